@@ -292,6 +292,73 @@ int snowverify_attention_ring(int pages);
  * the row tiles, on one XCD); 0 = automatic. Returns the previous value. */
 int snowverify_attention_row_groups(int groups);
 
+/* ---- attention over selected pages (extensions, no counterpart in the reference) ------
+ * Long contexts read a bounded number of pages per row: each page keeps the bounds of its keys,
+ * a row takes the pages whose bounds allow the largest scores, and attends to those. Rows are
+ * padded [batch, tokens]; pools and table as in snowverify_paged_attention, page 16, num_heads
+ * a multiple of num_kv_heads, head_size 64, 128 or 256. blocks: pages in the pools; a table
+ * entry outside 0 .. blocks - 1, and a page past table_stride, is no page: it is not written,
+ * not read, and scores lowest. bounds bf16 [blocks, num_kv_heads, 2, head_size]: the element-wise
+ * minimum and maximum of a page's keys, NaN where a key's element is NaN. Nothing here keeps
+ * library-owned scratch: calls on different streams need different scratch and no more. */
+
+/* The cache write of counts[b] rows of request b at positions starts[b], starts[b] + 1, ..: K per
+ * head normalised (k_gamma [head_size] bf16: RMSNorm with eps; NULL: not), its first 2 * half
+ * elements rotated in the pairs (i, i + half) by cos/sin [row, half] f32 (rows cs_stride apart),
+ * rounded once; V as it is. Row t of request b is row m = b * tokens + t: K head h at k + m *
+ * k_stride + h * head_size, V and q alike (strides in elements, multiples of 8; pointers 16-byte
+ * aligned). bounds (NULL: none kept): those of every page written, over its keys up to the last
+ * one written, whatever the page holds behind it. q (NULL: none): the same norm (q_gamma) and
+ * rotation into q_out [batch*tokens, num_heads, head_size]. counts above `tokens` count as
+ * tokens; a request with a count or start below 0 has no rows; rows past a request's count, in
+ * q_out too, are left as they were. half a multiple of 8, 2 * half <= head_size. Requests that
+ * write the same page race. */
+int snowverify_kv_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                         const void* q, int64_t q_stride, const float* cos_in,
+                         const float* sin_in, int64_t cs_stride, int64_t half,
+                         const void* q_gamma, const void* k_gamma, float eps, void* k_pool,
+                         void* v_pool, void* bounds, void* q_out, const int32_t* table,
+                         const int32_t* starts, const int32_t* counts, int64_t batch,
+                         int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                         int64_t head_size, int64_t table_stride, int64_t blocks, void* stream);
+/* The bounds of the pages that hold positions starts[b] .. starts[b] + counts[b] - 1, from the K
+ * pool: for pages that another writer filled. tokens: the most any counts[b] may be (larger ones
+ * count as tokens). */
+int snowverify_page_bounds(const void* k_pool, void* bounds, const int32_t* table,
+                           const int32_t* starts, const int32_t* counts, int64_t batch,
+                           int64_t tokens, int64_t num_kv_heads, int64_t head_size,
+                           int64_t table_stride, int64_t blocks, void* stream);
+/* Scratch bytes of snowverify_page_select (table_stride: pages per request, at most 2^17). */
+int64_t snowverify_page_select_scratch_bytes(int64_t batch, int64_t tokens, int64_t num_heads,
+                                             int64_t num_kv_heads, int64_t head_size,
+                                             int64_t table_stride);
+/* pages i32 [batch*tokens, num_kv_heads, budget]: the pages that each row (q bf16 [batch*tokens,
+ * num_heads, head_size], its last visible position positions[m], negative: none) reads per kv
+ * head, ascending, -1 behind the last. All of the row's pages where they are at most budget; else
+ * its first `sink`, its last `recent` (at least 1: the page of the row's own position is not
+ * judged by bounds that later rows are part of) and, of the others, those with the largest sum
+ * over the kv head's q heads g and elements d of max(q_gd low_d, q_gd high_d), in 64 bits, the
+ * lowest page first among equals; NaN counts as -inf. sink + recent <= budget. */
+int snowverify_page_select(const void* q, const void* bounds, const int32_t* table,
+                           const int32_t* positions, int32_t* pages, int64_t batch,
+                           int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                           int64_t head_size, int64_t table_stride, int64_t blocks,
+                           int64_t budget, int64_t sink, int64_t recent, void* scratch,
+                           int64_t scratch_bytes, void* stream);
+/* Scratch bytes of snowverify_sparse_attention (may be 0). */
+int64_t snowverify_sparse_attention_scratch_bytes(int64_t batch, int64_t tokens,
+                                                  int64_t num_heads, int64_t num_kv_heads,
+                                                  int64_t head_size, int64_t budget);
+/* out[m, h] = softmax(scale q k^T) v over the keys at positions <= positions[m] of the pages
+ * listed for (m, kv head), a page as often as it is listed; entries that are no page, or lie past
+ * the row's position, are passed over. A row that sees no key gets zeros. */
+int snowverify_sparse_attention(const void* q, const void* k_pool, const void* v_pool, void* out,
+                                const int32_t* table, const int32_t* positions,
+                                const int32_t* pages, int64_t batch, int64_t tokens,
+                                int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
+                                int64_t table_stride, int64_t blocks, int64_t budget, float scale,
+                                void* scratch, int64_t scratch_bytes, void* stream);
+
 /* ---- geometry-driven operator entry points (reference signatures) ---------------------
  * Shapes from the active geometry (see below); weights in the reference's _Weight descriptor
  * (snowllm/ops/inference.py:10-22) holding this library's repacked layouts: k-quant (quant,

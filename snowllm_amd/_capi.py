@@ -109,6 +109,14 @@ _SIGS = [
     ("snowverify_attention_d_split", c_int, [c_int]),
     ("snowverify_attention_ring", c_int, [c_int]),
     ("snowverify_attention_row_groups", c_int, [c_int]),
+    # attention over selected pages
+    ("snowverify_kv_append", c_int, [P, c_int64] * 3 + [P, P, c_int64, c_int64, P, P, c_float] +
+     [P] * 7 + [c_int64] * 7 + [S]),
+    ("snowverify_page_bounds", c_int, [P] * 5 + [c_int64] * 6 + [S]),
+    ("snowverify_page_select_scratch_bytes", c_int64, [c_int64] * 6),
+    ("snowverify_page_select", c_int, [P] * 5 + [c_int64] * 10 + [P, c_int64, S]),
+    ("snowverify_sparse_attention_scratch_bytes", c_int64, [c_int64] * 6),
+    ("snowverify_sparse_attention", c_int, [P] * 7 + [c_int64] * 8 + [c_float, P, c_int64, S]),
     # geometry-driven operator entry points (reference signatures)
     ("snowllm_qkv_proj_scratch_bytes", c_int64, [c_int64]),
     ("snowllm_attn_out_scale_oproj_scratch_bytes", c_int64, [c_int64]),

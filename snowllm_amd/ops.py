@@ -17,6 +17,8 @@ from .attention import (kv_pool_bytes, paged_attention_explicit,  # noqa: F401
                         paged_decode_num_slots, paged_decode_workspace_size,
                         paged_decode_plan_elems, paged_attn_decode_plan, paged_attn_decode,
                         prefill_q_plan)
+from .sparse import (kv_append, page_bounds, page_select, page_select_scratch_bytes,  # noqa: F401
+                     sparse_attention, sparse_attention_scratch_bytes)
 from .inference import (KQuantProjWeight, KQuantExpertWeight, inference_qkv,  # noqa: F401
                         qkv_proj_scratch_bytes, inference_mlp, mlp_workspace_bytes,
                         inference_moe, inference_moe_norm, inference_moe_workspace_bytes,
