@@ -286,17 +286,33 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(
 // ---------------------------------------------------------------------------------------
 // A page's score for a row and kv head is the sum over the group's heads of the largest q . k that
 // keys within the page's bounds could have:
-//   sum_g sum_d max(q_gd low_d, q_gd high_d) = sum_d P_d high_d - N_d low_d,
-//   P_d = sum_g max(q_gd, 0), N_d = sum_g max(-q_gd, 0),
-// one product of 2 D terms per (row, kv head, page). It is taken in 64 bits: the choice turns on
-// differences between nearly equal scores, and P and each product are then exact.
+//   s = sum_g sum_d max(q_gd low_d, q_gd high_d) = sum_d P_d high_d + N_d low_d,
+//   P_d = sum_g max(q_gd, 0), N_d = sum_g min(q_gd, 0),
+// one product of 2 D terms per (row, kv head, page). The choice turns on differences between nearly
+// equal scores, so it is made on 64-bit sums; but only few pages are near the border. The matrix
+// cores give every page a 32-bit s~ and a bound E on its error; with t the need-th largest s~, a
+// page above t + 2 E is chosen and one below t - 2 E is not whatever the exact sums are, and only
+// the pages between are summed in 64 bits.
+//
+// E: with A = sum_d |P_d high_d| + |N_d low_d|,
+//   P and N are 32-bit sums of G values                               <= G 2^-24 A
+//   each is multiplied as two bf16 pieces, what is left is            <= 2^-18 A
+//   2 . 2 D / 32 <= 32 matrix instructions add to one accumulator, each with at most 16 roundings
+//   of 2^-24 of what has been summed                                  <= 2^-15 A
+// so E = (2^-14 + G 2^-24) A, A from a third product of the larger pieces with |bounds| (2^-8 too
+// small at most: 1.01 A). Operands that the matrix cores could flush (below 2^-126) are kept out:
+// rows with a P or |N| between 0 and 2^-90, and anything not finite, have E = infinity, and all
+// their pages are summed in 64 bits; bounds below 2^-126 add at most 2^-126 sum |P| + |N|, products
+// that underflow at most 2^-110.
 struct SelectArgs {
   const uint16_t* q;        // [rows, Hq, D]
   const uint16_t* bounds;
   const int32_t* table;
   const int32_t* positions; // [rows] the last position a row sees, negative: none
   int32_t* pages;           // [rows, Hkv, budget]
-  double* scores;           // [requests, Hkv, T, width]
+  float* scores;            // [requests, Hkv, rows, width] s~
+  float* errors;            // [requests, Hkv, rows, width / 16] E of 16 pages
+  uint64_t* exact;          // [requests, Hkv, rows, width] keys, where a row needs them all
   int64_t table_stride, blocks, width, T, row0;   // row0: first row of every request in this launch
   int rows, Hq, Hkv, G, budget, sink, recent;     // rows: of a request in this launch
 };
@@ -307,86 +323,132 @@ __device__ __forceinline__ int64_t pages_seen(int pos, int64_t stride) {
   return n < stride ? n : stride;
 }
 
-constexpr int SCORE_TILES = 4;   // 16-page tiles per step of a score workgroup
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ float pos_part(float f) { return !(f <= 0.f) ? f : 0.f; }   // NaN stays
+__device__ __forceinline__ float neg_part(float f) { return !(f >= 0.f) ? f : 0.f; }
 
-// Four waves, each a quarter of the 2 D terms (waves 0, 1: -N and the minima; 2, 3: P and the
-// maxima), sixteen rows and sixteen pages a matrix instruction (v_mfma_f64_16x16x4_f64). The rows'
-// operand stays in registers; a lane's 16-byte load of a page's bounds feeds eight instructions.
-// The quarters are added in LDS.
+constexpr int SCORE_WAVES = 4;
+
+// A workgroup: sixteen rows of a request and kv head. Its threads sum the rows' P and N and leave
+// both pieces in LDS as operands of v_mfma_f32_16x16x32_bf16 (terms: D of N with the minima, then D
+// of P with the maxima), which every wave then holds in registers; the waves take sixteen pages at a
+// time, whose bounds are the other operand as they lie in memory.
 template <int D>
-__global__ void __launch_bounds__(256) score_kernel(SelectArgs a, int64_t pages_per_wg) {
-  constexpr int NS = D / 64;   // 16-byte loads of a lane per page: D / 2 terms of a wave
-  __shared__ double part[4][SCORE_TILES][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a, int64_t pages_per_wg) {
+  constexpr int NS = D / 16;   // steps of 32 terms
+  __shared__ u32x4 op[NS][2][64];
+  __shared__ float total[16];  // sum |P| + |N| of a row, infinite for a row that is not to be trusted
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
   const int tiles = (a.rows + 15) / 16;
   int64_t y = blockIdx.x;
   const int tile = (int)(y % tiles);
   y /= tiles;
   const int h = (int)(y % a.Hkv), b = (int)(y / a.Hkv);
-  const int64_t t0 = a.row0 + tile * 16;
-  const bool live = tile * 16 + col < a.rows;
-  const int64_t m = (int64_t)b * a.T + t0 + (live ? col : 0);
-  const int64_t n = live ? pages_seen(a.positions[m], a.table_stride) : 0;
+  const int64_t m0 = (int64_t)b * a.T + a.row0 + tile * 16;
+  const int live = a.rows - tile * 16 < 16 ? a.rows - tile * 16 : 16;
+  const int64_t n = col < live ? pages_seen(a.positions[m0 + col], a.table_stride) : 0;
   const int64_t last = (int64_t)wave_max<int>((int)n);
   const int64_t p0 = (int64_t)blockIdx.y * pages_per_wg;
   if (p0 >= last) return;
   const int64_t p1 = p0 + pages_per_wg < last ? p0 + pages_per_wg : last;
-  const int side = wave >> 1, d0 = (wave & 1) * (D / 2);
-  double w[NS * 8];
+  if (tid < 16) total[tid] = 0.f;
+  __syncthreads();
+  // unit u: row u % 16 and the eight elements 8 (u / 16) ..; lane (row, (u / 16) % 4) of step u / 64
+  for (int u = tid; u < 16 * (D / 8); u += 64 * SCORE_WAVES) {
+    const int r = u & 15, c = u >> 4;
+    float p[8], q[8];
 #pragma unroll
-  for (int i = 0; i < NS * 8; ++i) w[i] = 0.0;
-  if (live)
-    for (int e = 0; e < a.G; ++e) {
-      const uint16_t* qp = a.q + (m * a.Hq + h * a.G + e) * D + d0 + 8 * g;
+    for (int i = 0; i < 8; ++i) p[i] = q[i] = 0.f;
+    if (r < live) {
+      const uint16_t* qp = a.q + ((m0 + r) * a.Hq + (int64_t)h * a.G) * D + 8 * c;
+#pragma unroll 8
+      for (int e = 0; e < a.G; ++e) {
+        const u32x4 x = *(const u32x4*)(qp + (int64_t)e * D);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const u32x4 x = *(const u32x4*)(qp + 32 * s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float f = __uint_as_float(i & 1 ? x[i / 2] & 0xffff0000u : x[i / 2] << 16);
-          // max(q, 0) with the maxima, min(q, 0) = -N with the minima; NaN stays
-          if (side ? !(f <= 0.f) : !(f >= 0.f)) w[s * 8 + i] += (double)f;
+        for (int i = 0; i < 4; ++i) {
+          const float f0 = bf_lo(x[i]), f1 = bf_hi(x[i]);
+          p[2 * i] += pos_part(f0);
+          p[2 * i + 1] += pos_part(f1);
+          q[2 * i] += neg_part(f0);
+          q[2 * i + 1] += neg_part(f1);
         }
       }
     }
-  for (int64_t p = p0; p < p1; p += 16 * SCORE_TILES) {
-    u32x4 x[SCORE_TILES][NS];
+    float sum = 0.f;
+    u32x4 ph, pl, qh, ql;
 #pragma unroll
-    for (int i = 0; i < SCORE_TILES; ++i) {
-      const int64_t pg = p + 16 * i + col;
-      const int blk = page_block(a.table, a.table_stride, b, pg < last ? pg : last - 1, a.blocks);
-      const uint16_t* bp = a.bounds + (((int64_t)(blk < 0 ? 0 : blk) * a.Hkv + h) * 2 + side) * D + d0 + 8 * g;
+    for (int i = 0; i < 8; ++i) {
+      const float x = p[i] - q[i];
+      const bool small = (p[i] > 0.f && p[i] < 0x1p-90f) || (q[i] < 0.f && q[i] > -0x1p-90f);
+      sum += small ? __builtin_huge_valf() : x;
+    }
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        x[i][s] = *(const u32x4*)(bp + 32 * s);
-        if (blk < 0) x[i][s] = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};   // NaN
+    for (int i = 0; i < 4; ++i) {
+      ph[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+      qh[i] = pack_bf16x2(q[2 * i], q[2 * i + 1]);
+      pl[i] = pack_bf16x2(p[2 * i] - bf_lo(ph[i]), p[2 * i + 1] - bf_hi(ph[i]));
+      ql[i] = pack_bf16x2(q[2 * i] - bf_lo(qh[i]), q[2 * i + 1] - bf_hi(qh[i]));
+    }
+    const int s = c >> 2, l = (c & 3) * 16 + r;
+    op[s][0][l] = qh;
+    op[s][1][l] = ql;
+    op[NS / 2 + s][0][l] = ph;
+    op[NS / 2 + s][1][l] = pl;
+    if (r < live) atomicAdd(&total[r], sum);   // only a bound: its order is free
+  }
+  __syncthreads();
+  bf16x8 wh[NS], wl[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    wh[s] = __builtin_bit_cast(bf16x8, op[s][0][lane]);
+    wl[s] = __builtin_bit_cast(bf16x8, op[s][1][lane]);
+  }
+  const float tot = total[col];
+  const float rel = 1.01f * (0x1p-14f + (float)a.G * 0x1p-24f);
+  const int64_t item = ((int64_t)b * a.Hkv + h) * a.rows + tile * 16 + col;
+  float* sc = a.scores + item * a.width;
+  float* er = a.errors + item * (a.width / 16);
+  int64_t p = p0 + 16 * wave;
+  int blk = p < p1 ? page_block(a.table, a.table_stride, b, p + col < last ? p + col : last - 1, a.blocks) : -1;
+  for (; p < p1; p += 16 * SCORE_WAVES) {
+    const uint16_t* bp = a.bounds + ((int64_t)(blk < 0 ? 0 : blk) * a.Hkv + h) * 2 * D + 8 * g;
+    u32x4 x[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) x[s] = *(const u32x4*)(bp + 32 * s);
+    const uint64_t none = __ballot(blk < 0);   // bit i: page p + i is no page
+    const int64_t pn = p + 16 * SCORE_WAVES;
+    blk = pn < p1 ? page_block(a.table, a.table_stride, b, pn + col < last ? pn + col : last - 1, a.blocks) : -1;
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f}, mag = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const bf16x8 f = __builtin_bit_cast(bf16x8, x[s]);
+      // |bounds|, with the sign of the operand's piece: N is negative
+      u32x4 ab;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ab[i] = s < NS / 2 ? x[s][i] | 0x80008000u : x[s][i] & 0x7fff7fffu;
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, wh[s], acc, 0, 0, 0);
+      mag = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ab), wh[s], mag, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, wl[s], acc, 0, 0, 0);
+    }
+    // lane (row col, g): pages p + 4 g + r. The first pages, always chosen, do not count.
+    float e = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool no = none >> (4 * g + r) & 1;
+      if (no) acc[r] = -__builtin_huge_valf();
+      const int64_t pg = p + 4 * g + r;
+      if (!no && pg >= a.sink && pg < last) {
+        const float er1 = __builtin_fmaf(rel, mag[r], __builtin_fmaf(0x1p-126f, tot, 0x1p-110f));
+        e = er1 < 0x1p120f ? fmaxf(e, er1) : __builtin_huge_valf();   // NaN too
       }
     }
-#pragma unroll
-    for (int i = 0; i < SCORE_TILES; ++i) {
-      doublex4 acc = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = __uint_as_float(e & 1 ? x[i][s][e / 2] & 0xffff0000u : x[i][s][e / 2] << 16);
-          acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f, w[s * 8 + e], acc, 0, 0, 0);
-        }
-      // lane (row col, g): pages g + 4 r
-#pragma unroll
-      for (int r = 0; r < 4; ++r) part[wave][i][col * 16 + g + 4 * r] = acc[r];
+    e = fmaxf(e, __shfl_xor(e, 16, 64));
+    e = fmaxf(e, __shfl_xor(e, 32, 64));
+    if (col < live) {
+      *(floatx4*)(sc + p + 4 * g) = acc;
+      if (g == 0) er[p / 16] = tot < 0x1p120f ? e : __builtin_huge_valf();
     }
-    __syncthreads();
-    // thread: a row and pages of one tile
-#pragma unroll
-    for (int i = 0; i < SCORE_TILES; ++i) {
-      const int row = threadIdx.x >> 4, pg = threadIdx.x & 15;
-      const double s = (part[0][i][threadIdx.x] + part[1][i][threadIdx.x]) +
-                       (part[2][i][threadIdx.x] + part[3][i][threadIdx.x]);
-      if (tile * 16 + row < a.rows && p + 16 * i + pg < p1)
-        a.scores[(((int64_t)b * a.Hkv + h) * a.rows + tile * 16 + row) * a.width + p + 16 * i + pg] = s;
-    }
-    __syncthreads();
   }
 }
 
@@ -398,38 +460,282 @@ __device__ __forceinline__ uint64_t score_key(double s) {
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
-constexpr int PICK_THREADS = 256;
+constexpr int PICK_NEAR = 512;    // pages near the border that are ranked in LDS
+constexpr int PICK_KEYS = 16;     // scores a thread keeps in registers
 
-// One workgroup per (row, kv head): the need-th largest key by radix selection, eight bits a pass,
-// then the pages above it and the lowest-numbered of those equal to it, in ascending order, from
-// ballots kept in LDS.
-__global__ void __launch_bounds__(PICK_THREADS) pick_kernel(SelectArgs a) {
-  extern __shared__ uint64_t masks[];   // [words] chosen pages, then u32 [words] ranks before
-  __shared__ uint32_t hist[256];
+// The 64-bit score's key of one page, by a wave: lane l sums terms l, l + 64, .. in order, then a
+// fixed tree, so that equal pages have equal sums. pn [2 D]: N, then P.
+template <int D>
+__device__ __forceinline__ uint64_t exact_key(const SelectArgs& a, const double* pn, int b, int h, int64_t page) {
+  const int lane = threadIdx.x & 63;
+  const int blk = page_block(a.table, a.table_stride, b, page, a.blocks);
+  if (blk < 0) return score_key(-__builtin_huge_val());
+  const uint16_t* bp = a.bounds + ((int64_t)blk * a.Hkv + h) * 2 * D;
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 2 * D / 64; ++i) s += pn[64 * i + lane] * (double)bf16_to_f32(bp[64 * i + lane]);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+  return score_key(s);
+}
+
+// One workgroup per (row, kv head). CACHED: its scores fit the threads' registers.
+template <int D, int NT, bool CACHED>
+__global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
+  constexpr int BINS = 4 * NT, WAVES = NT / 64;
+  extern __shared__ uint64_t masks[];   // [words] chosen pages, [words] equal ones, u32 [words] ranks before
+  // a histogram, then the near pages' keys and numbers
+  __shared__ uint64_t lists[BINS / 2 > PICK_NEAR * 3 / 2 ? BINS / 2 : PICK_NEAR * 3 / 2];
+  uint32_t* hist = (uint32_t*)lists;
+  uint64_t* near_key = lists;
+  uint32_t* near_page = (uint32_t*)(lists + PICK_NEAR);
+  __shared__ double pn[2 * D];
+  __shared__ float red[3][WAVES];
+  __shared__ uint32_t redc[WAVES];
+  __shared__ float member[64];
+  __shared__ uint32_t sh[6];            // 0: members, 1: bin, 2: above the bin, 3: in the bin, 4: near, 5: chosen
   __shared__ uint64_t sh_prefix;
-  __shared__ uint32_t sh_need;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t item = blockIdx.x;      // (request, kv head, row)
   const int row = (int)(item % a.rows);
   const int h = (int)(item / a.rows % a.Hkv);
-  const int64_t b = item / a.rows / a.Hkv;
-  const int64_t m = b * a.T + a.row0 + row;
+  const int b = (int)(item / a.rows / a.Hkv);
+  const int64_t m = (int64_t)b * a.T + a.row0 + row;
   int32_t* out = a.pages + (m * a.Hkv + h) * a.budget;
   const int n = (int)pages_seen(a.positions[m], a.table_stride);
   if (n <= a.budget) {
-    for (int i = tid; i < a.budget; i += PICK_THREADS) out[i] = i < n ? i : -1;
+    for (int i = tid; i < a.budget; i += NT) out[i] = i < n ? i : -1;
     return;
   }
   const int first = a.sink, end = n - a.recent;   // candidates; n > budget >= sink + recent
-  const double* sc = a.scores + item * a.width;
-  uint32_t need = (uint32_t)(a.budget - a.sink - a.recent);
-  uint64_t prefix = 0;
-  if (need > 0)
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += PICK_THREADS) hist[i] = 0;
+  const uint32_t need0 = (uint32_t)(a.budget - a.sink - a.recent);
+  const float* sc = a.scores + item * a.width;
+  const int words = (n + 63) / 64;
+  uint64_t* equal = masks + words;
+  uint32_t* rank = (uint32_t*)(masks + 2 * words);
+  const float inf = __builtin_huge_valf();
+
+  float key[CACHED ? PICK_KEYS : 1];
+  // f(page, score) over the candidates, a word of 64 pages per wave and step
+  auto scan = [&](auto f) {
+    if constexpr (CACHED) {
+#pragma unroll
+      for (int j = 0; j < PICK_KEYS; ++j) f(j * NT + tid, key[j]);
+    } else {
+      for (int i = tid; i < words * 64; i += NT) f(i, i >= first && i < end ? sc[i] : -inf);
+    }
+  };
+  float e = 0.f, hi = -inf, lo = inf;
+  uint32_t pages = 0;                   // candidates that are pages
+  if (need0 > 0) {
+    if constexpr (CACHED) {
+#pragma unroll
+      for (int j = 0; j < PICK_KEYS; ++j) {
+        const int i = j * NT + tid;
+        key[j] = i >= first && i < end ? sc[i] : -inf;
+      }
+    }
+    const float* er = a.errors + item * (a.width / 16);
+    for (int i = tid; i < (n + 15) / 16; i += NT) e = fmaxf(e, er[i]);
+    scan([&](int i, float s) {
+      if (s > -inf) hi = fmaxf(hi, s), lo = fminf(lo, s), ++pages;
+    });
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) {
+      e = fmaxf(e, __shfl_xor(e, s, 64));
+      hi = fmaxf(hi, __shfl_xor(hi, s, 64));
+      lo = fminf(lo, __shfl_xor(lo, s, 64));
+    }
+    pages = wave_sum<uint32_t>(pages);
+    if (lane == 0) red[0][wave] = e, red[1][wave] = hi, red[2][wave] = lo, redc[wave] = pages;
+    __syncthreads();
+    pages = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      pages += redc[w];
+      e = fmaxf(e, red[0][w]);
+      hi = fmaxf(hi, red[1][w]);
+      lo = fminf(lo, red[2][w]);
+    }
+  }
+  // t, the need-th largest s~: histograms over [lo, hi], ever narrower, until 64 scores are left
+  float t = 0.f;
+  bool all = need0 > 0 && !(e < inf && hi < inf && pages >= need0);   // all pages in 64 bits
+  if (need0 > 0 && !all) {
+    uint32_t above = 0;                 // scores > hi
+    for (int round = 0;; ++round) {
+      if (lo == hi) {
+        t = lo;
+        break;
+      }
+      if (round == 32) {
+        all = true;
+        break;
+      }
+      const float inv = (float)(BINS - 1) / (hi - lo);
+      auto bin = [&](float s) {
+        const float x = (s - lo) * inv;
+        return x >= (float)(BINS - 1) ? BINS - 1 : x > 0.f ? (int)x : 0;
+      };
+      for (int i = tid; i < BINS; i += NT) hist[i] = 0;
+      if (tid == 0) sh[0] = 0;
       __syncthreads();
-      for (int i = first + tid; i < end; i += PICK_THREADS) {
-        const uint64_t k = score_key(sc[i]);
+      scan([&](int i, float s) {
+        if (s >= lo && s <= hi) atomicAdd(&hist[bin(s)], 1u);
+      });
+      __syncthreads();
+      // thread: four bins, from the top
+      const int top = BINS - 1 - 4 * tid;
+      uint32_t c[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += c[i] = hist[top - i];
+      uint32_t before = (uint32_t)wave_incl_sum_u64(sum);
+      if (lane == 63) redc[wave] = before;
+      before -= sum;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) before += redc[w];
+      before += above;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (before < need0 && before + c[i] >= need0) sh[1] = (uint32_t)(top - i), sh[2] = before, sh[3] = c[i];
+        before += c[i];
+      }
+      __syncthreads();
+      const int at = (int)sh[1];
+      const uint32_t count = sh[3];
+      above = sh[2];
+      if (count <= 64) {
+        scan([&](int i, float s) {
+          if (s >= lo && s <= hi && bin(s) == at) member[atomicAdd(&sh[0], 1u)] = s;
+        });
+        __syncthreads();
+        const float mine = lane < (int)count ? member[lane] : -inf;
+        uint32_t over = 0, same = 0;
+        for (int i = 0; i < (int)count; ++i) {
+          over += member[i] > mine;
+          same += member[i] == mine;
+        }
+        const uint32_t k = need0 - above;   // 1 .. count
+        const uint64_t is = __ballot(lane < (int)count && over < k && over + same >= k);
+        t = __shfl(mine, __builtin_ctzll(is), 64);
+        break;
+      }
+      float nh = -inf, nl = inf;
+      scan([&](int i, float s) {
+        if (s >= lo && s <= hi && bin(s) == at) nh = fmaxf(nh, s), nl = fminf(nl, s);
+      });
+#pragma unroll
+      for (int s = 32; s > 0; s >>= 1) {
+        nh = fmaxf(nh, __shfl_xor(nh, s, 64));
+        nl = fminf(nl, __shfl_xor(nl, s, 64));
+      }
+      __syncthreads();
+      if (lane == 0) red[1][wave] = nh, red[2][wave] = nl;
+      __syncthreads();
+      for (int w = 0; w < WAVES; ++w) {
+        nh = fmaxf(nh, red[1][w]);
+        nl = fminf(nl, red[2][w]);
+      }
+      hi = nh;
+      lo = nl;
+    }
+  }
+  // chosen for certain, and near
+  uint32_t need = 0;                    // of the pages in `equal`, the lowest that many
+  if (!all) {
+    const float over = t + 2.f * e, under = t - 2.f * e;
+    if (tid == 0) sh[4] = sh[5] = 0;
+    __syncthreads();
+    scan([&](int i, float s) {
+      const bool mid = i >= first && i < end;
+      const bool in = i < n && (!mid || (need0 > 0 && s > over));
+      const bool near = mid && need0 > 0 && s >= under && s <= over;
+      const uint64_t mi = __ballot(in), mn = __ballot(near);
+      if (i < words * 64) {             // uniform: a wave's word
+        uint32_t base = 0;
+        if (lane == 0) {
+          masks[i / 64] = mi;
+          equal[i / 64] = 0;
+          if (mn) base = atomicAdd(&sh[4], (uint32_t)__popcll(mn));
+          atomicAdd(&sh[5], (uint32_t)__popcll(mi));
+        }
+        if (mn) {
+          base = (uint32_t)__shfl((int)base, 0, 64);
+          const uint32_t to = base + (uint32_t)__popcll(mn & ((1ull << lane) - 1));
+          if (near && to < PICK_NEAR) near_page[to] = (uint32_t)i;
+        }
+      }
+    });
+    __syncthreads();
+    const uint32_t near = sh[4], left = (uint32_t)a.budget - sh[5];
+    if (need0 > 0 && near > PICK_NEAR && near > left) {
+      all = true;
+    } else if (near > PICK_NEAR) {      // all of them are chosen
+      __syncthreads();
+      scan([&](int i, float s) {
+        const uint64_t mi = __ballot(i < n && (i < first || i >= end || s >= under));
+        if (i < words * 64 && lane == 0) masks[i / 64] = mi;
+      });
+    } else if (near > 0) {
+      if (near > left) {
+        for (int d = tid; d < D; d += NT) {
+          double p = 0.0, q = 0.0;
+          const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D + d;
+#pragma unroll 8
+          for (int g = 0; g < a.G; ++g) {
+            const float f = bf16_to_f32(qp[(int64_t)g * D]);
+            p += (double)pos_part(f);
+            q += (double)neg_part(f);
+          }
+          pn[d] = q;
+          pn[D + d] = p;
+        }
+        __syncthreads();
+        for (uint32_t i = wave; i < near; i += WAVES) {
+          const uint64_t k = exact_key<D>(a, pn, b, h, near_page[i]);
+          if (lane == 0) near_key[i] = k;
+        }
+        __syncthreads();
+      }
+      for (uint32_t i = tid; i < near; i += NT) {
+        const uint32_t pg = near_page[i];
+        uint32_t ahead = 0;
+        if (near > left) {
+          const uint64_t k = near_key[i];
+          for (uint32_t j = 0; j < near; ++j) ahead += near_key[j] > k || (near_key[j] == k && near_page[j] < pg);
+        }
+        if (ahead < left) atomicOr((unsigned long long*)&masks[pg / 64], 1ull << (pg & 63));
+      }
+    }
+    __syncthreads();
+  }
+  if (all) {
+    // every candidate in 64 bits, the need-th largest key by radix selection, eight bits a pass
+    for (int d = tid; d < D; d += NT) {
+      double p = 0.0, q = 0.0;
+      const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D + d;
+      for (int g = 0; g < a.G; ++g) {
+        const float f = bf16_to_f32(qp[(int64_t)g * D]);
+        p += (double)pos_part(f);
+        q += (double)neg_part(f);
+      }
+      pn[d] = q;
+      pn[D + d] = p;
+    }
+    __syncthreads();
+    uint64_t* ex = a.exact + item * a.width;
+    for (int i = first + wave; i < end; i += WAVES) {
+      const uint64_t k = exact_key<D>(a, pn, b, h, i);
+      if (lane == 0) ex[i] = k;
+    }
+    __threadfence_block();
+    __syncthreads();
+    uint64_t prefix = 0;
+    need = need0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += NT) hist[i] = 0;
+      __syncthreads();
+      for (int i = first + tid; i < end; i += NT) {
+        const uint64_t k = ex[i];
         if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
           atomicAdd(&hist[(k >> shift) & 255], 1u);
       }
@@ -439,51 +745,50 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_kernel(SelectArgs a) {
         int d = 255;
         while (d > 0 && seen + hist[d] < need) seen += hist[d--];
         sh_prefix = prefix | (uint64_t)d << shift;
-        sh_need = need - seen;
+        sh[2] = need - seen;
       }
       __syncthreads();
       prefix = sh_prefix;
-      need = sh_need;
+      need = sh[2];
       __syncthreads();
     }
-  // `need` of the pages equal to the threshold, lowest first; all above it
-  const int words = (n + 63) / 64;
-  uint32_t* rank = (uint32_t*)(masks + words);
-  uint64_t* equal = masks + words + (words + 1) / 2;
-  for (int w = wave; w < words; w += PICK_THREADS / 64) {
-    const int i = w * 64 + lane;
-    const bool mid = i >= first && i < end;
-    const uint64_t k = mid && a.budget > a.sink + a.recent ? score_key(sc[i]) : 0;
-    const bool over = i < n && (!mid || (a.budget > a.sink + a.recent && k > prefix));
-    const bool eq = mid && a.budget > a.sink + a.recent && k == prefix;
-    const uint64_t mo = __ballot(over), me = __ballot(eq);
-    if (lane == 0) masks[w] = mo, equal[w] = me;
+    for (int i = tid; i < words * 64; i += NT) {
+      const bool mid = i >= first && i < end;
+      const uint64_t k = mid ? ex[i] : 0;
+      const uint64_t mo = __ballot(i < n && (!mid || k > prefix)), me = __ballot(mid && k == prefix);
+      if (lane == 0) masks[i / 64] = mo, equal[i / 64] = me;
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  // ranks of the words' first pages; of equal pages the lowest `need`
   if (wave == 0) {
     uint32_t eq_before = 0, before = 0;
     for (int w0 = 0; w0 < words; w0 += 64) {
       const int w = w0 + lane;
-      uint64_t mo = w < words ? masks[w] : 0, me = w < words ? equal[w] : 0;
-      const uint32_t ec = (uint32_t)__popcll(me);
-      const uint32_t ei = (uint32_t)wave_incl_sum_u64(ec);
-      const uint32_t eb = eq_before + ei - ec;
-      uint32_t take = eb >= need ? 0u : need - eb < ec ? need - eb : ec;
-      while (take > 0) {   // the lowest `take` set bits
-        const uint64_t bit = me & (~me + 1);
-        mo |= bit;
-        me ^= bit;
-        --take;
+      uint64_t mo = w < words ? masks[w] : 0;
+      if (need > 0) {
+        uint64_t me = w < words ? equal[w] : 0;
+        const uint32_t ec = (uint32_t)__popcll(me);
+        const uint32_t ei = (uint32_t)wave_incl_sum_u64(ec);
+        const uint32_t eb = eq_before + ei - ec;
+        uint32_t take = eb >= need ? 0u : need - eb < ec ? need - eb : ec;
+        while (take > 0) {   // the lowest `take` set bits
+          const uint64_t bit = me & (~me + 1);
+          mo |= bit;
+          me ^= bit;
+          --take;
+        }
+        eq_before += (uint32_t)__shfl((int)ei, 63, 64);
+        if (w < words) masks[w] = mo;
       }
       const uint32_t cnt = (uint32_t)__popcll(mo);
       const uint32_t ci = (uint32_t)wave_incl_sum_u64(cnt);
-      if (w < words) masks[w] = mo, rank[w] = before + ci - cnt;
-      eq_before += (uint32_t)__shfl((int)ei, 63, 64);
+      if (w < words) rank[w] = before + ci - cnt;
       before += (uint32_t)__shfl((int)ci, 63, 64);
     }
   }
   __syncthreads();
-  for (int w = wave; w < words; w += PICK_THREADS / 64) {
+  for (int w = wave; w < words; w += WAVES) {
     const uint64_t mo = masks[w];
     if (mo >> lane & 1) {
       const uint32_t at = rank[w] + (uint32_t)__popcll(mo & ((1ull << lane) - 1));
@@ -762,13 +1067,29 @@ int attend_splits(int64_t items, int64_t budget) {
   return (int)(s < 1 ? 1 : s);
 }
 
+// Workspace of one row's pages: scores, their errors, and keys where a row needs them all.
+int64_t select_width(int64_t pages) { return (pages + 15) / 16 * 16; }
+int64_t select_row_bytes(int64_t pages) { return select_width(pages) * 12 + select_width(pages) / 4; }
+
 // Rows of a request whose scores are in the workspace at a time (256 MiB).
-int64_t select_rows(int64_t batch, int64_t tokens, int64_t Hkv, int64_t width) {
-  const int64_t per_row = batch * Hkv * width * 8;
+int64_t select_rows(int64_t batch, int64_t tokens, int64_t Hkv, int64_t pages) {
+  const int64_t per_row = batch * Hkv * select_row_bytes(pages);
   int64_t r = per_row > 0 ? ((int64_t)256 << 20) / per_row : tokens;
   r = r / 16 * 16;
   if (r < 16) r = 16;
   return r < tokens ? r : tokens;
+}
+
+template <int D>
+auto pick_of(int64_t width) {
+  return width <= 256 * PICK_KEYS    ? pick_kernel<D, 256, true>
+         : width <= 1024 * PICK_KEYS ? pick_kernel<D, 1024, true>
+                                     : pick_kernel<D, 1024, false>;
+}
+// A thread holds up to sixteen scores: four waves up to 4096 pages, sixteen above, and past 16384
+// pages the scores are read again by every pass.
+auto pick_form(int64_t D, int64_t width) {
+  return D == 64 ? pick_of<64>(width) : D == 128 ? pick_of<128>(width) : pick_of<256>(width);
 }
 
 }  // namespace
@@ -861,7 +1182,8 @@ SV_API int64_t snowverify_page_select_scratch_bytes(int64_t batch, int64_t token
   if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
       table_stride > MAX_WIDTH)
     return 0;
-  return batch * select_rows(batch, tokens, num_kv_heads, table_stride) * num_kv_heads * table_stride * 8;
+  return batch * select_rows(batch, tokens, num_kv_heads, table_stride) * num_kv_heads *
+         select_row_bytes(table_stride);
 }
 
 SV_API int snowverify_page_select(const void* q, const void* bounds, const int32_t* table,
@@ -881,17 +1203,22 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
       (table_stride > 0 && !scratch))
     return SV_EINVAL;
   const int64_t chunk = select_rows(batch, tokens, num_kv_heads, table_stride);
-  if (!grid_ok(batch * num_kv_heads * chunk, PICK_THREADS)) return SV_EINVAL;
+  const int64_t width = select_width(table_stride);
+  const int threads = width <= 256 * PICK_KEYS ? 256 : 1024;
+  if (!grid_ok(batch * num_kv_heads * chunk, threads)) return SV_EINVAL;
   SelectArgs a{};
   a.q = (const uint16_t*)q;
   a.bounds = (const uint16_t*)bounds;
   a.table = table;
   a.positions = positions;
   a.pages = pages;
-  a.scores = (double*)scratch;
+  const int64_t cells = batch * num_kv_heads * chunk * width;
+  a.exact = (uint64_t*)scratch;
+  a.scores = (float*)(a.exact + cells);
+  a.errors = a.scores + cells;
   a.table_stride = table_stride;
   a.blocks = blocks;
-  a.width = table_stride;
+  a.width = width;
   a.T = tokens;
   a.Hq = (int)num_heads;
   a.Hkv = (int)num_kv_heads;
@@ -899,22 +1226,23 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
   a.budget = (int)budget;
   a.sink = (int)sink;
   a.recent = (int)recent;
-  const int64_t words = (table_stride + 63) / 64;
-  const size_t lds = (size_t)(2 * words + (words + 1) / 2) * 8;
+  const size_t lds = (size_t)((table_stride + 63) / 64) * 20;
+  auto score = head_size == 64 ? score_kernel<64> : head_size == 128 ? score_kernel<128> : score_kernel<256>;
+  auto pick = pick_form(head_size, width);
   for (int64_t r0 = 0; r0 < tokens; r0 += chunk) {
     a.row0 = r0;
     a.rows = (int)(tokens - r0 < chunk ? tokens - r0 : chunk);
     const int64_t tiles = batch * num_kv_heads * ((a.rows + 15) / 16);
     if (table_stride > budget) {   // otherwise every page of every row is taken
-      int64_t per = 16 * SCORE_TILES;
-      while (per < 1024 && tiles * ((table_stride + per - 1) / per) > 4096) per *= 2;
-      auto kern = head_size == 64 ? score_kernel<64> : head_size == 128 ? score_kernel<128> : score_kernel<256>;
-      hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)((table_stride + per - 1) / per)),
-                         dim3(256), 0, S(stream), a, per);
+      // about four workgroups a CU, each 64 to 2048 pages for the sixteen rows it prepares
+      int64_t per = (table_stride * tiles / 1024 + 63) / 64 * 64;
+      per = per < 64 ? 64 : per > 2048 ? 2048 : per;
+      hipLaunchKernelGGL(score, dim3((unsigned)tiles, (unsigned)((table_stride + per - 1) / per)),
+                         dim3(64 * SCORE_WAVES), 0, S(stream), a, per);
       SV_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(pick_kernel, dim3((unsigned)(batch * num_kv_heads * a.rows)),
-                       dim3(PICK_THREADS), lds, S(stream), a);
+    hipLaunchKernelGGL(pick, dim3((unsigned)(batch * num_kv_heads * a.rows)), dim3(threads), lds,
+                       S(stream), a);
     SV_CHECK_LAUNCH();
   }
   return SV_OK;

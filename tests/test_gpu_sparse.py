@@ -188,6 +188,9 @@ SELECT = [
     (2, 1, 256, 1, 17, 1030, 300, 3, 2),
     (8, 2, 64, 4, 3, 64, 1, 0, 1),
     (1, 1, 64, 1, 1, 1, 1, 0, 1),
+    (4, 2, 128, 1, 3, 5000, 128, 1, 2),
+    (2, 2, 64, 1, 2, 4096, 4000, 1, 2),
+    (2, 1, 64, 1, 2, 17000, 257, 0, 5),
 ]
 
 
@@ -210,18 +213,20 @@ def test_select(gpu, Hq, Hkv, d, B, T, width, budget, sink, recent):
     assert torch.equal(got, R.select(q, bounds, table, pos, budget, sink, recent))
 
 
-@pytest.mark.parametrize("kind", ["equal", "near", "nan", "inf", "holes", "past"])
-def test_select_borders(gpu, kind):
+@pytest.mark.parametrize("width,budget", [(300, 40), (1500, 40), (1500, 1400)])
+@pytest.mark.parametrize("kind", ["equal", "near", "same", "zero", "nan", "inf", "holes", "few", "past",
+                                  "tiny", "huge", "far"])
+def test_select_borders(gpu, kind, width, budget):
     """Equal and nearly equal scores, NaN and infinite bounds, pages that are none, positions past
-    the table."""
+    the table, values at the ends of the type's range, one page far above the others."""
     g = torch.Generator().manual_seed(11)
-    Hq, Hkv, d, T, width, budget = 8, 2, 128, 18, 300, 40
+    Hq, Hkv, d, T = 8, 2, 128, 18
     blocks = width + 5
     table = tables(g, 1, width, blocks)
     q = torch.randn(T, Hq, d, generator=g).bfloat16()
     x = torch.randn(blocks, Hkv, 2, d, generator=g)
     bounds = torch.stack([x.amin(2), x.amax(2)], 2).bfloat16()
-    pos = torch.randint(100 * PAGE, width * PAGE, (T,), generator=g, dtype=torch.int32)
+    pos = torch.randint(width // 2 * PAGE, width * PAGE, (T,), generator=g, dtype=torch.int32)
     if kind == "equal":                 # a few distinct pages, each many times
         bounds = bounds[torch.randint(0, 7, (blocks,), generator=g)].contiguous()
     if kind == "near":                  # all pages alike but for one element's last bit
@@ -230,6 +235,17 @@ def test_select_borders(gpu, kind):
         lines = bits(bounds).view(blocks, Hkv, 2, d)
         lines[torch.arange(blocks), :, 1, at] += 1
         bounds = lines.view(torch.bfloat16)
+    if kind == "same":                  # one page, many times
+        bounds[:] = bounds[:1]
+    if kind == "zero":
+        bounds[:] = 0.0
+    if kind == "tiny":                  # subnormal operands and products
+        bounds = (bounds.float() * 2.0 ** -125).bfloat16()
+        q[::2] = (q[::2].float() * 2.0 ** -100).bfloat16()
+    if kind == "huge":                  # scores past the 32-bit range
+        bounds = (bounds.float() * 2.0 ** 120).bfloat16()
+    if kind == "far":
+        bounds[5::400] *= 2.0 ** 30
     if kind == "nan":
         bounds[::2, :, 0, 3] = float("nan")
         q[3, 2, 5] = float("nan")       # every score of that row and kv head
@@ -240,6 +256,8 @@ def test_select_borders(gpu, kind):
     if kind == "holes":
         table[0, 5:60:3] = -1
         table[0, 6:60:3] = blocks
+    if kind == "few":                   # fewer pages than the budget
+        table[0, 7:] = -1
     if kind == "past":
         pos[::2] = 2 ** 31 - 1
     got = run_select(q, bounds, table, pos, budget, 1, 2, Hkv)
