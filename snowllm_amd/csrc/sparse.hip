@@ -300,10 +300,9 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(
 //   2 . 2 D / 32 <= 32 matrix instructions add to one accumulator, each with at most 16 roundings
 //   of 2^-24 of what has been summed                                  <= 2^-15 A
 // so E = (2^-14 + G 2^-24) A, A from a third product of the larger pieces with |bounds| (2^-8 too
-// small at most: 1.01 A). Operands that the matrix cores could flush (below 2^-126) are kept out:
-// rows with a P or |N| between 0 and 2^-90, and anything not finite, have E = infinity, and all
-// their pages are summed in 64 bits; bounds below 2^-126 add at most 2^-126 sum |P| + |N|, products
-// that underflow at most 2^-110.
+// small at most: 1.01 A). What the matrix cores could flush (below 2^-126) adds at most 2^-74: a row
+// has E = infinity, and all its pages summed in 64 bits, where a P or |N| is below 2^-90 (and not 0)
+// or above 2^40, or anything is not finite.
 struct SelectArgs {
   const uint16_t* q;        // [rows, Hq, D]
   const uint16_t* bounds;
@@ -330,124 +329,183 @@ __device__ __forceinline__ float neg_part(float f) { return !(f >= 0.f) ? f : 0.
 
 constexpr int SCORE_WAVES = 4;
 
-// A workgroup: sixteen rows of a request and kv head. Its threads sum the rows' P and N and leave
-// both pieces in LDS as operands of v_mfma_f32_16x16x32_bf16 (terms: D of N with the minima, then D
-// of P with the maxima), which every wave then holds in registers; the waves take sixteen pages at a
-// time, whose bounds are the other operand as they lie in memory.
-template <int D>
-__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a, int64_t pages_per_wg) {
+// A workgroup: RT times sixteen rows of a request and kv head. Its threads sum the rows' P and N and
+// leave both pieces in LDS as operands of v_mfma_f32_16x16x32_bf16 (terms: D of N with the minima,
+// then D of P with the maxima). A wave takes PT times sixteen pages at a time, whose bounds are the
+// other operand as they lie in memory: they are read ahead of the rows' sums, and each step's pages
+// while the last one's scores are stored. Two page tiles to each operand read keep LDS (85 bytes a
+// clock) behind the matrix cores, two row tiles halve the reads of the bounds.
+template <int D, int PT, int RT>
+__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a, uint32_t pages_per_wg) {
   constexpr int NS = D / 16;   // steps of 32 terms
-  __shared__ u32x4 op[NS][2][64];
-  __shared__ float total[16];  // sum |P| + |N| of a row, infinite for a row that is not to be trusted
+  __shared__ u32x4 op[RT][NS][2][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-  const int tiles = (a.rows + 15) / 16;
-  int64_t y = blockIdx.x;
-  const int tile = (int)(y % tiles);
-  y /= tiles;
-  const int h = (int)(y % a.Hkv), b = (int)(y / a.Hkv);
-  const int64_t m0 = (int64_t)b * a.T + a.row0 + tile * 16;
-  const int live = a.rows - tile * 16 < 16 ? a.rows - tile * 16 : 16;
-  const int64_t n = col < live ? pages_seen(a.positions[m0 + col], a.table_stride) : 0;
-  const int64_t last = (int64_t)wave_max<int>((int)n);
+  const uint32_t groups = (uint32_t)(a.rows + 16 * RT - 1) / (16 * RT);
+  uint32_t y = blockIdx.x;
+  const int row0 = (int)(y % groups) * 16 * RT;
+  y /= groups;
+  const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
+  const int64_t m0 = (int64_t)b * a.T + a.row0 + row0;
+  const int live = a.rows - row0 < 16 * RT ? a.rows - row0 : 16 * RT;
   const int64_t p0 = (int64_t)blockIdx.y * pages_per_wg;
+  const uint16_t* side = a.bounds + (int64_t)h * 2 * D + 8 * g;
+  const int64_t block_step = (int64_t)a.Hkv * 2 * D;
+  int blk[PT];
+  auto entries = [&](int64_t p) {   // lane: page p + 16 i + col, the table's last past its end
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int64_t pg = p + 16 * i + col;
+      blk[i] = page_block(a.table, a.table_stride, b, pg < a.table_stride ? pg : a.table_stride - 1, a.blocks);
+    }
+  };
+  u32x4 x[PT][NS];
+  auto fetch = [&] {
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const uint16_t* bp = side + (blk[i] < 0 ? 0 : blk[i]) * block_step;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) x[i][s] = *(const u32x4*)(bp + 32 * s);
+    }
+  };
+  int64_t p = p0 + 16 * PT * wave;
+  entries(p);
+  const int pos = lane < live ? a.positions[m0 + lane] : -1;
+  if constexpr (RT == 1) fetch();   // with more rows the registers are needed for their sums
+  const int64_t last = (int64_t)wave_max<int>((int)pages_seen(pos, a.table_stride));
   if (p0 >= last) return;
   const int64_t p1 = p0 + pages_per_wg < last ? p0 + pages_per_wg : last;
-  if (tid < 16) total[tid] = 0.f;
-  __syncthreads();
-  // unit u: row u % 16 and the eight elements 8 (u / 16) ..; lane (row, (u / 16) % 4) of step u / 64
-  for (int u = tid; u < 16 * (D / 8); u += 64 * SCORE_WAVES) {
-    const int r = u & 15, c = u >> 4;
-    float p[8], q[8];
+  // unit: four elements d .. of row r (D / 4 threads a row), of all heads at once; its row's slots in
+  // the operands are rotated by (d / 8) % 16, so that a row's threads write to different banks
+  constexpr int UNITS = RT * 16 * (D / 4) / (64 * SCORE_WAVES), PER = 256 / (D / 4);
+  {
+    float pp[UNITS][4], nn[UNITS][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = q[i] = 0.f;
-    if (r < live) {
-      const uint16_t* qp = a.q + ((m0 + r) * a.Hq + (int64_t)h * a.G) * D + 8 * c;
-#pragma unroll 8
-      for (int e = 0; e < a.G; ++e) {
-        const u32x4 x = *(const u32x4*)(qp + (int64_t)e * D);
+    for (int k = 0; k < UNITS; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float f0 = bf_lo(x[i]), f1 = bf_hi(x[i]);
-          p[2 * i] += pos_part(f0);
-          p[2 * i + 1] += pos_part(f1);
-          q[2 * i] += neg_part(f0);
-          q[2 * i + 1] += neg_part(f1);
-        }
+      for (int i = 0; i < 4; ++i) pp[k][i] = nn[k][i] = 0.f;
+    const int r0 = tid / (D / 4), d = tid % (D / 4) * 4;
+    const uint16_t* qp = a.q + ((m0 + r0) * a.Hq + (int64_t)h * a.G) * D + d;
+    const int64_t row_step = (int64_t)PER * a.Hq * D;
+#pragma unroll 4
+    for (int e = 0; e < a.G; ++e) {
+      uint2 w[UNITS];
+#pragma unroll
+      for (int k = 0; k < UNITS; ++k) {
+        w[k] = uint2{0u, 0u};
+        if (r0 + k * PER < live) w[k] = *(const uint2*)(qp + k * row_step + (int64_t)e * D);
       }
-    }
-    float sum = 0.f;
-    u32x4 ph, pl, qh, ql;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = p[i] - q[i];
-      const bool small = (p[i] > 0.f && p[i] < 0x1p-90f) || (q[i] < 0.f && q[i] > -0x1p-90f);
-      sum += small ? __builtin_huge_valf() : x;
-    }
+      for (int k = 0; k < UNITS; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ph[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-      qh[i] = pack_bf16x2(q[2 * i], q[2 * i + 1]);
-      pl[i] = pack_bf16x2(p[2 * i] - bf_lo(ph[i]), p[2 * i + 1] - bf_hi(ph[i]));
-      ql[i] = pack_bf16x2(q[2 * i] - bf_lo(qh[i]), q[2 * i + 1] - bf_hi(qh[i]));
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x2 = i ? w[k].y : w[k].x;
+          const short2v sign = __builtin_bit_cast(short2v, x2) >> (short)15;   // -1 where negative
+          const uint32_t ng = x2 & __builtin_bit_cast(uint32_t, sign), ps = x2 & ~__builtin_bit_cast(uint32_t, sign);
+          pp[k][2 * i] += bf_lo(ps);
+          pp[k][2 * i + 1] += bf_hi(ps);
+          nn[k][2 * i] += bf_lo(ng);
+          nn[k][2 * i + 1] += bf_hi(ng);
+        }
     }
-    const int s = c >> 2, l = (c & 3) * 16 + r;
-    op[s][0][l] = qh;
-    op[s][1][l] = ql;
-    op[NS / 2 + s][0][l] = ph;
-    op[NS / 2 + s][1][l] = pl;
-    if (r < live) atomicAdd(&total[r], sum);   // only a bound: its order is free
+    uint16_t* ops = (uint16_t*)op;
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+      const int r = r0 + k * PER;
+      uint2 ph, pl, nh, nl;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {   // NaN: the row's scores are not to be trusted
+        const float most = fmaxf(pp[k][i], -nn[k][i]);
+        const bool small = (pp[k][i] > 0.f && pp[k][i] < 0x1p-90f) || (nn[k][i] < 0.f && nn[k][i] > -0x1p-90f);
+        if (small || most > 0x1p40f) pp[k][i] = __builtin_nanf("");
+      }
+      ph.x = pack_bf16x2(pp[k][0], pp[k][1]);
+      ph.y = pack_bf16x2(pp[k][2], pp[k][3]);
+      nh.x = pack_bf16x2(nn[k][0], nn[k][1]);
+      nh.y = pack_bf16x2(nn[k][2], nn[k][3]);
+      pl.x = pack_bf16x2(pp[k][0] - bf_lo(ph.x), pp[k][1] - bf_hi(ph.x));
+      pl.y = pack_bf16x2(pp[k][2] - bf_lo(ph.y), pp[k][3] - bf_hi(ph.y));
+      nl.x = pack_bf16x2(nn[k][0] - bf_lo(nh.x), nn[k][1] - bf_hi(nh.x));
+      nl.y = pack_bf16x2(nn[k][2] - bf_lo(nh.y), nn[k][3] - bf_hi(nh.y));
+      const int st = d / 32, slot = (d / 8 % 4) * 16 + ((r + d / 8) & 15);
+      uint16_t* to = ops + ((((r / 16) * NS + st) * 2) * 64 + slot) * 8 + d % 8;
+      *(uint2*)to = nh;
+      *(uint2*)(to + 64 * 8) = nl;
+      *(uint2*)(to + NS * 64 * 8) = ph;           // NS / 2 steps of two pieces on
+      *(uint2*)(to + NS * 64 * 8 + 64 * 8) = pl;
+    }
   }
+  if constexpr (RT > 1) fetch();
   __syncthreads();
-  bf16x8 wh[NS], wl[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    wh[s] = __builtin_bit_cast(bf16x8, op[s][0][lane]);
-    wl[s] = __builtin_bit_cast(bf16x8, op[s][1][lane]);
-  }
-  const float tot = total[col];
   const float rel = 1.01f * (0x1p-14f + (float)a.G * 0x1p-24f);
-  const int64_t item = ((int64_t)b * a.Hkv + h) * a.rows + tile * 16 + col;
-  float* sc = a.scores + item * a.width;
-  float* er = a.errors + item * (a.width / 16);
-  int64_t p = p0 + 16 * wave;
-  int blk = p < p1 ? page_block(a.table, a.table_stride, b, p + col < last ? p + col : last - 1, a.blocks) : -1;
-  for (; p < p1; p += 16 * SCORE_WAVES) {
-    const uint16_t* bp = a.bounds + ((int64_t)(blk < 0 ? 0 : blk) * a.Hkv + h) * 2 * D + 8 * g;
-    u32x4 x[NS];
+  const int64_t item = ((int64_t)b * a.Hkv + h) * a.rows + row0 + col;
+  for (; p < p1; p += 16 * PT * SCORE_WAVES) {
+    uint32_t none[PT];   // bit i: page i of the tile is no page
 #pragma unroll
-    for (int s = 0; s < NS; ++s) x[s] = *(const u32x4*)(bp + 32 * s);
-    const uint64_t none = __ballot(blk < 0);   // bit i: page p + i is no page
-    const int64_t pn = p + 16 * SCORE_WAVES;
-    blk = pn < p1 ? page_block(a.table, a.table_stride, b, pn + col < last ? pn + col : last - 1, a.blocks) : -1;
-    floatx4 acc = {0.f, 0.f, 0.f, 0.f}, mag = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < PT; ++i) none[i] = (uint32_t)__ballot(blk[i] < 0);
+    const bool more = p + 16 * PT * SCORE_WAVES < p1;
+    if (more) entries(p + 16 * PT * SCORE_WAVES);
+    floatx4 acc[RT][PT], mag[RT][PT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int i = 0; i < PT; ++i) acc[r][i] = mag[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    u32x4 w[2][RT][2];
+    auto operand = [&](int s) {
+      const int slot = g * 16 + ((col + s % (NS / 2) * 4 + g) & 15);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) w[s & 1][r][0] = op[r][s][0][slot], w[s & 1][r][1] = op[r][s][1][slot];
+    };
+    operand(0);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const bf16x8 f = __builtin_bit_cast(bf16x8, x[s]);
-      // |bounds|, with the sign of the operand's piece: N is negative
-      u32x4 ab;
+      // one step ahead and no more: held over the loop they would not fit the registers
+      asm volatile("" ::: "memory");
+      if (s + 1 < NS) operand(s + 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ab[i] = s < NS / 2 ? x[s][i] | 0x80008000u : x[s][i] & 0x7fff7fffu;
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, wh[s], acc, 0, 0, 0);
-      mag = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ab), wh[s], mag, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, wl[s], acc, 0, 0, 0);
-    }
-    // lane (row col, g): pages p + 4 g + r. The first pages, always chosen, do not count.
-    float e = 0.f;
+      for (int r = 0; r < RT; ++r) {
+        const bf16x8 wh = __builtin_bit_cast(bf16x8, w[s & 1][r][0]);
+        const bf16x8 wl = __builtin_bit_cast(bf16x8, w[s & 1][r][1]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool no = none >> (4 * g + r) & 1;
-      if (no) acc[r] = -__builtin_huge_valf();
-      const int64_t pg = p + 4 * g + r;
-      if (!no && pg >= a.sink && pg < last) {
-        const float er1 = __builtin_fmaf(rel, mag[r], __builtin_fmaf(0x1p-126f, tot, 0x1p-110f));
-        e = er1 < 0x1p120f ? fmaxf(e, er1) : __builtin_huge_valf();   // NaN too
+        for (int i = 0; i < PT; ++i)
+          acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i][s]), wh, acc[r][i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+          // |bounds|, with the sign of the larger piece: N is negative
+          u32x4 ab;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ab[k] = s < NS / 2 ? x[i][s][k] | 0x80008000u : x[i][s][k] & 0x7fff7fffu;
+          mag[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ab), wh, mag[r][i], 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < PT; ++i)
+          acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i][s]), wl, acc[r][i], 0, 0, 0);
       }
     }
-    e = fmaxf(e, __shfl_xor(e, 16, 64));
-    e = fmaxf(e, __shfl_xor(e, 32, 64));
-    if (col < live) {
-      *(floatx4*)(sc + p + 4 * g) = acc;
-      if (g == 0) er[p / 16] = tot < 0x1p120f ? e : __builtin_huge_valf();
+    if (more) fetch();
+    // lane (row col, g): pages p + 16 i + 4 g + k. The first pages, always chosen, do not count.
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+#pragma unroll
+      for (int i = 0; i < PT; ++i) {
+        const int64_t pt = p + 16 * i;
+        float e = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool no = none[i] >> (4 * g + k) & 1;
+          if (no) acc[r][i][k] = -__builtin_huge_valf();
+          const int64_t pg = pt + 4 * g + k;
+          if (!no && pg >= a.sink && pg < last) {
+            const float e1 = __builtin_fmaf(rel, mag[r][i][k], 0x1p-74f);
+            e = e1 < 0x1p120f ? fmaxf(e, e1) : __builtin_huge_valf();   // NaN too
+          }
+        }
+        e = fmaxf(e, __shfl_xor(e, 16, 64));
+        e = fmaxf(e, __shfl_xor(e, 32, 64));
+        if (16 * r + col < live && pt < p1) {
+          *(floatx4*)(a.scores + (item + 16 * r) * a.width + pt + 4 * g) = acc[r][i];
+          if (g == 0) a.errors[(item + 16 * r) * (a.width / 16) + pt / 16] = e;
+        }
+      }
     }
   }
 }
@@ -460,8 +518,19 @@ __device__ __forceinline__ uint64_t score_key(double s) {
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
+// Inclusive sum over a wave.
+__device__ __forceinline__ uint32_t wave_incl_sum_u32(uint32_t v) {
+  v = row_scan_u32_dpp(v);
+  const int lane = threadIdx.x & 63;
+  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 15);
+  const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)v, 31);
+  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 47);
+  return v + (lane >= 16 ? a : 0u) + (lane >= 32 ? b : 0u) + (lane >= 48 ? c : 0u);
+}
+
 constexpr int PICK_NEAR = 512;    // pages near the border that are ranked in LDS
 constexpr int PICK_KEYS = 16;     // scores a thread keeps in registers
+constexpr int PICK_LIST = 1024;   // scores that the choice is made from
 
 // The 64-bit score's key of one page, by a wave: lane l sums terms l, l + 64, .. in order, then a
 // fixed tree, so that equal pages have equal sums. pn [2 D]: N, then P.
@@ -479,27 +548,33 @@ __device__ __forceinline__ uint64_t exact_key(const SelectArgs& a, const double*
   return score_key(s);
 }
 
-// One workgroup per (row, kv head). CACHED: its scores fit the threads' registers.
+// One workgroup per (row, kv head). CACHED: its scores fit the threads' registers. What bounds it is
+// the number of instructions per score, so the scores are looked at twice only: for each thread's
+// largest, of which the need-th largest is a lower bound of the row's (`low`), and for those not
+// clearly below it, which go to a list in LDS (a few more than are needed); t, the choice and the
+// near pages come from the list. Where more pass than the list holds (budgets of over about half
+// its length, many equal pages) the same steps go over all scores.
 template <int D, int NT, bool CACHED>
 __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
   constexpr int BINS = 4 * NT, WAVES = NT / 64;
-  extern __shared__ uint64_t masks[];   // [words] chosen pages, [words] equal ones, u32 [words] ranks before
+  extern __shared__ uint64_t masks[];   // [words] chosen pages, [words] equal ones
   // a histogram, then the near pages' keys and numbers
   __shared__ uint64_t lists[BINS / 2 > PICK_NEAR * 3 / 2 ? BINS / 2 : PICK_NEAR * 3 / 2];
   uint32_t* hist = (uint32_t*)lists;
   uint64_t* near_key = lists;
   uint32_t* near_page = (uint32_t*)(lists + PICK_NEAR);
+  __shared__ float top_score[PICK_LIST];
+  __shared__ uint32_t top_page[PICK_LIST];
   __shared__ double pn[2 * D];
-  __shared__ float red[3][WAVES];
-  __shared__ uint32_t redc[WAVES];
+  __shared__ uint32_t red[4][WAVES];
   __shared__ float member[64];
-  __shared__ uint32_t sh[6];            // 0: members, 1: bin, 2: above the bin, 3: in the bin, 4: near, 5: chosen
+  __shared__ uint32_t sh[8];            // 0: members, 1: bin, 2: above the bin, 3: in the bin, 4: near, 5: chosen, 6: listed
   __shared__ uint64_t sh_prefix;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t item = blockIdx.x;      // (request, kv head, row)
-  const int row = (int)(item % a.rows);
-  const int h = (int)(item / a.rows % a.Hkv);
-  const int b = (int)(item / a.rows / a.Hkv);
+  const uint32_t item = blockIdx.x;     // (request, kv head, row)
+  const int row = (int)(item % (uint32_t)a.rows);
+  const int h = (int)(item / (uint32_t)a.rows % (uint32_t)a.Hkv);
+  const int b = (int)(item / (uint32_t)a.rows / (uint32_t)a.Hkv);
   const int64_t m = (int64_t)b * a.T + a.row0 + row;
   int32_t* out = a.pages + (m * a.Hkv + h) * a.budget;
   const int n = (int)pages_seen(a.positions[m], a.table_stride);
@@ -509,103 +584,120 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
   }
   const int first = a.sink, end = n - a.recent;   // candidates; n > budget >= sink + recent
   const uint32_t need0 = (uint32_t)(a.budget - a.sink - a.recent);
-  const float* sc = a.scores + item * a.width;
+  const float* sc = a.scores + (int64_t)item * a.width;
   const int words = (n + 63) / 64;
   uint64_t* equal = masks + words;
-  uint32_t* rank = (uint32_t*)(masks + 2 * words);
+  uint32_t* rank = hist;                // pages chosen before a word's, at the end
   const float inf = __builtin_huge_valf();
 
   float key[CACHED ? PICK_KEYS : 1];
-  // f(page, score) over the candidates, a word of 64 pages per wave and step
-  auto scan = [&](auto f) {
+  float e = 0.f;
+  if (need0 > 0) {
+    if constexpr (CACHED) {
+#pragma unroll
+      for (int j = 0; j < PICK_KEYS; ++j) key[j] = sc[j * NT + tid < end ? j * NT + tid : end - 1];
+    }
+    const float* er = a.errors + (int64_t)item * (a.width / 16);
+    for (int i = tid; i < (n + 15) / 16; i += NT) e = fmaxf(e, er[i]);
+  }
+  // P and N in 64 bits, for the pages that are summed again
+  for (int d = tid; d < D; d += NT) {
+    double p = 0.0, q = 0.0;
+    const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D + d;
+#pragma unroll 8
+    for (int g = 0; g < a.G; ++g) {
+      const float f = bf16_to_f32(qp[(int64_t)g * D]);
+      p += (double)pos_part(f);
+      q += (double)neg_part(f);
+    }
+    pn[d] = q;
+    pn[D + d] = p;
+  }
+  // the chosen pages as a bit each, first the ones that always are
+  for (int w = tid; w < words; w += NT) {
+    const int p0 = w * 64;
+    auto below = [&](int x) { return x <= p0 ? 0ull : x - p0 >= 64 ? ~0ull : (1ull << (x - p0)) - 1; };
+    masks[w] = below(first) | (below(n) & ~below(end));
+  }
+  for (int i = tid; i < BINS; i += NT) hist[i] = 0;
+  if (tid < 8) sh[tid] = 0;
+  if constexpr (CACHED) {
+    if (need0 > 0) {
+#pragma unroll
+      for (int j = 0; j < PICK_KEYS; ++j)
+        if (j * NT + tid < first || j * NT + tid >= end) key[j] = -inf;
+    }
+  }
+  // f(page, score) over the row's candidates, from memory or (others then come as -inf) registers
+  auto over_row = [&](auto f) {
+    for (int i = first + tid; i < end; i += NT) f(i, sc[i]);
+  };
+  auto over_all = [&](auto f) {
     if constexpr (CACHED) {
 #pragma unroll
       for (int j = 0; j < PICK_KEYS; ++j) f(j * NT + tid, key[j]);
     } else {
-      for (int i = tid; i < words * 64; i += NT) f(i, i >= first && i < end ? sc[i] : -inf);
+      over_row(f);
     }
   };
-  float e = 0.f, hi = -inf, lo = inf;
-  uint32_t pages = 0;                   // candidates that are pages
-  if (need0 > 0) {
-    if constexpr (CACHED) {
-#pragma unroll
-      for (int j = 0; j < PICK_KEYS; ++j) {
-        const int i = j * NT + tid;
-        key[j] = i >= first && i < end ? sc[i] : -inf;
-      }
-    }
-    const float* er = a.errors + item * (a.width / 16);
-    for (int i = tid; i < (n + 15) / 16; i += NT) e = fmaxf(e, er[i]);
-    scan([&](int i, float s) {
-      if (s > -inf) hi = fmaxf(hi, s), lo = fminf(lo, s), ++pages;
-    });
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) {
-      e = fmaxf(e, __shfl_xor(e, s, 64));
-      hi = fmaxf(hi, __shfl_xor(hi, s, 64));
-      lo = fminf(lo, __shfl_xor(lo, s, 64));
-    }
-    pages = wave_sum<uint32_t>(pages);
-    if (lane == 0) red[0][wave] = e, red[1][wave] = hi, red[2][wave] = lo, redc[wave] = pages;
+  // largest and smallest of the threads' hi and lo, and the sum of their counts
+  auto reduce = [&](float& hi, float& lo, uint32_t& count) {
+    const uint32_t wh = wave_max_u32_all(ord_key(hi)), wl = wave_max_u32_all(~ord_key(lo)),
+                   wc = wave_sum_u32_dpp(count);
     __syncthreads();
-    pages = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      pages += redc[w];
-      e = fmaxf(e, red[0][w]);
-      hi = fmaxf(hi, red[1][w]);
-      lo = fminf(lo, red[2][w]);
+    if (lane == 0) red[1][wave] = wh, red[2][wave] = wl, red[3][wave] = wc;
+    __syncthreads();
+    const int w = lane % WAVES;
+    hi = ord_key_to_float(wave_max_u32_all(red[1][w]));
+    lo = ord_key_to_float(~wave_max_u32_all(red[2][w]));
+    count = wave_sum_u32_dpp(lane < WAVES ? red[3][w] : 0u);
+  };
+  auto bin_of = [&](float s, float lo, float inv) {
+    const float x = (s - lo) * inv;
+    return x >= (float)(BINS - 1) ? BINS - 1 : x > 0.f ? (int)x : 0;
+  };
+  // histogram (cleared before) -> the bin of the k-th largest: sh[1]; scores above it, of all that
+  // were counted and `above` more: sh[2]; in it: sh[3]. A barrier after it.
+  auto find_bin = [&](uint32_t k, uint32_t above) {
+    __syncthreads();
+    const int top = BINS - 1 - 4 * tid;   // thread: four bins, from the top
+    uint32_t c[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += c[i] = hist[top - i];
+    uint32_t before = wave_incl_sum_u32(sum);
+    if (lane == 63) red[0][wave] = before;
+    before -= sum;
+    __syncthreads();
+    before += above + wave_sum_u32_dpp(lane < wave ? red[0][lane % WAVES] : 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before < k && before + c[i] >= k) sh[1] = (uint32_t)(top - i), sh[2] = before, sh[3] = c[i];
+      before += c[i];
     }
-  }
-  // t, the need-th largest s~: histograms over [lo, hi], ever narrower, until 64 scores are left
-  float t = 0.f;
-  bool all = need0 > 0 && !(e < inf && hi < inf && pages >= need0);   // all pages in 64 bits
-  if (need0 > 0 && !all) {
+    __syncthreads();
+  };
+  // the k-th largest score that `scan` passes over, all of it in [lo, hi]: histograms, ever narrower,
+  // until 64 scores are left. False: not found in 32 of them.
+  auto kth = [&](auto scan, float hi, float lo, uint32_t k, float& t) {
     uint32_t above = 0;                 // scores > hi
-    for (int round = 0;; ++round) {
-      if (lo == hi) {
-        t = lo;
-        break;
-      }
-      if (round == 32) {
-        all = true;
-        break;
-      }
+    for (int round = 0; round < 32; ++round) {
+      t = lo;
+      if (lo == hi) return true;
       const float inv = (float)(BINS - 1) / (hi - lo);
-      auto bin = [&](float s) {
-        const float x = (s - lo) * inv;
-        return x >= (float)(BINS - 1) ? BINS - 1 : x > 0.f ? (int)x : 0;
-      };
+      __syncthreads();
       for (int i = tid; i < BINS; i += NT) hist[i] = 0;
       if (tid == 0) sh[0] = 0;
       __syncthreads();
       scan([&](int i, float s) {
-        if (s >= lo && s <= hi) atomicAdd(&hist[bin(s)], 1u);
+        if (s >= lo && s <= hi) atomicAdd(&hist[bin_of(s, lo, inv)], 1u);
       });
-      __syncthreads();
-      // thread: four bins, from the top
-      const int top = BINS - 1 - 4 * tid;
-      uint32_t c[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += c[i] = hist[top - i];
-      uint32_t before = (uint32_t)wave_incl_sum_u64(sum);
-      if (lane == 63) redc[wave] = before;
-      before -= sum;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) before += redc[w];
-      before += above;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (before < need0 && before + c[i] >= need0) sh[1] = (uint32_t)(top - i), sh[2] = before, sh[3] = c[i];
-        before += c[i];
-      }
-      __syncthreads();
+      find_bin(k, above);
       const int at = (int)sh[1];
       const uint32_t count = sh[3];
       above = sh[2];
       if (count <= 64) {
         scan([&](int i, float s) {
-          if (s >= lo && s <= hi && bin(s) == at) member[atomicAdd(&sh[0], 1u)] = s;
+          if (s >= lo && s <= hi && bin_of(s, lo, inv) == at) member[atomicAdd(&sh[0], 1u)] = s;
         });
         __syncthreads();
         const float mine = lane < (int)count ? member[lane] : -inf;
@@ -614,82 +706,105 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
           over += member[i] > mine;
           same += member[i] == mine;
         }
-        const uint32_t k = need0 - above;   // 1 .. count
-        const uint64_t is = __ballot(lane < (int)count && over < k && over + same >= k);
-        t = __shfl(mine, __builtin_ctzll(is), 64);
-        break;
+        const uint32_t r = k - above;   // 1 .. count
+        const uint64_t is = __ballot(lane < (int)count && over < r && over + same >= r);
+        t = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(mine), __builtin_ctzll(is)));
+        return true;
       }
       float nh = -inf, nl = inf;
+      uint32_t none = 0;
       scan([&](int i, float s) {
-        if (s >= lo && s <= hi && bin(s) == at) nh = fmaxf(nh, s), nl = fminf(nl, s);
+        if (s >= lo && s <= hi && bin_of(s, lo, inv) == at) nh = fmaxf(nh, s), nl = fminf(nl, s);
       });
-#pragma unroll
-      for (int s = 32; s > 0; s >>= 1) {
-        nh = fmaxf(nh, __shfl_xor(nh, s, 64));
-        nl = fminf(nl, __shfl_xor(nl, s, 64));
-      }
-      __syncthreads();
-      if (lane == 0) red[1][wave] = nh, red[2][wave] = nl;
-      __syncthreads();
-      for (int w = 0; w < WAVES; ++w) {
-        nh = fmaxf(nh, red[1][w]);
-        nl = fminf(nl, red[2][w]);
-      }
+      reduce(nh, nl, none);
       hi = nh;
       lo = nl;
     }
-  }
-  // chosen for certain, and near
-  uint32_t need = 0;                    // of the pages in `equal`, the lowest that many
-  if (!all) {
+    return false;
+  };
+  // marks the pages above t + 2 E, lists those within 2 E of t
+  auto classify = [&](auto scan, float t) {
     const float over = t + 2.f * e, under = t - 2.f * e;
-    if (tid == 0) sh[4] = sh[5] = 0;
-    __syncthreads();
     scan([&](int i, float s) {
-      const bool mid = i >= first && i < end;
-      const bool in = i < n && (!mid || (need0 > 0 && s > over));
-      const bool near = mid && need0 > 0 && s >= under && s <= over;
-      const uint64_t mi = __ballot(in), mn = __ballot(near);
-      if (i < words * 64) {             // uniform: a wave's word
-        uint32_t base = 0;
-        if (lane == 0) {
-          masks[i / 64] = mi;
-          equal[i / 64] = 0;
-          if (mn) base = atomicAdd(&sh[4], (uint32_t)__popcll(mn));
-          atomicAdd(&sh[5], (uint32_t)__popcll(mi));
-        }
-        if (mn) {
-          base = (uint32_t)__shfl((int)base, 0, 64);
-          const uint32_t to = base + (uint32_t)__popcll(mn & ((1ull << lane) - 1));
-          if (near && to < PICK_NEAR) near_page[to] = (uint32_t)i;
+      if (s >= under) {
+        if (s > over) {
+          atomicOr((unsigned long long*)&masks[i / 64], 1ull << (i & 63));
+          atomicAdd(&sh[5], 1u);
+        } else {
+          const uint32_t to = atomicAdd(&sh[4], 1u);
+          if (to < PICK_NEAR) near_page[to] = (uint32_t)i;
         }
       }
     });
     __syncthreads();
-    const uint32_t near = sh[4], left = (uint32_t)a.budget - sh[5];
-    if (need0 > 0 && near > PICK_NEAR && near > left) {
-      all = true;
-    } else if (near > PICK_NEAR) {      // all of them are chosen
-      __syncthreads();
-      scan([&](int i, float s) {
-        const uint64_t mi = __ballot(i < n && (i < first || i >= end || s >= under));
-        if (i < words * 64 && lane == 0) masks[i / 64] = mi;
-      });
-    } else if (near > 0) {
-      if (near > left) {
-        for (int d = tid; d < D; d += NT) {
-          double p = 0.0, q = 0.0;
-          const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D + d;
-#pragma unroll 8
-          for (int g = 0; g < a.G; ++g) {
-            const float f = bf16_to_f32(qp[(int64_t)g * D]);
-            p += (double)pos_part(f);
-            q += (double)neg_part(f);
-          }
-          pn[d] = q;
-          pn[D + d] = p;
+  };
+
+  bool all = false;                     // all candidates summed in 64 bits
+  if (need0 > 0) {
+    float most = -inf;                  // of this thread
+    over_all([&](int i, float s) { most = fmaxf(most, s); });
+    uint32_t pages = 0;                 // candidates that are pages, where that may be too few
+    e = __uint_as_float(wave_max_u32_all(__float_as_uint(e)));
+    if (lane == 0) red[0][wave] = __float_as_uint(e);
+    float hi = most, lo = most > -inf ? most : inf;
+    uint32_t maxima = most > -inf;
+    reduce(hi, lo, maxima);
+    e = __uint_as_float(wave_max_u32_all(red[0][lane % WAVES]));
+    all = !(e < inf && hi < inf && maxima > 0);
+    if (!all) {
+      float low = -inf;                 // at least need0 scores are not below it
+      if (maxima >= need0) {
+        const float inv = hi > lo ? (float)(BINS - 1) / (hi - lo) : 0.f;
+        const int bin = bin_of(most, lo, inv);
+        if (most > -inf) atomicAdd(&hist[bin], 1u);
+        find_bin(need0, 0);
+        float ignore = -inf;
+        uint32_t none = 0;
+        low = most > -inf && bin >= (int)sh[1] ? most : inf;
+        reduce(ignore, low, none);
+      }
+      const float from = low - 2.f * e;
+      over_all([&](int i, float s) {
+        if (s >= from && s > -inf) {
+          const uint32_t to = atomicAdd(&sh[6], 1u);
+          if (to < PICK_LIST) top_score[to] = s, top_page[to] = (uint32_t)i;
         }
+      });
+      __syncthreads();
+      const uint32_t listed = sh[6];
+      float t;
+      if (listed < need0) {             // fewer pages than are needed
+        all = true;
+      } else if (listed <= PICK_LIST) {
+        auto over_list = [&](auto f) {
+          for (uint32_t i = tid; i < listed; i += NT) f((int)top_page[i], top_score[i]);
+        };
+        float l2 = inf, h2 = -inf;
+        over_list([&](int i, float s) { l2 = fminf(l2, s), h2 = fmaxf(h2, s); });
+        reduce(h2, l2, pages);
+        all = !kth(over_list, h2, l2, need0, t);
         __syncthreads();
+        if (!all) classify(over_list, t);
+      } else {
+        float l2 = inf;
+        over_row([&](int i, float s) {
+          if (s > -inf) l2 = fminf(l2, s);
+        });
+        reduce(hi, l2, pages);
+        all = !kth(over_row, hi, l2, need0, t);
+        __syncthreads();
+        if (!all) classify(over_row, t);
+      }
+    }
+  }
+  __syncthreads();
+  uint32_t need = 0;                    // of the pages in `equal`, the lowest that many
+  if (need0 > 0 && !all) {
+    const uint32_t near = sh[4], left = need0 - sh[5];   // of the near ones, `left` are chosen
+    if (near > PICK_NEAR) {
+      all = true;
+    } else {
+      if (near > left) {
         for (uint32_t i = wave; i < near; i += WAVES) {
           const uint64_t k = exact_key<D>(a, pn, b, h, near_page[i]);
           if (lane == 0) near_key[i] = k;
@@ -710,19 +825,7 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
   }
   if (all) {
     // every candidate in 64 bits, the need-th largest key by radix selection, eight bits a pass
-    for (int d = tid; d < D; d += NT) {
-      double p = 0.0, q = 0.0;
-      const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D + d;
-      for (int g = 0; g < a.G; ++g) {
-        const float f = bf16_to_f32(qp[(int64_t)g * D]);
-        p += (double)pos_part(f);
-        q += (double)neg_part(f);
-      }
-      pn[d] = q;
-      pn[D + d] = p;
-    }
-    __syncthreads();
-    uint64_t* ex = a.exact + item * a.width;
+    uint64_t* ex = a.exact + (int64_t)item * a.width;
     for (int i = first + wave; i < end; i += WAVES) {
       const uint64_t k = exact_key<D>(a, pn, b, h, i);
       if (lane == 0) ex[i] = k;
@@ -759,18 +862,15 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
       if (lane == 0) masks[i / 64] = mo, equal[i / 64] = me;
     }
     __syncthreads();
-  }
-  // ranks of the words' first pages; of equal pages the lowest `need`
-  if (wave == 0) {
-    uint32_t eq_before = 0, before = 0;
-    for (int w0 = 0; w0 < words; w0 += 64) {
-      const int w = w0 + lane;
-      uint64_t mo = w < words ? masks[w] : 0;
-      if (need > 0) {
-        uint64_t me = w < words ? equal[w] : 0;
+    // of equal pages the lowest `need`
+    if (wave == 0) {
+      uint32_t before = 0;
+      for (int w0 = 0; w0 < words; w0 += 64) {
+        const int w = w0 + lane;
+        uint64_t mo = w < words ? masks[w] : 0, me = w < words ? equal[w] : 0;
         const uint32_t ec = (uint32_t)__popcll(me);
-        const uint32_t ei = (uint32_t)wave_incl_sum_u64(ec);
-        const uint32_t eb = eq_before + ei - ec;
+        const uint32_t ei = wave_incl_sum_u32(ec);
+        const uint32_t eb = before + ei - ec;
         uint32_t take = eb >= need ? 0u : need - eb < ec ? need - eb : ec;
         while (take > 0) {   // the lowest `take` set bits
           const uint64_t bit = me & (~me + 1);
@@ -778,14 +878,24 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
           me ^= bit;
           --take;
         }
-        eq_before += (uint32_t)__shfl((int)ei, 63, 64);
+        before += (uint32_t)__builtin_amdgcn_readlane((int)ei, 63);
         if (w < words) masks[w] = mo;
       }
-      const uint32_t cnt = (uint32_t)__popcll(mo);
-      const uint32_t ci = (uint32_t)wave_incl_sum_u64(cnt);
-      if (w < words) rank[w] = before + ci - cnt;
-      before += (uint32_t)__shfl((int)ci, 63, 64);
     }
+    __syncthreads();
+  }
+  // ranks of the words' first pages
+  uint32_t before = 0;
+  for (int w0 = 0; w0 < words; w0 += NT) {
+    const int w = w0 + tid;
+    const uint32_t cnt = w < words ? (uint32_t)__popcll(masks[w]) : 0u;
+    const uint32_t ci = wave_incl_sum_u32(cnt);
+    __syncthreads();
+    if (lane == 63) red[0][wave] = ci;
+    __syncthreads();
+    const uint32_t t0 = lane < WAVES ? red[0][lane] : 0u;
+    if (w < words) rank[w] = before + wave_sum_u32_dpp(lane < wave ? t0 : 0u) + ci - cnt;
+    before += wave_sum_u32_dpp(t0);
   }
   __syncthreads();
   for (int w = wave; w < words; w += WAVES) {
@@ -1081,6 +1191,13 @@ int64_t select_rows(int64_t batch, int64_t tokens, int64_t Hkv, int64_t pages) {
 }
 
 template <int D>
+auto score_of(int pt, int rt) {
+  return rt == 2 ? score_kernel<D, 2, 2> : pt == 2 ? score_kernel<D, 2, 1> : score_kernel<D, 1, 1>;
+}
+auto score_form(int64_t D, int pt, int rt) {
+  return D == 64 ? score_of<64>(pt, rt) : D == 128 ? score_of<128>(pt, rt) : score_of<256>(pt, rt);
+}
+template <int D>
 auto pick_of(int64_t width) {
   return width <= 256 * PICK_KEYS    ? pick_kernel<D, 256, true>
          : width <= 1024 * PICK_KEYS ? pick_kernel<D, 1024, true>
@@ -1226,19 +1343,24 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
   a.budget = (int)budget;
   a.sink = (int)sink;
   a.recent = (int)recent;
-  const size_t lds = (size_t)((table_stride + 63) / 64) * 20;
-  auto score = head_size == 64 ? score_kernel<64> : head_size == 128 ? score_kernel<128> : score_kernel<256>;
+  const size_t lds = (size_t)((table_stride + 63) / 64) * 16;
   auto pick = pick_form(head_size, width);
   for (int64_t r0 = 0; r0 < tokens; r0 += chunk) {
     a.row0 = r0;
     a.rows = (int)(tokens - r0 < chunk ? tokens - r0 : chunk);
-    const int64_t tiles = batch * num_kv_heads * ((a.rows + 15) / 16);
     if (table_stride > budget) {   // otherwise every page of every row is taken
-      // about four workgroups a CU, each 64 to 2048 pages for the sixteen rows it prepares
-      int64_t per = (table_stride * tiles / 1024 + 63) / 64 * 64;
-      per = per < 64 ? 64 : per > 2048 ? 2048 : per;
-      hipLaunchKernelGGL(score, dim3((unsigned)tiles, (unsigned)((table_stride + per - 1) / per)),
-                         dim3(64 * SCORE_WAVES), 0, S(stream), a, per);
+      const int rt = a.rows > 16 ? 2 : 1;
+      const int64_t groups = batch * num_kv_heads * ((a.rows + 16 * rt - 1) / (16 * rt));
+      // workgroups: two a CU, one where the sums over the rows' heads would take longer than the
+      // pages they are for
+      const int64_t wgs = a.rows > 4 && rt == 1 ? 256 : 512;
+      const int pt = rt == 2 || table_stride * groups >= 128 * wgs ? 2 : 1;
+      const int64_t step = 16 * pt * SCORE_WAVES;
+      int64_t per = (table_stride * groups + wgs * step - 1) / (wgs * step) * step;
+      per = per > 4096 ? 4096 : per;
+      hipLaunchKernelGGL(score_form(head_size, pt, rt),
+                         dim3((unsigned)groups, (unsigned)((table_stride + per - 1) / per)),
+                         dim3(64 * SCORE_WAVES), 0, S(stream), a, (uint32_t)per);
       SV_CHECK_LAUNCH();
     }
     hipLaunchKernelGGL(pick, dim3((unsigned)(batch * num_kv_heads * a.rows)), dim3(threads), lds,
