@@ -55,30 +55,39 @@ def test_checks_of_shapes_and_strides():
         def data_ptr(self):
             return self._p
 
-        def dim(self):
-            return len(self.shape)
+        def get_device(self):
+            return 0 if self.is_cuda else -1
 
         def is_contiguous(self):
             return True
 
-    assert sparse._rows(Fake((3, 2, 64), (200, 64, 1)), "k", 3, 2, 64) == 200
-    assert sparse._rows(Fake((1, 2, 64), (7, 64, 1)), "k", 1, 2, 64) == 128
-    assert sparse._rows(Fake((3, 1, 64), (64, 5, 1)), "k", 3, 1, 64) == 64
+    rows = (3, 2, 64)
+    assert sparse._rows(Fake(rows, (200, 64, 1), ptr=32), "k", rows, 0) == (32, 200)
+    assert sparse._rows(Fake((1, 2, 64), (7, 64, 1)), "k", (1, 2, 64), 0) == (0, 128)
+    assert sparse._rows(Fake((3, 1, 64), (64, 5, 1)), "k", (3, 1, 64), 0) == (0, 64)
     for shape, stride, ptr, dtype in (((3, 2, 64), (200, 64, 2), 0, BF), ((3, 2, 64), (200, 72, 1), 0, BF),
                                       ((3, 2, 64), (129, 64, 1), 0, BF), ((3, 2, 64), (64, 64, 1), 0, BF),
                                       ((3, 2, 64), (200, 64, 1), 8, BF),
                                       ((3, 2, 64), (200, 64, 1), 0, torch.float16),
                                       ((4, 2, 64), (200, 64, 1), 0, BF)):
         with pytest.raises(Err):
-            sparse._rows(Fake(shape, stride, dtype, ptr), "k", 3, 2, 64)
+            sparse._rows(Fake(shape, stride, dtype, ptr), "k", rows, 0)
+    with pytest.raises(Err, match="on cuda:1"):
+        sparse._rows(Fake(rows, (200, 64, 1)), "k", rows, 1)
+    with pytest.raises(Err, match="on cuda:1"):
+        sparse._need(Fake((3,), (1,), I32), "x", I32, (3,), 1)
     with pytest.raises(Err, match="16-byte"):
-        sparse._need(Fake((3,), (1,), I32, 4), "x", I32, (3,))
+        sparse._need(Fake((3,), (1,), I32, 4), "x", I32, (3,), 0)
+    with pytest.raises(Err, match="shape"):
+        sparse._need(Fake((3,), (1,), I32), "x", I32, (4,), 0)
     with pytest.raises(Err, match="whole number"):
-        sparse._requests(Fake((2, 5), (5, 1), I32), 3)
+        sparse._requests(Fake((2, 5), (5, 1), I32), 3, 0)
     with pytest.raises(Err, match="whole number"):
-        sparse._requests(Fake((0, 5), (5, 1), I32), 3)
+        sparse._requests(Fake((0, 5), (5, 1), I32), 3, 0)
     with pytest.raises(Err, match="batch, pages"):
-        sparse._requests(Fake((5,), (1,), I32), 5)
+        sparse._requests(Fake((5,), (1,), I32), 5, 0)
+    with pytest.raises(Err, match="scratch bytes"):
+        sparse._scratch(None, 8, "x", 0)
 
 
 EINVAL = 1
