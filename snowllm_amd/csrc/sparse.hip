@@ -12,6 +12,9 @@
 // Rows are padded [batch, tokens]; request b's page p is block table[b, p].
 #include "common.h"
 
+#include <algorithm>
+#include <atomic>
+
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -24,6 +27,9 @@ constexpr int PAGE = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 inline hipStream_t S(void* s) { return (hipStream_t)s; }
+
+// This wave of the workgroup, as a scalar: what depends on it alone is scalar work then.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
 // The block of request b's page, or -1 past the table's width or where the entry is no block.
 __device__ __forceinline__ int page_block(const int32_t* __restrict__ table, int64_t stride, int b,
@@ -339,7 +345,7 @@ template <int D, int PT, int RT>
 __global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a, uint32_t pages_per_wg) {
   constexpr int NS = D / 16;   // steps of 32 terms
   __shared__ u32x4 op[RT][NS][2][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
   const uint32_t groups = (uint32_t)(a.rows + 16 * RT - 1) / (16 * RT);
   uint32_t y = blockIdx.x;
   const int row0 = (int)(y % groups) * 16 * RT;
@@ -570,7 +576,7 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
   __shared__ float member[64];
   __shared__ uint32_t sh[8];            // 0: members, 1: bin, 2: above the bin, 3: in the bin, 4: near, 5: chosen, 6: listed
   __shared__ uint64_t sh_prefix;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const uint32_t item = blockIdx.x;     // (request, kv head, row)
   const int row = (int)(item % (uint32_t)a.rows);
   const int h = (int)(item / (uint32_t)a.rows % (uint32_t)a.Hkv);
@@ -922,10 +928,78 @@ struct AttendArgs {
   float* part_ml;           // [rows * Hq, splits, 2]
   int64_t table_stride, blocks, items;
   int T, Hq, Hkv, G, GT, budget, splits;
+  int rpt, ring_bytes;      // attend_rows_kernel: rows of a wave, LDS in front of the union
   float qk_scale;           // softmax scale * log2(e)
 };
 
 constexpr int ATT_WAVES = 4;
+
+// s_waitcnt on the vector-memory counter only (gfx9 encoding: vmcnt in bits 3:0 and 15:14, no wait on
+// the others).
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// On the LDS counter only: this wave's LDS reads have ended.
+__device__ __forceinline__ void wait_lgkmcnt0() {
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+}
+
+// Workgroup barrier without the wait of __syncthreads for every load in flight.
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The V^T operands of elements d and d + 1 over two pages' keys, from a 16-byte load of each page
+// (d's four keys, then d + 1's): the middle pairs change places.
+__device__ __forceinline__ void v_operands(u32x4 a, u32x4 b, bf16x8& f0, bf16x8& f1) {
+  uint32_t a2 = a[2], a3 = a[3], b0 = b[0], b1 = b[1];
+  asm("v_swap_b32 %0, %1" : "+v"(a2), "+v"(b0));
+  asm("v_swap_b32 %0, %1" : "+v"(a3), "+v"(b1));
+  f0 = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], a2, a3});
+  f1 = __builtin_bit_cast(bf16x8, u32x4{b0, b1, b[2], b[3]});
+}
+
+// One step of the running softmax over a wave's 32 keys: exponents e (lane (head col, g): keys 4 g ..
+// of two pages, masked ones -inf) to weights 2^(e - m), as a bf16 pair hi + lo (16 bits of
+// mantissa: hi is the upper half of the word, lo what is left, rounded; single bf16 weights would add
+// about two thirds of the output's own rounding to its error). m moves, and O and l are scaled, only
+// where a score passes it by 2^8, for all of a wave's columns at once; all in 32 bits.
+constexpr float RESCALE = 8.f;
+
+template <int D>
+__device__ __forceinline__ void softmax_step(const float (&e)[8], float& m, float& l,
+                                             floatx4 (&acc)[D / 16], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  const float inf = __builtin_huge_valf();
+  float top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+  if (__ballot(top > m + RESCALE)) {
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float nm = fmaxf(m, top);
+    const float c = m == nm ? 1.f : __builtin_amdgcn_exp2f(m - nm);   // 0 at the first keys
+    m = nm;
+    l *= c;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) acc[i] *= c;
+  }
+  const float ref = m == -inf ? 0.f : m;
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(e[i] - ref);
+    l += p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = __float_as_uint(p[2 * i]), v = __float_as_uint(p[2 * i + 1]);
+    hi[i] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+    lo[i] = pack_bf16x2(p[2 * i] - __uint_as_float(u & 0xffff0000u), p[2 * i + 1] - __uint_as_float(v & 0xffff0000u));
+  }
+}
 
 // One workgroup per (row, kv head, 16 heads of its group, split of the list), one page pair per wave
 // and step. Per pair (32 keys):
@@ -933,27 +1007,12 @@ constexpr int ATT_WAVES = 4;
 //                                  (its layout is the operand's: 1 KiB per wave load)
 //   O^T[d, head]  += V^T . P^T     over the 32 keys, A = V^T (a 16-byte load holds a lane's keys of
 //                                  elements d and d + 1: two operands), B = P^T from S^T's registers
-// so neither K, V nor P passes through LDS. P is a bf16 hi + lo pair (16 bits of mantissa): single
-// bf16 weights would add about two thirds of the output's own rounding to its error.
-// The running maximum and sum, and O, are 32-bit.
-template <int D>
-__global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a) {
+// so neither K, V nor P passes through LDS.
+template <int D, int NW>
+__device__ __forceinline__ void attend_row(const AttendArgs& a, int b, int h, int gt, int t, int split,
+                                           float* so, float (*sml)[16][2]) {
   constexpr int KS = D / 32;
-  extern __shared__ float so[];   // [waves][heads][elements of a round + 4]
-  __shared__ float sml[ATT_WAVES][16][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  // neighbouring rows, which list many of the same pages, run on one XCD
-  const int64_t per_xcd = (int64_t)gridDim.x / 8;
-  int64_t item = (int64_t)(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-  if (item >= a.items) return;
-  const int split = (int)(item % a.splits);
-  item /= a.splits;
-  const int t = (int)(item % a.T);
-  item /= a.T;
-  const int gt = (int)(item % a.GT);
-  item /= a.GT;
-  const int h = (int)(item % a.Hkv);
-  const int b = (int)(item / a.Hkv);
+  const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
   const int64_t m = (int64_t)b * a.T + t;
   const int heads = a.G - gt * 16 < 16 ? a.G - gt * 16 : 16;
   const int64_t head0 = (int64_t)h * a.G + gt * 16;
@@ -972,7 +1031,7 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
   for (int i = 0; i < D / 16; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float mx = -__builtin_huge_valf(), l = 0.f;
 
-  const int parts = a.splits * ATT_WAVES, part = split * ATT_WAVES + wave;
+  const int parts = a.splits * NW, part = split * NW + wave;
   const int64_t page_elems = (int64_t)PAGE * D;
   for (int e0 = part; e0 < a.budget; e0 += 64 * parts) {
     const int64_t e = e0 + (int64_t)lane * parts;
@@ -1013,37 +1072,16 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
         sb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xb[s]), qf[s], sb, 0, 0, 0);
       }
       // lane (head col, g): keys 4 g + r of both pages
-      float p[8];
-      float top = -__builtin_huge_valf();
+      float x[8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[r] = 4 * g + r < left_a ? sa[r] * a.qk_scale : -__builtin_huge_valf();
-        p[4 + r] = 4 * g + r < left_b ? sb[r] * a.qk_scale : -__builtin_huge_valf();
+        x[r] = 4 * g + r < left_a ? sa[r] * a.qk_scale : -__builtin_huge_valf();
+        x[4 + r] = 4 * g + r < left_b ? sb[r] * a.qk_scale : -__builtin_huge_valf();
       }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) top = fmaxf(top, p[r]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__ballot(top > mx)) {
-        const float nm = fmaxf(mx, top);
-        const float c = mx == nm ? 1.f : __builtin_amdgcn_exp2f(mx - nm);   // 0 at the first pair
-        mx = nm;
-        l *= c;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) acc[i] *= c;
-      }
-      const float ref = mx == -__builtin_huge_valf() ? 0.f : mx;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(p[r] - ref);
-        l += p[r];
-      }
-      bf16x8 hi, lo;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        hi[r] = (__bf16)p[r];
-        lo[r] = (__bf16)(p[r] - (float)hi[r]);
-      }
+      uint32_t ph[4], pl[4];
+      softmax_step<D>(x, mx, l, acc, ph, pl);
+      const bf16x8 hi = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
+      const bf16x8 lo = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
       // what lies behind the row's last position never enters: 0 . NaN would
       if (left_a < PAGE || left_b < PAGE) {
 #pragma unroll
@@ -1062,9 +1100,8 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
       }
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        const u32x4 v0 = {ya[j][0], ya[j][1], yb[j][0], yb[j][1]};
-        const u32x4 v1 = {ya[j][2], ya[j][3], yb[j][2], yb[j][3]};
-        const bf16x8 f0 = __builtin_bit_cast(bf16x8, v0), f1 = __builtin_bit_cast(bf16x8, v1);
+        bf16x8 f0, f1;
+        v_operands(ya[j], yb[j], f0, f1);
         acc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f0, hi, acc[2 * j], 0, 0, 0);
         acc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f1, hi, acc[2 * j + 1], 0, 0, 0);
         acc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f0, lo, acc[2 * j], 0, 0, 0);
@@ -1079,7 +1116,7 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
   __syncthreads();
   float top = sml[0][col][0];
 #pragma unroll
-  for (int w = 1; w < ATT_WAVES; ++w) top = fmaxf(top, sml[w][col][0]);
+  for (int w = 1; w < NW; ++w) top = fmaxf(top, sml[w][col][0]);
   const float c = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - top);
   // in two rounds of D / 2 elements where the waves' sums would pass 64 KiB of LDS
   const int rounds = D == 256 && heads > 8 ? 2 : 1, DR = D / rounds, ld = DR + 4;
@@ -1096,15 +1133,15 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
       }
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < heads * (DR / 4); u += 64 * ATT_WAVES) {
+    for (int u = threadIdx.x; u < heads * (DR / 4); u += 64 * NW) {
       const int hd = u / (DR / 4), dr = u % (DR / 4) * 4, d = rd * DR + dr;
       float hm = sml[0][hd][0];
 #pragma unroll
-      for (int w = 1; w < ATT_WAVES; ++w) hm = fmaxf(hm, sml[w][hd][0]);
+      for (int w = 1; w < NW; ++w) hm = fmaxf(hm, sml[w][hd][0]);
       float sum = 0.f;
       floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < ATT_WAVES; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float wm = sml[w][hd][0];
         sum += sml[w][hd][1] * (wm == hm ? 1.f : __builtin_amdgcn_exp2f(wm - hm));
         o += *(const floatx4*)(so + (w * heads + hd) * ld + dr);
@@ -1125,6 +1162,279 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
       }
     }
   }
+}
+
+template <int D>
+__global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a) {
+  extern __shared__ float so[];   // [waves][heads][elements of a round + 4]
+  __shared__ float sml[ATT_WAVES][16][2];
+  // neighbouring rows, which list many of the same pages, run on one XCD
+  const uint32_t per_xcd = gridDim.x / 8;
+  uint32_t item = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+  if (item >= (uint64_t)a.items) return;
+  const int split = (int)(item % (uint32_t)a.splits);
+  item /= (uint32_t)a.splits;
+  const int t = (int)(item % (uint32_t)a.T);
+  item /= (uint32_t)a.T;
+  const int gt = (int)(item % (uint32_t)a.GT);
+  item /= (uint32_t)a.GT;
+  attend_row<D, ATT_WAVES>(a, (int)(item / (uint32_t)a.Hkv), (int)(item % (uint32_t)a.Hkv), gt, t, split, so, sml);
+}
+
+// Many rows: neighbouring rows of a request list many of the same pages. A workgroup takes R = 4 rpt
+// rows of one kv head (rpt rows fill the 16 columns of a matrix instruction) and goes once over the
+// union of their lists, each page with the set of rows that list it: the pages stream through LDS
+// (global_load_lds, 1 KiB per wave instruction), two pairs in use and the next two on their way. Four
+// waves, one for each rpt rows, multiply the first pair of a step and four the second, with the columns
+// of rows that do not list a page masked; the two halves are joined at the end. A page that not all
+// rows see whole is entered once for each row. Two waves a SIMD, so that one's softmax and LDS reads
+// run beside the other's products: with one (the same step with four waves) 81 us for 1024 rows of 64
+// pages instead of TIME_ROWS.
+// What is masked in a row's column is multiplied by a weight of zero, so a V that is not finite in a
+// page of another row would reach it as NaN: rows whose result is not finite are computed again alone,
+// as are those of a workgroup with a list in which a page stands twice.
+constexpr int ROWS_MAX = 16, ROWS_GROUPS = 4, ROWS_WAVES = 8;
+constexpr int ROWS_LDS = 160 * 1024 - 2048;   // dynamic LDS at most
+
+// LDS image of one (page, kv head): K, then V, as they are in memory (a lane's 16 bytes of either
+// operand are next to its neighbours': no two lanes that are served together share a bank).
+template <int D>
+struct PageImage {
+  static constexpr int HALF = PAGE * D * 2, GROUP = D * 8, BYTES = 2 * HALF, CHUNKS = BYTES / 1024;
+};
+
+template <int D>
+__global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendArgs a) {
+  typedef __attribute__((address_space(3))) void lds_void;
+  using Image = PageImage<D>;
+  constexpr int KS = D / 32, NT = 64 * ROWS_WAVES, CPW = 4 * Image::CHUNKS / ROWS_WAVES;   // loads of a wave per step
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // two steps' pages (first the rows of every page), union
+  __shared__ float sml[ROWS_WAVES][16][2];
+  __shared__ int spos[ROWS_MAX];
+  __shared__ uint32_t counts[ROWS_WAVES];
+  __shared__ uint32_t again, twice;   // rows to compute alone; a list names a page twice
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
+  const uint32_t per_xcd = gridDim.x / 8;
+  uint32_t item = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+  if (item >= (uint64_t)a.items) return;
+  const int rpt = a.rpt, R = ROWS_GROUPS * rpt, K = a.budget;
+  const uint32_t groups = (uint32_t)(a.T + R - 1) / R;
+  const int t0 = (int)(item % groups) * R;
+  item /= groups;
+  const int h = (int)(item % (uint32_t)a.Hkv), b = (int)(item / (uint32_t)a.Hkv);
+  const int64_t m0 = (int64_t)b * a.T + t0;
+  const int live = a.T - t0 < R ? a.T - t0 : R;
+  uint32_t* page_rows = (uint32_t*)lds;         // 16 bits a page
+  uint2* merged = (uint2*)(lds + a.ring_bytes); // the union: block, page << 16 | rows
+  if (tid < ROWS_MAX) spos[tid] = tid < live ? a.positions[m0 + tid] : -1;
+  if (tid == 0) again = twice = 0;
+  // this wave's queries: column col is head col % G of row wave * rpt + col / G
+  const int rg = wave % ROWS_GROUPS, half = wave / ROWS_GROUPS;
+  const int row = col < rpt * a.G ? rg * rpt + col / a.G : ROWS_MAX;
+  bf16x8 qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (row < live) x = *(const u32x4*)(a.q + ((m0 + row) * a.Hq + (int64_t)h * a.G + col % a.G) * D + 32 * s + 8 * g);
+    qf[s] = __builtin_bit_cast(bf16x8, x);
+  }
+  const int32_t* lists = a.pages + (m0 * a.Hkv + h) * K;
+  const int64_t list_step = (int64_t)a.Hkv * K;
+  const int entries = live * K;
+  __syncthreads();
+  int low = 0x7fffffff;
+  for (int r = 0; r < live; ++r) low = spos[r] >= 0 && spos[r] < low ? spos[r] : low;
+  // entry e of the lists: its page, or -1
+  auto entry = [&](int e, int& r) {
+    r = e / K;
+    const int p = lists[r * list_step + e % K];
+    return p >= 0 && spos[r] >= 0 && p <= spos[r] / PAGE && p < a.table_stride ? p : -1;
+  };
+  auto whole = [&](int p) { return p * PAGE + PAGE - 1 <= low; };
+  for (int e = tid; e < entries; e += NT) {
+    int r;
+    const int p = entry(e, r);
+    if (p >= 0) page_rows[p >> 1] = 0;
+  }
+  __syncthreads();
+  for (int e = tid; e < entries; e += NT) {
+    int r;
+    const int p = entry(e, r);
+    if (p >= 0) {
+      const uint32_t bit = 1u << (r + (p & 1) * 16);
+      if (atomicOr(&page_rows[p >> 1], bit) & bit) twice = 1;
+    }
+  }
+  __syncthreads();
+  const bool merge = twice == 0;
+  uint32_t total = 0, bad = 0;
+  if (merge)
+    for (int e0 = 0; e0 < entries; e0 += NT) {
+      int r = 0, blk = -1, p = -1;
+      uint32_t rows = 0;
+      if (e0 + tid < entries) p = entry(e0 + tid, r);
+      if (p >= 0) {
+        rows = whole(p) ? page_rows[p >> 1] >> (p & 1) * 16 & 0xffffu : 1u << r;
+        if (__builtin_ctz(rows) == r) blk = page_block(a.table, a.table_stride, b, p, a.blocks);
+      }
+      const uint64_t have = __ballot(blk >= 0);
+      if (lane == 0) counts[wave] = (uint32_t)__popcll(have);
+      __syncthreads();
+      uint32_t at = total + (uint32_t)__popcll(have & ((1ull << lane) - 1));
+      for (int w = 0; w < ROWS_WAVES; ++w) {
+        if (w < wave) at += counts[w];
+        total += counts[w];
+      }
+      if (blk >= 0) {
+        merged[at] = uint2{(uint32_t)blk, (uint32_t)p << 16 | rows};
+      }
+      __syncthreads();
+    }
+
+  floatx4 acc[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float mx = -__builtin_huge_valf(), l = 0.f;
+  const int pos = row < live ? spos[row] : -1;
+  const uint32_t mine = ((1u << rpt) - 1) << (rg * rpt);   // the wave's rows
+  const uint32_t pairs = (total + 1) / 2;
+  const uint32_t steps = (pairs + 1) / 2;
+  // The four pages of step j into its half of the ring, the last pair again past the end.
+  auto fetch = [&](uint32_t j) {
+    uint8_t* to = lds + (j & 1) * (4 * Image::BYTES);
+    int64_t base[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t e = 4 * j + i;
+      e = e < total ? e : total - 1;
+      base[i] = ((int64_t)__builtin_amdgcn_readfirstlane((int)merged[e].x) * a.Hkv + h) * Image::HALF;
+    }
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) {
+      const int c = i * ROWS_WAVES + wave, cc = c % Image::CHUNKS;
+      // which of the four pages: known at compile time but for two per eight chunks
+      const int pg0 = i * ROWS_WAVES / Image::CHUNKS, pg = Image::CHUNKS < ROWS_WAVES ? c / Image::CHUNKS : pg0;
+      const int64_t from = Image::CHUNKS < ROWS_WAVES ? (pg & 1 ? base[(2 * i + 1) & 3] : base[(2 * i) & 3]) : base[pg0];
+      const bool is_v = cc >= Image::CHUNKS / 2;
+      const int off = (is_v ? cc - Image::CHUNKS / 2 : cc) * 1024;
+      const uint8_t* src = (const uint8_t*)(is_v ? a.v_pool : a.k_pool) + from + off + lane * 16;
+      __builtin_amdgcn_global_load_lds((const void*)src, (lds_void*)(to + c * 1024), 16, 0, 0);
+    }
+  };
+  const uint32_t k_at = (g >> 1) * 512 + col * 32 + (g & 1) * 16, v_at = Image::HALF + g * Image::GROUP + col * 16;
+  if (pairs) fetch(0);
+  for (uint32_t j = 0; j < steps; ++j) {
+    // this step's pages have landed, for every wave, and every wave is done with the last step's
+    wait_vmcnt<0>();
+    wait_lgkmcnt0();
+    block_barrier();
+    if (j + 1 < steps) fetch(j + 1);
+    const uint32_t e = 4 * j + 2 * half;
+    if (e >= total) continue;
+    const bool two = e + 1 < total;
+    const uint32_t info_a = (uint32_t)__builtin_amdgcn_readfirstlane((int)merged[e].y);
+    const uint32_t info_b = two ? (uint32_t)__builtin_amdgcn_readfirstlane((int)merged[e + 1].y) : 0u;
+    const uint32_t rows_a = info_a & 0xffffu, rows_b = info_b & 0xffffu;
+    if (!((rows_a | rows_b) & mine)) continue;   // by none of the wave's rows
+    const int page_a = (int)(info_a >> 16), page_b = (int)(info_b >> 16);
+    // a page that one row sees in part: what lies behind its last position never enters
+    int end_a = PAGE, end_b = two ? PAGE : 0;
+    if (!whole(page_a)) end_a = __builtin_amdgcn_readfirstlane(spos[__builtin_ctz(rows_a)]) - page_a * PAGE + 1;
+    if (two && !whole(page_b)) end_b = __builtin_amdgcn_readfirstlane(spos[__builtin_ctz(rows_b)]) - page_b * PAGE + 1;
+    const uint8_t* slot = lds + (j & 1) * (4 * Image::BYTES) + half * (2 * Image::BYTES);
+    // all of K is asked for before the first is used, all of V before the softmax
+    u32x4 ka[KS], kb[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      ka[s] = *(const u32x4*)(slot + k_at + 1024 * s);
+      kb[s] = *(const u32x4*)(slot + Image::BYTES + k_at + 1024 * s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    floatx4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ka[s]), qf[s], s0, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kb[s]), qf[s], s1, 0, 0, 0);
+    }
+    u32x4 va[KS], vb[KS];   // keys 4 g .. 4 g + 3 of d = 32 s + 2 col and of the next
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      va[s] = *(const u32x4*)(slot + v_at + 256 * s);
+      vb[s] = *(const u32x4*)(slot + Image::BYTES + v_at + 256 * s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const int left_a = rows_a >> row & 1 ? pos - page_a * PAGE + 1 : 0;
+    const int left_b = rows_b >> row & 1 ? pos - page_b * PAGE + 1 : 0;
+    float x[8];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[r] = 4 * g + r < left_a ? s0[r] * a.qk_scale : -__builtin_huge_valf();
+      x[4 + r] = 4 * g + r < left_b ? s1[r] * a.qk_scale : -__builtin_huge_valf();
+    }
+    uint32_t hi[4], lo[4];
+    softmax_step<D>(x, mx, l, acc, hi, lo);
+    const bf16x8 ph = __builtin_bit_cast(bf16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
+    const bf16x8 pl = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
+    if (end_a < PAGE || end_b < PAGE) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int k0 = 4 * g + 2 * w;
+        const uint32_t ma = k0 + 1 < end_a ? 0xffffffffu : k0 < end_a ? 0xffffu : 0u;
+        const uint32_t mb = k0 + 1 < end_b ? 0xffffffffu : k0 < end_b ? 0xffffu : 0u;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) va[s][w] &= ma, va[s][2 + w] &= ma, vb[s][w] &= mb, vb[s][2 + w] &= mb;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      bf16x8 f0, f1;
+      v_operands(va[s], vb[s], f0, f1);
+      acc[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f0, ph, acc[2 * s], 0, 0, 0);
+      acc[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f1, ph, acc[2 * s + 1], 0, 0, 0);
+      acc[2 * s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f0, pl, acc[2 * s], 0, 0, 0);
+      acc[2 * s + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f1, pl, acc[2 * s + 1], 0, 0, 0);
+    }
+  }
+  // join the halves: the second leaves its sums in LDS
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  __syncthreads();
+  floatx4* other = (floatx4*)lds + rg * (D / 16) * 64 + lane;
+  if (half) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) other[i * 64] = acc[i];
+    if (g == 0) sml[rg][col][0] = mx, sml[rg][col][1] = l;
+  }
+  __syncthreads();
+  if (!half && merge && row < live) {
+    const float m2 = sml[rg][col][0], top = fmaxf(mx, m2);
+    const float c1 = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - top);
+    const float c2 = m2 == top ? 1.f : __builtin_amdgcn_exp2f(m2 - top);
+    l = l * c1 + sml[rg][col][1] * c2;
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // nothing seen: zeros
+    uint16_t* o = a.out + ((m0 + row) * a.Hq + (int64_t)h * a.G + col % a.G) * D + 8 * g;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {   // register r of tiles 2 s, 2 s + 1: d = 32 s + 8 g + 2 r, + 1
+      const floatx4 y = (acc[2 * s] * c1 + other[2 * s * 64] * c2) * inv;
+      const floatx4 z = (acc[2 * s + 1] * c1 + other[(2 * s + 1) * 64] * c2) * inv;
+      u32x4 w;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sum += __builtin_fabsf(y[r]) + __builtin_fabsf(z[r]);
+        w[r] = pack_bf16x2(y[r], z[r]);
+      }
+      *(u32x4*)(o + 32 * s) = w;
+    }
+    if (!(sum < __builtin_huge_valf())) atomicOr(&again, 1u << row);
+  }
+  __syncthreads();
+  const uint32_t alone = merge ? again : ~0u;
+  for (int r = 0; r < live; ++r)
+    if (alone >> r & 1) {
+      __syncthreads();
+      attend_row<D, ROWS_WAVES>(a, b, h, 0, t0 + r, 0, (float*)lds, sml);
+    }
 }
 
 // The splits of one (row, head) joined: D / 4 threads a head.
@@ -1160,6 +1470,18 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const float* __restric
 constexpr int64_t MAX_BATCH_ROWS = 1 << 24;   // batch * tokens
 constexpr int64_t MAX_WIDTH = 1 << 17;        // pages of a request that the choice covers (2M tokens)
 
+// More than 64 KiB of dynamic LDS has to be allowed, once per kernel and device.
+hipError_t raise_lds_limit(const void* kernel, std::atomic<uint64_t>& devices, int bytes) {
+  int dev = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err != hipSuccess) return err;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (devices.load() & bit) return hipSuccess;
+  err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == hipSuccess) devices |= bit;
+  return err;
+}
+
 // A launch holds fewer than 2^32 threads.
 bool grid_ok(int64_t wgs, int64_t threads) { return wgs <= 0xffffffffll / threads; }
 
@@ -1175,6 +1497,27 @@ int attend_splits(int64_t items, int64_t budget) {
   int64_t s = items > 0 ? (512 + items - 1) / items : 1;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : s);
+}
+
+// LDS of attend_rows_kernel in front of the union: the ring, and before it two bytes a page.
+int64_t rows_ring_bytes(int64_t D, int64_t pages) {
+  const int64_t image = D == 64 ? PageImage<64>::BYTES : D == 128 ? PageImage<128>::BYTES : PageImage<256>::BYTES;
+  return std::max(8 * image, (pages + 1) / 2 * 4);
+}
+
+// Rows of a wave where rows go over the union of their lists (attend_rows_kernel), or 0: a group of
+// at most sixteen heads, a table (16 bits a page) and lists that fit LDS, rows for more than one
+// wave, and workgroups for half the CUs. Fewer rows run faster one by one with their lists split.
+int attend_rows_per_wave(int64_t batch, int64_t tokens, int64_t Hkv, int64_t G, int64_t D, int64_t pages,
+                         int64_t budget) {
+  if (G > 16) return 0;
+  const int64_t most = ROWS_MAX / ROWS_GROUPS;
+  int64_t rpt = 16 / G < most ? 16 / G : most;
+  const int64_t room = ROWS_LDS - rows_ring_bytes(D, pages);
+  while (rpt > 0 && ROWS_GROUPS * rpt * budget * 8 > room) --rpt;
+  if (rpt < 1 || tokens <= rpt || pages > 65536) return 0;
+  const int64_t R = ROWS_GROUPS * rpt;
+  return batch * Hkv * ((tokens + R - 1) / R) >= 128 ? (int)rpt : 0;
 }
 
 // Workspace of one row's pages: scores, their errors, and keys where a row needs them all.
@@ -1421,7 +1764,24 @@ SV_API int snowverify_sparse_attention(const void* q, const void* k_pool, const 
   a.part_ml = a.splits > 1 ? a.part_o + batch * tokens * num_heads * a.splits * head_size : nullptr;
   const int hm = a.G < 16 ? a.G : 16;
   const int64_t dr = head_size == 256 && hm > 8 ? 128 : head_size;
-  const size_t lds = (size_t)ATT_WAVES * hm * (dr + 4) * 4;
+  size_t lds = (size_t)ATT_WAVES * hm * (dr + 4) * 4;
+  const int rpt = attend_rows_per_wave(batch, tokens, num_kv_heads, a.G, head_size, table_stride, budget);
+  if (rpt) {
+    a.rpt = rpt;
+    a.splits = 1;
+    const int64_t R = ROWS_GROUPS * rpt, ring = rows_ring_bytes(head_size, table_stride);
+    a.items = batch * num_kv_heads * ((tokens + R - 1) / R);
+    a.ring_bytes = (int)ring;
+    lds = std::max(lds / ATT_WAVES * ROWS_WAVES, (size_t)(ring + R * budget * 8));
+    auto kern = head_size == 64 ? attend_rows_kernel<64> : head_size == 128 ? attend_rows_kernel<128> : attend_rows_kernel<256>;
+    static std::atomic<uint64_t> raised[3];
+    const hipError_t err = raise_lds_limit((const void*)kern, raised[head_size / 128], ROWS_LDS);
+    if (err != hipSuccess) return (int)err;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3(64 * ROWS_WAVES), lds,
+                       S(stream), a);
+    SV_CHECK_LAUNCH();
+    return SV_OK;
+  }
   auto kern = head_size == 64 ? attend_kernel<64> : head_size == 128 ? attend_kernel<128> : attend_kernel<256>;
   hipLaunchKernelGGL(kern, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3(64 * ATT_WAVES), lds,
                      S(stream), a);

@@ -320,7 +320,8 @@ def check_attend(got, q, kp, vp, table, positions, pages, scale):
     weight = (q.shape[2] + 4) * U * reach + 2.0 ** -16 + (keys + 64) * U
     tol = BF * want.abs() + 2 * weight * size + 1e-30
     err = (got.double() - want).abs()
-    assert (err <= tol).all(), float((err / tol).max())
+    ok = (err <= tol) | (want.isnan() & got.isnan()) | (got.double() == want)
+    assert ok.all(), float((err / tol).nan_to_num(1e9).max())
 
 
 ATTEND = [
@@ -336,6 +337,13 @@ ATTEND = [
     (16, 2, 64, 2, 150, 8, 7),
     (3, 3, 256, 1, 1, 140, 131),
     (8, 8, 64, 2, 40, 20, 17),
+    # rows over the union of their lists: 2, 4, 1, 3 rows a tile, a last group that is not full
+    (16, 2, 256, 1, 517, 30, 12),
+    (8, 2, 128, 2, 600, 25, 20),
+    (16, 1, 64, 1, 520, 20, 20),
+    (5, 1, 256, 3, 515, 12, 9),
+    (20, 4, 128, 1, 400, 40, 130),
+    (3, 3, 64, 1, 700, 6, 1),
 ]
 
 
@@ -351,6 +359,12 @@ def test_attend(gpu, Hq, Hkv, d, B, T, width, budget):
     pos[-1] = width * PAGE - 1
     # lists in any order, -1 among them, pages past the row's position
     pages = torch.randint(-1, width, (M, Hkv, budget), generator=g, dtype=torch.int32)
+    if T > 300:        # ascending, as they are chosen; a few rows in any order
+        keep = pages[::97].clone()
+        pages = torch.stack([torch.randperm(width, generator=g)[:min(budget, width)].sort().values
+                             for _ in range(M * Hkv)]).int()
+        pages = torch.nn.functional.pad(pages, (0, max(0, budget - width)), value=-1).view(M, Hkv, budget)
+        pages[::97] = keep
     if M > 2:
         pos[0], pos[1] = 0, -1
         pages[2] = -1
@@ -361,8 +375,8 @@ def test_attend(gpu, Hq, Hkv, d, B, T, width, budget):
         assert (got[1:3] == 0).all()
 
 
-@pytest.mark.parametrize("kind", ["dead", "holes", "twice", "past", "large", "tiny"])
-@pytest.mark.parametrize("T", [1, 130])
+@pytest.mark.parametrize("kind", ["dead", "holes", "twice", "past", "large", "tiny", "other", "ends"])
+@pytest.mark.parametrize("T", [1, 130, 600])
 def test_attend_borders(gpu, kind, T):
     """NaN and infinities behind the last position, table entries that are no page, listed pages
     outside the table or listed twice, scores that differ by hundreds."""
@@ -377,6 +391,10 @@ def test_attend_borders(gpu, kind, T):
     pages = torch.stack([torch.randperm(21, generator=g)[:budget] for _ in range(T * Hkv)])
     pages = pages.view(T, Hkv, budget).int()
     pages[:, :, 3] = 20                  # the page that the row ends in
+    if T == 600:                         # ascending: rows over the union of their lists
+        pages = torch.stack([torch.randperm(20, generator=g)[:budget - 2].sort().values
+                             for _ in range(T * Hkv)]).view(T, Hkv, -1).int()
+        pages = torch.cat([pages, torch.full((T, Hkv, 1), 20), torch.full((T, Hkv, 1), -1)], 2).int()
     if kind == "dead":
         blk = int(table[0, 20])
         kp[blk, :, :, 5:] = float("nan")
@@ -391,6 +409,15 @@ def test_attend_borders(gpu, kind, T):
         pages[:, :, 1::3] = -2 ** 31
     if kind == "large":
         q *= 64
+    if kind == "other":                  # pages that only some rows list hold no numbers
+        bad = table[0, 7].long()
+        vp[bad, 0, 2, 5, 1], vp[bad, 1, 0, 3, 2], kp[bad, 1, 2, 4, 5] = float("nan"), float("inf"), float("nan")
+        pages[::2] = torch.where(pages[::2] == 7, -1, pages[::2]).sort(dim=2, descending=False).values
+        pages[::2] = torch.where(pages[::2] == -1, 2 ** 30, pages[::2]).sort(dim=2).values
+    if kind == "ends":                   # rows of a group end in the same page, or pages apart
+        pos = (last - torch.arange(T) % 37).int()
+        vp[int(table[0, 20]), :, 1:, :, 1:] = float("nan")
+        pos[5::11] = -1
     if kind == "tiny":
         q *= 2.0 ** -100
     got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
