@@ -39,6 +39,34 @@ __device__ __forceinline__ int page_block(const int32_t* __restrict__ table, int
   return e >= 0 && e < blocks ? e : -1;
 }
 
+// s_waitcnt on the vector-memory counter only (gfx9 encoding: vmcnt in bits 3:0 and 15:14, no wait on
+// the others).
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// On the LDS counter only: this wave's LDS reads have ended.
+__device__ __forceinline__ void wait_lgkmcnt0() {
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+}
+
+// Workgroup barrier without the wait of __syncthreads for every load in flight.
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The maximum over the four lanes of a column (lanes col, col + 16, ..), by row and half-wave swaps.
+__device__ __forceinline__ float column_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
 // bf16 pairs as signed 16-bit keys in the order of their values (and back: it is an involution),
 // so that minima and maxima are one packed integer operation for two elements. NaNs lie outside
 // the infinities: above +inf or below -inf, by their sign.
@@ -318,6 +346,8 @@ struct SelectArgs {
   float* scores;            // [requests, Hkv, rows, width] s~
   float* errors;            // [requests, Hkv, rows, width / 16] E of 16 pages
   uint64_t* exact;          // [requests, Hkv, rows, width] keys, where a row needs them all
+  u32x4* operands;          // [requests, Hkv, row tiles] of more than sixteen rows
+  int32_t* tile_last;       // [requests, row tiles] pages seen
   int64_t table_stride, blocks, width, T, row0;   // row0: first row of every request in this launch
   int rows, Hq, Hkv, G, budget, sink, recent;     // rows: of a request in this launch
 };
@@ -335,185 +365,306 @@ __device__ __forceinline__ float neg_part(float f) { return !(f >= 0.f) ? f : 0.
 
 constexpr int SCORE_WAVES = 4;
 
-// A workgroup: RT times sixteen rows of a request and kv head. Its threads sum the rows' P and N and
-// leave both pieces in LDS as operands of v_mfma_f32_16x16x32_bf16 (terms: D of N with the minima,
-// then D of P with the maxima). A wave takes PT times sixteen pages at a time, whose bounds are the
-// other operand as they lie in memory: they are read ahead of the rows' sums, and each step's pages
-// while the last one's scores are stored. Two page tiles to each operand read keep LDS (85 bytes a
-// clock) behind the matrix cores, two row tiles halve the reads of the bounds.
-template <int D, int PT, int RT>
-__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a, uint32_t pages_per_wg) {
-  constexpr int NS = D / 16;   // steps of 32 terms
-  __shared__ u32x4 op[RT][NS][2][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
-  const uint32_t groups = (uint32_t)(a.rows + 16 * RT - 1) / (16 * RT);
-  uint32_t y = blockIdx.x;
-  const int row0 = (int)(y % groups) * 16 * RT;
-  y /= groups;
-  const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
-  const int64_t m0 = (int64_t)b * a.T + a.row0 + row0;
-  const int live = a.rows - row0 < 16 * RT ? a.rows - row0 : 16 * RT;
-  const int64_t p0 = (int64_t)blockIdx.y * pages_per_wg;
-  const uint16_t* side = a.bounds + (int64_t)h * 2 * D + 8 * g;
-  const int64_t block_step = (int64_t)a.Hkv * 2 * D;
+// The sums P and N of sixteen rows, of which `live` are rows, both pieces, as operands of
+// v_mfma_f32_16x16x32_bf16 in LDS: [D / 16 steps of 32 terms][piece][64 lanes], D terms of N (for the
+// minima), then D of P. By 256 threads, four elements d .. of a row at a time (D / 4 threads a row), all
+// heads of them; a row's slots are rotated by (d / 8) % 16, so that its threads write to different banks.
+template <int D>
+__device__ __forceinline__ void rows_operand(const SelectArgs& a, int64_t m0, int h, int live, uint16_t* ops) {
+  constexpr int NS = D / 16, UNITS = 16 * (D / 4) / (64 * SCORE_WAVES), PER = 64 * SCORE_WAVES / (D / 4);
+  const int tid = threadIdx.x;
+  float pp[UNITS][4], nn[UNITS][4];
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pp[k][i] = nn[k][i] = 0.f;
+  const int r0 = tid / (D / 4), d = tid % (D / 4) * 4;
+  const uint16_t* qp = a.q + ((m0 + r0) * a.Hq + (int64_t)h * a.G) * D + d;
+  const int64_t row_step = (int64_t)PER * a.Hq * D;
+#pragma unroll 4
+  for (int e = 0; e < a.G; ++e) {
+    uint2 w[UNITS];
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+      w[k] = uint2{0u, 0u};
+      if (r0 + k * PER < live) w[k] = *(const uint2*)(qp + k * row_step + (int64_t)e * D);
+    }
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t x2 = i ? w[k].y : w[k].x;
+        const short2v sign = __builtin_bit_cast(short2v, x2) >> (short)15;   // -1 where negative
+        const uint32_t ng = x2 & __builtin_bit_cast(uint32_t, sign), ps = x2 & ~__builtin_bit_cast(uint32_t, sign);
+        pp[k][2 * i] += bf_lo(ps);
+        pp[k][2 * i + 1] += bf_hi(ps);
+        nn[k][2 * i] += bf_lo(ng);
+        nn[k][2 * i + 1] += bf_hi(ng);
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k) {
+    const int r = r0 + k * PER;
+    uint2 ph, pl, nh, nl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // NaN: the row's scores are not to be trusted
+      const float most = fmaxf(pp[k][i], -nn[k][i]);
+      const bool small = (pp[k][i] > 0.f && pp[k][i] < 0x1p-90f) || (nn[k][i] < 0.f && nn[k][i] > -0x1p-90f);
+      if (small || most > 0x1p40f) pp[k][i] = __builtin_nanf("");
+    }
+    ph.x = pack_bf16x2(pp[k][0], pp[k][1]);
+    ph.y = pack_bf16x2(pp[k][2], pp[k][3]);
+    nh.x = pack_bf16x2(nn[k][0], nn[k][1]);
+    nh.y = pack_bf16x2(nn[k][2], nn[k][3]);
+    pl.x = pack_bf16x2(pp[k][0] - bf_lo(ph.x), pp[k][1] - bf_hi(ph.x));
+    pl.y = pack_bf16x2(pp[k][2] - bf_lo(ph.y), pp[k][3] - bf_hi(ph.y));
+    nl.x = pack_bf16x2(nn[k][0] - bf_lo(nh.x), nn[k][1] - bf_hi(nh.x));
+    nl.y = pack_bf16x2(nn[k][2] - bf_lo(nh.y), nn[k][3] - bf_hi(nh.y));
+    const int st = d / 32, slot = (d / 8 % 4) * 16 + ((r + d / 8) & 15);
+    uint16_t* to = ops + (st * 2 * 64 + slot) * 8 + d % 8;
+    *(uint2*)to = nh;
+    *(uint2*)(to + 64 * 8) = nl;
+    *(uint2*)(to + NS * 64 * 8) = ph;           // NS / 2 steps of two pieces on
+    *(uint2*)(to + NS * 64 * 8 + 64 * 8) = pl;
+  }
+}
+
+// Lane (col, g)'s slot in step s of such an operand.
+template <int D>
+__device__ __forceinline__ int operand_slot(int s, int col, int g) {
+  return g * 16 + ((col + s % (D / 32) * 4 + g) & 15);
+}
+
+// One step of 32 terms for PT times sixteen pages: s~ and the sum of the terms' magnitudes.
+template <int PT>
+__device__ __forceinline__ void score_step(bool minima, const u32x4* x, u32x4 hi, u32x4 lo, floatx4 (&acc)[PT],
+                                           floatx4 (&mag)[PT], int pitch) {
+  const bf16x8 wh = __builtin_bit_cast(bf16x8, hi), wl = __builtin_bit_cast(bf16x8, lo);
+  u32x4 ab[PT];   // |bounds|, with the sign of the larger piece: N is negative
+#pragma unroll
+  for (int i = 0; i < PT; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ab[i][k] = minima ? x[i * pitch][k] | 0x80008000u : x[i * pitch][k] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 0; i < PT; ++i)
+    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i * pitch]), wh, acc[i], 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < PT; ++i)
+    mag[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ab[i]), wh, mag[i], 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < PT; ++i)
+    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i * pitch]), wl, acc[i], 0, 0, 0);
+}
+
+// E of a tile of sixteen pages from page pt (lane (row col, g): pages pt + 4 g + k), whose first
+// `sink`, always chosen, and those from `last` on do not count; what is no page (bits of none) scores
+// -inf.
+__device__ __forceinline__ float tile_error(const SelectArgs& a, int64_t pt, int64_t last, uint32_t none, int g,
+                                            floatx4& acc, floatx4 mag) {
+  const float rel = 1.01f * (0x1p-14f + (float)a.G * 0x1p-24f), inf = __builtin_huge_valf();
+  float e = 0.f;
+  if (none == 0 && pt >= a.sink && pt + 16 <= last) {
+    const float sum = (mag[0] + mag[1]) + (mag[2] + mag[3]);   // infinite or NaN where one of them is
+    e = sum < 0x1p120f ? __builtin_fmaf(rel, fmaxf(fmaxf(mag[0], mag[1]), fmaxf(mag[2], mag[3])), 0x1p-74f) : inf;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool no = none >> (4 * g + k) & 1;
+      if (no) acc[k] = -inf;
+      const int64_t pg = pt + 4 * g + k;
+      if (!no && pg >= a.sink && pg < last) {
+        const float e1 = __builtin_fmaf(rel, mag[k], 0x1p-74f);
+        e = e1 < 0x1p120f ? fmaxf(e, e1) : inf;   // NaN too
+      }
+    }
+  }
+  return column_max(e);
+}
+
+// This lane's bounds of PT times sixteen pages from page p: blocks (-1: no page; past the table's end
+// its last page's), then 16-byte loads of each step.
+template <int D, int PT>
+struct PageTiles {
   int blk[PT];
-  auto entries = [&](int64_t p) {   // lane: page p + 16 i + col, the table's last past its end
+  u32x4 x[PT][D / 16];
+  __device__ __forceinline__ void entries(const SelectArgs& a, int b, int64_t p, int col) {
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int64_t pg = p + 16 * i + col;
       blk[i] = page_block(a.table, a.table_stride, b, pg < a.table_stride ? pg : a.table_stride - 1, a.blocks);
     }
-  };
-  u32x4 x[PT][NS];
-  auto fetch = [&] {
+  }
+  __device__ __forceinline__ void fetch(const SelectArgs& a, int h, int g) {
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
-      const uint16_t* bp = side + (blk[i] < 0 ? 0 : blk[i]) * block_step;
+      const uint16_t* bp = a.bounds + ((int64_t)(blk[i] < 0 ? 0 : blk[i]) * a.Hkv + h) * 2 * D + 8 * g;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) x[i][s] = *(const u32x4*)(bp + 32 * s);
+      for (int s = 0; s < D / 16; ++s) x[i][s] = *(const u32x4*)(bp + 32 * s);
     }
-  };
+  }
+};
+
+// Up to sixteen rows of a request and kv head a workgroup, which sums them for itself. A wave takes
+// PT times sixteen pages at a time, whose bounds are an operand as they lie in memory: they are read
+// ahead of the rows' sums, and each step's pages while the last one's scores are stored. Two page
+// tiles to each read of the rows' operand keep LDS (85 bytes a clock) behind the matrix cores.
+template <int D, int PT>
+__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a, uint32_t pages_per_wg) {
+  constexpr int NS = D / 16;
+  __shared__ u32x4 op[NS][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
+  uint32_t y = blockIdx.x;
+  const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
+  const int64_t m0 = (int64_t)b * a.T + a.row0;
+  const int live = a.rows;
+  const int64_t p0 = (int64_t)blockIdx.y * pages_per_wg;
+  PageTiles<D, PT> t;
   int64_t p = p0 + 16 * PT * wave;
-  entries(p);
+  t.entries(a, b, p, col);
   const int pos = lane < live ? a.positions[m0 + lane] : -1;
-  if constexpr (RT == 1) fetch();   // with more rows the registers are needed for their sums
+  t.fetch(a, h, g);
   const int64_t last = (int64_t)wave_max<int>((int)pages_seen(pos, a.table_stride));
   if (p0 >= last) return;
   const int64_t p1 = p0 + pages_per_wg < last ? p0 + pages_per_wg : last;
-  // unit: four elements d .. of row r (D / 4 threads a row), of all heads at once; its row's slots in
-  // the operands are rotated by (d / 8) % 16, so that a row's threads write to different banks
-  constexpr int UNITS = RT * 16 * (D / 4) / (64 * SCORE_WAVES), PER = 256 / (D / 4);
-  {
-    float pp[UNITS][4], nn[UNITS][4];
-#pragma unroll
-    for (int k = 0; k < UNITS; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pp[k][i] = nn[k][i] = 0.f;
-    const int r0 = tid / (D / 4), d = tid % (D / 4) * 4;
-    const uint16_t* qp = a.q + ((m0 + r0) * a.Hq + (int64_t)h * a.G) * D + d;
-    const int64_t row_step = (int64_t)PER * a.Hq * D;
-#pragma unroll 4
-    for (int e = 0; e < a.G; ++e) {
-      uint2 w[UNITS];
-#pragma unroll
-      for (int k = 0; k < UNITS; ++k) {
-        w[k] = uint2{0u, 0u};
-        if (r0 + k * PER < live) w[k] = *(const uint2*)(qp + k * row_step + (int64_t)e * D);
-      }
-#pragma unroll
-      for (int k = 0; k < UNITS; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t x2 = i ? w[k].y : w[k].x;
-          const short2v sign = __builtin_bit_cast(short2v, x2) >> (short)15;   // -1 where negative
-          const uint32_t ng = x2 & __builtin_bit_cast(uint32_t, sign), ps = x2 & ~__builtin_bit_cast(uint32_t, sign);
-          pp[k][2 * i] += bf_lo(ps);
-          pp[k][2 * i + 1] += bf_hi(ps);
-          nn[k][2 * i] += bf_lo(ng);
-          nn[k][2 * i + 1] += bf_hi(ng);
-        }
-    }
-    uint16_t* ops = (uint16_t*)op;
-#pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-      const int r = r0 + k * PER;
-      uint2 ph, pl, nh, nl;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {   // NaN: the row's scores are not to be trusted
-        const float most = fmaxf(pp[k][i], -nn[k][i]);
-        const bool small = (pp[k][i] > 0.f && pp[k][i] < 0x1p-90f) || (nn[k][i] < 0.f && nn[k][i] > -0x1p-90f);
-        if (small || most > 0x1p40f) pp[k][i] = __builtin_nanf("");
-      }
-      ph.x = pack_bf16x2(pp[k][0], pp[k][1]);
-      ph.y = pack_bf16x2(pp[k][2], pp[k][3]);
-      nh.x = pack_bf16x2(nn[k][0], nn[k][1]);
-      nh.y = pack_bf16x2(nn[k][2], nn[k][3]);
-      pl.x = pack_bf16x2(pp[k][0] - bf_lo(ph.x), pp[k][1] - bf_hi(ph.x));
-      pl.y = pack_bf16x2(pp[k][2] - bf_lo(ph.y), pp[k][3] - bf_hi(ph.y));
-      nl.x = pack_bf16x2(nn[k][0] - bf_lo(nh.x), nn[k][1] - bf_hi(nh.x));
-      nl.y = pack_bf16x2(nn[k][2] - bf_lo(nh.y), nn[k][3] - bf_hi(nh.y));
-      const int st = d / 32, slot = (d / 8 % 4) * 16 + ((r + d / 8) & 15);
-      uint16_t* to = ops + ((((r / 16) * NS + st) * 2) * 64 + slot) * 8 + d % 8;
-      *(uint2*)to = nh;
-      *(uint2*)(to + 64 * 8) = nl;
-      *(uint2*)(to + NS * 64 * 8) = ph;           // NS / 2 steps of two pieces on
-      *(uint2*)(to + NS * 64 * 8 + 64 * 8) = pl;
-    }
-  }
-  if constexpr (RT > 1) fetch();
+  rows_operand<D>(a, m0, h, live, (uint16_t*)op);
   __syncthreads();
-  const float rel = 1.01f * (0x1p-14f + (float)a.G * 0x1p-24f);
-  const int64_t item = ((int64_t)b * a.Hkv + h) * a.rows + row0 + col;
+  const int64_t item = ((int64_t)b * a.Hkv + h) * a.rows + col;
   for (; p < p1; p += 16 * PT * SCORE_WAVES) {
-    uint32_t none[PT];   // bit i: page i of the tile is no page
+    uint32_t none[PT];
 #pragma unroll
-    for (int i = 0; i < PT; ++i) none[i] = (uint32_t)__ballot(blk[i] < 0);
+    for (int i = 0; i < PT; ++i) none[i] = (uint32_t)__ballot(t.blk[i] < 0);
     const bool more = p + 16 * PT * SCORE_WAVES < p1;
-    if (more) entries(p + 16 * PT * SCORE_WAVES);
-    floatx4 acc[RT][PT], mag[RT][PT];
+    if (more) t.entries(a, b, p + 16 * PT * SCORE_WAVES, col);
+    floatx4 acc[PT], mag[PT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int i = 0; i < PT; ++i) acc[r][i] = mag[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    u32x4 w[2][RT][2];
+    for (int i = 0; i < PT; ++i) acc[i] = mag[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    u32x4 w[3][2];
     auto operand = [&](int s) {
-      const int slot = g * 16 + ((col + s % (NS / 2) * 4 + g) & 15);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) w[s & 1][r][0] = op[r][s][0][slot], w[s & 1][r][1] = op[r][s][1][slot];
+      const int slot = operand_slot<D>(s, col, g);
+      w[s % 3][0] = op[s][0][slot], w[s % 3][1] = op[s][1][slot];
     };
     operand(0);
+    operand(1);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      // one step ahead and no more: held over the loop they would not fit the registers
+      // two steps ahead and no more: held over the loop they would not fit the registers
       asm volatile("" ::: "memory");
-      if (s + 1 < NS) operand(s + 1);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const bf16x8 wh = __builtin_bit_cast(bf16x8, w[s & 1][r][0]);
-        const bf16x8 wl = __builtin_bit_cast(bf16x8, w[s & 1][r][1]);
-#pragma unroll
-        for (int i = 0; i < PT; ++i)
-          acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i][s]), wh, acc[r][i], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < PT; ++i) {
-          // |bounds|, with the sign of the larger piece: N is negative
-          u32x4 ab;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) ab[k] = s < NS / 2 ? x[i][s][k] | 0x80008000u : x[i][s][k] & 0x7fff7fffu;
-          mag[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ab), wh, mag[r][i], 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < PT; ++i)
-          acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[i][s]), wl, acc[r][i], 0, 0, 0);
-      }
+      if (s + 2 < NS) operand(s + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      score_step<PT>(s < NS / 2, &t.x[0][s], w[s % 3][0], w[s % 3][1], acc, mag, NS);
     }
-    if (more) fetch();
-    // lane (row col, g): pages p + 16 i + 4 g + k. The first pages, always chosen, do not count.
+    if (more) t.fetch(a, h, g);
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-#pragma unroll
-      for (int i = 0; i < PT; ++i) {
-        const int64_t pt = p + 16 * i;
-        float e = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool no = none[i] >> (4 * g + k) & 1;
-          if (no) acc[r][i][k] = -__builtin_huge_valf();
-          const int64_t pg = pt + 4 * g + k;
-          if (!no && pg >= a.sink && pg < last) {
-            const float e1 = __builtin_fmaf(rel, mag[r][i][k], 0x1p-74f);
-            e = e1 < 0x1p120f ? fmaxf(e, e1) : __builtin_huge_valf();   // NaN too
-          }
-        }
-        e = fmaxf(e, __shfl_xor(e, 16, 64));
-        e = fmaxf(e, __shfl_xor(e, 32, 64));
-        if (16 * r + col < live && pt < p1) {
-          *(floatx4*)(a.scores + (item + 16 * r) * a.width + pt + 4 * g) = acc[r][i];
-          if (g == 0) a.errors[(item + 16 * r) * (a.width / 16) + pt / 16] = e;
-        }
+    for (int i = 0; i < PT; ++i) {
+      const int64_t pt = p + 16 * i;
+      const float e = tile_error(a, pt, last, none[i], g, acc[i], mag[i]);
+      if (col < live && pt < p1) {
+        *(floatx4*)(a.scores + item * a.width + pt + 4 * g) = acc[i];
+        if (g == 0) a.errors[item * (a.width / 16) + pt / 16] = e;
       }
     }
   }
+}
+
+// More rows: their operands once, into the workspace, in tiles of sixteen; with each the most pages
+// that one of its rows sees.
+template <int D>
+__global__ void __launch_bounds__(64 * SCORE_WAVES) operand_kernel(SelectArgs a) {
+  constexpr int NS = D / 16;
+  __shared__ u32x4 op[NS * 2 * 64];
+  const int tiles = (a.rows + 15) / 16, lane = threadIdx.x & 63;
+  uint32_t y = blockIdx.x;
+  const int tile = (int)(y % (uint32_t)tiles);
+  y /= (uint32_t)tiles;
+  const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
+  const int64_t m0 = (int64_t)b * a.T + a.row0 + tile * 16;
+  const int live = a.rows - tile * 16 < 16 ? a.rows - tile * 16 : 16;
+  rows_operand<D>(a, m0, h, live, (uint16_t*)op);
+  const int last = wave_max<int>((int)pages_seen(lane < live ? a.positions[m0 + lane] : -1, a.table_stride));
+  if (h == 0 && threadIdx.x == 0) a.tile_last[b * tiles + tile] = last;
+  __syncthreads();
+  u32x4* out = a.operands + (int64_t)blockIdx.x * (NS * 2 * 64);
+#pragma unroll
+  for (int i = 0; i < NS * 2 / SCORE_WAVES; ++i) out[i * 256 + threadIdx.x] = op[i * 256 + threadIdx.x];
+}
+
+// A wave keeps the bounds of 32 pages in registers and goes over the row tiles of its part of the
+// rows, whose operands come through LDS for all four waves (global_load_lds), the next tile's while
+// one is used. A tile's scores are stored a step later, so that the one wait of a step is for loads
+// and stores that have had a step's time.
+template <int D>
+__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_rows_kernel(SelectArgs a, uint32_t tiles_per_wg) {
+  typedef __attribute__((address_space(3))) void lds_void;
+  constexpr int NS = D / 16, PT = 2, TILE = NS * 2 * 64;   // 16-byte words of a row tile's operands
+  __shared__ u32x4 op[2][TILE];
+  const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
+  const int tiles = (a.rows + 15) / 16;
+  const uint32_t parts = ((uint32_t)tiles + tiles_per_wg - 1) / tiles_per_wg;
+  uint32_t y = blockIdx.y;
+  const int t0 = (int)(y % parts * tiles_per_wg);
+  y /= parts;
+  const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
+  const int t1 = t0 + (int)tiles_per_wg < tiles ? t0 + (int)tiles_per_wg : tiles;
+  const int64_t p = (int64_t)blockIdx.x * (16 * PT * SCORE_WAVES) + 16 * PT * wave;
+  const u32x4* src = a.operands + ((int64_t)b * a.Hkv + h) * tiles * TILE + lane;
+  auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < TILE / 64 / SCORE_WAVES; ++i) {
+      const int c = i * SCORE_WAVES + wave;
+      __builtin_amdgcn_global_load_lds((const void*)(src + (int64_t)t * TILE + c * 64), (lds_void*)&op[t & 1][c * 64], 16, 0, 0);
+    }
+  };
+  PageTiles<D, PT> t;
+  t.entries(a, b, p, col);
+  load(t0);
+  t.fetch(a, h, g);
+  uint32_t none[PT];
+#pragma unroll
+  for (int i = 0; i < PT; ++i) none[i] = (uint32_t)__ballot(t.blk[i] < 0);
+  floatx4 acc[PT], mag[PT];
+  float err[PT] = {};
+  const int lasts = t0 + lane < t1 ? a.tile_last[b * tiles + t0 + lane] : 0;   // at most 64 tiles
+  int64_t done_last = 0;   // pages that the last tile's rows see: what of it is stored
+  auto store = [&](int r) {
+    const int64_t item = ((int64_t)b * a.Hkv + h) * a.rows + r * 16 + col;
+#pragma unroll
+    for (int i = 0; i < PT; ++i)
+      if (p + 16 * i < done_last && r * 16 + col < a.rows) {
+        *(floatx4*)(a.scores + item * a.width + p + 16 * i + 4 * g) = acc[i];
+        if (g == 0) a.errors[item * (a.width / 16) + p / 16 + i] = err[i];
+      }
+  };
+  for (int r = t0; r < t1; ++r) {
+    wait_vmcnt<0>();
+    wait_lgkmcnt0();
+    block_barrier();
+    store(r - 1);
+    if (r + 1 < t1) load(r + 1);
+    done_last = __builtin_amdgcn_readlane(lasts, r - t0);
+    if (p >= done_last) continue;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) acc[i] = mag[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    u32x4 w[3][2];
+    auto operand = [&](int s) {
+      const u32x4* o = op[r & 1] + s * 128 + operand_slot<D>(s, col, g);
+      w[s % 3][0] = o[0], w[s % 3][1] = o[64];
+    };
+    operand(0);
+    operand(1);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      asm volatile("" ::: "memory");
+      // or the loop would hold |bounds| too
+#pragma unroll
+      for (int i = 0; i < PT; ++i) asm volatile("" : "+v"(t.x[i][s]));
+      if (s + 2 < NS) operand(s + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      score_step<PT>(s < NS / 2, &t.x[0][s], w[s % 3][0], w[s % 3][1], acc, mag, NS);
+    }
+#pragma unroll
+    for (int i = 0; i < PT; ++i) err[i] = tile_error(a, p + 16 * i, done_last, none[i], g, acc[i], mag[i]);
+  }
+  store(t1 - 1);
 }
 
 // 64-bit keys in the order of the scores; NaN is -inf, -0 is +0 (the rule of ord_key).
@@ -536,7 +687,6 @@ __device__ __forceinline__ uint32_t wave_incl_sum_u32(uint32_t v) {
 
 constexpr int PICK_NEAR = 512;    // pages near the border that are ranked in LDS
 constexpr int PICK_KEYS = 16;     // scores a thread keeps in registers
-constexpr int PICK_LIST = 1024;   // scores that the choice is made from
 
 // The 64-bit score's key of one page, by a wave: lane l sums terms l, l + 64, .. in order, then a
 // fixed tree, so that equal pages have equal sums. pn [2 D]: N, then P.
@@ -561,16 +711,16 @@ __device__ __forceinline__ uint64_t exact_key(const SelectArgs& a, const double*
 // near pages come from the list. Where more pass than the list holds (budgets of over about half
 // its length, many equal pages) the same steps go over all scores.
 template <int D, int NT, bool CACHED>
-__global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
-  constexpr int BINS = 4 * NT, WAVES = NT / 64;
+__global__ void __launch_bounds__(NT, NT == 256 ? 8 : 2) pick_kernel(SelectArgs a) {
+  constexpr int BINS = 4 * NT, WAVES = NT / 64, LIST = NT == 256 ? 512 : 1024;   // scores the choice is made from
   extern __shared__ uint64_t masks[];   // [words] chosen pages, [words] equal ones
   // a histogram, then the near pages' keys and numbers
   __shared__ uint64_t lists[BINS / 2 > PICK_NEAR * 3 / 2 ? BINS / 2 : PICK_NEAR * 3 / 2];
   uint32_t* hist = (uint32_t*)lists;
   uint64_t* near_key = lists;
   uint32_t* near_page = (uint32_t*)(lists + PICK_NEAR);
-  __shared__ float top_score[PICK_LIST];
-  __shared__ uint32_t top_page[PICK_LIST];
+  __shared__ __attribute__((aligned(16))) float top_score[LIST];
+  __shared__ uint32_t top_page[LIST];
   __shared__ double pn[2 * D];
   __shared__ uint32_t red[4][WAVES];
   __shared__ float member[64];
@@ -773,7 +923,7 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
       over_all([&](int i, float s) {
         if (s >= from && s > -inf) {
           const uint32_t to = atomicAdd(&sh[6], 1u);
-          if (to < PICK_LIST) top_score[to] = s, top_page[to] = (uint32_t)i;
+          if (to < LIST) top_score[to] = s, top_page[to] = (uint32_t)i;
         }
       });
       __syncthreads();
@@ -781,15 +931,33 @@ __global__ void __launch_bounds__(NT) pick_kernel(SelectArgs a) {
       float t;
       if (listed < need0) {             // fewer pages than are needed
         all = true;
-      } else if (listed <= PICK_LIST) {
+      } else if (listed <= LIST) {
+        if (listed <= 256) {            // few: each against all
+          for (uint32_t i = listed + tid; i < (listed + 3) / 4 * 4; i += NT) top_score[i] = -inf;
+          __syncthreads();
+          if (tid < (int)listed) {
+            const float mine = top_score[tid];
+            uint32_t over = 0, same = 0;
+            for (uint32_t i = 0; i < listed; i += 4) {
+              const floatx4 x = *(const floatx4*)(top_score + i);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) over += x[k] > mine, same += x[k] == mine;
+            }
+            if (over < need0 && over + same >= need0) red[1][0] = __float_as_uint(mine);   // equal ones write the same
+          }
+          __syncthreads();
+          t = __uint_as_float(red[1][0]);
+        }
         auto over_list = [&](auto f) {
           for (uint32_t i = tid; i < listed; i += NT) f((int)top_page[i], top_score[i]);
         };
-        float l2 = inf, h2 = -inf;
-        over_list([&](int i, float s) { l2 = fminf(l2, s), h2 = fmaxf(h2, s); });
-        reduce(h2, l2, pages);
-        all = !kth(over_list, h2, l2, need0, t);
-        __syncthreads();
+        if (listed > 256) {
+          float l2 = inf, h2 = -inf;
+          over_list([&](int i, float s) { l2 = fminf(l2, s), h2 = fmaxf(h2, s); });
+          reduce(h2, l2, pages);
+          all = !kth(over_list, h2, l2, need0, t);
+          __syncthreads();
+        }
         if (!all) classify(over_list, t);
       } else {
         float l2 = inf;
@@ -934,26 +1102,6 @@ struct AttendArgs {
 
 constexpr int ATT_WAVES = 4;
 
-// s_waitcnt on the vector-memory counter only (gfx9 encoding: vmcnt in bits 3:0 and 15:14, no wait on
-// the others).
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt is six bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
-// On the LDS counter only: this wave's LDS reads have ended.
-__device__ __forceinline__ void wait_lgkmcnt0() {
-  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
-}
-
-// Workgroup barrier without the wait of __syncthreads for every load in flight.
-__device__ __forceinline__ void block_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // The V^T operands of elements d and d + 1 over two pages' keys, from a 16-byte load of each page
 // (d's four keys, then d + 1's): the middle pairs change places.
 __device__ __forceinline__ void v_operands(u32x4 a, u32x4 b, bf16x8& f0, bf16x8& f1) {
@@ -977,9 +1125,7 @@ __device__ __forceinline__ void softmax_step(const float (&e)[8], float& m, floa
   const float inf = __builtin_huge_valf();
   float top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
   if (__ballot(top > m + RESCALE)) {
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float nm = fmaxf(m, top);
+    const float nm = fmaxf(m, column_max(top));
     const float c = m == nm ? 1.f : __builtin_amdgcn_exp2f(m - nm);   // 0 at the first keys
     m = nm;
     l *= c;
@@ -1520,25 +1666,35 @@ int attend_rows_per_wave(int64_t batch, int64_t tokens, int64_t Hkv, int64_t G, 
   return batch * Hkv * ((tokens + R - 1) / R) >= 128 ? (int)rpt : 0;
 }
 
-// Workspace of one row's pages: scores, their errors, and keys where a row needs them all.
-int64_t select_width(int64_t pages) { return (pages + 15) / 16 * 16; }
-int64_t select_row_bytes(int64_t pages) { return select_width(pages) * 12 + select_width(pages) / 4; }
+// The choice's workspace for some rows of every request: keys for where a row needs them all, scores,
+// their errors, and, of more than sixteen rows, the operands.
+struct SelectSpace {
+  int64_t width, scores, errors, operands, lasts, bytes;   // pages, rounded up; offsets
+};
+SelectSpace select_space(int64_t batch, int64_t rows, int64_t Hkv, int64_t D, int64_t pages) {
+  SelectSpace s;
+  s.width = (pages + 15) / 16 * 16;
+  const int64_t cells = batch * Hkv * rows * s.width, tiles = rows > 16 ? (rows + 15) / 16 : 0;
+  s.scores = cells * 8;
+  s.errors = s.scores + cells * 4;
+  s.operands = (s.errors + cells / 4 + 255) / 256 * 256;
+  s.lasts = s.operands + batch * Hkv * tiles * D * 128;
+  s.bytes = s.lasts + batch * tiles * 4;
+  return s;
+}
 
-// Rows of a request whose scores are in the workspace at a time (256 MiB).
-int64_t select_rows(int64_t batch, int64_t tokens, int64_t Hkv, int64_t pages) {
-  const int64_t per_row = batch * Hkv * select_row_bytes(pages);
-  int64_t r = per_row > 0 ? ((int64_t)256 << 20) / per_row : tokens;
-  r = r / 16 * 16;
+// Rows of a request whose scores are in the workspace at a time: sixteen, or what 256 MiB hold.
+int64_t select_rows(int64_t batch, int64_t tokens, int64_t Hkv, int64_t D, int64_t pages) {
+  const int64_t sixteen = select_space(batch, 32, Hkv, D, pages).bytes / 2;
+  int64_t r = sixteen > 0 ? ((int64_t)256 << 20) / sixteen * 16 : tokens;
   if (r < 16) r = 16;
   return r < tokens ? r : tokens;
 }
 
-template <int D>
-auto score_of(int pt, int rt) {
-  return rt == 2 ? score_kernel<D, 2, 2> : pt == 2 ? score_kernel<D, 2, 1> : score_kernel<D, 1, 1>;
-}
-auto score_form(int64_t D, int pt, int rt) {
-  return D == 64 ? score_of<64>(pt, rt) : D == 128 ? score_of<128>(pt, rt) : score_of<256>(pt, rt);
+auto score_form(int64_t D, bool two) {
+  return D == 64    ? two ? score_kernel<64, 2> : score_kernel<64, 1>
+         : D == 128 ? two ? score_kernel<128, 2> : score_kernel<128, 1>
+                    : two ? score_kernel<256, 2> : score_kernel<256, 1>;
 }
 template <int D>
 auto pick_of(int64_t width) {
@@ -1642,8 +1798,8 @@ SV_API int64_t snowverify_page_select_scratch_bytes(int64_t batch, int64_t token
   if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
       table_stride > MAX_WIDTH)
     return 0;
-  return batch * select_rows(batch, tokens, num_kv_heads, table_stride) * num_kv_heads *
-         select_row_bytes(table_stride);
+  const int64_t rows = select_rows(batch, tokens, num_kv_heads, head_size, table_stride);
+  return select_space(batch, rows, num_kv_heads, head_size, table_stride).bytes;
 }
 
 SV_API int snowverify_page_select(const void* q, const void* bounds, const int32_t* table,
@@ -1662,8 +1818,9 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
                                                            head_size, table_stride) ||
       (table_stride > 0 && !scratch))
     return SV_EINVAL;
-  const int64_t chunk = select_rows(batch, tokens, num_kv_heads, table_stride);
-  const int64_t width = select_width(table_stride);
+  const int64_t chunk = select_rows(batch, tokens, num_kv_heads, head_size, table_stride);
+  const SelectSpace space = select_space(batch, chunk, num_kv_heads, head_size, table_stride);
+  const int64_t width = space.width;
   const int threads = width <= 256 * PICK_KEYS ? 256 : 1024;
   if (!grid_ok(batch * num_kv_heads * chunk, threads)) return SV_EINVAL;
   SelectArgs a{};
@@ -1672,10 +1829,12 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
   a.table = table;
   a.positions = positions;
   a.pages = pages;
-  const int64_t cells = batch * num_kv_heads * chunk * width;
-  a.exact = (uint64_t*)scratch;
-  a.scores = (float*)(a.exact + cells);
-  a.errors = a.scores + cells;
+  uint8_t* base = (uint8_t*)scratch;
+  a.exact = (uint64_t*)base;
+  a.scores = (float*)(base + space.scores);
+  a.errors = (float*)(base + space.errors);
+  a.operands = (u32x4*)(base + space.operands);
+  a.tile_last = (int32_t*)(base + space.lasts);
   a.table_stride = table_stride;
   a.blocks = blocks;
   a.width = width;
@@ -1692,18 +1851,31 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
     a.row0 = r0;
     a.rows = (int)(tokens - r0 < chunk ? tokens - r0 : chunk);
     if (table_stride > budget) {   // otherwise every page of every row is taken
-      const int rt = a.rows > 16 ? 2 : 1;
-      const int64_t groups = batch * num_kv_heads * ((a.rows + 16 * rt - 1) / (16 * rt));
-      // workgroups: two a CU, one where the sums over the rows' heads would take longer than the
-      // pages they are for
-      const int64_t wgs = a.rows > 4 && rt == 1 ? 256 : 512;
-      const int pt = rt == 2 || table_stride * groups >= 128 * wgs ? 2 : 1;
-      const int64_t step = 16 * pt * SCORE_WAVES;
-      int64_t per = (table_stride * groups + wgs * step - 1) / (wgs * step) * step;
-      per = per > 4096 ? 4096 : per;
-      hipLaunchKernelGGL(score_form(head_size, pt, rt),
-                         dim3((unsigned)groups, (unsigned)((table_stride + per - 1) / per)),
-                         dim3(64 * SCORE_WAVES), 0, S(stream), a, (uint32_t)per);
+      const int64_t groups = batch * num_kv_heads, tiles = (a.rows + 15) / 16;
+      if (tiles > 1) {
+        auto prepare = head_size == 64 ? operand_kernel<64> : head_size == 128 ? operand_kernel<128> : operand_kernel<256>;
+        hipLaunchKernelGGL(prepare, dim3((unsigned)(groups * tiles)), dim3(64 * SCORE_WAVES), 0, S(stream), a);
+        SV_CHECK_LAUNCH();
+        // two workgroups a CU (what LDS holds of a 256-wide head), at most 64 row tiles each
+        const int64_t columns = (table_stride + 32 * SCORE_WAVES - 1) / (32 * SCORE_WAVES);
+        int64_t per = tiles * groups * columns / 512;
+        per = per < 1 ? 1 : per > 64 ? 64 : per;
+        const int64_t parts = (tiles + per - 1) / per;
+        if (groups * parts > 65535) return SV_EINVAL;
+        auto score = head_size == 64 ? score_rows_kernel<64> : head_size == 128 ? score_rows_kernel<128> : score_rows_kernel<256>;
+        hipLaunchKernelGGL(score, dim3((unsigned)columns, (unsigned)(groups * parts)), dim3(64 * SCORE_WAVES),
+                           0, S(stream), a, (uint32_t)per);
+      } else {
+        // workgroups: two a CU, one where the sums over the rows' heads would take longer than the
+        // pages they are for
+        const int64_t wgs = a.rows > 4 ? 256 : 512;
+        const int pt = table_stride * groups >= 128 * wgs ? 2 : 1;
+        const int64_t step = 16 * pt * SCORE_WAVES;
+        int64_t per = (table_stride * groups + wgs * step - 1) / (wgs * step) * step;
+        per = per > 4096 ? 4096 : per;
+        hipLaunchKernelGGL(score_form(head_size, pt == 2), dim3((unsigned)groups, (unsigned)((table_stride + per - 1) / per)),
+                           dim3(64 * SCORE_WAVES), 0, S(stream), a, (uint32_t)per);
+      }
       SV_CHECK_LAUNCH();
     }
     hipLaunchKernelGGL(pick, dim3((unsigned)(batch * num_kv_heads * a.rows)), dim3(threads), lds,
