@@ -25,6 +25,8 @@ the experts' gate/up in Q4_K, Q5_K or Q6_K and their down in the same format or 
 experts' formats. Formats may change from layer to layer.
 Anything else raises SnowLLMError naming the tensor; nothing falls back to another path.
 """
+from dataclasses import replace
+
 import torch
 
 from . import layers as Lops
@@ -351,15 +353,17 @@ def save_gguf(path, cfg: VerifyConfig, tensors, *, parts: int = 1):
 
 
 def load_gguf(path, *, context: int, block: int, tree_parents=(), kv_std: float = 1.0,
-              seed: int = 0, name: str = None) -> VerifyModel:
+              seed: int = 0, name: str = None, sparse_pages: int = 0) -> VerifyModel:
     """A VerifyModel whose weights come from the GGUF checkpoint at `path` (one file or the
     first part of a split one). The KV cache is random (kv_std, seed) and holds `context` prior
-    tokens; `block` rows are verified per step. Installs the checkpoint's geometry (the repack
+    tokens; `block` rows are verified per step, over selected pages of the context where
+    sparse_pages says how many. Installs the checkpoint's geometry (the repack
     entry points read their shapes from it) and leaves it active."""
     g = GGUF(path)
     try:
         cfg = config_from_gguf(g, context=context, block=block, tree_parents=tree_parents,
                                name=name)
+        cfg = replace(cfg, sparse_pages=sparse_pages)
         ops.define_geometry(**geometry_fields(cfg))
 
         def install(model: VerifyModel):

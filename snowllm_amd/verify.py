@@ -12,6 +12,10 @@ qwen3_5.py:32-78, layers.py:75-228) and its verify drivers (snowllm/engine/spec_
 263-309, 527-581). Every launch goes to torch's current stream and nothing allocates or
 synchronises inside step(), so the step can be captured in one HIP graph.
 
+With VerifyConfig.sparse_pages the attention is the one over selected pages (snowllm_amd.sparse):
+the cache write keeps the bounds of each page's keys, every row chooses the pages it reads, and
+only those are read, however long the context.
+
 Weights are either random-initialised on the GPU from seeded generators, in the formats of
 the BASELINE configs (Q4_K/Q8_0 GGUF blocks repacked with snowllm_gemm_kquant_shuffle_b, fp16
 embedding and LM head, bf16 router and norms), or read from a GGUF checkpoint
@@ -59,6 +63,11 @@ class VerifyConfig:
     page: int = 16
     qk_norm: bool = True
     centered: bool = True    # zero-mean Q4_K model weights (gguf_random); False: config 2's
+    # attention over selected pages: pages that each row reads per kv head (0: the whole context),
+    # of which the first sparse_sink and the last sparse_recent always
+    sparse_pages: int = 0
+    sparse_sink: int = 1
+    sparse_recent: int = 2
 
     @property
     def moe(self):
@@ -233,6 +242,14 @@ class VerifyModel:
         MAX_STEP_ROWS."""
         if batch < 1 or batch * cfg.block > MAX_STEP_ROWS:
             raise SnowLLMError(f"a verify step holds at most {MAX_STEP_ROWS} rows")
+        if cfg.sparse_pages:
+            if cfg.tree_parents:
+                raise SnowLLMError("attention over selected pages takes chains, not trees: a row "
+                                   "sees every key up to its position")
+            if (cfg.sparse_sink < 0 or cfg.sparse_recent < 1
+                    or cfg.sparse_sink + cfg.sparse_recent > cfg.sparse_pages):
+                raise SnowLLMError(f"sparse_pages {cfg.sparse_pages} does not hold the first "
+                                   f"{cfg.sparse_sink} and the last {cfg.sparse_recent} (at least 1)")
         self.batch = batch
         self.cfg = c = cfg
         self.keep_raw = keep_raw
@@ -280,6 +297,14 @@ class VerifyModel:
         perm = torch.randperm(self.blocks, device=dev, generator=kvg)[:batch * self.pages]
         self.table = perm.int().view(batch, -1).contiguous()
         self._alloc_step_buffers()
+        if c.sparse_pages:
+            # the prior tokens' pages come from elsewhere: their bounds, once
+            self.bounds = [torch.zeros(self.blocks, c.kv_heads, 2, c.head_dim, dtype=torch.bfloat16,
+                                       device=dev) for _ in range(c.layers)]
+            whole = torch.full((batch,), self.pages * c.page, dtype=torch.int32, device=dev)
+            for k, bounds in zip(self.k_pools, self.bounds):
+                ops.page_bounds(k, bounds, self.table, torch.zeros_like(whole), whole,
+                                self.pages * c.page)
 
     def _random_weights(self, seed, keep_raw):
         c, dev = self.cfg, "cuda"
@@ -368,6 +393,16 @@ class VerifyModel:
             ops.paged_attention_explicit_scratch_bytes(B, c.block, c.heads, c.kv_heads,
                                                        c.head_dim),
             dtype=torch.uint8, device=dev)
+        if c.sparse_pages:
+            i32 = dict(dtype=torch.int32, device=dev)
+            self.starts, self.counts = torch.zeros(B, **i32), torch.full((B,), c.block, **i32)
+            self.row_positions = torch.zeros(T, **i32)       # -1: a padding row
+            self.row_pages = torch.empty(T, c.kv_heads, c.sparse_pages, **i32)
+            shape = (B, c.block, c.heads, c.kv_heads, c.head_dim)
+            self.select_scratch = ops.empty_bytes(
+                ops.page_select_scratch_bytes(*shape, self.pages))
+            self.attn_scratch = ops.empty_bytes(
+                max(16, ops.sparse_attention_scratch_bytes(*shape, c.sparse_pages)))
         self.ws_tile = ops.gemm_kquant_a_ws_bytes(16, H)   # one 16-row tile of ws_h / ws_h2
         if c.moe:
             E, F, K = c.experts, c.expert_ffn, c.topk
@@ -430,6 +465,13 @@ class VerifyModel:
         self.slots.copy_(torch.tensor(slots, dtype=torch.int32, device=dev))
         self.lens.copy_(torch.tensor([x + T for x in contexts], dtype=torch.int32, device=dev))
         self.lengths = lengths
+        if c.sparse_pages:
+            self.starts.copy_(torch.tensor(contexts, dtype=torch.int32, device=dev))
+            self.counts.copy_(torch.tensor(lengths, dtype=torch.int32, device=dev))
+            self.row_positions.copy_(torch.tensor(
+                [x + t if t < n else -1 for x, n in zip(contexts, lengths) for t in range(T)],
+                dtype=torch.int32, device=dev))
+            return   # positions say what a row sees: no masks
         if not c.tree_parents:
             if all(n == T for n in lengths):
                 self.tree = None
@@ -480,7 +522,9 @@ class VerifyModel:
                                            self.proj, T, nqk, H, self.ws_h, col=0)
                 ops.gemm_kquant_a_prepared(lw.v_fmt, lw.v[0], lw.v[1], self.proj, T,
                                            c.qkv_n - nqk, H, self.ws_h, col=nqk)
-            if c.rot_half <= ops.FUSED_QK_MAX_HALF:
+            if c.sparse_pages:
+                self._sparse_attention(i, lw)
+            elif c.rot_half <= ops.FUSED_QK_MAX_HALF:
                 # QK-norm + RoPE + the block's K/V cache write inside the attention's launches
                 # with 256-wide heads the merge also writes the O projection's operands
                 ws_o = self.ws_a if c.head_dim == 256 else None
@@ -497,7 +541,7 @@ class VerifyModel:
                 ops.paged_attention_explicit(self.q, self.k_pools[i], self.v_pools[i], self.attn,
                                              self.table, self.lens, c.head_dim ** -0.5,
                                              self.attn_scratch, tree=self.tree)
-            if c.rot_half <= ops.FUSED_QK_MAX_HALF and c.head_dim == 256:
+            if not c.sparse_pages and c.rot_half <= ops.FUSED_QK_MAX_HALF and c.head_dim == 256:
                 ops.gemm_kquant_a_prepared(lw.o_fmt or c.attn_fmt, lw.o[0], lw.o[1], self.o, T,
                                            H, c.heads * c.head_dim, self.ws_a)
             else:
@@ -567,6 +611,23 @@ class VerifyModel:
                 Lops.dense_gemv(Lops.WT_F16, self.lm_head, self.ws_f, self.logits, T, c.vocab, H)
         self.final_residual = res_out
         return self.logits
+
+    def _sparse_attention(self, i, lw):
+        """Layer i's cache write with the bounds of its pages, the rows' choice of pages, and the
+        attention over them: self.proj -> self.attn."""
+        c = self.cfg
+        nq, nk = c.heads * c.head_dim, c.kv_heads * c.head_dim
+        q = self.proj[:, :nq].unflatten(1, (c.heads, c.head_dim))
+        k = self.proj[:, nq:nq + nk].unflatten(1, (c.kv_heads, c.head_dim))
+        v = self.proj[:, nq + nk:].unflatten(1, (c.kv_heads, c.head_dim))
+        ops.kv_append(k, v, self.cos, self.sin, self.k_pools[i], self.v_pools[i], self.table,
+                      self.starts, self.counts, bounds=self.bounds[i], q=q, q_out=self.q,
+                      q_gamma=lw.q_norm, k_gamma=lw.k_norm, eps=c.eps)
+        ops.page_select(self.q, self.bounds[i], self.table, self.row_positions, self.row_pages,
+                        self.select_scratch, sink=c.sparse_sink, recent=c.sparse_recent)
+        ops.sparse_attention(self.q, self.k_pools[i], self.v_pools[i], self.attn, self.table,
+                             self.row_positions, self.row_pages, c.head_dim ** -0.5,
+                             self.attn_scratch)
 
     def _ws_rows(self, ws, r0):
         """The operand-workspace view whose first tile is rows r0.. (r0 a multiple of 16 or
