@@ -114,6 +114,8 @@ struct AppendArgs {
   int64_t page_wgs;        // workgroups over (request, page, kv head); the rest rotate queries
 };
 
+constexpr int Q_HEADS = 4;   // heads of a row that a thread rotates: their loads are in flight at once
+
 // Eight elements d = 8 c .. 8 c + 7 of a head, normalised and rotated; the D / 8 threads of a head
 // are neighbours in one wave. The rotation partner's raw words come from its thread.
 template <int D>
@@ -180,18 +182,26 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t vs[PAGE * LD];
   const int tid = threadIdx.x, r = tid / W, c = tid % W;
   int64_t wg = blockIdx.x;
-  if (wg >= a.page_wgs) {   // queries: sixteen (row, head) units
-    const int64_t u = (wg - a.page_wgs) * 16 + r;
-    const int64_t m = u / a.Hq;
-    const int head = (int)(u % a.Hq);
-    const int64_t b = m / a.T;
-    const bool live = b < a.batch && m % a.T < a.counts[b] && a.starts[b] >= 0;
+  if (wg >= a.page_wgs) {   // queries: sixteen units of a row and Q_HEADS heads
+    const uint32_t u = (uint32_t)(wg - a.page_wgs) * 16 + r, groups = (uint32_t)(a.Hq + Q_HEADS - 1) / Q_HEADS;
+    const uint32_t m = u / groups;
+    const int head = (int)(u % groups) * Q_HEADS;
+    const uint32_t b = m / (uint32_t)a.T;
+    const bool live = b < (uint32_t)a.batch && (int)(m % (uint32_t)a.T) < a.counts[b] && a.starts[b] >= 0;
     const int64_t mr = live ? m : 0;
-    u32x4 raw = {0u, 0u, 0u, 0u};
-    if (live) raw = *(const u32x4*)(a.q + mr * a.q_stride + (int64_t)head * D + 8 * c);
-    const u32x4 o = rotate_norm<D>(raw, c, a.q_gamma, a.eps, a.cosv + mr * a.cs_stride,
-                                   a.sinv + mr * a.cs_stride, a.half);
-    if (live) *(u32x4*)(a.q_out + (m * a.Hq + head) * D + 8 * c) = o;
+    const int heads = live ? a.Hq - head < Q_HEADS ? a.Hq - head : Q_HEADS : 0;
+    u32x4 raw[Q_HEADS];
+#pragma unroll
+    for (int i = 0; i < Q_HEADS; ++i) {
+      raw[i] = u32x4{0u, 0u, 0u, 0u};
+      if (i < heads) raw[i] = *(const u32x4*)(a.q + mr * a.q_stride + (int64_t)(head + i) * D + 8 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < Q_HEADS; ++i) {
+      const u32x4 o = rotate_norm<D>(raw[i], c, a.q_gamma, a.eps, a.cosv + mr * a.cs_stride,
+                                     a.sinv + mr * a.cs_stride, a.half);
+      if (i < heads) *(u32x4*)(a.q_out + (mr * a.Hq + head + i) * D + 8 * c) = o;
+    }
     return;
   }
   const int h = (int)(wg % a.Hkv);
@@ -268,17 +278,30 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
 // ---------------------------------------------------------------------------------------
 // bounds
 // ---------------------------------------------------------------------------------------
-// D / 8 threads per (page, kv head), eight elements each, all sixteen tokens in flight at once; a
-// page's dead tokens are read as its last live one.
+// Lane swaps for the bounds: with the lane 2 away, and with one 4 or 6 away (the values of those two
+// are equal by then).
+__device__ __forceinline__ short2v lanes_xor2(short2v v) {
+  return __builtin_bit_cast(short2v, dpp_u32<DPP_QUAD_XOR2>(__builtin_bit_cast(uint32_t, v)));
+}
+__device__ __forceinline__ short2v lanes_xor4(short2v v) {
+  return __builtin_bit_cast(short2v, dpp_u32<DPP_QUAD_XOR1>(dpp_u32<DPP_HALF_MIRROR>(__builtin_bit_cast(uint32_t, v))));
+}
+
+// A half wave takes 64 elements of a (page, kv head), that is four chunks of [16 tokens][16], in four
+// loads that are whole 128-byte lines: lane (chunk, token % 4, half chunk). A lane's four tokens meet in
+// its registers, the four lanes of an element by lane swaps. A page's dead tokens are read as its last
+// live one. Bound by the read of K: WIDE_BOUNDS.
 template <int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(
     const uint16_t* __restrict__ k_pool, uint16_t* __restrict__ bounds,
     const int32_t* __restrict__ table, const int32_t* __restrict__ starts,
     const int32_t* __restrict__ counts, int64_t table_stride, int64_t blocks, int batch, int Hkv,
     int tokens, int64_t pages) {
-  constexpr int W = D / 8;
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / W;
-  const int c = threadIdx.x % W;
+  constexpr int SLABS = D / 64;
+  int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32;
+  const int lane = threadIdx.x & 31, half = lane & 1, quarter = lane >> 1 & 3, chunk = lane >> 3;
+  const int slab = (int)(unit % SLABS);
+  unit /= SLABS;
   const int h = (int)(unit % Hkv);
   const int64_t j = unit / Hkv % pages, b = unit / Hkv / pages;
   if (b >= batch) return;
@@ -291,28 +314,35 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(
   const int blk = page_block(table, table_stride, (int)b, page, blocks);
   if (blk < 0) return;
   const int last = left < PAGE ? (int)left - 1 : PAGE - 1;
-  const uint16_t* kp = k_pool + ((int64_t)blk * Hkv + h) * PAGE * D + (c / 2) * 256 + (c % 2) * 8;
-  u32x4 x[PAGE];
+  const uint16_t* kp = k_pool + ((int64_t)blk * Hkv + h) * PAGE * D + (slab * 4 + chunk) * 256 + half * 8;
+  u32x4 x[4];
 #pragma unroll
-  for (int t = 0; t < PAGE; ++t) x[t] = *(const u32x4*)(kp + (t < last ? t : last) * 16);
+  for (int i = 0; i < 4; ++i) {
+    const int t = 4 * i + quarter;
+    x[i] = *(const u32x4*)(kp + (t < last ? t : last) * 16);
+  }
   u32x4 wl, wu;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     short2v l = order_keys(x[0][i]), u = l;
 #pragma unroll
-    for (int t = 1; t < PAGE; ++t) {
+    for (int t = 1; t < 4; ++t) {
       const short2v k = order_keys(x[t][i]);
       l = min2(l, k);
       u = max2(u, k);
     }
+    l = min2(l, lanes_xor2(l));
+    u = max2(u, lanes_xor2(u));
+    l = min2(l, lanes_xor4(l));
+    u = max2(u, lanes_xor4(u));
     uint32_t a0, b0;
     bounds_words(l, u, a0, b0);
     wl[i] = a0;
     wu[i] = b0;
   }
-  uint16_t* bp = bounds + ((int64_t)blk * Hkv + h) * 2 * D + 8 * c;
-  *(u32x4*)bp = wl;
-  *(u32x4*)(bp + D) = wu;
+  uint16_t* bp = bounds + ((int64_t)blk * Hkv + h) * 2 * D + slab * 64 + chunk * 16 + half * 8;
+  if (quarter == 0) *(u32x4*)bp = wl;
+  if (quarter == 1) *(u32x4*)(bp + D) = wu;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1595,9 +1625,11 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const float* __restric
   const float* ml = part_ml + row * splits * 2;
   const float* po = part_o + row * splits * D + d;
   float top = -__builtin_huge_valf();
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[2 * s]);
   float sum = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
     const float c = ml[2 * s] == top ? 1.f : __builtin_amdgcn_exp2f(ml[2 * s] - top);
     sum = __builtin_fmaf(ml[2 * s + 1], c, sum);
@@ -1760,7 +1792,8 @@ SV_API int snowverify_kv_append(const void* k, int64_t k_stride, const void* v, 
   a.half = (int)half;
   a.pages = (int)((tokens + PAGE - 2) / PAGE + 1);
   a.page_wgs = batch * a.pages * num_kv_heads;
-  const int64_t grid = a.page_wgs + (q ? (batch * tokens * num_heads + 15) / 16 : 0);
+  const int64_t groups = (num_heads + Q_HEADS - 1) / Q_HEADS;
+  const int64_t grid = a.page_wgs + (q ? (batch * tokens * groups + 15) / 16 : 0);
   if (!grid_ok(grid, 2 * head_size)) return SV_EINVAL;
   auto kern = head_size == 64 ? append_kernel<64> : head_size == 128 ? append_kernel<128> : append_kernel<256>;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3((unsigned)(2 * head_size)), 0, S(stream), a);
@@ -1780,9 +1813,9 @@ SV_API int snowverify_page_bounds(const void* k_pool, void* bounds, const int32_
   if ((blocks && (!k_pool || !bounds)) || (table_stride && !table) || !starts || !counts)
     return SV_EINVAL;
   const int64_t pages = (tokens + PAGE - 2) / PAGE + 1;
-  const int64_t per_wg = 256 / (head_size / 8);
+  const int64_t per_wg = 8;   // 64 elements of a page and head each
   if (pages > ((int64_t)1 << 40) / num_kv_heads / batch) return SV_EINVAL;
-  const int64_t grid = (batch * pages * num_kv_heads + per_wg - 1) / per_wg;
+  const int64_t grid = (batch * pages * num_kv_heads * (head_size / 64) + per_wg - 1) / per_wg;
   if (!grid_ok(grid, 256)) return SV_EINVAL;
   auto kern = head_size == 64 ? page_bounds_kernel<64> : head_size == 128 ? page_bounds_kernel<128> : page_bounds_kernel<256>;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), 0, S(stream), (const uint16_t*)k_pool,
