@@ -360,13 +360,14 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(
 //
 // E: with A = sum_d |P_d high_d| + |N_d low_d|,
 //   P and N are 32-bit sums of G values                               <= G 2^-24 A
-//   each is multiplied as two bf16 pieces, what is left is            <= 2^-18 A
-//   2 . 2 D / 32 <= 32 matrix instructions add to one accumulator, each with at most 16 roundings
-//   of 2^-24 of what has been summed                                  <= 2^-15 A
-// so E = (2^-14 + G 2^-24) A, A from a third product of the larger pieces with |bounds| (2^-8 too
-// small at most: 1.01 A). What the matrix cores could flush (below 2^-126) adds at most 2^-74: a row
-// has E = infinity, and all its pages summed in 64 bits, where a P or |N| is below 2^-90 (and not 0)
-// or above 2^40, or anything is not finite.
+//   each is multiplied as two bf16 pieces, what is left is            <= 2^-16 A
+//   2 . 2 D / 32 matrix instructions add to one accumulator, each taken to make at most 16 roundings
+//   of 2^-24 of what has been summed                                  <= 2 D 2^-24 A
+// (over normal, positive, rising and heavy-tailed operands of 64- to 256-wide heads the whole error came
+// to 2^-17.7 A at most, nearly all of it the second), A from a third product of the larger pieces with
+// |bounds| (2^-8 too small at most: 1.01 A). What the matrix cores could flush (below 2^-126) adds at
+// most 2^-74: a row has E = infinity, and all its pages summed in 64 bits, where a P or |N| is below
+// 2^-90 (and not 0) or above 2^40, or anything is not finite.
 struct SelectArgs {
   const uint16_t* q;        // [rows, Hq, D]
   const uint16_t* bounds;
@@ -489,9 +490,10 @@ __device__ __forceinline__ void score_step(bool minima, const u32x4* x, u32x4 hi
 // E of a tile of sixteen pages from page pt (lane (row col, g): pages pt + 4 g + k), whose first
 // `sink`, always chosen, and those from `last` on do not count; what is no page (bits of none) scores
 // -inf.
+template <int D>
 __device__ __forceinline__ float tile_error(const SelectArgs& a, int64_t pt, int64_t last, uint32_t none, int g,
                                             floatx4& acc, floatx4 mag) {
-  const float rel = 1.01f * (0x1p-14f + (float)a.G * 0x1p-24f), inf = __builtin_huge_valf();
+  const float rel = 1.01f * (0x1p-16f + (float)(2 * D + a.G) * 0x1p-24f), inf = __builtin_huge_valf();
   float e = 0.f;
   if (none == 0 && pt >= a.sink && pt + 16 <= last) {
     const float sum = (mag[0] + mag[1]) + (mag[2] + mag[3]);   // infinite or NaN where one of them is
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_kernel(SelectArgs a
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int64_t pt = p + 16 * i;
-      const float e = tile_error(a, pt, last, none[i], g, acc[i], mag[i]);
+      const float e = tile_error<D>(a, pt, last, none[i], g, acc[i], mag[i]);
       if (col < live && pt < p1) {
         *(floatx4*)(a.scores + item * a.width + pt + 4 * g) = acc[i];
         if (g == 0) a.errors[item * (a.width / 16) + pt / 16] = e;
@@ -692,7 +694,7 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_rows_kernel(SelectA
       score_step<PT>(s < NS / 2, &t.x[0][s], w[s % 3][0], w[s % 3][1], acc, mag, NS);
     }
 #pragma unroll
-    for (int i = 0; i < PT; ++i) err[i] = tile_error(a, p + 16 * i, done_last, none[i], g, acc[i], mag[i]);
+    for (int i = 0; i < PT; ++i) err[i] = tile_error<D>(a, p + 16 * i, done_last, none[i], g, acc[i], mag[i]);
   }
   store(t1 - 1);
 }
@@ -1370,6 +1372,7 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
 // page of another row would reach it as NaN: rows whose result is not finite are computed again alone,
 // as are those of a workgroup with a list in which a page stands twice.
 constexpr int ROWS_MAX = 16, ROWS_GROUPS = 4, ROWS_WAVES = 8;
+constexpr int ROWS_ENTRIES = 4;               // of the rows' lists, that a thread holds
 constexpr int ROWS_LDS = 160 * 1024 - 2048;   // dynamic LDS at most
 
 // LDS image of one (page, kv head): K, then V, as they are in memory (a lane's 16 bytes of either
@@ -1420,38 +1423,40 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
   __syncthreads();
   int low = 0x7fffffff;
   for (int r = 0; r < live; ++r) low = spos[r] >= 0 && spos[r] < low ? spos[r] : low;
-  // entry e of the lists: its page, or -1
-  auto entry = [&](int e, int& r) {
-    r = e / K;
-    const int p = lists[r * list_step + e % K];
-    return p >= 0 && spos[r] >= 0 && p <= spos[r] / PAGE && p < a.table_stride ? p : -1;
-  };
   auto whole = [&](int p) { return p * PAGE + PAGE - 1 <= low; };
-  for (int e = tid; e < entries; e += NT) {
-    int r;
-    const int p = entry(e, r);
-    if (p >= 0) page_rows[p >> 1] = 0;
+  // this thread's entries of the lists: pages, or -1
+  int page[ROWS_ENTRIES], from[ROWS_ENTRIES];
+#pragma unroll
+  for (int i = 0; i < ROWS_ENTRIES; ++i) {
+    const int e = i * NT + tid, r = e < entries ? e / K : 0;
+    from[i] = r;
+    page[i] = e < entries ? lists[r * list_step + e % K] : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS_ENTRIES; ++i) {
+    const int p = page[i], seen = spos[from[i]];
+    if (!(p >= 0 && seen >= 0 && p <= seen / PAGE && p < a.table_stride)) page[i] = -1;
+    if (page[i] >= 0) page_rows[p >> 1] = 0;
   }
   __syncthreads();
-  for (int e = tid; e < entries; e += NT) {
-    int r;
-    const int p = entry(e, r);
-    if (p >= 0) {
-      const uint32_t bit = 1u << (r + (p & 1) * 16);
-      if (atomicOr(&page_rows[p >> 1], bit) & bit) twice = 1;
+#pragma unroll
+  for (int i = 0; i < ROWS_ENTRIES; ++i)
+    if (page[i] >= 0) {
+      const uint32_t bit = 1u << (from[i] + (page[i] & 1) * 16);
+      if (atomicOr(&page_rows[page[i] >> 1], bit) & bit) twice = 1;
     }
-  }
   __syncthreads();
   const bool merge = twice == 0;
-  uint32_t total = 0, bad = 0;
-  if (merge)
-    for (int e0 = 0; e0 < entries; e0 += NT) {
-      int r = 0, blk = -1, p = -1;
+  uint32_t total = 0;
+  if (merge) {
+#pragma unroll
+    for (int i = 0; i < ROWS_ENTRIES; ++i) {
+      if (i * NT >= entries) break;
+      int blk = -1;
       uint32_t rows = 0;
-      if (e0 + tid < entries) p = entry(e0 + tid, r);
-      if (p >= 0) {
-        rows = whole(p) ? page_rows[p >> 1] >> (p & 1) * 16 & 0xffffu : 1u << r;
-        if (__builtin_ctz(rows) == r) blk = page_block(a.table, a.table_stride, b, p, a.blocks);
+      if (page[i] >= 0) {
+        rows = whole(page[i]) ? page_rows[page[i] >> 1] >> (page[i] & 1) * 16 & 0xffffu : 1u << from[i];
+        if (__builtin_ctz(rows) == from[i]) blk = page_block(a.table, a.table_stride, b, page[i], a.blocks);
       }
       const uint64_t have = __ballot(blk >= 0);
       if (lane == 0) counts[wave] = (uint32_t)__popcll(have);
@@ -1461,11 +1466,10 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
         if (w < wave) at += counts[w];
         total += counts[w];
       }
-      if (blk >= 0) {
-        merged[at] = uint2{(uint32_t)blk, (uint32_t)p << 16 | rows};
-      }
+      if (blk >= 0) merged[at] = uint2{(uint32_t)blk, (uint32_t)page[i] << 16 | rows};
       __syncthreads();
     }
+  }
 
   floatx4 acc[D / 16];
 #pragma unroll
@@ -1692,7 +1696,9 @@ int attend_rows_per_wave(int64_t batch, int64_t tokens, int64_t Hkv, int64_t G, 
   const int64_t most = ROWS_MAX / ROWS_GROUPS;
   int64_t rpt = 16 / G < most ? 16 / G : most;
   const int64_t room = ROWS_LDS - rows_ring_bytes(D, pages);
-  while (rpt > 0 && ROWS_GROUPS * rpt * budget * 8 > room) --rpt;
+  while (rpt > 0 && (ROWS_GROUPS * rpt * budget * 8 > room ||
+                     ROWS_GROUPS * rpt * budget > 64 * ROWS_WAVES * ROWS_ENTRIES))
+    --rpt;
   if (rpt < 1 || tokens <= rpt || pages > 65536) return 0;
   const int64_t R = ROWS_GROUPS * rpt;
   return batch * Hkv * ((tokens + R - 1) / R) >= 128 ? (int)rpt : 0;
