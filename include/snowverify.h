@@ -300,14 +300,14 @@ int snowverify_attention_row_groups(int groups);
  * entry outside 0 .. blocks - 1, and a page past table_stride, is no page: it is not written,
  * not read, and scores lowest. bounds bf16 [blocks, num_kv_heads, 2, head_size]: the element-wise
  * minimum and maximum of a page's keys, NaN where a key's element is NaN. Nothing here keeps
- * library-owned scratch: calls on different streams need different scratch and no more. */
+ * library-owned scratch: calls on different streams need different scratch and no more. bf16
+ * tensors and scratch 16-byte aligned. */
 
 /* The cache write of counts[b] rows of request b at positions starts[b], starts[b] + 1, ..: K per
  * head normalised (k_gamma [head_size] bf16: RMSNorm with eps; NULL: not), its first 2 * half
  * elements rotated in the pairs (i, i + half) by cos/sin [row, half] f32 (rows cs_stride apart),
  * rounded once; V as it is. Row t of request b is row m = b * tokens + t: K head h at k + m *
- * k_stride + h * head_size, V and q alike (strides in elements, multiples of 8; pointers 16-byte
- * aligned). bounds (NULL: none kept): those of every page written, over its keys up to the last
+ * k_stride + h * head_size, V and q alike (strides in elements, multiples of 8). bounds (NULL: none kept): those of every page written, over its keys up to the last
  * one written, whatever the page holds behind it. q (NULL: none): the same norm (q_gamma) and
  * rotation into q_out [batch*tokens, num_heads, head_size]. counts above `tokens` count as
  * tokens; a request with a count or start below 0 has no rows; rows past a request's count, in

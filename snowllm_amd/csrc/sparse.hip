@@ -19,7 +19,6 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef double doublex4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short short2v __attribute__((ext_vector_type(2)));
 
@@ -632,12 +631,12 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_rows_kernel(SelectA
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
   const int tiles = (a.rows + 15) / 16;
   const uint32_t parts = ((uint32_t)tiles + tiles_per_wg - 1) / tiles_per_wg;
-  uint32_t y = blockIdx.y;
+  uint32_t y = blockIdx.x;
   const int t0 = (int)(y % parts * tiles_per_wg);
   y /= parts;
   const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
   const int t1 = t0 + (int)tiles_per_wg < tiles ? t0 + (int)tiles_per_wg : tiles;
-  const int64_t p = (int64_t)blockIdx.x * (16 * PT * SCORE_WAVES) + 16 * PT * wave;
+  const int64_t p = (int64_t)blockIdx.y * (16 * PT * SCORE_WAVES) + 16 * PT * wave;
   const u32x4* src = a.operands + ((int64_t)b * a.Hkv + h) * tiles * TILE + lane;
   auto load = [&](int t) {
 #pragma unroll
@@ -1900,9 +1899,8 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
         int64_t per = tiles * groups * columns / 512;
         per = per < 1 ? 1 : per > 64 ? 64 : per;
         const int64_t parts = (tiles + per - 1) / per;
-        if (groups * parts > 65535) return SV_EINVAL;
         auto score = head_size == 64 ? score_rows_kernel<64> : head_size == 128 ? score_rows_kernel<128> : score_rows_kernel<256>;
-        hipLaunchKernelGGL(score, dim3((unsigned)columns, (unsigned)(groups * parts)), dim3(64 * SCORE_WAVES),
+        hipLaunchKernelGGL(score, dim3((unsigned)(groups * parts), (unsigned)columns), dim3(64 * SCORE_WAVES),
                            0, S(stream), a, (uint32_t)per);
       } else {
         // workgroups: two a CU, one where the sums over the rows' heads would take longer than the

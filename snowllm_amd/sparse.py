@@ -25,11 +25,11 @@ BF16, I32, F32 = torch.bfloat16, torch.int32, torch.float32
 # The checks are most of what a small call costs on the host, so a tensor that passes is looked at
 # once per property; what is wrong is found out afterwards.
 def _need(t, name, dtype, shape, dev):
-    """The address of a contiguous, 16-byte aligned tensor of this dtype, shape and device."""
+    """The address of a contiguous tensor of this dtype, shape and device (bf16: 16-byte aligned)."""
     if t.dtype != dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
         _refuse(t, name, dtype, shape, dev)
     p = t.data_ptr()
-    if p & 15:
+    if p & 15 and dtype is BF16:
         raise SnowLLMError(f"{name}: must be 16-byte aligned")
     return p
 
@@ -242,5 +242,5 @@ def sparse_attention(q, k_pool, v_pool, out, table, positions, pages, scale, scr
     need = sparse_attention_scratch_bytes(batch, tokens, heads, hkv, d, budget)
     scp, scn = _scratch(scratch, need, "sparse attention", dev)
     check(lib.snowverify_sparse_attention(qp, kp, vp, op, tp, at, lp, batch, tokens, heads, hkv, d,
-                                          width, blocks, budget, scale, scp, scn, _stream(dev)),
+                                          width, blocks, budget, float(scale), scp, scn, _stream(dev)),
           "sparse_attention")

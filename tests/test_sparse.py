@@ -77,7 +77,8 @@ def test_checks_of_shapes_and_strides():
     with pytest.raises(Err, match="on cuda:1"):
         sparse._need(Fake((3,), (1,), I32), "x", I32, (3,), 1)
     with pytest.raises(Err, match="16-byte"):
-        sparse._need(Fake((3,), (1,), I32, 4), "x", I32, (3,), 0)
+        sparse._need(Fake((3,), (1,), BF, 8), "x", BF, (3,), 0)
+    assert sparse._need(Fake((3,), (1,), I32, 4), "x", I32, (3,), 0) == 4      # a slice of positions
     with pytest.raises(Err, match="shape"):
         sparse._need(Fake((3,), (1,), I32), "x", I32, (4,), 0)
     with pytest.raises(Err, match="whole number"):
