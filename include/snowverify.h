@@ -307,9 +307,10 @@ int snowverify_attention_row_groups(int groups);
  * head normalised (k_gamma [head_size] bf16: RMSNorm with eps; NULL: not), its first 2 * half
  * elements rotated in the pairs (i, i + half) by cos/sin [row, half] f32 (rows cs_stride apart),
  * rounded once; V as it is. Row t of request b is row m = b * tokens + t: K head h at k + m *
- * k_stride + h * head_size, V and q alike (strides in elements, multiples of 8). bounds (NULL: none kept): those of every page written, over its keys up to the last
- * one written, whatever the page holds behind it. q (NULL: none): the same norm (q_gamma) and
- * rotation into q_out [batch*tokens, num_heads, head_size]. counts above `tokens` count as
+ * k_stride + h * head_size, V and q alike (strides in elements, multiples of 8). bounds (NULL:
+ * none kept): those of every page written, over its keys up to the last one written, whatever the
+ * page holds behind it. q (NULL: none): the same norm (q_gamma) and rotation into q_out
+ * [batch*tokens, num_heads, head_size], which may be q. counts above `tokens` count as
  * tokens; a request with a count or start below 0 has no rows; rows past a request's count, in
  * q_out too, are left as they were. half a multiple of 8, 2 * half <= head_size. Requests that
  * write the same page race. */
@@ -351,7 +352,7 @@ int64_t snowverify_sparse_attention_scratch_bytes(int64_t batch, int64_t tokens,
                                                   int64_t head_size, int64_t budget);
 /* out[m, h] = softmax(scale q k^T) v over the keys at positions <= positions[m] of the pages
  * listed for (m, kv head), a page as often as it is listed; entries that are no page, or lie past
- * the row's position, are passed over. A row that sees no key gets zeros. */
+ * the row's position, are passed over. A row that sees no key gets zeros. out must not overlap q. */
 int snowverify_sparse_attention(const void* q, const void* k_pool, const void* v_pool, void* out,
                                 const int32_t* table, const int32_t* positions,
                                 const int32_t* pages, int64_t batch, int64_t tokens,

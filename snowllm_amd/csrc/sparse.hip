@@ -289,7 +289,8 @@ __device__ __forceinline__ short2v lanes_xor4(short2v v) {
 // A half wave takes 64 elements of a (page, kv head), that is four chunks of [16 tokens][16], in four
 // loads that are whole 128-byte lines: lane (chunk, token % 4, half chunk). A lane's four tokens meet in
 // its registers, the four lanes of an element by lane swaps. A page's dead tokens are read as its last
-// live one. Bound by the read of K: WIDE_BOUNDS.
+// live one. Bound by the read of K: 220K
+// tokens of two 256-wide heads 54 us (4.7 TB/s) from HBM, 36 from the last-level cache.
 template <int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(
     const uint16_t* __restrict__ k_pool, uint16_t* __restrict__ bounds,
@@ -624,19 +625,20 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES) operand_kernel(SelectArgs a)
 // one is used. A tile's scores are stored a step later, so that the one wait of a step is for loads
 // and stores that have had a step's time.
 template <int D>
-__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_rows_kernel(SelectArgs a, uint32_t tiles_per_wg) {
+__global__ void __launch_bounds__(64 * SCORE_WAVES, 2) score_rows_kernel(SelectArgs a, uint32_t tiles_per_wg,
+                                                                       uint32_t columns) {
   typedef __attribute__((address_space(3))) void lds_void;
   constexpr int NS = D / 16, PT = 2, TILE = NS * 2 * 64;   // 16-byte words of a row tile's operands
   __shared__ u32x4 op[2][TILE];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
   const int tiles = (a.rows + 15) / 16;
   const uint32_t parts = ((uint32_t)tiles + tiles_per_wg - 1) / tiles_per_wg;
-  uint32_t y = blockIdx.x;
+  uint32_t y = blockIdx.x / columns;
   const int t0 = (int)(y % parts * tiles_per_wg);
   y /= parts;
   const int h = (int)(y % (uint32_t)a.Hkv), b = (int)(y / (uint32_t)a.Hkv);
   const int t1 = t0 + (int)tiles_per_wg < tiles ? t0 + (int)tiles_per_wg : tiles;
-  const int64_t p = (int64_t)blockIdx.y * (16 * PT * SCORE_WAVES) + 16 * PT * wave;
+  const int64_t p = (int64_t)(blockIdx.x % columns) * (16 * PT * SCORE_WAVES) + 16 * PT * wave;
   const u32x4* src = a.operands + ((int64_t)b * a.Hkv + h) * tiles * TILE + lane;
   auto load = [&](int t) {
 #pragma unroll
@@ -1127,7 +1129,7 @@ struct AttendArgs {
   float* part_ml;           // [rows * Hq, splits, 2]
   int64_t table_stride, blocks, items;
   int T, Hq, Hkv, G, GT, budget, splits;
-  int rpt, ring_bytes;      // attend_rows_kernel: rows of a wave, LDS in front of the union
+  int rpt, ring_bytes, union_most;   // attend_rows_kernel: rows of a wave, LDS in front of the union, its entries
   float qk_scale;           // softmax scale * log2(e)
 };
 
@@ -1178,6 +1180,12 @@ __device__ __forceinline__ void softmax_step(const float (&e)[8], float& m, floa
   }
 }
 
+// The waves' sums meet in LDS: in rounds of D / 2 elements where they would pass 64 KiB; floats.
+__host__ __device__ __forceinline__ int attend_rounds(int D, int heads) { return D == 256 && heads > 8 ? 2 : 1; }
+__host__ __device__ __forceinline__ int attend_lds(int D, int heads) {
+  return ATT_WAVES * heads * (D / attend_rounds(D, heads) + 4);
+}
+
 // One workgroup per (row, kv head, 16 heads of its group, split of the list), one page pair per wave
 // and step. Per pair (32 keys):
 //   S^T[key, head] = K . q^T       v_mfma_f32_16x16x32_bf16 over d, A = K straight from the page
@@ -1185,11 +1193,12 @@ __device__ __forceinline__ void softmax_step(const float (&e)[8], float& m, floa
 //   O^T[d, head]  += V^T . P^T     over the 32 keys, A = V^T (a 16-byte load holds a lane's keys of
 //                                  elements d and d + 1: two operands), B = P^T from S^T's registers
 // so neither K, V nor P passes through LDS.
-template <int D, int NW>
+// By four waves, whose threads are tid; `write`: or the result is dropped.
+template <int D>
 __device__ __forceinline__ void attend_row(const AttendArgs& a, int b, int h, int gt, int t, int split,
-                                           float* so, float (*sml)[16][2]) {
-  constexpr int KS = D / 32;
-  const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, g = lane >> 4;
+                                           int tid, int wave, bool write, float* so, float (*sml)[16][2]) {
+  constexpr int KS = D / 32, NW = ATT_WAVES;
+  const int lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int64_t m = (int64_t)b * a.T + t;
   const int heads = a.G - gt * 16 < 16 ? a.G - gt * 16 : 16;
   const int64_t head0 = (int64_t)h * a.G + gt * 16;
@@ -1295,8 +1304,7 @@ __device__ __forceinline__ void attend_row(const AttendArgs& a, int b, int h, in
 #pragma unroll
   for (int w = 1; w < NW; ++w) top = fmaxf(top, sml[w][col][0]);
   const float c = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - top);
-  // in two rounds of D / 2 elements where the waves' sums would pass 64 KiB of LDS
-  const int rounds = D == 256 && heads > 8 ? 2 : 1, DR = D / rounds, ld = DR + 4;
+  const int rounds = attend_rounds(D, heads), DR = D / rounds, ld = DR + 4;
   for (int rd = 0; rd < rounds; ++rd) {
     if (rd) __syncthreads();
     if (col < heads) {
@@ -1310,7 +1318,7 @@ __device__ __forceinline__ void attend_row(const AttendArgs& a, int b, int h, in
       }
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < heads * (DR / 4); u += 64 * NW) {
+    for (int u = write ? tid : heads * (DR / 4); u < heads * (DR / 4); u += 64 * NW) {
       const int hd = u / (DR / 4), dr = u % (DR / 4) * 4, d = rd * DR + dr;
       float hm = sml[0][hd][0];
 #pragma unroll
@@ -1355,7 +1363,8 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
   item /= (uint32_t)a.T;
   const int gt = (int)(item % (uint32_t)a.GT);
   item /= (uint32_t)a.GT;
-  attend_row<D, ATT_WAVES>(a, (int)(item / (uint32_t)a.Hkv), (int)(item % (uint32_t)a.Hkv), gt, t, split, so, sml);
+  attend_row<D>(a, (int)(item / (uint32_t)a.Hkv), (int)(item % (uint32_t)a.Hkv), gt, t, split, threadIdx.x,
+                wave_id(), true, so, sml);
 }
 
 // Many rows: neighbouring rows of a request list many of the same pages. A workgroup takes R = 4 rpt
@@ -1366,7 +1375,12 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
 // of rows that do not list a page masked; the two halves are joined at the end. A page that not all
 // rows see whole is entered once for each row. Two waves a SIMD, so that one's softmax and LDS reads
 // run beside the other's products: with one (the same step with four waves) 81 us for 1024 rows of 64
-// pages instead of TIME_ROWS.
+// pages and two 256-wide kv heads instead of 62. Of these, a step's products, softmax and LDS reads alone
+// take 37 us and its loads alone 29 (13 TB/s from L2).
+// Time grows with the union where the per-row form's does not: those 1024 rows take 44 us where all
+// lists are one, 64 with 1.8 lists' pages in a union of eight rows, 86 with 2.6, 121 with 3.9, and row
+// by row 77 to 90. A workgroup whose union is past union_most therefore computes its rows alone, two
+// at a time (92 to 97 us).
 // What is masked in a row's column is multiplied by a weight of zero, so a V that is not finite in a
 // page of another row would reach it as NaN: rows whose result is not finite are computed again alone,
 // as are those of a workgroup with a list in which a page stands twice.
@@ -1385,6 +1399,7 @@ template <int D>
 __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendArgs a) {
   typedef __attribute__((address_space(3))) void lds_void;
   using Image = PageImage<D>;
+  static_assert(Image::CHUNKS % ROWS_WAVES == 0, "a load of all waves is of one page");
   constexpr int KS = D / 32, NT = 64 * ROWS_WAVES, CPW = 4 * Image::CHUNKS / ROWS_WAVES;   // loads of a wave per step
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // two steps' pages (first the rows of every page), union
   __shared__ float sml[ROWS_WAVES][16][2];
@@ -1445,7 +1460,7 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
       if (atomicOr(&page_rows[page[i] >> 1], bit) & bit) twice = 1;
     }
   __syncthreads();
-  const bool merge = twice == 0;
+  bool merge = twice == 0;
   uint32_t total = 0;
   if (merge) {
 #pragma unroll
@@ -1468,6 +1483,7 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
       if (blk >= 0) merged[at] = uint2{(uint32_t)blk, (uint32_t)page[i] << 16 | rows};
       __syncthreads();
     }
+    if (total > (uint32_t)a.union_most) merge = false, total = 0;
   }
 
   floatx4 acc[D / 16];
@@ -1491,9 +1507,7 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
 #pragma unroll
     for (int i = 0; i < CPW; ++i) {
       const int c = i * ROWS_WAVES + wave, cc = c % Image::CHUNKS;
-      // which of the four pages: known at compile time but for two per eight chunks
-      const int pg0 = i * ROWS_WAVES / Image::CHUNKS, pg = Image::CHUNKS < ROWS_WAVES ? c / Image::CHUNKS : pg0;
-      const int64_t from = Image::CHUNKS < ROWS_WAVES ? (pg & 1 ? base[(2 * i + 1) & 3] : base[(2 * i) & 3]) : base[pg0];
+      const int64_t from = base[i * ROWS_WAVES / Image::CHUNKS];
       const bool is_v = cc >= Image::CHUNKS / 2;
       const int off = (is_v ? cc - Image::CHUNKS / 2 : cc) * 1024;
       const uint8_t* src = (const uint8_t*)(is_v ? a.v_pool : a.k_pool) + from + off + lane * 16;
@@ -1608,41 +1622,75 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
     if (!(sum < __builtin_huge_valf())) atomicOr(&again, 1u << row);
   }
   __syncthreads();
-  const uint32_t alone = merge ? again : ~0u;
-  for (int r = 0; r < live; ++r)
-    if (alone >> r & 1) {
-      __syncthreads();
-      attend_row<D, ROWS_WAVES>(a, b, h, 0, t0 + r, 0, (float*)lds, sml);
-    }
+  uint32_t alone = merge ? again : (1u << live) - 1;
+  while (alone) {   // two at a time, each by four waves
+    const int r0 = __builtin_ctz(alone);
+    alone &= alone - 1;
+    const bool two = alone != 0;
+    const int r1 = two ? __builtin_ctz(alone) : r0;
+    alone &= alone - 1;
+    __syncthreads();
+    attend_row<D>(a, b, h, 0, t0 + (half ? r1 : r0), 0, tid & 255, rg, !half || two,
+                  (float*)lds + half * attend_lds(D, a.G), sml + half * ATT_WAVES);
+  }
 }
 
-// The splits of one (row, head) joined: D / 4 threads a head.
+// The splits joined: D / 4 threads a head. Two round trips to memory bound it, so all loads of eight
+// splits are in flight at once, and a list is taken on the XCD where attend_kernel computed (its first
+// split): that XCD's L2 has the sums. Both kernels for one token's two lists of 64 pages 9.9 us from
+// HBM, 11.3 with loads as the compiler places them.
+constexpr int JOIN = 8;  // splits whose sums are loaded at once
+
 template <int D>
-__global__ void __launch_bounds__(256) attend_join_kernel(const float* __restrict__ part_o,
-                                                          const float* __restrict__ part_ml,
-                                                          uint16_t* __restrict__ out, int64_t rows,
-                                                          int splits) {
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (D / 4);
+__global__ void __launch_bounds__(256, 4) attend_join_kernel(AttendArgs a, uint32_t per_xcd) {
+  const int splits = a.splits, heads = a.G < 16 ? a.G : 16;
+  const uint32_t x = blockIdx.x % 8, unit = (blockIdx.x / 8 * 256 + threadIdx.x) / (D / 4);
+  const uint32_t l0 = (x * per_xcd + splits - 1) / splits, l1 = ((x + 1) * per_xcd + splits - 1) / splits;
+  uint32_t item = l0 + unit / heads;
+  if (item >= l1 || item >= (uint64_t)a.items / splits) return;
+  const int t = (int)(item % (uint32_t)a.T);
+  item /= (uint32_t)a.T;
+  const int head = (int)(item % (uint32_t)a.GT * 16 + unit % heads);
+  item /= (uint32_t)a.GT;
+  if (head >= a.G) return;
+  const int64_t m = (int64_t)(item / (uint32_t)a.Hkv) * a.T + t;
+  const int64_t row = m * a.Hq + (int64_t)(item % (uint32_t)a.Hkv) * a.G + head;
   const int d = threadIdx.x % (D / 4) * 4;
-  if (row >= rows) return;
-  const float* ml = part_ml + row * splits * 2;
-  const float* po = part_o + row * splits * D + d;
-  float top = -__builtin_huge_valf();
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[2 * s]);
-  float sum = 0.f;
+  const float* ml = a.part_ml + row * splits * 2;
+  const float* po = a.part_o + row * splits * D + d;
+  float top = -__builtin_huge_valf(), sum = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    const float c = ml[2 * s] == top ? 1.f : __builtin_amdgcn_exp2f(ml[2 * s] - top);
-    sum = __builtin_fmaf(ml[2 * s + 1], c, sum);
-    o += *(const floatx4*)(po + (int64_t)s * D) * c;
+  for (int s0 = 0; s0 < splits; s0 += JOIN) {
+    // the last split again past the end, without weight
+    float2 w[JOIN];
+    floatx4 x[JOIN];
+#pragma unroll
+    for (int i = 0; i < JOIN; ++i) {
+      const int s = s0 + i < splits ? s0 + i : splits - 1;
+      w[i] = *(const float2*)(ml + 2 * s);
+      x[i] = *(const floatx4*)(po + s * D);
+    }
+    __builtin_amdgcn_sched_barrier(0);   // all in flight, or the compiler takes them one by one
+    float nt = top;
+#pragma unroll
+    for (int i = 0; i < JOIN; ++i) nt = fmaxf(nt, w[i].x);
+    const float k = top == nt ? 1.f : __builtin_amdgcn_exp2f(top - nt);   // 0 at first
+    top = nt;
+    sum *= k;
+    o *= k;
+#pragma unroll
+    for (int i = 0; i < JOIN; ++i) {
+      const bool in = s0 + i < splits;
+      const float c = w[i].x == top ? 1.f : __builtin_amdgcn_exp2f(w[i].x - top);
+      sum = in ? __builtin_fmaf(w[i].y, c, sum) : sum;
+      o = in ? o + x[i] * c : o;
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint2 y;
   y.x = pack_bf16x2(o[0] * inv, o[1] * inv);
   y.y = pack_bf16x2(o[2] * inv, o[3] * inv);
-  *(uint2*)(out + row * D + d) = y;
+  *(uint2*)(a.out + row * D + d) = y;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1672,35 +1720,43 @@ bool head_shape_ok(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64
          (tokens == 0 || batch <= MAX_BATCH_ROWS / tokens);
 }
 
-// Splits of a list: enough workgroups for two on each of 256 CUs, a page pair or more per wave.
+// Splits of a list: for 256 workgroups, a page pair or more per wave, and whole rounds of the join
+// (whose second starts when the first is added up). With lists from HBM: eighteen of 128 pages and
+// 256-wide heads take 32 us whole, 13.8 in sixteen splits, 15.1 in fifteen; 128 of 64 pages and 128-wide
+// heads 19.6 whole, 20.2 in two, of 256 pages 60 and 53. Short lists are done before a second launch would
+// start (16 pages of 256-wide heads: 7.5 us, 8.9 split; 32 pages: 10.3, 9.2 split).
 int attend_splits(int64_t items, int64_t budget) {
+  if (items <= 0 || budget <= 24) return 1;
   const int64_t most = (budget + 2 * ATT_WAVES - 1) / (2 * ATT_WAVES);
-  int64_t s = items > 0 ? (512 + items - 1) / items : 1;
-  s = s < most ? s : most;
-  return (int)(s < 1 ? 1 : s);
+  int64_t s = (256 + items - 1) / items;
+  if (s > JOIN) s = (s + JOIN - 1) / JOIN * JOIN;
+  return (int)(s < most ? s : most);
 }
 
 // LDS of attend_rows_kernel in front of the union: the ring, and before it two bytes a page.
 int64_t rows_ring_bytes(int64_t D, int64_t pages) {
-  const int64_t image = D == 64 ? PageImage<64>::BYTES : D == 128 ? PageImage<128>::BYTES : PageImage<256>::BYTES;
+  const int64_t image = D == 128 ? PageImage<128>::BYTES : PageImage<256>::BYTES;
   return std::max(8 * image, (pages + 1) / 2 * 4);
 }
 
-// Rows of a wave where rows go over the union of their lists (attend_rows_kernel), or 0: a group of
-// at most sixteen heads, a table (16 bits a page) and lists that fit LDS, rows for more than one
-// wave, and workgroups for half the CUs. Fewer rows run faster one by one with their lists split.
+// Rows of a wave where rows go over the union of their lists (attend_rows_kernel), or 0: two rows or
+// more for the columns of a matrix instruction, heads that are wide enough (1024 rows of 64 pages and
+// two 64-wide kv heads take 26 us row by row, 40 at best over the union; sixteen 256-wide heads a group 46
+// and 41 to 93), a table (16 bits a page) and lists that fit LDS, and rows that fill the rounds of 256
+// workgroups to three quarters, as a round takes as long when it is not full (1024 rows of two 256-wide
+// kv heads, one round: 77 us row by row, 64 over the union; 512 rows 42 and 57).
 int attend_rows_per_wave(int64_t batch, int64_t tokens, int64_t Hkv, int64_t G, int64_t D, int64_t pages,
                          int64_t budget) {
-  if (G > 16) return 0;
+  if (D < 128 || G > 8) return 0;
   const int64_t most = ROWS_MAX / ROWS_GROUPS;
   int64_t rpt = 16 / G < most ? 16 / G : most;
   const int64_t room = ROWS_LDS - rows_ring_bytes(D, pages);
   while (rpt > 0 && (ROWS_GROUPS * rpt * budget * 8 > room ||
                      ROWS_GROUPS * rpt * budget > 64 * ROWS_WAVES * ROWS_ENTRIES))
     --rpt;
-  if (rpt < 1 || tokens <= rpt || pages > 65536) return 0;
-  const int64_t R = ROWS_GROUPS * rpt;
-  return batch * Hkv * ((tokens + R - 1) / R) >= 128 ? (int)rpt : 0;
+  if (rpt < 2 || pages > 65536) return 0;
+  const int64_t R = ROWS_GROUPS * rpt, wgs = batch * Hkv * ((tokens + R - 1) / R);
+  return 4 * batch * Hkv * tokens >= 3 * R * ((wgs + 255) / 256 * 256) ? (int)rpt : 0;
 }
 
 // The choice's workspace for some rows of every request: keys for where a row needs them all, scores,
@@ -1900,13 +1956,14 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
         per = per < 1 ? 1 : per > 64 ? 64 : per;
         const int64_t parts = (tiles + per - 1) / per;
         auto score = head_size == 64 ? score_rows_kernel<64> : head_size == 128 ? score_rows_kernel<128> : score_rows_kernel<256>;
-        hipLaunchKernelGGL(score, dim3((unsigned)(groups * parts), (unsigned)columns), dim3(64 * SCORE_WAVES),
-                           0, S(stream), a, (uint32_t)per);
+        hipLaunchKernelGGL(score, dim3((unsigned)(groups * parts * columns)), dim3(64 * SCORE_WAVES),
+                           0, S(stream), a, (uint32_t)per, (uint32_t)columns);
       } else {
-        // workgroups: two a CU, one where the sums over the rows' heads would take longer than the
-        // pages they are for
-        const int64_t wgs = a.rows > 4 ? 256 : 512;
-        const int pt = table_stride * groups >= 128 * wgs ? 2 : 1;
+        // two workgroups a CU; two page tiles a step where there are pages for about all waves then
+        // (eleven rows of 13751 pages and two kv heads 25.1 us, 25.9 with one; of 2048 pages 20.4 with
+        // one, 22.7 with two)
+        const int64_t wgs = 512;
+        const int pt = table_stride * groups >= 48 * wgs ? 2 : 1;
         const int64_t step = 16 * pt * SCORE_WAVES;
         int64_t per = (table_stride * groups + wgs * step - 1) / (wgs * step) * step;
         per = per > 4096 ? 4096 : per;
@@ -1944,7 +2001,7 @@ SV_API int snowverify_sparse_attention(const void* q, const void* k_pool, const 
   if (batch * tokens == 0) return SV_OK;
   const int64_t need = snowverify_sparse_attention_scratch_bytes(batch, tokens, num_heads,
                                                                  num_kv_heads, head_size, budget);
-  if (!q || (blocks && (!k_pool || !v_pool)) || !out || (table_stride && !table) || !positions ||
+  if (!q || (blocks && (!k_pool || !v_pool)) || !out || out == q || (table_stride && !table) || !positions ||
       (budget && !pages) ||
       scratch_bytes < need || (need && !scratch))
     return SV_EINVAL;
@@ -1972,8 +2029,7 @@ SV_API int snowverify_sparse_attention(const void* q, const void* k_pool, const 
   a.part_o = (float*)scratch;
   a.part_ml = a.splits > 1 ? a.part_o + batch * tokens * num_heads * a.splits * head_size : nullptr;
   const int hm = a.G < 16 ? a.G : 16;
-  const int64_t dr = head_size == 256 && hm > 8 ? 128 : head_size;
-  size_t lds = (size_t)ATT_WAVES * hm * (dr + 4) * 4;
+  size_t lds = (size_t)attend_lds((int)head_size, hm) * 4;
   const int rpt = attend_rows_per_wave(batch, tokens, num_kv_heads, a.G, head_size, table_stride, budget);
   if (rpt) {
     a.rpt = rpt;
@@ -1981,10 +2037,13 @@ SV_API int snowverify_sparse_attention(const void* q, const void* k_pool, const 
     const int64_t R = ROWS_GROUPS * rpt, ring = rows_ring_bytes(head_size, table_stride);
     a.items = batch * num_kv_heads * ((tokens + R - 1) / R);
     a.ring_bytes = (int)ring;
-    lds = std::max(lds / ATT_WAVES * ROWS_WAVES, (size_t)(ring + R * budget * 8));
-    auto kern = head_size == 64 ? attend_rows_kernel<64> : head_size == 128 ? attend_rows_kernel<128> : attend_rows_kernel<256>;
-    static std::atomic<uint64_t> raised[3];
-    const hipError_t err = raise_lds_limit((const void*)kern, raised[head_size / 128], ROWS_LDS);
+    // where a workgroup's rows alone take as long (eight rows of 256-wide heads: 2.7 lists' pages; sixteen
+    // rows of 128-wide ones: 4 lists', 92 us for 512 rows of 64 pages and eight kv heads, 45 at 1.5 lists')
+    a.union_most = (int)(R * budget / (head_size == 256 ? 3 : 4));
+    lds = std::max(2 * lds, (size_t)(ring + R * budget * 8));
+    auto kern = head_size == 128 ? attend_rows_kernel<128> : attend_rows_kernel<256>;
+    static std::atomic<uint64_t> raised[2];
+    const hipError_t err = raise_lds_limit((const void*)kern, raised[head_size / 256], ROWS_LDS);
     if (err != hipSuccess) return (int)err;
     hipLaunchKernelGGL(kern, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3(64 * ROWS_WAVES), lds,
                        S(stream), a);
@@ -1996,10 +2055,10 @@ SV_API int snowverify_sparse_attention(const void* q, const void* k_pool, const 
                      S(stream), a);
   SV_CHECK_LAUNCH();
   if (a.splits > 1) {
-    const int64_t rows = batch * tokens * num_heads;
+    const int64_t per_xcd = (a.items + 7) / 8, lists = (per_xcd + a.splits - 1) / a.splits;   // of an XCD, at most
     auto join = head_size == 64 ? attend_join_kernel<64> : head_size == 128 ? attend_join_kernel<128> : attend_join_kernel<256>;
-    hipLaunchKernelGGL(join, dim3((unsigned)((rows * (head_size / 4) + 255) / 256)), dim3(256), 0,
-                       S(stream), a.part_o, a.part_ml, a.out, rows, a.splits);
+    hipLaunchKernelGGL(join, dim3((unsigned)((lists * hm * (head_size / 4) + 255) / 256 * 8)), dim3(256), 0,
+                       S(stream), a, (uint32_t)per_xcd);
     SV_CHECK_LAUNCH();
   }
   return SV_OK;

@@ -121,8 +121,8 @@ def kv_append(k, v, cos, sin, k_pool, v_pool, table, starts, counts, *, bounds=N
     projection); cos, sin [batch*tokens, half] f32, half % 8 == 0; starts, counts int32 [batch].
     K (and q, into q_out) is normalised per head where its gamma [d] is given, its first 2 half
     elements rotated in the pairs (i, i + half), and rounded once. bounds: those of the pages
-    written, over their keys up to the last one written. Rows past a request's count are left as
-    they were, in q_out too. Requests must not share the pages they write.
+    written, over their keys up to the last one written. q_out may be q. Rows past a request's count
+    are left as they were, in q_out too. Requests must not share the pages they write.
     """
     kp, blocks, hkv, d, dev = _pool(k_pool, "K pool")
     M = k.shape[0]
@@ -224,7 +224,8 @@ def sparse_attention(q, k_pool, v_pool, out, table, positions, pages, scale, scr
     q, out [batch*tokens, Hq, d]; positions int32 [batch*tokens]; pages int32 [batch*tokens, Hkv,
     budget] as page_select gives them, or any other: -1, pages past the row's position and pages
     outside the table are passed over, a page counts as often as it is listed, order is free. A
-    row that sees no key gets zeros. scratch: sparse_attention_scratch_bytes (may be 0: None).
+    row that sees no key gets zeros. out must not overlap q. scratch:
+    sparse_attention_scratch_bytes (may be 0: None).
     """
     kp, blocks, hkv, d, dev = _pool(k_pool, "K pool")
     qs, ps = q.shape, pages.shape
@@ -235,6 +236,8 @@ def sparse_attention(q, k_pool, v_pool, out, table, positions, pages, scale, scr
     rows = (M, heads, d)
     qp = _need(q, "q", BF16, rows, dev)
     op = _need(out, "out", BF16, rows, dev)
+    if op == qp and M:
+        raise SnowLLMError("out must not be q")
     _groups(heads, hkv)
     vp = _need(v_pool, "V pool", BF16, (blocks, hkv, PAGE // 4, d, 4), dev)
     at = _need(positions, "positions", I32, (M,), dev)

@@ -337,13 +337,21 @@ ATTEND = [
     (16, 2, 64, 2, 150, 8, 7),
     (3, 3, 256, 1, 1, 140, 131),
     (8, 8, 64, 2, 40, 20, 17),
-    # rows over the union of their lists: 2, 4, 1, 3 rows a tile, a last group that is not full
+    # many rows one by one
     (16, 2, 256, 1, 517, 30, 12),
     (8, 2, 128, 2, 600, 25, 20),
     (16, 1, 64, 1, 520, 20, 20),
-    (5, 1, 256, 3, 515, 12, 9),
-    (20, 4, 128, 1, 400, 40, 130),
     (3, 3, 64, 1, 700, 6, 1),
+    # rows over the union of their lists: 2, 4, 4, 3, 4 rows a tile, a last group that is not full
+    (32, 4, 256, 1, 397, 30, 12),
+    (8, 2, 128, 2, 789, 25, 20),
+    (15, 5, 256, 2, 310, 12, 9),
+    (20, 4, 128, 1, 590, 40, 130),
+    (4, 4, 128, 1, 799, 6, 1),
+    # the same with lists that have little in common
+    (32, 4, 256, 1, 397, 90, 12),
+    (16, 4, 128, 1, 801, 200, 20),
+    (24, 8, 256, 1, 390, 40, 9),
 ]
 
 
@@ -376,12 +384,12 @@ def test_attend(gpu, Hq, Hkv, d, B, T, width, budget):
 
 
 @pytest.mark.parametrize("kind", ["dead", "holes", "twice", "past", "large", "tiny", "other", "ends"])
-@pytest.mark.parametrize("T", [1, 130, 600])
+@pytest.mark.parametrize("T", [1, 130, 799])
 def test_attend_borders(gpu, kind, T):
     """NaN and infinities behind the last position, table entries that are no page, listed pages
     outside the table or listed twice, scores that differ by hundreds."""
     g = torch.Generator().manual_seed(8)
-    Hq, Hkv, d, width, budget = 8, 2, 128, 24, 20
+    Hq, Hkv, d, width, budget = (16, 4, 128, 24, 20) if T == 799 else (8, 2, 128, 24, 20)
     blocks = width + 4
     table = tables(g, 1, width, blocks)
     kp, vp = pools(g, blocks, Hkv, d)
@@ -391,7 +399,7 @@ def test_attend_borders(gpu, kind, T):
     pages = torch.stack([torch.randperm(21, generator=g)[:budget] for _ in range(T * Hkv)])
     pages = pages.view(T, Hkv, budget).int()
     pages[:, :, 3] = 20                  # the page that the row ends in
-    if T == 600:                         # ascending: rows over the union of their lists
+    if T == 799:                         # ascending: rows over the union of their lists
         pages = torch.stack([torch.randperm(20, generator=g)[:budget - 2].sort().values
                              for _ in range(T * Hkv)]).view(T, Hkv, -1).int()
         pages = torch.cat([pages, torch.full((T, Hkv, 1), 20), torch.full((T, Hkv, 1), -1)], 2).int()
@@ -572,6 +580,76 @@ def test_step_in_a_graph_and_on_another_stream(gpu):
         graph.replay()
         c.check()
         assert torch.equal(bits(c.out.cpu()), bits(eager.cpu()))
+
+
+def test_many_rows_in_two_graphs(gpu):
+    """A prompt chunk's step, captured for two caches, replayed in turn and on two streams at once,
+    between eager steps."""
+    caches = [Cache(32, 4, 256, 32, 1, 397, 60, 8, seed=s) for s in (11, 12)]
+    graphs = []
+    for c in caches:
+        c.at([500])
+        c.step()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            c.step()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for n, contexts in enumerate(([500], [530], [101])):
+        say("replay", contexts)
+        for c in caches:
+            c.at(contexts)
+        eager = [c.step().clone() for c in caches]
+        for c in caches:
+            c.out.fill_(5.0)
+            c.pages.fill_(3)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream if n == 2 else torch.cuda.current_stream()):
+                graph.replay()
+        torch.cuda.synchronize()
+        for c, e in zip(caches, eager):
+            assert torch.equal(bits(c.out.cpu()), bits(e.cpu()))
+    caches[0].check()
+
+
+def test_in_place_and_unaligned_views(gpu):
+    """q rotated in place, and positions, tables, lists, starts and angles that begin anywhere in
+    their buffers."""
+    from snowllm_amd import ops
+    def inside(t):
+        t = t.cuda()
+        return torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)
+    g = torch.Generator().manual_seed(77)
+    Hq, Hkv, d, half, B, T, width, budget = 8, 2, 128, 32, 2, 21, 20, 7
+    blocks, M = B * width + 1, B * T
+    table = tables(g, B, width, blocks)
+    kp, vp = pools(g, blocks, Hkv, d)
+    bounds = torch.zeros(blocks, Hkv, 2, d, dtype=torch.bfloat16)
+    c = [t.cuda() for t in (kp, vp, bounds)]
+    proj = torch.randn(M, Hq + 2 * Hkv, d, generator=g).bfloat16()
+    q, k, v = proj[:, :Hq].contiguous(), proj[:, Hq:Hq + Hkv], proj[:, Hq + Hkv:]
+    cos, sin = torch.rand(M, half, generator=g), torch.rand(M, half, generator=g)
+    st, ct = torch.tensor([200, 31], dtype=torch.int32), torch.tensor([21, 20], dtype=torch.int32)
+    pos = (st[:, None] + torch.arange(T, dtype=torch.int32)).view(-1)
+    out, qd = torch.zeros_like(q).cuda(), q.cuda()
+    ops.page_bounds(c[0], c[2], inside(table), inside(torch.zeros_like(st)), inside(st), 200)
+    ops.kv_append(k.cuda(), v.cuda(), inside(cos), inside(sin), c[0], c[1], inside(table), inside(st),
+                  inside(ct), bounds=c[2], q=qd, q_out=qd)
+    other = torch.full_like(q, 4.0).cuda()
+    ops.kv_append(k.cuda(), v.cuda(), cos.cuda(), sin.cuda(), c[0], c[1], table.cuda(), st.cuda(),
+                  ct.cuda(), bounds=c[2], q=q.cuda(), q_out=other)
+    assert torch.equal(bits(qd[:-1].cpu()), bits(other[:-1].cpu()))
+    assert torch.equal(bits(qd[-1].cpu()), bits(q[-1])) and (other[-1] == 4).all()
+    scratch = ops.empty_bytes(ops.page_select_scratch_bytes(B, T, Hq, Hkv, d, width))
+    pages = inside(torch.zeros(M, Hkv, budget, dtype=torch.int32))
+    assert pages.data_ptr() % 16 and pages.is_contiguous()
+    ops.page_select(qd, c[2], inside(table), inside(pos), pages, scratch)
+    assert torch.equal(pages.cpu(), R.select(qd.cpu(), c[2].cpu(), table, pos, budget, 1, 2))
+    need = ops.sparse_attention_scratch_bytes(B, T, Hq, Hkv, d, budget)
+    ops.sparse_attention(qd, c[0], c[1], out, inside(table), inside(pos), pages, d ** -0.5,
+                         ops.empty_bytes(need) if need else None)
+    check_attend(out.cpu(), qd.cpu(), c[0].cpu(), c[1].cpu(), table, pos, pages.cpu(), d ** -0.5)
 
 
 def test_two_streams_at_once(gpu):

@@ -124,11 +124,11 @@ def test_entry_points_refuse_sizes():
                 dict(Hq=5), dict(sink=1 << 62, recent=1 << 62), dict(budget=1 << 40)):
         assert select(**bad) == EINVAL, bad
 
-    def attend(budget=8, T=1, B=1, d=64, Hq=4, Hkv=2, q=16, pages=16, scratch=16, nbytes=1 << 40):
-        return lib.snowverify_sparse_attention(q, 16, 16, 16, 16, 16, pages, B, T, Hq, Hkv, d, 64, 9,
+    def attend(budget=8, T=1, B=1, d=64, Hq=4, Hkv=2, q=16, out=32, pages=16, scratch=16, nbytes=1 << 40):
+        return lib.snowverify_sparse_attention(q, 16, 16, out, 16, 16, pages, B, T, Hq, Hkv, d, 64, 9,
                                                budget, 1.0, scratch, nbytes, 0)
     assert attend(B=0) == 0
-    for bad in (dict(budget=-1), dict(d=48), dict(Hq=0), dict(q=0), dict(pages=0), dict(T=1 << 30),
+    for bad in (dict(budget=-1), dict(d=48), dict(Hq=0), dict(q=0), dict(out=16), dict(pages=0), dict(T=1 << 30),
                 dict(budget=1000, nbytes=0), dict(budget=1000, scratch=0), dict(budget=1 << 30),
                 dict(T=1 << 23, Hq=4096, Hkv=4096)):
         assert attend(**bad) == EINVAL, bad
