@@ -169,6 +169,9 @@ __device__ __forceinline__ u32x4 rotate_norm(u32x4 raw, int c, const uint16_t* g
   return o;
 }
 
+// Bound by its bytes: four prompts of about 2048 rows (q and k normalised, 150 MB) take 41 us (3.7 TB/s),
+// 34 of them in the kernel; one row of a 128-wide model 4 us, a dependent load of start, table entry and
+// rows each. A thread's four heads of queries: 41 us against 47 with one.
 // 2 D threads: sixteen heads of D / 8 threads each. A page workgroup owns one (request, page, kv
 // head): its threads take a token's row each, normalise and rotate it, and pass it through LDS into
 // the page's layout, so that global reads and writes are both contiguous. The page's bounds are
@@ -536,7 +539,10 @@ struct PageTiles {
   }
 };
 
-// Up to sixteen rows of a request and kv head a workgroup, which sums them for itself. A wave takes
+// Bound by the bytes of the bounds where the cache is long: 32 requests of 16K to 32K tokens and eight
+// 128-wide kv heads, 205 MB read in 46 us (4.5 TB/s); eleven rows at 220K and two 256-wide heads 12 us
+// (28 MB from the last-level cache); 8 us for one row at 8K, a chain of loads (position, table, bounds) and
+// of the rows' sums. Up to sixteen rows of a request and kv head a workgroup, which sums them for itself. A wave takes
 // PT times sixteen pages at a time, whose bounds are an operand as they lie in memory: they are read
 // ahead of the rows' sums, and each step's pages while the last one's scores are stored. Two page
 // tiles to each read of the rows' operand keep LDS (85 bytes a clock) behind the matrix cores.
@@ -620,6 +626,10 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES) operand_kernel(SelectArgs a)
   for (int i = 0; i < NS * 2 / SCORE_WAVES; ++i) out[i * 256 + threadIdx.x] = op[i * 256 + threadIdx.x];
 }
 
+// Many rows are bound by the products, three of 16 x 16 x 2 D per page tile and row tile: 1024 rows over
+// 4064 pages, two 256-wide kv heads, 34 us (8.5 GFLOP that are needed, 13 with the products for E; matrix
+// cores 39 % busy, the rest LDS reads of the operands and the stores of the scores). With workgroups of
+// the other form, one for each sixteen rows, which read and sum everything again, 48 us.
 // A wave keeps the bounds of 32 pages in registers and goes over the row tiles of its part of the
 // rows, whose operands come through LDS for all four waves (global_load_lds), the next tile's while
 // one is used. A tile's scores are stored a step later, so that the one wait of a step is for loads
@@ -737,8 +747,9 @@ __device__ __forceinline__ uint64_t exact_key(const SelectArgs& a, const double*
   return score_key(s);
 }
 
-// One workgroup per (row, kv head). CACHED: its scores fit the threads' registers. What bounds it is
-// the number of instructions per score, so the scores are looked at twice only: for each thread's
+// One workgroup per (row, kv head). CACHED: its scores fit the threads' registers. One row is bound by the
+// chain of its barriers and reductions (8 us over 512 pages, 14 over 13751), many rows by the number of
+// instructions per score (1024 rows over 4064 pages and two kv heads 26 us), so the scores are looked at twice only: for each thread's
 // largest, of which the need-th largest is a lower bound of the row's (`low`), and for those not
 // clearly below it, which go to a list in LDS (a few more than are needed); t, the choice and the
 // near pages come from the list. Where more pass than the list holds (budgets of over about half
@@ -1192,7 +1203,11 @@ __host__ __device__ __forceinline__ int attend_lds(int D, int heads) {
 //                                  (its layout is the operand's: 1 KiB per wave load)
 //   O^T[d, head]  += V^T . P^T     over the 32 keys, A = V^T (a 16-byte load holds a lane's keys of
 //                                  elements d and d + 1: two operands), B = P^T from S^T's registers
-// so neither K, V nor P passes through LDS.
+// so neither K, V nor P passes through LDS. Bound by the bytes of the pages where rows have their own (64
+// requests of 64 pages and eight 128-wide kv heads, 270 MB in 50 us, 5.3 TB/s; their reads from HBM 263
+// MB), by L2 where neighbouring rows share them (1024 rows of 64 pages and two 256-wide kv heads, 2.1 GB in
+// 77 to 90 us, 25 TB/s), by a chain of loads (position, list, table, pages) where there are few (one row of 64
+// pages 6.3 us).
 // By four waves, whose threads are tid; `write`: or the result is dropped.
 template <int D>
 __device__ __forceinline__ void attend_row(const AttendArgs& a, int b, int h, int gt, int t, int split,
@@ -1635,29 +1650,21 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
   }
 }
 
-// The splits joined: D / 4 threads a head. Two round trips to memory bound it, so all loads of eight
-// splits are in flight at once, and a list is taken on the XCD where attend_kernel computed (its first
-// split): that XCD's L2 has the sums. Both kernels for one token's two lists of 64 pages 9.9 us from
-// HBM, 11.3 with loads as the compiler places them.
-constexpr int JOIN = 8;  // splits whose sums are loaded at once
+// The splits of one (row, head) joined: D / 4 threads a head. A round trip to memory bounds it, so all
+// loads of eight splits are in flight at once (2.4 us; both kernels for two lists of 48 pages of 256-wide
+// heads, six splits each, 8.7 us from HBM, 9.9 with the loads as the compiler places them).
+constexpr int JOIN = 8;
 
 template <int D>
-__global__ void __launch_bounds__(256, 4) attend_join_kernel(AttendArgs a, uint32_t per_xcd) {
-  const int splits = a.splits, heads = a.G < 16 ? a.G : 16;
-  const uint32_t x = blockIdx.x % 8, unit = (blockIdx.x / 8 * 256 + threadIdx.x) / (D / 4);
-  const uint32_t l0 = (x * per_xcd + splits - 1) / splits, l1 = ((x + 1) * per_xcd + splits - 1) / splits;
-  uint32_t item = l0 + unit / heads;
-  if (item >= l1 || item >= (uint64_t)a.items / splits) return;
-  const int t = (int)(item % (uint32_t)a.T);
-  item /= (uint32_t)a.T;
-  const int head = (int)(item % (uint32_t)a.GT * 16 + unit % heads);
-  item /= (uint32_t)a.GT;
-  if (head >= a.G) return;
-  const int64_t m = (int64_t)(item / (uint32_t)a.Hkv) * a.T + t;
-  const int64_t row = m * a.Hq + (int64_t)(item % (uint32_t)a.Hkv) * a.G + head;
+__global__ void __launch_bounds__(256, 4) attend_join_kernel(const float* __restrict__ part_o,
+                                                             const float* __restrict__ part_ml,
+                                                             uint16_t* __restrict__ out, int64_t rows,
+                                                             int splits) {
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (D / 4);
   const int d = threadIdx.x % (D / 4) * 4;
-  const float* ml = a.part_ml + row * splits * 2;
-  const float* po = a.part_o + row * splits * D + d;
+  if (row >= rows) return;
+  const float* ml = part_ml + row * splits * 2;
+  const float* po = part_o + row * splits * D + d;
   float top = -__builtin_huge_valf(), sum = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < splits; s0 += JOIN) {
@@ -1690,7 +1697,7 @@ __global__ void __launch_bounds__(256, 4) attend_join_kernel(AttendArgs a, uint3
   uint2 y;
   y.x = pack_bf16x2(o[0] * inv, o[1] * inv);
   y.y = pack_bf16x2(o[2] * inv, o[3] * inv);
-  *(uint2*)(a.out + row * D + d) = y;
+  *(uint2*)(out + row * D + d) = y;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1722,9 +1729,9 @@ bool head_shape_ok(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64
 
 // Splits of a list: for 256 workgroups, a page pair or more per wave, and whole rounds of the join
 // (whose second starts when the first is added up). With lists from HBM: eighteen of 128 pages and
-// 256-wide heads take 32 us whole, 13.8 in sixteen splits, 15.1 in fifteen; 128 of 64 pages and 128-wide
-// heads 19.6 whole, 20.2 in two, of 256 pages 60 and 53. Short lists are done before a second launch would
-// start (16 pages of 256-wide heads: 7.5 us, 8.9 split; 32 pages: 10.3, 9.2 split).
+// 256-wide heads take 32 us whole, 12.9 in sixteen splits; 128 of 64 pages and 128-wide heads 19.6 whole,
+// 19.0 in two, of 256 pages 60 and 53. Short lists are done before a second launch would start (of 16
+// pages of 256-wide heads, from L2: 6.8 us whole, 7.7 split; of 32, from HBM: 10.3 and 9.2).
 int attend_splits(int64_t items, int64_t budget) {
   if (items <= 0 || budget <= 24) return 1;
   const int64_t most = (budget + 2 * ATT_WAVES - 1) / (2 * ATT_WAVES);
@@ -1796,7 +1803,9 @@ auto pick_of(int64_t width) {
                                      : pick_kernel<D, 1024, false>;
 }
 // A thread holds up to sixteen scores: four waves up to 4096 pages, sixteen above, and past 16384
-// pages the scores are read again by every pass.
+// pages the scores are read again by every pass. The whole choice: 256 rows over 4096 pages and two kv
+// heads 39 us with four waves, 46 with sixteen (one row the same with both); eleven rows over 13751 pages
+// 25 us with the scores in registers, 29 read again.
 auto pick_form(int64_t D, int64_t width) {
   return D == 64 ? pick_of<64>(width) : D == 128 ? pick_of<128>(width) : pick_of<256>(width);
 }
@@ -1950,7 +1959,8 @@ SV_API int snowverify_page_select(const void* q, const void* bounds, const int32
         auto prepare = head_size == 64 ? operand_kernel<64> : head_size == 128 ? operand_kernel<128> : operand_kernel<256>;
         hipLaunchKernelGGL(prepare, dim3((unsigned)(groups * tiles)), dim3(64 * SCORE_WAVES), 0, S(stream), a);
         SV_CHECK_LAUNCH();
-        // two workgroups a CU (what LDS holds of a 256-wide head), at most 64 row tiles each
+        // two workgroups a CU (what LDS holds of a 256-wide head), at most 64 row tiles each: choice of
+        // 1024 rows over 4064 pages 65.5 us, 70.9 for one a CU, 67.9 for four
         const int64_t columns = (table_stride + 32 * SCORE_WAVES - 1) / (32 * SCORE_WAVES);
         int64_t per = tiles * groups * columns / 512;
         per = per < 1 ? 1 : per > 64 ? 64 : per;
@@ -2055,10 +2065,10 @@ SV_API int snowverify_sparse_attention(const void* q, const void* k_pool, const 
                      S(stream), a);
   SV_CHECK_LAUNCH();
   if (a.splits > 1) {
-    const int64_t per_xcd = (a.items + 7) / 8, lists = (per_xcd + a.splits - 1) / a.splits;   // of an XCD, at most
+    const int64_t rows = batch * tokens * num_heads;
     auto join = head_size == 64 ? attend_join_kernel<64> : head_size == 128 ? attend_join_kernel<128> : attend_join_kernel<256>;
-    hipLaunchKernelGGL(join, dim3((unsigned)((lists * hm * (head_size / 4) + 255) / 256 * 8)), dim3(256), 0,
-                       S(stream), a, (uint32_t)per_xcd);
+    hipLaunchKernelGGL(join, dim3((unsigned)((rows * (head_size / 4) + 255) / 256)), dim3(256), 0,
+                       S(stream), a.part_o, a.part_ml, a.out, rows, a.splits);
     SV_CHECK_LAUNCH();
   }
   return SV_OK;
