@@ -628,8 +628,8 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES) operand_kernel(SelectArgs a)
 
 // Many rows are bound by the products, three of 16 x 16 x 2 D per page tile and row tile: 1024 rows over
 // 4064 pages, two 256-wide kv heads, 34 us (8.5 GFLOP that are needed, 13 with the products for E; matrix
-// cores 39 % busy, the rest LDS reads of the operands and the stores of the scores). With workgroups of
-// the other form, one for each sixteen rows, which read and sum everything again, 48 us.
+// cores 39 % busy, the rest LDS reads of the operands and the stores of the scores); the whole choice 62 us,
+// 82 with workgroups of the other form, one for each sixteen rows, which read and sum everything again.
 // A wave keeps the bounds of 32 pages in registers and goes over the row tiles of its part of the
 // rows, whose operands come through LDS for all four waves (global_load_lds), the next tile's while
 // one is used. A tile's scores are stored a step later, so that the one wait of a step is for loads
