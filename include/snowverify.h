@@ -346,7 +346,7 @@ int snowverify_page_select(const void* q, const void* bounds, const int32_t* tab
                            int64_t head_size, int64_t table_stride, int64_t blocks,
                            int64_t budget, int64_t sink, int64_t recent, void* scratch,
                            int64_t scratch_bytes, void* stream);
-/* Scratch bytes of snowverify_sparse_attention (may be 0). */
+/* Scratch bytes of snowverify_sparse_attention (may be 0; few rows may need more than many). */
 int64_t snowverify_sparse_attention_scratch_bytes(int64_t batch, int64_t tokens,
                                                   int64_t num_heads, int64_t num_kv_heads,
                                                   int64_t head_size, int64_t budget);

@@ -213,6 +213,7 @@ def page_select(q, bounds, table, positions, pages, scratch, *, sink=1, recent=2
 
 @lru_cache(maxsize=256)
 def sparse_attention_scratch_bytes(batch, tokens, num_heads, num_kv_heads, head_size, budget) -> int:
+    """For this shape: few rows' lists are split, so fewer rows may need more than many."""
     return int(lib.snowverify_sparse_attention_scratch_bytes(batch, tokens, num_heads, num_kv_heads,
                                                              head_size, budget))
 
