@@ -1111,8 +1111,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 2) pick_kernel(SelectArgs 
     __syncthreads();
     if (lane == 63) red[0][wave] = ci;
     __syncthreads();
+    // every lane takes part in the sums, also those past the last word
     const uint32_t t0 = lane < WAVES ? red[0][lane] : 0u;
-    if (w < words) rank[w] = before + wave_sum_u32_dpp(lane < wave ? t0 : 0u) + ci - cnt;
+    const uint32_t earlier = wave_sum_u32_dpp(lane < wave ? t0 : 0u);
+    if (w < words) rank[w] = before + earlier + ci - cnt;
     before += wave_sum_u32_dpp(t0);
   }
   __syncthreads();

@@ -213,6 +213,22 @@ def test_select(gpu, Hq, Hkv, d, B, T, width, budget, sink, recent):
     assert torch.equal(got, R.select(q, bounds, table, pos, budget, sink, recent))
 
 
+@pytest.mark.parametrize("width,budget", [(4096, 40), (8400, 40), (17000, 300)])
+def test_select_every_length(gpu, width, budget):
+    """Rows that end in every group of 64 pages, at its start, in it and at its end."""
+    g = torch.Generator().manual_seed(width)
+    table = tables(g, 1, width, width)
+    x = torch.randn(width, 1, 2, 64, generator=g)
+    bounds = torch.stack([x.amin(2), x.amax(2)], 2).bfloat16()
+    groups = torch.arange((width + 63) // 64)
+    last = torch.stack([groups * 64, groups * 64 + torch.randint(1, 63, groups.shape, generator=g),
+                        groups * 64 + 63], 1).view(-1).clamp(max=width - 1)
+    pos = (last * PAGE + 5).int()
+    q = torch.randn(len(pos), 2, 64, generator=g).bfloat16()
+    got = run_select(q, bounds, table, pos, budget, 1, 2, 1)
+    assert torch.equal(got, R.select(q, bounds, table, pos, budget, 1, 2))
+
+
 @pytest.mark.parametrize("width,budget", [(300, 40), (1500, 40), (1500, 1400)])
 @pytest.mark.parametrize("kind", ["equal", "near", "same", "zero", "nan", "inf", "holes", "few", "past",
                                   "tiny", "huge", "far"])
