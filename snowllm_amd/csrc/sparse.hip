@@ -540,7 +540,7 @@ struct PageTiles {
 };
 
 // Bound by the bytes of the bounds where the cache is long: 32 requests of 16K to 32K tokens and eight
-// 128-wide kv heads, 205 MB read in 46 us (4.5 TB/s); eleven rows at 220K and two 256-wide heads 12 us
+// 128-wide kv heads, 205 MB read in 48 us (4.3 TB/s); eleven rows at 220K and two 256-wide heads 12 us
 // (28 MB from the last-level cache); 8 us for one row at 8K, a chain of loads (position, table, bounds) and
 // of the rows' sums. Up to sixteen rows of a request and kv head a workgroup, which sums them for itself. A wave takes
 // PT times sixteen pages at a time, whose bounds are an operand as they lie in memory: they are read
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(64 * SCORE_WAVES) operand_kernel(SelectArgs a)
 
 // Many rows are bound by the products, three of 16 x 16 x 2 D per page tile and row tile: 1024 rows over
 // 4064 pages, two 256-wide kv heads, 34 us (8.5 GFLOP that are needed, 13 with the products for E; matrix
-// cores 39 % busy, the rest LDS reads of the operands and the stores of the scores); the whole choice 62 us,
+// cores 38 % busy, the rest LDS reads of the operands and the stores of the scores); the whole choice 62 us,
 // 82 with workgroups of the other form, one for each sixteen rows, which read and sum everything again.
 // A wave keeps the bounds of 32 pages in registers and goes over the row tiles of its part of the
 // rows, whose operands come through LDS for all four waves (global_load_lds), the next tile's while
