@@ -339,7 +339,8 @@ int64_t snowverify_page_select_scratch_bytes(int64_t batch, int64_t tokens, int6
  * its first `sink`, its last `recent` (at least 1: the page of the row's own position is not
  * judged by bounds that later rows are part of) and, of the others, those with the largest sum
  * over the kv head's q heads g and elements d of max(q_gd low_d, q_gd high_d), in 64 bits, the
- * lowest page first among equals; NaN counts as -inf. sink + recent <= budget. */
+ * lowest page first among equals; a sum with a NaN product (0 . inf) counts as -inf. sink + recent
+ * <= budget. */
 int snowverify_page_select(const void* q, const void* bounds, const int32_t* table,
                            const int32_t* positions, int32_t* pages, int64_t batch,
                            int64_t tokens, int64_t num_heads, int64_t num_kv_heads,

@@ -79,6 +79,11 @@ def scores(q, bounds, table, b, head, hkv):
     group = q[head * G:(head + 1) * G].double()
     up, down = group.clamp(min=0).sum(0), group.clamp(max=0).sum(0)
     s = (up * box[:, 1]).sum(-1) + (down * box[:, 0]).sum(-1)
+    # the same only for finite values (0 . inf): otherwise as it is defined, NaN where a term is
+    odd = ~box.isfinite().all(-1).all(-1) | ~group.isfinite().all()
+    if odd.any():
+        terms = group[:, None, None] * box[odd]                           # [G, pages, 2, d]
+        s[odd] = torch.maximum(terms[:, :, 0], terms[:, :, 1]).sum((0, 2))
     return s.masked_fill(~ok, float("nan"))
 
 

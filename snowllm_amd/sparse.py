@@ -183,7 +183,8 @@ def page_select(q, bounds, table, positions, pages, scratch, *, sink=1, recent=2
     a padding row, all -1). Every page where there are at most budget; else the first `sink`, the
     last `recent` (at least 1) and, of the others, those with the largest sum over the kv head's q
     heads and the elements of max(q low, q high), the most that a key within the bounds could
-    score; taken in 64 bits, the lowest page first among equals, NaN as -inf.
+    score; taken in 64 bits, the lowest page first among equals, a sum with a NaN product (0 . inf)
+    as -inf.
     """
     qs, bs, ps = q.shape, bounds.shape, pages.shape
     if len(qs) != 3 or len(ps) != 3 or len(bs) != 4:

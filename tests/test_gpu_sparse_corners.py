@@ -1,0 +1,55 @@
+"""Corner inputs of the operators over selected pages against their definition in 64 bits
+(oracle/sparse.py), with the tolerances of tests/test_gpu_sparse.py."""
+import pytest
+import torch
+
+from oracle import sparse as R
+from tests.test_gpu_sparse import check_attend, pools, run_attend, run_select, say, tables
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+PAGE = 16
+
+
+# ------------------------------------------------------------------------------------------
+# select
+# ------------------------------------------------------------------------------------------
+def test_select_page_with_an_infinite_minimum(gpu):
+    """Positive queries score a page by its maxima, whatever its minima: the second page, whose
+    maxima are the largest, holds a key of -inf."""
+    bounds = torch.ones(6, 1, 2, 128, dtype=torch.bfloat16)
+    bounds[:, :, 0] = -1.0
+    bounds[1, :, 1] = 3.0
+    bounds[1, 0, 0, 7] = -INF
+    table = torch.arange(6, dtype=torch.int32).view(1, 6)
+    pos = torch.tensor([95], dtype=torch.int32)
+    for sign, low, high in ((1.0, bounds[:, :, 0], bounds[:, :, 1]), (-1.0, -bounds[:, :, 1], -bounds[:, :, 0])):
+        q = torch.full((1, 2, 128), sign).bfloat16()
+        got = run_select(q, torch.stack([low, high], 2), table, pos, 2, 0, 1, 1)
+        assert got.tolist() == [[[1, 5]]], sign
+
+
+@pytest.mark.parametrize("Hq,Hkv,d", [(8, 2, 128), (6, 1, 64), (3, 3, 256)])
+@pytest.mark.parametrize("T", [1, 15, 40])
+def test_select_infinite_bounds(gpu, Hq, Hkv, d, T):
+    """Infinite keys among ordinary ones, for queries of one sign, of both, with zeros and with
+    infinities: scores that are finite, infinite and NaN."""
+    say("select inf", Hq, Hkv, d, T)
+    g = torch.Generator().manual_seed(d + T)
+    width, budget = 90, 20
+    table = tables(g, 1, width, width)
+    x = torch.randn(width, Hkv, 2, d, generator=g)
+    bounds = torch.stack([x.amin(2), x.amax(2)], 2).bfloat16()
+    bounds[::4, :, 0, 3] = -INF
+    bounds[1::4, :, 1, 5] = INF
+    bounds[2::8, :, 0, 7], bounds[2::8, :, 1, 7] = -INF, INF
+    bounds[6::8, :, :, 9] = INF
+    q = torch.randn(T, Hq, d, generator=g).bfloat16()
+    q[0::5] = q[0::5].abs()
+    q[1::5] = -q[1::5].abs()
+    q[3::5, :, 3:6] = 0.0
+    q[4::5, ::2, 11] = -INF
+    pos = torch.full((T,), width * PAGE - 1, dtype=torch.int32)
+    got = run_select(q, bounds, table, pos, budget, 1, 2, Hkv)
+    assert torch.equal(got, R.select(q, bounds, table, pos, budget, 1, 2))
