@@ -1174,6 +1174,13 @@ struct AttendArgs {
 
 constexpr int ATT_WAVES = 4;
 
+// Keys of a page that a row at `pos` sees, PAGE of a whole one; the page is not past the row's position.
+// pos may be 2^31 - 1, so the one is added last.
+__device__ __forceinline__ int keys_seen(int pos, int page) {
+  const int before = pos - page * PAGE;
+  return (before < PAGE - 1 ? before : PAGE - 1) + 1;
+}
+
 // The V^T operands of elements d and d + 1 over two pages' keys, from a 16-byte load of each page
 // (d's four keys, then d + 1's): the middle pairs change places.
 __device__ __forceinline__ void v_operands(u32x4 a, u32x4 b, bf16x8& f0, bf16x8& f1) {
@@ -1275,8 +1282,8 @@ __device__ __forceinline__ void attend_row(const AttendArgs& a, int b, int h, in
       const int ib = two ? __builtin_ctzll(todo) : ia;
       if (two) todo &= todo - 1;
       const int ba = __builtin_amdgcn_readlane(blk, ia), bb = __builtin_amdgcn_readlane(blk, ib);
-      const int left_a = pos - __builtin_amdgcn_readlane(pg, ia) * PAGE + 1;
-      const int left_b = two ? pos - __builtin_amdgcn_readlane(pg, ib) * PAGE + 1 : 0;
+      const int left_a = keys_seen(pos, __builtin_amdgcn_readlane(pg, ia));
+      const int left_b = two ? keys_seen(pos, __builtin_amdgcn_readlane(pg, ib)) : 0;
       const int64_t offa = ((int64_t)ba * a.Hkv + h) * page_elems, offb = ((int64_t)bb * a.Hkv + h) * page_elems;
       // K: lane (key col, g) holds d = 32 s + 8 g .. of its key
       const uint16_t* ka = a.k_pool + offa + (g >> 1) * 256 + col * 16 + (g & 1) * 8;
@@ -1575,8 +1582,8 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
     const int page_a = (int)(info_a >> 16), page_b = (int)(info_b >> 16);
     // a page that one row sees in part: what lies behind its last position never enters
     int end_a = PAGE, end_b = two ? PAGE : 0;
-    if (!whole(page_a)) end_a = __builtin_amdgcn_readfirstlane(spos[__builtin_ctz(rows_a)]) - page_a * PAGE + 1;
-    if (two && !whole(page_b)) end_b = __builtin_amdgcn_readfirstlane(spos[__builtin_ctz(rows_b)]) - page_b * PAGE + 1;
+    if (!whole(page_a)) end_a = keys_seen(__builtin_amdgcn_readfirstlane(spos[__builtin_ctz(rows_a)]), page_a);
+    if (two && !whole(page_b)) end_b = keys_seen(__builtin_amdgcn_readfirstlane(spos[__builtin_ctz(rows_b)]), page_b);
     const uint8_t* slot = lds + (j & 1) * (4 * Image::BYTES) + half * (2 * Image::BYTES);
     // all of K is asked for before the first is used, all of V before the softmax
     u32x4 ka[KS], kb[KS];
@@ -1599,8 +1606,8 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) attend_rows_kernel(AttendA
       vb[s] = *(const u32x4*)(slot + Image::BYTES + v_at + 256 * s);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const int left_a = rows_a >> row & 1 ? pos - page_a * PAGE + 1 : 0;
-    const int left_b = rows_b >> row & 1 ? pos - page_b * PAGE + 1 : 0;
+    const int left_a = rows_a >> row & 1 ? keys_seen(pos, page_a) : 0;
+    const int left_b = rows_b >> row & 1 ? keys_seen(pos, page_b) : 0;
     float x[8];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {

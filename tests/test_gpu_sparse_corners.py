@@ -53,3 +53,28 @@ def test_select_infinite_bounds(gpu, Hq, Hkv, d, T):
     pos = torch.full((T,), width * PAGE - 1, dtype=torch.int32)
     got = run_select(q, bounds, table, pos, budget, 1, 2, Hkv)
     assert torch.equal(got, R.select(q, bounds, table, pos, budget, 1, 2))
+
+
+# ------------------------------------------------------------------------------------------
+# attend
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 130, 799])
+def test_attend_at_the_last_position(gpu, T):
+    """Rows at position 2^31 - 1, which see every listed page whole, page 0 among them as the first
+    and as the second page of a pair: a wave takes every fourth entry of a list, the union of the
+    lists of many rows begins with the first one's."""
+    say("attend at 2^31 - 1", T)
+    g = torch.Generator().manual_seed(T)
+    Hq, Hkv, d, width, budget = (16, 4, 128, 24, 20) if T == 799 else (8, 2, 128, 24, 20)
+    table = tables(g, 1, width, width + 2)
+    kp, vp = pools(g, width + 2, Hkv, d)
+    q = torch.randn(T, Hq, d, generator=g).bfloat16()
+    pos = torch.full((T,), 2 ** 31 - 1, dtype=torch.int32)
+    pages = torch.stack([torch.randperm(width - 1, generator=g)[:budget] + 1 for _ in range(T * Hkv)])
+    pages = pages.view(T, Hkv, budget).int()
+    pages[:, :, 1 if T == 799 else 4] = 0
+    pages[3::7, :, 0] = 0
+    pages[3::7, :, 1:5] = pages[3::7, :, 5:9]
+    pages[3::7, :, 5:9] = -1
+    got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
+    check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
