@@ -1193,9 +1193,11 @@ __device__ __forceinline__ void v_operands(u32x4 a, u32x4 b, bf16x8& f0, bf16x8&
 
 // One step of the running softmax over a wave's 32 keys: exponents e (lane (head col, g): keys 4 g ..
 // of two pages, masked ones -inf) to weights 2^(e - m), as a bf16 pair hi + lo (16 bits of
-// mantissa: hi is the upper half of the word, lo what is left, rounded; single bf16 weights would add
-// about two thirds of the output's own rounding to its error). m moves, and O and l are scaled, only
-// where a score passes it by 2^8, for all of a wave's columns at once; all in 32 bits.
+// mantissa: hi is the upper half of the word below the weight's, lo what is left, rounded; single bf16
+// weights would add about two thirds of the output's own rounding to its error). That word is one
+// less so that lo is not 0 where the weight is a bf16 itself, as the largest key's 1 is: an infinite V
+// times 0 would be NaN. m moves, and O and l are scaled, only where a score passes it by 2^8, for all
+// of a wave's columns at once; all in 32 bits.
 constexpr float RESCALE = 8.f;
 
 template <int D>
@@ -1220,7 +1222,8 @@ __device__ __forceinline__ void softmax_step(const float (&e)[8], float& m, floa
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t u = __float_as_uint(p[2 * i]), v = __float_as_uint(p[2 * i + 1]);
+    const uint32_t u = __builtin_elementwise_sub_sat(__float_as_uint(p[2 * i]), 1u);   // 0 stays 0
+    const uint32_t v = __builtin_elementwise_sub_sat(__float_as_uint(p[2 * i + 1]), 1u);
     hi[i] = __builtin_amdgcn_perm(v, u, 0x07060302u);
     lo[i] = pack_bf16x2(p[2 * i] - __uint_as_float(u & 0xffff0000u), p[2 * i + 1] - __uint_as_float(v & 0xffff0000u));
   }

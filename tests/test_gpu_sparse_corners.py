@@ -78,3 +78,27 @@ def test_attend_at_the_last_position(gpu, T):
     pages[3::7, :, 5:9] = -1
     got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
     check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
+
+
+@pytest.mark.parametrize("T,budget", [(1, 20), (1, 131), (130, 20), (799, 20)])
+def test_attend_infinite_values(gpu, T, budget):
+    """An infinite value that a row sees makes its element infinite, and NaN only together with one
+    of the other sign: also under the largest weight, which is a power of two."""
+    say("attend infinite v", T, budget)
+    g = torch.Generator().manual_seed(T + budget)
+    Hq, Hkv, d, width = (16, 4, 128, 140) if T == 799 else (8, 2, 128, 140)
+    table = tables(g, 1, width, width)
+    kp, vp = pools(g, width, Hkv, d)
+    vp[:, :, :, 5], vp[:, :, :, 6] = INF, -INF         # [blocks, Hkv, 4, d, 4]
+    vp[table[0, 0].long(), :, 0, 7, 0] = INF           # one key
+    vp[table[0, 1].long(), :, 0, 8, 1], vp[table[0, 2].long(), :, 0, 8, 1] = INF, -INF
+    q = torch.randn(T, Hq, d, generator=g).bfloat16()
+    pos = torch.full((T,), width * PAGE - 1, dtype=torch.int32)
+    pages = torch.stack([torch.randperm(width - 3, generator=g)[:budget].sort().values + 3
+                         for _ in range(T * Hkv)]).view(T, Hkv, budget).int()
+    pages[::2, :, 0], pages[1::4, :, 1], pages[::3, :, 2] = 0, 1, 2
+    if T > 1:
+        pos[4], pos[6] = 0, 2                          # one key, whose weight is 1, and three
+    got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
+    check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
+    assert (got[:, :, 5] == INF).all(-1)[pos > 15].all() and (got[:, :, 6] == -INF).all(-1)[pos > 15].all()
