@@ -301,10 +301,34 @@ class VerifyModel:
             # the prior tokens' pages come from elsewhere: their bounds, once
             self.bounds = [torch.zeros(self.blocks, c.kv_heads, 2, c.head_dim, dtype=torch.bfloat16,
                                        device=dev) for _ in range(c.layers)]
-            whole = torch.full((batch,), self.pages * c.page, dtype=torch.int32, device=dev)
-            for k, bounds in zip(self.k_pools, self.bounds):
-                ops.page_bounds(k, bounds, self.table, torch.zeros_like(whole), whole,
-                                self.pages * c.page)
+            # per request, the pages whose bounds may leave out keys behind a block that ended in them
+            self.cut_pages = [set() for _ in range(batch)]
+            self._page_bounds([(0, self.pages)] * batch)
+
+    def _page_bounds(self, spans):
+        """Every layer's bounds of whole pages, from the K pools: request b's pages spans[b][0] ..
+        spans[b][1] - 1."""
+        page = self.cfg.page
+        at = torch.tensor(spans, dtype=torch.int32) * page
+        starts, counts = at[:, 0].to("cuda"), (at[:, 1] - at[:, 0]).to("cuda")
+        for k, bounds in zip(self.k_pools, self.bounds):
+            ops.page_bounds(k, bounds, self.table, starts, counts,
+                            page * max(hi - lo for lo, hi in spans))
+
+    def _stage_bounds(self, contexts, lengths):
+        """Before blocks of `lengths` rows at `contexts`: the bounds of the pages in front of them
+        hold all of their keys again. The cache write keeps those of a block's last page up to the
+        block's last row; a context behind the page sees it whole, without a write of it in between
+        where contexts jump or a staged block is not run."""
+        page, spans = self.cfg.page, []
+        for cut, x, n in zip(self.cut_pages, contexts, lengths):
+            seen = {p for p in cut if p < x // page}
+            spans.append((min(seen), max(seen) + 1) if seen else (0, 0))
+            cut -= seen
+            if (x + n) % page:
+                cut.add((x + n) // page)
+        if any(hi for _, hi in spans):
+            self._page_bounds(spans)
 
     def _random_weights(self, seed, keep_raw):
         c, dev = self.cfg, "cuda"
@@ -440,7 +464,9 @@ class VerifyModel:
         (a length below the block) keep the padded layout [batch, T]: the padding rows write no
         cache (slot -1) and see only themselves, the real rows never see them (ancestor masks
         of the chain), and their logits are ignored. Host-side, outside the captured step; a
-        graph captured with one ragged/uniform shape must be replayed with the same kind."""
+        graph captured with one ragged/uniform shape must be replayed with the same kind. With
+        sparse_pages the contexts may move back and forth, and keys that something else writes into
+        the pools need ops.page_bounds."""
         c, B, T = self.cfg, self.batch, self.cfg.block
         dev = "cuda"
         ids = torch.as_tensor(ids, dtype=torch.int64).view(B, T)
@@ -466,6 +492,7 @@ class VerifyModel:
         self.lens.copy_(torch.tensor([x + T for x in contexts], dtype=torch.int32, device=dev))
         self.lengths = lengths
         if c.sparse_pages:
+            self._stage_bounds(contexts, lengths)
             self.starts.copy_(torch.tensor(contexts, dtype=torch.int32, device=dev))
             self.counts.copy_(torch.tensor(lengths, dtype=torch.int32, device=dev))
             self.row_positions.copy_(torch.tensor(
