@@ -329,7 +329,9 @@ int snowverify_page_bounds(const void* k_pool, void* bounds, const int32_t* tabl
                            const int32_t* starts, const int32_t* counts, int64_t batch,
                            int64_t tokens, int64_t num_kv_heads, int64_t head_size,
                            int64_t table_stride, int64_t blocks, void* stream);
-/* Scratch bytes of snowverify_page_select (table_stride: pages per request, at most 2^17). */
+/* Scratch bytes of snowverify_page_select (table_stride: pages per request, at most 2^17): those of
+ * all rows, or 256 MiB, or those of sixteen rows of every request where these are more. They never
+ * fall where a size grows. */
 int64_t snowverify_page_select_scratch_bytes(int64_t batch, int64_t tokens, int64_t num_heads,
                                              int64_t num_kv_heads, int64_t head_size,
                                              int64_t table_stride);

@@ -1821,12 +1821,23 @@ SelectSpace select_space(int64_t batch, int64_t rows, int64_t Hkv, int64_t D, in
   return s;
 }
 
-// Rows of a request whose scores are in the workspace at a time: sixteen, or what 256 MiB hold.
+// The choice's workspace holds the scores of all rows, or of a part of them: what 256 MiB hold, sixteen
+// at least. It never falls where the shape grows, so that one for the largest shape serves them all.
+int64_t select_bytes(int64_t batch, int64_t tokens, int64_t Hkv, int64_t D, int64_t pages) {
+  const int64_t part = std::max((int64_t)256 << 20, select_space(batch, 16, Hkv, D, pages).bytes);
+  return std::min(part, select_space(batch, tokens, Hkv, D, pages).bytes);
+}
+
+// Rows of a request in a part: a multiple of sixteen, or all.
 int64_t select_rows(int64_t batch, int64_t tokens, int64_t Hkv, int64_t D, int64_t pages) {
-  const int64_t sixteen = select_space(batch, 32, Hkv, D, pages).bytes / 2;
-  int64_t r = sixteen > 0 ? ((int64_t)256 << 20) / sixteen * 16 : tokens;
-  if (r < 16) r = 16;
-  return r < tokens ? r : tokens;
+  const int64_t bytes = select_bytes(batch, tokens, Hkv, D, pages);
+  if (select_space(batch, tokens, Hkv, D, pages).bytes <= bytes) return tokens;
+  int64_t lo = 1, hi = (tokens + 15) / 16;   // row tiles: lo fit (sixteen rows always do), hi do not
+  while (hi - lo > 1) {
+    const int64_t mid = lo + (hi - lo) / 2;
+    (select_space(batch, mid * 16, Hkv, D, pages).bytes <= bytes ? lo : hi) = mid;
+  }
+  return lo * 16;
 }
 
 auto score_form(int64_t D, bool two) {
@@ -1937,10 +1948,9 @@ SV_API int64_t snowverify_page_select_scratch_bytes(int64_t batch, int64_t token
                                                     int64_t num_kv_heads, int64_t head_size,
                                                     int64_t table_stride) {
   if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
-      table_stride > MAX_WIDTH)
+      table_stride > MAX_WIDTH || batch * tokens == 0)
     return 0;
-  const int64_t rows = select_rows(batch, tokens, num_kv_heads, head_size, table_stride);
-  return select_space(batch, rows, num_kv_heads, head_size, table_stride).bytes;
+  return select_bytes(batch, tokens, num_kv_heads, head_size, table_stride);
 }
 
 SV_API int snowverify_page_select(const void* q, const void* bounds, const int32_t* table,

@@ -171,7 +171,8 @@ def page_bounds(k_pool, bounds, table, starts, counts, tokens):
 
 @lru_cache(maxsize=256)
 def page_select_scratch_bytes(batch, tokens, num_heads, num_kv_heads, head_size, width) -> int:
-    """width: pages per request (the table's second dimension)."""
+    """width: pages per request (the table's second dimension). Scratch for the largest of each size
+    is enough for smaller ones."""
     return int(lib.snowverify_page_select_scratch_bytes(batch, tokens, num_heads, num_kv_heads,
                                                         head_size, width))
 

@@ -55,6 +55,32 @@ def test_select_infinite_bounds(gpu, Hq, Hkv, d, T):
     assert torch.equal(got, R.select(q, bounds, table, pos, budget, 1, 2))
 
 
+@pytest.mark.parametrize("T", [150, 140, 129])
+def test_select_two_requests_in_parts_of_row_tiles(gpu, T):
+    """Rows of two requests that pass the scratch in parts of four row tiles, the last part of two,
+    of less than one and of a single row; rows at the parts' ends."""
+    from snowllm_amd import ops
+    say("select in parts", T)
+    g = torch.Generator().manual_seed(T)
+    B, Hq, Hkv, d, width, blocks, budget = 2, 16, 8, 64, 20000, 700, 90
+    need = ops.page_select_scratch_bytes(B, T, Hq, Hkv, d, width)
+    # a part is a multiple of sixteen rows: 64 rows fit, 80 do not
+    fits = [r for r in range(16, T, 16) if ops.page_select_scratch_bytes(B, r, Hq, Hkv, d, width) < need]
+    assert fits == [16, 32, 48, 64]
+    table = torch.randint(0, blocks, (B, width), generator=g, dtype=torch.int32)
+    x = torch.randn(blocks, Hkv, 2, d, generator=g)
+    bounds = torch.stack([x.amin(2), x.amax(2)], 2).bfloat16()
+    q = torch.randn(B * T, Hq, d, generator=g).bfloat16()
+    pos = torch.randint(width // 2 * PAGE, width * PAGE, (B * T,), generator=g, dtype=torch.int32)
+    pos[T - 1], pos[70], pos[T + 65] = width * PAGE - 1, -1, 50 * PAGE
+    got = run_select(q, bounds, table, pos, budget, 1, 2, Hkv)
+    for b in range(B):
+        for t in (0, 15, 16, 63, 64, 65, 70, 127, 128, T - 1):
+            m = b * T + t
+            one = R.select(q[m:m + 1], bounds, table[b:b + 1], pos[m:m + 1], budget, 1, 2)
+            assert torch.equal(got[m:m + 1], one), (b, t)
+
+
 # ------------------------------------------------------------------------------------------
 # attend
 # ------------------------------------------------------------------------------------------

@@ -26,3 +26,24 @@ def test_oracle_scores_of_infinite_bounds():
     assert R.scores(q[0], bounds, table, 0, 0, 1)[1] == INF
     bounds[3, 0, 1, 9] = float("nan")
     assert R.scores(q[0], bounds, table, 0, 0, 1)[3].isnan()
+
+
+def test_select_scratch_grows_with_the_shape():
+    """A workspace that is enough for the longest tables, the most rows and the largest batch is
+    enough for less of each."""
+    from snowllm_amd import ops
+    need = ops.page_select_scratch_bytes
+    assert need(1 << 60, 0, 32, 8, 128, 4096) == 0
+    assert need(1, 1024, 32, 8, 128, 4096) <= need(1, 1024, 32, 8, 128, 8192)
+    assert need(4, 512, 32, 8, 128, 2432) <= need(4, 512, 32, 8, 128, 3840)
+    widths = [0, 1, 15, 16, 17, 100, 513, 1000, 2432, 3840, 4064, 4096, 8192, 13751, 20000, 40000, 1 << 17]
+    rows = [1, 9, 15, 16, 17, 31, 32, 33, 64, 100, 500, 512, 1000, 1024, 2048, 10000]
+    for hkv, d in ((1, 64), (8, 128), (2, 256)):
+        table = torch.tensor([[[need(b, t, 4 * hkv, hkv, d, w) for w in widths] for t in rows]
+                              for b in (1, 2, 3, 4, 16, 64, 256)])
+        for dim in range(3):
+            assert (table.diff(dim=dim) >= 0).all(), (hkv, d, dim)
+        # and 256 MiB do, or sixteen rows' part
+        sixteen = torch.tensor([[[need(b, 16, 4 * hkv, hkv, d, w) for w in widths] for _ in rows]
+                                for b in (1, 2, 3, 4, 16, 64, 256)])
+        assert (table <= sixteen.clamp(min=256 << 20)).all()
