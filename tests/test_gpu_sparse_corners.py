@@ -128,3 +128,108 @@ def test_attend_infinite_values(gpu, T, budget):
     got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
     check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
     assert (got[:, :, 5] == INF).all(-1)[pos > 15].all() and (got[:, :, 6] == -INF).all(-1)[pos > 15].all()
+
+
+# rows of a wave that go over the union of their lists, and the most pages of a union, as the host
+# chooses them: without these the tests below would test the form row by row
+def union_form(G, d, budget):
+    rows = 4 * min(16 // G, 4)
+    return rows, rows * budget // (3 if d == 256 else 4)
+
+
+def unions(pos, pages, G, d):
+    """(pages, pages that several rows share) of the unions of every group of rows and kv head."""
+    T, Hkv, budget = pages.shape
+    R_, _ = union_form(G, d, budget)
+    found = []
+    for h in range(Hkv):
+        for t0 in range(0, T, R_):
+            here = range(t0, min(T, t0 + R_))
+            low = min([int(pos[t]) for t in here if pos[t] >= 0], default=-1)
+            count = {}
+            for t in here:
+                for p in pages[t, h].tolist():
+                    if p >= 0 and pos[t] >= 0 and p <= int(pos[t]) // PAGE:
+                        k = p if p * PAGE + PAGE - 1 <= low else (p, t)
+                        count[k] = count.get(k, 0) + 1
+            found.append((len(count), sum(n > 1 for n in count.values())))
+    return found
+
+
+UNION = [
+    # Hq, Hkv, d, batch, T, width, budget: 2, 2, 4, 4, 4, 4, 3, 3 rows of a matrix instruction
+    (16, 2, 256, 1, 781, 200, 64),
+    (32, 4, 128, 1, 397, 160, 70),
+    (8, 8, 128, 2, 199, 300, 100),
+    (4, 4, 256, 1, 800, 180, 64),
+    (15, 5, 256, 1, 623, 150, 64),
+    (15, 5, 128, 1, 623, 150, 65),
+    (20, 4, 128, 1, 590, 400, 130),
+    (10, 2, 256, 1, 1204, 170, 64),
+]
+
+
+@pytest.mark.parametrize("Hq,Hkv,d,B,T,width,budget", UNION)
+def test_attend_over_unions(gpu, Hq, Hkv, d, B, T, width, budget):
+    """A chunk of a prompt: consecutive positions behind a long context, lists that the rows of a
+    group have mostly in common, the first page and the row's last two in each; a few rows with a
+    short list or none, and padding rows. Rows of some groups against the definition, all rows
+    against the form that takes them one by one."""
+    say("attend over unions", Hq, Hkv, d, B, T, width, budget)
+    g = torch.Generator().manual_seed(budget * 7 + d)
+    G, M = Hq // Hkv, B * T
+    rows, most = union_form(G, d, budget)
+    groups = B * Hkv * ((T + rows - 1) // rows)
+    assert 4 * B * Hkv * T >= 3 * rows * ((groups + 255) // 256 * 256)      # rows fill the workgroups
+    table = tables(g, B, width, B * width + 3)
+    kp, vp = pools(g, B * width + 3, Hkv, d)
+    q = torch.randn(M, Hq, d, generator=g).bfloat16()
+    context = width * PAGE - T - 3
+    pos = (context + torch.arange(T)).repeat(B).int()
+    first = context // PAGE - 1                     # pages 1 .. first - 1 are whole to every row
+    pages = torch.empty(B, T, Hkv, budget, dtype=torch.int32)
+    for b in range(B):
+        for t in range(T):
+            if t % rows == 0:
+                common = [torch.randperm(first - 1, generator=g)[:budget * 5 // 4] + 1 for _ in range(Hkv)]
+            last = int(pos[t]) // PAGE
+            for h in range(Hkv):
+                pick = common[h][torch.randperm(len(common[h]), generator=g)[:budget - 3]].sort().values
+                pages[b, t, h] = torch.cat([torch.tensor([0]), pick, torch.tensor([last - 1, last])])
+    pages = pages.view(M, Hkv, budget)
+    pages[5::41, :, budget // 3:] = -1
+    pages[17::97] = -1
+    pos[rows + 1::89] = -1
+    for b in range(B):
+        found = unions(pos[b * T:(b + 1) * T], pages[b * T:(b + 1) * T], G, d)
+        assert all(n <= most and shared >= budget // 2 for n, shared in found), (most, found)
+    scale = d ** -0.5
+    got = run_attend(q, kp, vp, table, pos, pages, scale)
+    assert (got[pos < 0] == 0).all() and (got[17::97] == 0).all()
+    for b in range(B):
+        some = torch.cat([torch.arange(rows), torch.arange(T // 2 // rows * rows, T // 2 // rows * rows + rows),
+                          torch.arange((T - 1) // rows * rows, T)]) + b * T
+        check_attend(got[some], q[some], kp, vp, table[b:b + 1], pos[some], pages[some], scale)
+        # one by one. Each form is within one rounding (2^-8) and twice the weights' error times the sum
+        # of weights times |v| (at most 1.3 here) of the definition; weights are off by at most (d + 4) u
+        # of a score's terms (at most 14) + 2^-16 + (keys + 64) u = 3.7e-4: 2 . 2 . 3.7e-4 . 1.3 < 2^-9
+        for t0 in range(b * T, b * T + T, 32):
+            part = slice(t0, min(t0 + 32, b * T + T))
+            alone = run_attend(q[part], kp, vp, table[b:b + 1], pos[part], pages[part], scale)
+            err = (alone.double() - got[part].double()).abs()
+            assert (err <= 2.0 ** -7 * alone.double().abs() + 2.0 ** -9).all(), (t0, err.max())
+
+
+@pytest.mark.parametrize("Hq,Hkv,d,T,budget", [(40, 1, 128, 2, 9), (33, 1, 256, 1, 33), (80, 2, 64, 3, 20)])
+def test_attend_three_head_tiles(gpu, Hq, Hkv, d, T, budget):
+    say("attend", Hq, Hkv, d, T, budget)
+    g = torch.Generator().manual_seed(Hq)
+    width = 40
+    table = tables(g, 1, width, width)
+    kp, vp = pools(g, width, Hkv, d)
+    q = torch.randn(T, Hq, d, generator=g).bfloat16()
+    pos = torch.randint(20 * PAGE, width * PAGE, (T,), generator=g, dtype=torch.int32)
+    pages = torch.stack([torch.randperm(width, generator=g)[:budget] for _ in range(T * Hkv)])
+    pages = pages.view(T, Hkv, budget).int()
+    got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
+    check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
