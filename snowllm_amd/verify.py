@@ -413,10 +413,6 @@ class VerifyModel:
         self.ws_h2 = torch.empty(wsH, dtype=torch.uint8, device=dev)
         self.ws_a = torch.empty(ops.gemm_kquant_a_ws_bytes(T, c.heads * c.head_dim),
                                 dtype=torch.uint8, device=dev)
-        self.attn_scratch = torch.empty(
-            ops.paged_attention_explicit_scratch_bytes(B, c.block, c.heads, c.kv_heads,
-                                                       c.head_dim),
-            dtype=torch.uint8, device=dev)
         if c.sparse_pages:
             i32 = dict(dtype=torch.int32, device=dev)
             self.starts, self.counts = torch.zeros(B, **i32), torch.full((B,), c.block, **i32)
@@ -427,6 +423,11 @@ class VerifyModel:
                 ops.page_select_scratch_bytes(*shape, self.pages))
             self.attn_scratch = ops.empty_bytes(
                 max(16, ops.sparse_attention_scratch_bytes(*shape, c.sparse_pages)))
+        else:
+            self.attn_scratch = torch.empty(
+                ops.paged_attention_explicit_scratch_bytes(B, c.block, c.heads, c.kv_heads,
+                                                           c.head_dim),
+                dtype=torch.uint8, device=dev)
         self.ws_tile = ops.gemm_kquant_a_ws_bytes(16, H)   # one 16-row tile of ws_h / ws_h2
         if c.moe:
             E, F, K = c.experts, c.expert_ffn, c.topk
