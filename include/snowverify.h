@@ -355,7 +355,8 @@ int64_t snowverify_sparse_attention_scratch_bytes(int64_t batch, int64_t tokens,
                                                   int64_t head_size, int64_t budget);
 /* out[m, h] = softmax(scale q k^T) v over the keys at positions <= positions[m] of the pages
  * listed for (m, kv head), a page as often as it is listed; entries that are no page, or lie past
- * the row's position, are passed over. A row that sees no key gets zeros. out must not overlap q. */
+ * the row's position, are passed over. A row that sees no key, or only keys that score -inf, gets
+ * zeros. out must not overlap q. */
 int snowverify_sparse_attention(const void* q, const void* k_pool, const void* v_pool, void* out,
                                 const int32_t* table, const int32_t* positions,
                                 const int32_t* pages, int64_t batch, int64_t tokens,

@@ -227,7 +227,7 @@ def sparse_attention(q, k_pool, v_pool, out, table, positions, pages, scale, scr
     q, out [batch*tokens, Hq, d]; positions int32 [batch*tokens]; pages int32 [batch*tokens, Hkv,
     budget] as page_select gives them, or any other: -1, pages past the row's position and pages
     outside the table are passed over, a page counts as often as it is listed, order is free. A
-    row that sees no key gets zeros. out must not overlap q. scratch:
+    row that sees no key, or only keys that score -inf, gets zeros. out must not overlap q. scratch:
     sparse_attention_scratch_bytes (may be 0: None).
     """
     kp, blocks, hkv, d, dev = _pool(k_pool, "K pool")

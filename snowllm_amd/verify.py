@@ -321,7 +321,7 @@ class VerifyModel:
         block's last row; a context behind the page sees it whole, without a write of it in between
         where contexts jump or a staged block is not run."""
         page, spans = self.cfg.page, []
-        for cut, x, n in zip(self.cut_pages, contexts, lengths):
+        for cut, x, n in zip(self.cut_pages, map(int, contexts), lengths):
             seen = {p for p in cut if p < x // page}
             spans.append((min(seen), max(seen) + 1) if seen else (0, 0))
             cut -= seen

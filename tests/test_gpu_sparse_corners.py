@@ -120,7 +120,8 @@ def test_attend_infinite_values(gpu, T, budget):
     vp[table[0, 1].long(), :, 0, 8, 1], vp[table[0, 2].long(), :, 0, 8, 1] = INF, -INF
     q = torch.randn(T, Hq, d, generator=g).bfloat16()
     pos = torch.full((T,), width * PAGE - 1, dtype=torch.int32)
-    pages = torch.stack([torch.randperm(width - 3, generator=g)[:budget].sort().values + 3
+    spread = 60 if T == 799 else width - 3             # few pages: rows over the union of their lists
+    pages = torch.stack([torch.randperm(spread, generator=g)[:budget].sort().values + 3
                          for _ in range(T * Hkv)]).view(T, Hkv, budget).int()
     pages[::2, :, 0], pages[1::4, :, 1], pages[::3, :, 2] = 0, 1, 2
     if T > 1:
@@ -232,4 +233,32 @@ def test_attend_three_head_tiles(gpu, Hq, Hkv, d, T, budget):
     pages = torch.stack([torch.randperm(width, generator=g)[:budget] for _ in range(T * Hkv)])
     pages = pages.view(T, Hkv, budget).int()
     got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
+    check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
+
+
+@pytest.mark.parametrize("T,budget", [(1, 20), (1, 131), (130, 20), (799, 20)])
+def test_attend_keys_of_minus_infinity(gpu, T, budget):
+    """Keys that score -inf have no weight beside others; alone they leave nothing, and the row is
+    zeros as one without keys is."""
+    say("attend -inf keys", T, budget)
+    g = torch.Generator().manual_seed(T + budget)
+    Hq, Hkv, d, width = (16, 4, 128, 140) if T == 799 else (8, 2, 128, 140)
+    table = tables(g, 1, width, width)
+    kp, vp = pools(g, width, Hkv, d)
+    kp[table[0, :70].long(), :, 2, ::3, 5] = -INF
+    kp[table[0, 133].long(), :, 2, :, 5] = -INF
+    q = torch.randn(T, Hq, d, generator=g).abs().bfloat16()
+    pos = torch.full((T,), width * PAGE - 1, dtype=torch.int32)
+    spread = 60 if T == 799 else 133                   # few pages: rows over the union of their lists
+    pages = torch.stack([torch.randperm(spread, generator=g)[:budget].sort().values + 133 - spread
+                         for _ in range(T * Hkv)]).view(T, Hkv, budget).int()
+    alone = torch.zeros(T, dtype=torch.bool)
+    alone[5::9] = True
+    pages[alone], pages[alone, :, 0] = -1, 133
+    if T == 1:
+        got = run_attend(q, kp, vp, table, pos, torch.full_like(pages, 133), d ** -0.5)
+        assert (got == 0).all()
+    got = run_attend(q, kp, vp, table, pos, pages, d ** -0.5)
+    assert (got[alone] == 0).all()
+    pages[alone] = -1                    # zeros by the definition too
     check_attend(got, q, kp, vp, table, pos, pages, d ** -0.5)
