@@ -732,44 +732,35 @@ constexpr int PICK_NEAR = 512;    // pages near the border that are ranked in LD
 constexpr int PICK_KEYS = 16;     // scores a thread keeps in registers
 
 // The 64-bit score's key of one page for row m, by a wave: lane l sums terms l, l + 64, .. in order, then
-// a fixed tree, so that equal pages have equal sums. pn [2 D]: N, then P. Where something of an element
-// is not finite, N low + P high is not the sum over g of max(q_gd low, q_gd high) (N = 0 and low = -inf:
-// NaN for q_gd high), so that element is summed head by head, NaN where one of its products is.
-template <int D>
+// a fixed tree, so that equal pages have equal sums. pn [2 D]: N, then P. N low + P high is not the sum
+// over g of max(q_gd low, q_gd high) where one of them is not finite (N = 0 and low = -inf: NaN for
+// q_gd high); its sum is not finite then, and the page is summed head by head, NaN where a product is.
+// FINITE: there is no such page, as everywhere where E is finite.
+template <int D, bool FINITE>
 __device__ __forceinline__ uint64_t exact_key(const SelectArgs& a, const double* pn, int64_t m, int b, int h,
                                               int64_t page) {
   const int lane = threadIdx.x & 63;
   const int blk = page_block(a.table, a.table_stride, b, page, a.blocks);
   if (blk < 0) return score_key(-__builtin_huge_val());
   const uint16_t* bp = a.bounds + ((int64_t)blk * a.Hkv + h) * 2 * D;
-  double lo[D / 64], hi[D / 64], s = 0.0;
-  bool finite[D / 64];
+  double s = 0.0;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int d = 64 * i + lane;
-    lo[i] = bf16_to_f32(bp[d]);
-    hi[i] = bf16_to_f32(bp[D + d]);
-    finite[i] = __builtin_isfinite(lo[i]) && __builtin_isfinite(hi[i]) && __builtin_isfinite(pn[d]) &&
-                __builtin_isfinite(pn[D + d]);
-  }
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int d = 64 * i + lane;
-    if (finite[i]) {
-      s += pn[d] * lo[i];
-    } else {
-      const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D + d;
-      for (int g = 0; g < a.G; ++g) {
-        const double q = bf16_to_f32(qp[(int64_t)g * D]), x = q * lo[i], y = q * hi[i];
-        s += x > y ? x : y >= x ? y : __builtin_nan("");
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    if (finite[i]) s += pn[D + 64 * i + lane] * hi[i];
+  for (int i = 0; i < 2 * D / 64; ++i) s += pn[64 * i + lane] * (double)bf16_to_f32(bp[64 * i + lane]);
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+  if (!FINITE && !__builtin_isfinite(s)) {   // the same in all lanes
+    const uint16_t* qp = a.q + (m * a.Hq + (int64_t)h * a.G) * D;
+    s = 0.0;
+    int i = lane;
+    asm volatile("" : "+v"(i));   // no address of it is held before
+#pragma unroll 1
+    for (; i < a.G * D; i += 64) {   // head i / D, element i % D
+      const double q = bf16_to_f32(qp[i]), x = q * bf16_to_f32(bp[i % D]), y = q * bf16_to_f32(bp[D + i % D]);
+      s += x > y ? x : y >= x ? y : __builtin_nan("");
+    }
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+  }
   return score_key(s);
 }
 
@@ -1050,7 +1041,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 2) pick_kernel(SelectArgs 
     } else {
       if (near > left) {
         for (uint32_t i = wave; i < near; i += WAVES) {
-          const uint64_t k = exact_key<D>(a, pn, m, b, h, near_page[i]);
+          const uint64_t k = exact_key<D, true>(a, pn, m, b, h, near_page[i]);
           if (lane == 0) near_key[i] = k;
         }
         __syncthreads();
@@ -1071,7 +1062,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 2) pick_kernel(SelectArgs 
     // every candidate in 64 bits, the need-th largest key by radix selection, eight bits a pass
     uint64_t* ex = a.exact + (int64_t)item * a.width;
     for (int i = first + wave; i < end; i += WAVES) {
-      const uint64_t k = exact_key<D>(a, pn, m, b, h, i);
+      const uint64_t k = exact_key<D, false>(a, pn, m, b, h, i);
       if (lane == 0) ex[i] = k;
     }
     __threadfence_block();
