@@ -293,7 +293,7 @@ __device__ __forceinline__ short2v lanes_xor4(short2v v) {
 // loads that are whole 128-byte lines: lane (chunk, token % 4, half chunk). A lane's four tokens meet in
 // its registers, the four lanes of an element by lane swaps. A page's dead tokens are read as its last
 // live one. Bound by the read of K: 220K
-// tokens of two 256-wide heads 54 us (4.7 TB/s) from HBM, 36 from the last-level cache.
+// tokens of two 256-wide heads 52 us (4.9 TB/s) from HBM, 36 from the last-level cache.
 template <int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(
     const uint16_t* __restrict__ k_pool, uint16_t* __restrict__ bounds,
@@ -1424,7 +1424,9 @@ __global__ void __launch_bounds__(64 * ATT_WAVES, 2) attend_kernel(AttendArgs a)
 // Time grows with the union where the per-row form's does not: those 1024 rows take 44 us where all
 // lists are one, 64 with 1.8 lists' pages in a union of eight rows, 86 with 2.6, 121 with 3.9, and row
 // by row 77 to 90. A workgroup whose union is past union_most therefore computes its rows alone, two
-// at a time (92 to 97 us).
+// at a time (92 to 97 us). Lists that the choice gives have little in common where the queries have: of
+// independent ones 5.7 lists' pages in eight rows (136 us, 140 in two calls that go row by row), of
+// queries correlated 0.5 4.1 (133 and 117), 0.9 2.1 (104 and 101), 0.97 1.6 (73 and 97).
 // What is masked in a row's column is multiplied by a weight of zero, so a V that is not finite in a
 // page of another row would reach it as NaN: rows whose result is not finite are computed again alone,
 // as are those of a workgroup with a list in which a page stands twice.
