@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(
 // keys within the page's bounds could have:
 //   s = sum_g sum_d max(q_gd low_d, q_gd high_d) = sum_d P_d high_d + N_d low_d,
 //   P_d = sum_g max(q_gd, 0), N_d = sum_g min(q_gd, 0),
-// one product of 2 D terms per (row, kv head, page) as long as all is finite. The choice turns on differences between nearly
-// equal scores, so it is made on 64-bit sums; but only few pages are near the border. The matrix
-// cores give every page a 32-bit s~ and a bound E on its error; with t the need-th largest s~, a
-// page above t + 2 E is chosen and one below t - 2 E is not whatever the exact sums are, and only
-// the pages between are summed in 64 bits.
+// one product of 2 D terms per (row, kv head, page), as long as all is finite. The choice turns on
+// differences between nearly equal scores, so it is made on 64-bit sums; but only few pages are near
+// the border. The matrix cores give every page a 32-bit s~ and a bound E on its error; with t the
+// need-th largest s~, a page above t + 2 E is chosen and one below t - 2 E is not whatever the exact
+// sums are, and only the pages between are summed in 64 bits.
 //
 // E: with A = sum_d |P_d high_d| + |N_d low_d|,
 //   P and N are 32-bit sums of G values                               <= G 2^-24 A
