@@ -2,7 +2,7 @@
 
 python bench.py [--gpus 1] [--steps K] [--warmup W] [--workload NAME]
 
-Prints ONE JSON line: the metric of BASELINE.json ("verify-step us + accepted tok/s (block 8);
+Prints ONE JSON line: the metric ("verify-step us + accepted tok/s (block 8);
 achieved HBM GB/s vs peak"), the roofline of the dominant kernel (algorithmic bytes per launch
 / its average launch duration, HIP events on the launch stream) and the reference CPU path
 timed on this host's cores over a bounded sample.
@@ -464,7 +464,7 @@ def bench_step(args, name):
             "us": round(us, 3), "alg_bytes": int(sb), "gbs": round(sb / (us * 1e-6) / 1e9, 1)}
     adaptive = None
     if cfg.name == CONFIGS["config4"].name and B == 1:
-        # BASELINE config 1 (the acceptance alone) beside the north-star step
+        # BASELINE config 1 (the acceptance alone) beside the whole step
         kern["config1_acceptance"] = dict(time_acceptance(reps=200), outside_step=True)
         # the draft heads that produce the next proposal, and the adaptive prefix scheduler
         # on this step's measured costs

@@ -80,7 +80,7 @@ class VerifyConfig:
         return (self.heads + 2 * self.kv_heads) * self.head_dim
 
 
-# BASELINE.json configs. RoPE: config 3 rotates the full head (theta 1e6); the 35B-A3B shape
+# The benchmark configurations. RoPE: config 3 rotates the full head (theta 1e6); the 35B-A3B shape
 # rotates 64 of 256 dims (partial_rotary_factor 0.25, as the reference's Qwen3.5 loader
 # requires at snowllm/models/qwen3_5/qwen3_5_weights.py:443-445) with theta 1e7.
 # Config 3's linear weights are Q4_K "as in config 2" (its generator exactly); the MoE shapes
