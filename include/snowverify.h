@@ -364,6 +364,54 @@ int snowverify_sparse_attention(const void* q, const void* k_pool, const void* v
                                 int64_t table_stride, int64_t blocks, int64_t budget, float scale,
                                 void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---- the paged KV cache in 8 bits (extensions) -----------------------------------------
+ * Codes int8 with one fp32 scale per (token, kv head): a head's row x is held as rint(x / s) * s, s =
+ * max(max |x|, 2^-100) / 127; a row with an element that is not finite has a NaN scale and zero codes.
+ * Pages of 16 tokens: K [blocks, Hkv, 4, d/16, 4, 16] (token t is group t / 4, place t % 4), V [blocks,
+ * Hkv, d, 16], scales [blocks, Hkv, 16], all 16-byte aligned; head_size 64, 128 or 256. Rows, table,
+ * starts and counts as in snowverify_kv_append. */
+/* cosv, sinv f32 [rows, half]: cos and sin of pos[axis(i), m] * inv_freq[i], the product in 64 bits. pos
+ * i64 [axes, rows], axes 1 .. 4; sections (host memory): the pairs of every axis, half <= 4096 in all,
+ * one axis behind the other or, interleaved, in turn: pair i is of axis i % axes while i / axes <
+ * sections[axis], of axis 0 else (an axis' last pair must lie below half). */
+int snowverify_rope_axes(const int64_t* pos, const float* inv_freq, float* cosv, float* sinv,
+                         int64_t rows, int64_t half, int64_t axes, const int64_t* sections,
+                         int interleaved, void* stream);
+/* snowverify_kv_append's cache write into a cache in 8 bits: K (normalised, rotated) and V quantised
+ * from fp32, queries rotated alongside. */
+int snowverify_kv8_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const void* q, int64_t q_stride, const float* cos_in,
+                          const float* sin_in, int64_t cs_stride, int64_t half,
+                          const void* q_gamma, const void* k_gamma, float eps, void* k_pool,
+                          void* v_pool, float* k_scale, float* v_scale, void* q_out,
+                          const int32_t* table, const int32_t* starts, const int32_t* counts,
+                          int64_t batch, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                          int64_t head_size, int64_t table_stride, int64_t blocks, void* stream);
+/* k, v bf16 [batch*tokens, num_kv_heads, head_size]: the cached rows at positions starts[b] ..
+ * starts[b] + counts[b] - 1; other rows, and those of pages without a block, are left as they were. */
+int snowverify_kv8_read(const void* k_pool, const void* v_pool, const float* k_scale,
+                        const float* v_scale, const int32_t* table, const int32_t* starts,
+                        const int32_t* counts, void* k, void* v, int64_t batch, int64_t tokens,
+                        int64_t num_kv_heads, int64_t head_size, int64_t table_stride,
+                        int64_t blocks, void* stream);
+/* Scratch bytes of snowverify_kv8_attention (may be 0; few rows may need more than many). */
+int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t num_heads,
+                                               int64_t num_kv_heads, int64_t head_size,
+                                               int64_t table_stride);
+/* out[m, h] = softmax(scale q k^T) v: row t of request b (q row m = b * tokens + t at q + m * q_stride)
+ * sees the positions up to starts[b] + t, or, with tree (ancestor masks u64 [batch*tokens], tokens <=
+ * 64), those before starts[b] and the block's rows j < counts[b] whose bit j is set. Keys in pages
+ * without a block or past the table are passed over; a row that sees none gets zeros; rows past a
+ * request's count are left as they were. out must not overlap q; scale is finite. At most 65535
+ * requests, and 65535 * 16 rows of (tokens * num_heads). */
+int snowverify_kv8_attention(const void* q, int64_t q_stride, const void* k_pool,
+                             const void* v_pool, const float* k_scale, const float* v_scale,
+                             void* out, const int32_t* table, const int32_t* starts,
+                             const int32_t* counts, const uint64_t* tree, int64_t batch,
+                             int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                             int64_t head_size, int64_t table_stride, int64_t blocks, float scale,
+                             void* scratch, int64_t scratch_bytes, void* stream);
+
 /* ---- geometry-driven operator entry points (reference signatures) ---------------------
  * Shapes from the active geometry (see below); weights in the reference's _Weight descriptor
  * (snowllm/ops/inference.py:10-22) holding this library's repacked layouts: k-quant (quant,

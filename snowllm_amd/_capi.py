@@ -117,6 +117,14 @@ _SIGS = [
     ("snowverify_page_select", c_int, [P] * 5 + [c_int64] * 10 + [P, c_int64, S]),
     ("snowverify_sparse_attention_scratch_bytes", c_int64, [c_int64] * 6),
     ("snowverify_sparse_attention", c_int, [P] * 7 + [c_int64] * 8 + [c_float, P, c_int64, S]),
+    # the cache in 8 bits
+    ("snowverify_rope_axes", c_int, [P] * 4 + [c_int64] * 3 + [P, c_int, S]),
+    ("snowverify_kv8_append", c_int, [P, c_int64] * 3 + [P, P, c_int64, c_int64, P, P, c_float] +
+     [P] * 8 + [c_int64] * 7 + [S]),
+    ("snowverify_kv8_read", c_int, [P] * 9 + [c_int64] * 6 + [S]),
+    ("snowverify_kv8_attention_scratch_bytes", c_int64, [c_int64] * 6),
+    ("snowverify_kv8_attention", c_int, [P, c_int64] + [P] * 9 + [c_int64] * 7 +
+     [c_float, P, c_int64, S]),
     # geometry-driven operator entry points (reference signatures)
     ("snowllm_qkv_proj_scratch_bytes", c_int64, [c_int64]),
     ("snowllm_attn_out_scale_oproj_scratch_bytes", c_int64, [c_int64]),

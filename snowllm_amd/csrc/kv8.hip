@@ -1,0 +1,772 @@
+// The paged KV cache in 8 bits, in four operators:
+//
+//   axes      cos and sin of rotary positions with several axes
+//   append    the cache write of new rows: optional per-head RMSNorm, rotate-half RoPE, quantised
+//   read      cached rows back in bf16
+//   attend    softmax attention of new rows over the cache, causal or by ancestor masks
+//
+// The cache: codes of a (token, kv head)'s row x with one fp32 scale,
+//   scale = max(max_d |x_d|, 2^-100) / 127,  code_d = rint(x_d / scale),  x_d ~ code_d * scale,
+// in pages of 16 tokens: K [blocks, Hkv, 4, d/16, 4, 16] (token t is group t / 4, place t % 4), V
+// [blocks, Hkv, d, 16], scales [blocks, Hkv, 16]. A row with an element that is not finite has a NaN
+// scale and zero codes. The least scale keeps 127 / max finite and every scale a normal number; rows
+// below 2^-100 read back as zeros.
+//
+// The layouts are the operands of the attention's 64-key products (v_mfma_i32_16x16x64_i8): 16 bytes
+// of K are 16 elements of a token, 16 bytes of V the 16 tokens of a page at one element, and a lane's
+// scores are of one page, see attend.
+#include "common.h"
+#include "pages.h"
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float LEAST = 0x1p-100f;
+
+struct Cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+};
+
+// ---------------------------------------------------------------------------------------
+// axes
+// ---------------------------------------------------------------------------------------
+constexpr int MAX_AXES = 4;
+
+struct AxesArgs {
+  const int64_t* pos;      // [axes, rows]
+  const float* inv_freq;   // [half]
+  float* cosv;             // [rows, half]
+  float* sinv;
+  int64_t rows;
+  int half, axes, interleaved;
+  int count[MAX_AXES];     // pairs of each axis
+};
+
+// The angle in turns, pos * inv_freq / 2 pi, is taken in 64 bits and without its whole turns: a
+// 32-bit product at position 220000 is off by up to 2^-7 of a radian.
+__global__ void __launch_bounds__(256) axes_kernel(AxesArgs a) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= a.rows * a.half) return;
+  const int64_t m = idx / a.half;
+  const int i = (int)(idx % a.half);
+  int axis = 0;
+  if (a.interleaved) {
+    axis = i % a.axes;
+    if (i / a.axes >= a.count[axis]) axis = 0;
+  } else {
+    int end = a.count[0];
+    while (i >= end && axis + 1 < a.axes) end += a.count[++axis];
+  }
+  const double turns = (double)a.pos[axis * a.rows + m] * (double)a.inv_freq[i] * 0.15915494309189533577;
+  const float x = 2.f * (float)(turns - rint(turns));
+  float s, c;
+  sincospif(x, &s, &c);
+  a.cosv[idx] = c;
+  a.sinv[idx] = s;
+}
+
+// ---------------------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------------------
+struct AppendArgs {
+  QueryRows rows;          // the queries, rotated alongside
+  const uint16_t* k;       // row m, head h at k + m * k_stride + h * D
+  const uint16_t* v;
+  int64_t k_stride, v_stride;
+  const uint16_t* k_gamma; // null: no norm
+  Cache cache;
+  const int32_t* table;
+  int64_t table_stride, blocks;
+  int Hkv, pages;          // pages: most pages that T rows touch
+  int64_t page_wgs;        // workgroups over (request, page, kv head); the rest rotate queries
+};
+
+// Eight codes of a row whose D / 8 threads are neighbours in a wave, and its scale. Magnitudes are
+// compared as integers, in which infinities and NaN lie above all finite values.
+template <int D>
+__device__ __forceinline__ u32x2 quantise(const float (&y)[8], float& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+#pragma unroll
+  for (int s = D / 16; s > 0; s >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)top, s, D / 8);
+    top = o > top ? o : top;
+  }
+  const bool fine = top < 0x7f800000u;
+  const float most = fmaxf(__uint_as_float(top), LEAST);
+  scale = fine ? __fdiv_rn(most, 127.f) : __uint_as_float(0x7fc00000u);
+  const float inv = __fdiv_rn(127.f, most);
+  u32x2 w = {0u, 0u};
+  if (fine)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      w[e >> 2] |= (uint32_t)((int)rintf(y[e] * inv) & 255) << (8 * (e & 3));
+  return w;
+}
+
+// 2 D threads: sixteen rows of D / 8 threads each. A page workgroup owns one (request, page, kv head):
+// its threads take a token's row each, and the codes go through LDS into the page's layout.
+template <int D>
+__global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
+  constexpr int W = D / 8, VP = D + 8;   // VP: pitch of V's codes in LDS, by token
+  __shared__ __attribute__((aligned(16))) uint8_t ks[PAGE * D];
+  __shared__ __attribute__((aligned(16))) uint8_t vs[PAGE * VP];
+  const int tid = threadIdx.x, r = tid / W, c = tid % W;
+  int64_t wg = blockIdx.x;
+  if (wg >= a.page_wgs) {
+    rotate_queries<D>((uint32_t)(wg - a.page_wgs) * 16 + r, c, a.rows);
+    return;
+  }
+  const int h = (int)(wg % a.Hkv);
+  wg /= a.Hkv;
+  const int j = (int)(wg % a.pages), b = (int)(wg / a.pages);
+  const int64_t start = a.rows.starts[b];
+  int64_t count = a.rows.counts[b];
+  count = count < a.rows.T ? count : a.rows.T;
+  if (start < 0 || count <= 0) return;
+  const int64_t page = start / PAGE + j, first = page * PAGE;
+  const int64_t end = start + count;   // one past the last position
+  if (first >= end) return;
+  const int blk = page_block(a.table, a.table_stride, b, page, a.blocks);
+  if (blk < 0) return;
+  const int lo = start > first ? (int)(start - first) : 0;             // new tokens lo .. hi - 1
+  const int hi = end - first < PAGE ? (int)(end - first) : PAGE;
+  const int64_t at = (int64_t)blk * a.Hkv + h;
+  {
+    const bool live = r >= lo && r < hi;
+    const int64_t m = (int64_t)b * a.rows.T + (live ? first + r - start : 0);
+    u32x4 kraw = {0u, 0u, 0u, 0u}, vraw = {0u, 0u, 0u, 0u};
+    if (live) {
+      kraw = *(const u32x4*)(a.k + m * a.k_stride + (int64_t)h * D + 8 * c);
+      vraw = *(const u32x4*)(a.v + m * a.v_stride + (int64_t)h * D + 8 * c);
+    }
+    float y[8], z[8], k_scale, v_scale;
+    rotate_norm_f32<D>(y, kraw, c, a.k_gamma, a.rows.eps, a.rows.cosv + m * a.rows.cs_stride,
+                       a.rows.sinv + m * a.rows.cs_stride, a.rows.half);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[2 * i] = __uint_as_float(vraw[i] << 16);
+      z[2 * i + 1] = __uint_as_float(vraw[i] & 0xffff0000u);
+    }
+    const u32x2 kc = quantise<D>(y, k_scale), vc = quantise<D>(z, v_scale);
+    *(u32x2*)(ks + ((r / 4) * (D / 16) + c / 2) * 64 + (r % 4) * 16 + (c % 2) * 8) = kc;
+    *(u32x2*)(vs + r * VP + 8 * c) = vc;
+    if (live && c == 0) {
+      a.cache.k_scale[at * PAGE + r] = k_scale;
+      a.cache.v_scale[at * PAGE + r] = v_scale;
+    }
+  }
+  __syncthreads();
+  if (tid < D) {   // 16 bytes of K: token, sixteen elements
+    const int tok = tid / (D / 4) * 4 + tid % 4;
+    if (tok >= lo && tok < hi)
+      *(u32x4*)(a.cache.k + at * PAGE * D + tid * 16) = *(const u32x4*)(ks + tid * 16);
+  } else {         // an element of V: its tokens
+    const int d = tid - D;
+    int8_t* vp = a.cache.v + at * PAGE * D + d * 16;
+    if (hi - lo == PAGE) {
+      u32x4 w = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int t = 0; t < PAGE; ++t) w[t >> 2] |= (uint32_t)vs[t * VP + d] << (8 * (t & 3));
+      *(u32x4*)vp = w;
+    } else {
+      for (int t = lo; t < hi; ++t) vp[t] = (int8_t)vs[t * VP + d];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// read
+// ---------------------------------------------------------------------------------------
+struct ReadArgs {
+  Cache cache;
+  const int32_t* table;
+  const int32_t* starts;
+  const int32_t* counts;
+  uint16_t* k;             // [rows, Hkv, D]
+  uint16_t* v;
+  int64_t table_stride, blocks;
+  int T, Hkv, pages;
+};
+
+// Eight codes times their scale, rounded once to bf16.
+__device__ __forceinline__ u32x4 values(u32x2 w, float scale) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x = (int)w[i >> 1] >> (16 * (i & 1));
+    o[i] = pack_bf16x2((float)(int8_t)(x & 255) * scale, (float)(int8_t)(x >> 8 & 255) * scale);
+  }
+  return o;
+}
+
+// 2 D threads take a (request, page, kv head): sixteen rows of D / 8 threads each.
+template <int D>
+__global__ void __launch_bounds__(2 * D) read_kernel(ReadArgs a) {
+  constexpr int W = D / 8, VP = D + 8;
+  __shared__ __attribute__((aligned(16))) uint8_t vs[PAGE * VP];
+  const int tid = threadIdx.x, r = tid / W, c = tid % W;
+  int64_t wg = blockIdx.x;
+  const int h = (int)(wg % a.Hkv);
+  wg /= a.Hkv;
+  const int j = (int)(wg % a.pages), b = (int)(wg / a.pages);
+  const int64_t start = a.starts[b];
+  int64_t count = a.counts[b];
+  count = count < a.T ? count : a.T;
+  if (start < 0 || count <= 0) return;
+  const int64_t page = start / PAGE + j, first = page * PAGE, end = start + count;
+  if (first >= end) return;
+  const int blk = page_block(a.table, a.table_stride, b, page, a.blocks);
+  if (blk < 0) return;
+  const int64_t at = (int64_t)blk * a.Hkv + h;
+  const u32x2 kc = *(const u32x2*)(a.cache.k + at * PAGE * D + ((r / 4) * (D / 16) + c / 2) * 64 +
+                                   (r % 4) * 16 + (c % 2) * 8);
+  const float k_scale = a.cache.k_scale[at * PAGE + r], v_scale = a.cache.v_scale[at * PAGE + r];
+  {   // half of an element's tokens, by token into LDS
+    const int d = tid % D, t0 = tid / D * 8;
+    const u32x2 w = *(const u32x2*)(a.cache.v + at * PAGE * D + d * 16 + t0);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) vs[(t0 + t) * VP + d] = (uint8_t)(w[t >> 2] >> (8 * (t & 3)));
+  }
+  __syncthreads();
+  const int64_t pos = first + r;
+  if (pos < start || pos >= end) return;
+  const int64_t o = (((int64_t)b * a.T + pos - start) * a.Hkv + h) * D + 8 * c;
+  *(u32x4*)(a.k + o) = values(kc, k_scale);
+  *(u32x4*)(a.v + o) = values(*(const u32x2*)(vs + r * VP + 8 * c), v_scale);
+}
+
+// ---------------------------------------------------------------------------------------
+// attend
+// ---------------------------------------------------------------------------------------
+// The products run on the 8-bit matrix cores, exactly, with q and the weights as two 8-bit terms:
+//   q_d = qs (256 h_d + l_d),   qs = max |q| / 32512: off by at most 2^-16 of the row's largest
+//   S_k = scale qs ks_k (256 K_k.h + K_k.l)
+//   p_k = 2^(S_k log2 e - m),   l = sum p_k,   m the row's maximum
+//   p_k vs_k = g (256 a_k + b_k),  g = max_k (p_k vs_k) / 32512 over 64 keys
+//   o_d += g (256 V_d.a + V_d.b),  sums of integers below 2^31, o and l in fp32
+// h and l are signed bytes; a is in 0 .. 127, b signed. Because g follows the 64 keys, a key with a
+// large weight costs only its neighbours' weights precision (2^-16 of it), not the whole context's.
+//
+// Rows of a kv head are ordered r = t * G + g, in tiles of 16 (columns of the products). For four
+// pages, product n = 0 .. 3 takes row 4 q + i of its K operand from page q, token 4 n + i; then the
+// lane (column, q) holds the scores of page q's sixteen tokens, in the order of the V operand's bytes
+// (16 bytes: the page's tokens at one element), and the weights go from the scores' registers into the
+// second product's operand without leaving the lane.
+struct AttendArgs {
+  const uint16_t* q;       // row m at q + m * q_stride
+  int64_t q_stride;
+  Cache cache;
+  uint16_t* out;           // [rows, Hq, D]
+  const int32_t* table;
+  const int32_t* starts;
+  const int32_t* counts;
+  const uint64_t* tree;    // [rows] ancestor masks or null (causal)
+  float* part_o;           // [batch, Hkv, tiles, splits, 16, D]
+  float* part_ml;          // [batch, Hkv, tiles, splits, 16, 2]
+  int64_t table_stride, blocks;
+  int T, Hq, Hkv, G, tiles, splits, chunks;   // chunks: of 64 keys per split
+  float scale;
+};
+
+constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float TERM = 32512.f;      // the largest value of two terms, 127 * 256
+constexpr float RESCALE = 8.f;       // the maximum moves when a score exceeds it by 2^8
+typedef __attribute__((address_space(4))) const int32_t cint32;
+
+// One row of a lane's column: it sees the positions below `end`, and those from there on by its mask.
+struct Row {
+  int64_t m;               // its index, -1: no row
+  int head, end;
+  uint64_t mask;
+};
+
+template <int D>
+struct RowState {
+  floatx4 o[D / 16];
+  float m, l;
+};
+
+template <int D>
+struct Query {
+  i32x4 h[D / 64], l[D / 64];
+  float s;                 // scores' factor, as an exponent of 2
+};
+
+__device__ __forceinline__ int clamp_pos(int64_t p) { return p < 0x7fffffff ? (int)p : 0x7fffffff; }
+
+__device__ __forceinline__ Row find_row(const AttendArgs& a, int b, int h, int r, int64_t start, int count) {
+  Row x{-1, 0, 0, 0};
+  const int t = r / a.G, g = r % a.G;
+  if (t >= count) return x;
+  x.m = (int64_t)b * a.T + t;
+  x.head = h * a.G + g;
+  x.end = clamp_pos(start + t + 1);
+  if (a.tree) {
+    x.end = clamp_pos(start);
+    x.mask = a.tree[x.m] & (count < 64 ? (1ull << count) - 1 : ~0ull);
+  }
+  return x;
+}
+
+// Which of the sixteen positions from p on a row sees, by bits.
+__device__ __forceinline__ uint32_t seen_from(const Row& x, int p) {
+  const int n = x.end - p;
+  if (n >= 16) return 0xffffu;
+  const uint32_t below = n > 0 ? (1u << n) - 1 : 0u;
+  const uint64_t own = n >= 0 ? x.mask << n : -n < 64 ? x.mask >> -n : 0ull;
+  return below | ((uint32_t)own & 0xffffu);
+}
+
+// Four values as two terms each, in bytes: z = x + 2^23 (+ 2^22) + 128 has x + 128 in its low bits, of
+// which the second byte is the larger term and the first, less 128, the smaller.
+__device__ __forceinline__ void two_terms(const float (&z)[4], int& h, int& l) {
+  const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(z[1]), __float_as_uint(z[0]), 0x05010400u);
+  const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(z[3]), __float_as_uint(z[2]), 0x05010400u);
+  l = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+  h = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+template <int D>
+__device__ __forceinline__ void load_query(Query<D>& q, const AttendArgs& a, const Row& x, int quad) {
+  float v[D / 64][16], top = 0.f;
+  const uint16_t* p = a.q + x.m * a.q_stride + (int64_t)x.head * D + 16 * quad;
+#pragma unroll
+  for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      u32x4 w = {0u, 0u, 0u, 0u};
+      if (x.m >= 0) w = *(const u32x4*)(p + 64 * s + 8 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[s][8 * i + 2 * e] = __uint_as_float(w[e] << 16);
+        v[s][8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      }
+    }
+#pragma unroll
+  for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[s][e]));   // NaN stays
+  top = column_maximum(top);
+  // rows below 2^-100 as zeros, as in the cache; an element that is not finite makes the scores NaN
+  const float most = fmaxf(top, LEAST);
+  const float f = a.scale < 0.f ? -TERM / most : TERM / most;
+  // (never zero: a hidden key's -inf times it stays -inf)
+  q.s = top < __builtin_huge_valf()
+            ? fmaxf(most * (1.f / TERM) * __builtin_fabsf(a.scale) * kLog2e, 0x1p-126f)
+            : __uint_as_float(0x7fc00000u);
+#pragma unroll
+  for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float z[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = __builtin_fmaf(v[s][4 * e + i], f, 12583040.f);
+      int h, l;
+      two_terms(z, h, l);
+      q.h[s][e] = h;
+      q.l[s][e] = l;
+    }
+}
+
+// 64 keys, four pages: k(n, s) the K operand of product n, elements 64 s .., v(t) the V operand of
+// elements 16 t .., ks(n) and vs(n) the scales of this lane's page, tokens 4 n ... Where !all, this
+// lane's row sees the tokens of its page whose bits `seen` has.
+template <int D, typename K, typename V, typename KS, typename VS>
+__device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, K k, V v, KS ks, VS vs,
+                                            bool all, uint32_t seen) {
+  constexpr int NS = D / 64;
+  float x[16], p[16];   // scores; scales of V, then weights times them
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const i32x4 w = k(n, s);
+      hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q.h[s], hi, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q.l[s], lo, 0, 0, 0);
+    }
+    const floatx4 f = ks(n), g = vs(n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[4 * n + i] = (float)(int)(((uint32_t)hi[i] << 8) + (uint32_t)lo[i]) * f[i];
+      p[4 * n + i] = g[i];
+    }
+  }
+  if (!all)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {   // the scales of a key that is not there may be anything
+      const bool s = seen >> j & 1;
+      x[j] = s ? x[j] : NEG_INF;
+      p[j] = s ? p[j] : 0.f;
+    }
+  float top = x[0];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+  top *= q.s;
+  // The maximum (the same in the four lanes of a row) moves only when a score is above it by more than
+  // 2^8 somewhere in the wave; weights are at most 2^8 then.
+  if (__builtin_amdgcn_ballot_w64(top > st.m + RESCALE) != 0) {
+    const float m = fmaxf(st.m, column_max(top));
+    const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) st.o[t] *= f;
+    st.l *= f;
+    st.m = m;
+  }
+  const float nm = st.m == NEG_INF ? 0.f : -st.m;
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], q.s, nm));
+    st.l += e;
+    p[j] *= e;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) most = __builtin_elementwise_maximum(most, p[j]);   // NaN stays
+  most = column_maximum(most);
+  const float g = most * (1.f / TERM);
+  const float f = fminf(__builtin_amdgcn_rcpf(g), 0x1p120f);
+  i32x4 pa, pb;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    float z[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = __builtin_fmaf(p[4 * n + i], f, 8388736.f);
+    int h, l;
+    two_terms(z, h, l);
+    pa[n] = h;
+    pb[n] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) {
+    const i32x4 w = v(t), zero = {0, 0, 0, 0};
+    const i32x4 hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pa, zero, 0, 0, 0);
+    const i32x4 lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pb, zero, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      st.o[t][i] = __builtin_fmaf((float)(int)(((uint32_t)hi[i] << 8) + (uint32_t)lo[i]), g, st.o[t][i]);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void clear(RowState<D>& st) {
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) st.o[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  st.m = NEG_INF;
+  st.l = 0.f;
+}
+
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }   // NaN stays
+
+// A (request, kv head, tile, split) each; its waves take the split's 64-key chunks in turn, operands
+// straight from memory, and join their states through LDS.
+constexpr int WAVES = 4;
+
+template <int D>
+__global__ void __launch_bounds__(64 * WAVES) attend_kernel(AttendArgs a) {
+  constexpr int OP = D + 4;   // pitch of a row in LDS
+  __shared__ __attribute__((aligned(16))) float os[WAVES][16][OP];
+  __shared__ float ml[WAVES][16][2];
+  const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
+  const int split = blockIdx.x, tile = (int)(blockIdx.y % (unsigned)a.tiles), h = (int)(blockIdx.y / (unsigned)a.tiles);
+  const int b = blockIdx.z;
+  const int64_t start = a.starts[b];
+  int count = a.counts[b];
+  count = count < a.T ? count : a.T;
+  if (start < 0 || count <= 0 || tile * 16 >= count * a.G) return;
+  const Row x = find_row(a, b, h, tile * 16 + col, start, count);
+  // chunks up to the last position that a row of the tile sees
+  int t_last = (tile * 16 + 15) / a.G;
+  t_last = t_last < count ? t_last : count - 1;
+  int64_t end = a.tree ? start + count : start + t_last + 1;
+  end = end < a.table_stride * PAGE ? end : a.table_stride * PAGE;
+  const int c0 = split * a.chunks;
+  int c1 = (int)((end + 63) / 64);
+  c1 = c1 < c0 + a.chunks ? c1 : c0 + a.chunks;
+  // every row of the tile sees the positions below
+  const int common = a.tree ? clamp_pos(start) : clamp_pos(start + tile * 16 / a.G + 1);
+  RowState<D> st;
+  clear(st);
+  Query<D> q;
+  load_query(q, a, x, quad);
+  const int64_t page_bytes = PAGE * D, block_bytes = page_bytes * a.Hkv;
+  const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
+  const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
+  const int32_t* trow = a.table + (int64_t)b * a.table_stride;
+  for (int c = c0 + wave; c < c1; c += WAVES) {
+    const int64_t pk = 4ll * c + (col >> 2), pv = 4ll * c + quad;
+    int bk = pk < a.table_stride ? trow[pk] : -1, bv = pv < a.table_stride ? trow[pv] : -1;
+    const bool there = bv >= 0 && bv < a.blocks;
+    bk = bk >= 0 && bk < a.blocks ? bk : 0;
+    bv = there ? bv : 0;
+    const int8_t* kp = kh + bk * block_bytes;
+    const int8_t* vp = vh + bv * block_bytes;
+    const float* ksp = a.cache.k_scale + ((int64_t)bv * a.Hkv + h) * PAGE;
+    const float* vsp = a.cache.v_scale + ((int64_t)bv * a.Hkv + h) * PAGE;
+    const bool all = __builtin_amdgcn_ballot_w64(!there) == 0 && c * 64 + 64 <= common;
+    attend_keys<D>(
+        st, q, [&](int n, int s) { return *(const i32x4*)(kp + n * 4 * D + s * 256); },
+        [&](int t) { return *(const i32x4*)(vp + t * 256); },
+        [&](int n) { return *(const floatx4*)(ksp + 4 * n); },
+        [&](int n) { return *(const floatx4*)(vsp + 4 * n); }, all,
+        there ? seen_from(x, c * 64 + quad * 16) : 0u);
+  }
+  float l = column_sum(st.l);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) *(floatx4*)&os[wave][col][t * 16 + 4 * quad] = st.o[t];
+  if (quad == 0) {
+    ml[wave][col][0] = st.m;
+    ml[wave][col][1] = l;
+  }
+  __syncthreads();
+  const int64_t part = (((int64_t)b * a.Hkv + h) * a.tiles + tile) * a.splits + split;
+  for (int u = threadIdx.x; u < 16 * (D / 4); u += 64 * WAVES) {
+    const int r = u / (D / 4), d = u % (D / 4) * 4;
+    const int t = (tile * 16 + r) / a.G;
+    if (t >= count) break;   // rows only grow
+    float m = ml[0][r][0], w[WAVES], sum = 0.f;
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) m = fmaxf(m, ml[i][r][0]);
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      w[i] = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[i][r][0] - m);
+      sum += w[i] * ml[i][r][1];
+      o += w[i] * *(const floatx4*)&os[i][r][d];
+    }
+    if (a.splits == 1) {
+      const float f = inverse_sum(sum);
+      const int64_t row = (int64_t)b * a.T + t;
+      *(u32x2*)(a.out + (row * a.Hq + h * a.G + (tile * 16 + r) % a.G) * D + d) =
+          u32x2{pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f)};
+    } else {
+      *(floatx4*)(a.part_o + (part * 16 + r) * D + d) = o;
+      if (d == 0) {
+        a.part_ml[(part * 16 + r) * 2] = m;
+        a.part_ml[(part * 16 + r) * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+constexpr int JOIN = 256;
+
+template <int D>
+__global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
+  constexpr int W = D / 4, GROUPS = JOIN / W;
+  __shared__ floatx4 red[GROUPS][W];
+  const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = r / a.G;
+  int count = a.counts[b];
+  count = count < a.T ? count : a.T;
+  if (a.starts[b] < 0 || t >= count) return;
+  const int lane = threadIdx.x & 63, g = threadIdx.x / W, c = threadIdx.x % W;
+  const int64_t part = (((int64_t)b * a.Hkv + h) * a.tiles + r / 16) * a.splits;
+  const float* ml = a.part_ml + (part * 16 + r % 16) * 2;
+  float m = NEG_INF, l = 0.f;
+  for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[s * 32]);
+  m = wave_max(m);
+  const float base = m == NEG_INF ? 0.f : m;
+  for (int s = lane; s < a.splits; s += 64) l += __builtin_amdgcn_exp2f(ml[s * 32] - base) * ml[s * 32 + 1];
+  l = wave_sum(l);
+  const float* po = a.part_o + (part * 16 + r % 16) * D + 4 * c;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = g; s < a.splits; s += GROUPS)
+    o += __builtin_amdgcn_exp2f(ml[s * 32] - base) * *(const floatx4*)(po + (int64_t)s * 16 * D);
+  red[g][c] = o;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) o += red[i][c];
+  const float f = inverse_sum(l);
+  const int64_t row = (int64_t)b * a.T + t;
+  *(u32x2*)(a.out + (row * a.Hq + h * a.G + r % a.G) * D + 4 * c) =
+      u32x2{pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f)};
+}
+
+// ---------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------
+constexpr int64_t MAX_PAGES = 1 << 26;   // of a request: positions stay below 2^30
+
+struct Plan {
+  int64_t tiles, splits, chunks;
+};
+
+Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t width) {
+  Plan p;
+  p.tiles = (tokens * (Hq / Hkv) + 15) / 16;
+  const int64_t chunks = (width + 3) / 4, items = batch * Hkv * p.tiles;
+  int64_t splits = items < 512 ? 512 / items : 1;
+  const int64_t most = (chunks + WAVES - 1) / WAVES;
+  splits = splits < most ? splits : most;
+  if (splits < 1) splits = 1;
+  p.chunks = (chunks + splits - 1) / splits;
+  p.chunks = p.chunks > 0 ? p.chunks : 1;
+  p.splits = (chunks + p.chunks - 1) / p.chunks;
+  p.splits = p.splits > 0 ? p.splits : 1;
+  return p;
+}
+
+}  // namespace
+
+SV_API int snowverify_rope_axes(const int64_t* pos, const float* inv_freq, float* cosv, float* sinv,
+                                int64_t rows, int64_t half, int64_t axes, const int64_t* sections,
+                                int interleaved, void* stream) {
+  if (rows < 0 || half <= 0 || half > 4096 || axes <= 0 || axes > MAX_AXES || !sections) return SV_EINVAL;
+  AxesArgs a{pos, inv_freq, cosv, sinv, rows, (int)half, (int)axes, interleaved != 0, {}};
+  int64_t sum = 0;
+  for (int i = 0; i < axes; ++i) {
+    if (sections[i] < 0 || sections[i] > half) return SV_EINVAL;
+    // the pairs in turn: an axis' last pair has to be there
+    if (interleaved && i && sections[i] && i + axes * (sections[i] - 1) >= half) return SV_EINVAL;
+    a.count[i] = (int)sections[i];
+    sum += sections[i];
+  }
+  if (sum != half) return SV_EINVAL;
+  if (rows == 0) return SV_OK;
+  if (!pos || !inv_freq || !cosv || !sinv || rows > ((int64_t)1 << 40) / half) return SV_EINVAL;
+  const int64_t grid = (rows * half + 255) / 256;
+  if (!grid_ok(grid, 256)) return SV_EINVAL;
+  hipLaunchKernelGGL(axes_kernel, dim3((unsigned)grid), dim3(256), 0, S(stream), a);
+  SV_CHECK_LAUNCH();
+  return SV_OK;
+}
+
+SV_API int snowverify_kv8_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                                 const void* q, int64_t q_stride, const float* cos_in,
+                                 const float* sin_in, int64_t cs_stride, int64_t half,
+                                 const void* q_gamma, const void* k_gamma, float eps, void* k_pool,
+                                 void* v_pool, float* k_scale, float* v_scale, void* q_out,
+                                 const int32_t* table, const int32_t* starts, const int32_t* counts,
+                                 int64_t batch, int64_t tokens, int64_t num_heads,
+                                 int64_t num_kv_heads, int64_t head_size, int64_t table_stride,
+                                 int64_t blocks, void* stream) {
+  if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || half < 0 || half % 8 ||
+      2 * half > head_size || table_stride < 0 || blocks < 0 || k_stride % 8 || v_stride % 8 ||
+      q_stride % 8 || (q && !q_out))
+    return SV_EINVAL;
+  if (batch * tokens == 0) return SV_OK;
+  if (!k || !v || (blocks && (!k_pool || !v_pool || !k_scale || !v_scale)) ||
+      (table_stride && !table) || !starts || !counts || (half && (!cos_in || !sin_in)))
+    return SV_EINVAL;
+  AppendArgs a{};
+  a.rows = {(const uint16_t*)q, q_stride, (const uint16_t*)q_gamma, cos_in, sin_in, cs_stride, eps,
+            (uint16_t*)q_out, starts, counts, (int)batch, (int)tokens, (int)num_heads, (int)half};
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.k_gamma = (const uint16_t*)k_gamma;
+  a.cache = {(int8_t*)k_pool, (int8_t*)v_pool, k_scale, v_scale};
+  a.table = table;
+  a.table_stride = table_stride;
+  a.blocks = blocks;
+  a.Hkv = (int)num_kv_heads;
+  a.pages = (int)((tokens + PAGE - 2) / PAGE + 1);
+  a.page_wgs = batch * a.pages * num_kv_heads;
+  const int64_t groups = (num_heads + Q_HEADS - 1) / Q_HEADS;
+  const int64_t grid = a.page_wgs + (q ? (batch * tokens * groups + 15) / 16 : 0);
+  if (!grid_ok(grid, 2 * head_size)) return SV_EINVAL;
+  auto kern = head_size == 64 ? append_kernel<64> : head_size == 128 ? append_kernel<128> : append_kernel<256>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3((unsigned)(2 * head_size)), 0, S(stream), a);
+  SV_CHECK_LAUNCH();
+  return SV_OK;
+}
+
+SV_API int snowverify_kv8_read(const void* k_pool, const void* v_pool, const float* k_scale,
+                               const float* v_scale, const int32_t* table, const int32_t* starts,
+                               const int32_t* counts, void* k, void* v, int64_t batch, int64_t tokens,
+                               int64_t num_kv_heads, int64_t head_size, int64_t table_stride,
+                               int64_t blocks, void* stream) {
+  if (!head_shape_ok(batch, tokens, num_kv_heads, num_kv_heads, head_size) || table_stride < 0 || blocks < 0)
+    return SV_EINVAL;
+  if (batch * tokens == 0) return SV_OK;
+  if ((blocks && (!k_pool || !v_pool || !k_scale || !v_scale)) || (table_stride && !table) || !starts ||
+      !counts || !k || !v)
+    return SV_EINVAL;
+  ReadArgs a{{(int8_t*)k_pool, (int8_t*)v_pool, (float*)k_scale, (float*)v_scale}, table, starts, counts,
+             (uint16_t*)k, (uint16_t*)v, table_stride, blocks, (int)tokens, (int)num_kv_heads,
+             (int)((tokens + PAGE - 2) / PAGE + 1)};
+  const int64_t grid = batch * a.pages * num_kv_heads;
+  if (!grid_ok(grid, 2 * head_size)) return SV_EINVAL;
+  auto kern = head_size == 64 ? read_kernel<64> : head_size == 128 ? read_kernel<128> : read_kernel<256>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3((unsigned)(2 * head_size)), 0, S(stream), a);
+  SV_CHECK_LAUNCH();
+  return SV_OK;
+}
+
+SV_API int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t num_heads,
+                                                      int64_t num_kv_heads, int64_t head_size,
+                                                      int64_t table_stride) {
+  if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
+      table_stride > MAX_PAGES || batch * tokens == 0)
+    return 0;
+  const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
+  return p.splits == 1 ? 0 : batch * num_kv_heads * p.tiles * p.splits * 16 * (head_size + 2) * 4;
+}
+
+SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void* k_pool,
+                                    const void* v_pool, const float* k_scale, const float* v_scale,
+                                    void* out, const int32_t* table, const int32_t* starts,
+                                    const int32_t* counts, const uint64_t* tree, int64_t batch,
+                                    int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                                    int64_t head_size, int64_t table_stride, int64_t blocks, float scale,
+                                    void* scratch, int64_t scratch_bytes, void* stream) {
+  if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
+      table_stride > MAX_PAGES || blocks < 0 || q_stride % 8 || !(scale - scale == 0.f) ||
+      (tree && tokens > 64))
+    return SV_EINVAL;
+  if (batch * tokens == 0) return SV_OK;
+  const int64_t need = snowverify_kv8_attention_scratch_bytes(batch, tokens, num_heads, num_kv_heads,
+                                                              head_size, table_stride);
+  if (!q || !out || out == q || (blocks && (!k_pool || !v_pool || !k_scale || !v_scale)) ||
+      (table_stride && !table) || !starts || !counts || scratch_bytes < need || (need && !scratch))
+    return SV_EINVAL;
+  const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
+  if (batch > 65535 || p.tiles * num_kv_heads > 65535) return SV_ENOTSUP;
+  AttendArgs a{};
+  a.q = (const uint16_t*)q;
+  a.q_stride = q_stride;
+  a.cache = {(int8_t*)k_pool, (int8_t*)v_pool, (float*)k_scale, (float*)v_scale};
+  a.out = (uint16_t*)out;
+  a.table = table;
+  a.starts = starts;
+  a.counts = counts;
+  a.tree = tree;
+  a.table_stride = blocks ? table_stride : 0;   // no block, no key
+  a.blocks = blocks;
+  a.T = (int)tokens;
+  a.Hq = (int)num_heads;
+  a.Hkv = (int)num_kv_heads;
+  a.G = (int)(num_heads / num_kv_heads);
+  a.tiles = (int)p.tiles;
+  a.splits = (int)p.splits;
+  a.chunks = (int)p.chunks;
+  a.scale = scale;
+  a.part_o = (float*)scratch;
+  a.part_ml = (float*)scratch + batch * num_kv_heads * p.tiles * p.splits * 16 * head_size;
+  const dim3 grid((unsigned)p.splits, (unsigned)(p.tiles * num_kv_heads), (unsigned)batch);
+  auto kern = head_size == 64 ? attend_kernel<64> : head_size == 128 ? attend_kernel<128> : attend_kernel<256>;
+  hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), 0, S(stream), a);
+  SV_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    auto join = head_size == 64 ? join_kernel<64> : head_size == 128 ? join_kernel<128> : join_kernel<256>;
+    hipLaunchKernelGGL(join, dim3((unsigned)(tokens * a.G), (unsigned)num_kv_heads, (unsigned)batch),
+                       dim3(JOIN), 0, S(stream), a);
+    SV_CHECK_LAUNCH();
+  }
+  return SV_OK;
+}

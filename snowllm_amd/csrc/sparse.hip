@@ -11,6 +11,7 @@
 // 16, bf16. Bounds are [blocks, Hkv, 2, d] bf16 (minima, then maxima), 1/16 of the K and V bytes.
 // Rows are padded [batch, tokens]; request b's page p is block table[b, p].
 #include "common.h"
+#include "pages.h"
 
 #include <algorithm>
 #include <atomic>
@@ -19,52 +20,7 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short short2v __attribute__((ext_vector_type(2)));
-
-constexpr int PAGE = 16;
-constexpr float kLog2e = 1.4426950408889634f;
-
-inline hipStream_t S(void* s) { return (hipStream_t)s; }
-
-// This wave of the workgroup, as a scalar: what depends on it alone is scalar work then.
-__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
-
-// The block of request b's page, or -1 past the table's width or where the entry is no block.
-__device__ __forceinline__ int page_block(const int32_t* __restrict__ table, int64_t stride, int b,
-                                          int64_t page, int64_t blocks) {
-  if (page < 0 || page >= stride) return -1;
-  const int e = table[(int64_t)b * stride + page];
-  return e >= 0 && e < blocks ? e : -1;
-}
-
-// s_waitcnt on the vector-memory counter only (gfx9 encoding: vmcnt in bits 3:0 and 15:14, no wait on
-// the others).
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt is six bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
-// On the LDS counter only: this wave's LDS reads have ended.
-__device__ __forceinline__ void wait_lgkmcnt0() {
-  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
-}
-
-// Workgroup barrier without the wait of __syncthreads for every load in flight.
-__device__ __forceinline__ void block_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// The maximum over the four lanes of a column (lanes col, col + 16, ..), by row and half-wave swaps.
-__device__ __forceinline__ float column_max(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
-}
 
 // bf16 pairs as signed 16-bit keys in the order of their values (and back: it is an involution),
 // so that minima and maxima are one packed integer operation for two elements. NaNs lie outside
@@ -93,81 +49,23 @@ __device__ __forceinline__ void bounds_words(short2v lo, short2v hi, uint32_t& w
 struct AppendArgs {
   const uint16_t* k;       // row m, head h at k + m * k_stride + h * D
   const uint16_t* v;
-  const uint16_t* q;       // null: no queries
-  int64_t k_stride, v_stride, q_stride;
+  QueryRows rows;          // the queries, rotated alongside
+  int64_t k_stride, v_stride;
   const float* cosv;       // [rows, half], rows cs_stride apart
   const float* sinv;
   int64_t cs_stride;
-  const uint16_t* q_gamma; // null: no norm
-  const uint16_t* k_gamma;
+  const uint16_t* k_gamma; // null: no norm
   float eps;
   uint16_t* k_pool;
   uint16_t* v_pool;
   uint16_t* bounds;        // null: none kept
-  uint16_t* q_out;         // [rows, Hq, D]
   const int32_t* table;
   const int32_t* starts;   // [batch] position of a request's first row
   const int32_t* counts;   // [batch] its rows
   int64_t table_stride, blocks;
-  int batch, T, Hq, Hkv, half, pages;   // pages: most pages that T rows touch
+  int batch, T, Hkv, half, pages;   // pages: most pages that T rows touch
   int64_t page_wgs;        // workgroups over (request, page, kv head); the rest rotate queries
 };
-
-constexpr int Q_HEADS = 4;   // heads of a row that a thread rotates: their loads are in flight at once
-
-// Eight elements d = 8 c .. 8 c + 7 of a head, normalised and rotated; the D / 8 threads of a head
-// are neighbours in one wave. The rotation partner's raw words come from its thread.
-template <int D>
-__device__ __forceinline__ u32x4 rotate_norm(u32x4 raw, int c, const uint16_t* gamma, float eps,
-                                             const float* cr, const float* sr, int half) {
-  constexpr int W = D / 8;
-  float inv = 1.f;
-  if (gamma) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = __uint_as_float(raw[i] << 16), b = __uint_as_float(raw[i] & 0xffff0000u);
-      ss = __builtin_fmaf(a, a, ss);
-      ss = __builtin_fmaf(b, b, ss);
-    }
-#pragma unroll
-    for (int s = W / 2; s > 0; s >>= 1) ss += __shfl_xor(ss, s, W);
-    inv = __frsqrt_rn(ss / (float)D + eps);
-  }
-  const int h8 = half / 8;
-  const int pc = c < h8 ? c + h8 : c < 2 * h8 ? c - h8 : c;
-  u32x4 other;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)raw[i], pc, W);
-  float y[8], z[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    y[2 * i] = __uint_as_float(raw[i] << 16) * inv;
-    y[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u) * inv;
-    z[2 * i] = __uint_as_float(other[i] << 16) * inv;
-    z[2 * i + 1] = __uint_as_float(other[i] & 0xffff0000u) * inv;
-  }
-  if (gamma) {
-    const u32x4 g = *(const u32x4*)(gamma + 8 * c), go = *(const u32x4*)(gamma + 8 * pc);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[2 * i] *= __uint_as_float(g[i] << 16);
-      y[2 * i + 1] *= __uint_as_float(g[i] & 0xffff0000u);
-      z[2 * i] *= __uint_as_float(go[i] << 16);
-      z[2 * i + 1] *= __uint_as_float(go[i] & 0xffff0000u);
-    }
-  }
-  if (c < 2 * h8) {
-    const int i0 = c < h8 ? 8 * c : 8 * (c - h8);
-    const float sign = c < h8 ? -1.f : 1.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(y[e], cr[i0 + e], sign * (z[e] * sr[i0 + e]));
-  }
-  u32x4 o;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
-  return o;
-}
 
 // Bound by its bytes: four prompts of about 2048 rows (q and k normalised, 150 MB) take 41 us (3.7 TB/s),
 // 34 of them in the kernel; one row of a 128-wide model 4 us, a dependent load of start, table entry and
@@ -185,25 +83,7 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   const int tid = threadIdx.x, r = tid / W, c = tid % W;
   int64_t wg = blockIdx.x;
   if (wg >= a.page_wgs) {   // queries: sixteen units of a row and Q_HEADS heads
-    const uint32_t u = (uint32_t)(wg - a.page_wgs) * 16 + r, groups = (uint32_t)(a.Hq + Q_HEADS - 1) / Q_HEADS;
-    const uint32_t m = u / groups;
-    const int head = (int)(u % groups) * Q_HEADS;
-    const uint32_t b = m / (uint32_t)a.T;
-    const bool live = b < (uint32_t)a.batch && (int)(m % (uint32_t)a.T) < a.counts[b] && a.starts[b] >= 0;
-    const int64_t mr = live ? m : 0;
-    const int heads = live ? a.Hq - head < Q_HEADS ? a.Hq - head : Q_HEADS : 0;
-    u32x4 raw[Q_HEADS];
-#pragma unroll
-    for (int i = 0; i < Q_HEADS; ++i) {
-      raw[i] = u32x4{0u, 0u, 0u, 0u};
-      if (i < heads) raw[i] = *(const u32x4*)(a.q + mr * a.q_stride + (int64_t)(head + i) * D + 8 * c);
-    }
-#pragma unroll
-    for (int i = 0; i < Q_HEADS; ++i) {
-      const u32x4 o = rotate_norm<D>(raw[i], c, a.q_gamma, a.eps, a.cosv + mr * a.cs_stride,
-                                     a.sinv + mr * a.cs_stride, a.half);
-      if (i < heads) *(u32x4*)(a.q_out + (mr * a.Hq + head + i) * D + 8 * c) = o;
-    }
+    rotate_queries<D>((uint32_t)(wg - a.page_wgs) * 16 + r, c, a.rows);
     return;
   }
   const int h = (int)(wg % a.Hkv);
@@ -1734,7 +1614,6 @@ __global__ void __launch_bounds__(256, 4) attend_join_kernel(const float* __rest
 // ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
-constexpr int64_t MAX_BATCH_ROWS = 1 << 24;   // batch * tokens
 constexpr int64_t MAX_WIDTH = 1 << 17;        // pages of a request that the choice covers (2M tokens)
 
 // More than 64 KiB of dynamic LDS has to be allowed, once per kernel and device.
@@ -1747,15 +1626,6 @@ hipError_t raise_lds_limit(const void* kernel, std::atomic<uint64_t>& devices, i
   err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (err == hipSuccess) devices |= bit;
   return err;
-}
-
-// A launch holds fewer than 2^32 threads.
-bool grid_ok(int64_t wgs, int64_t threads) { return wgs <= 0xffffffffll / threads; }
-
-bool head_shape_ok(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D) {
-  return batch >= 0 && tokens >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq <= 4096 &&
-         (D == 64 || D == 128 || D == 256) &&
-         (tokens == 0 || batch <= MAX_BATCH_ROWS / tokens);
 }
 
 // Splits of a list: for 256 workgroups, a page pair or more per wave, and whole rounds of the join
@@ -1878,20 +1748,16 @@ SV_API int snowverify_kv_append(const void* k, int64_t k_stride, const void* v, 
   AppendArgs a{};
   a.k = (const uint16_t*)k;
   a.v = (const uint16_t*)v;
-  a.q = (const uint16_t*)q;
   a.k_stride = k_stride;
   a.v_stride = v_stride;
-  a.q_stride = q_stride;
   a.cosv = cos_in;
   a.sinv = sin_in;
   a.cs_stride = cs_stride;
-  a.q_gamma = (const uint16_t*)q_gamma;
   a.k_gamma = (const uint16_t*)k_gamma;
   a.eps = eps;
   a.k_pool = (uint16_t*)k_pool;
   a.v_pool = (uint16_t*)v_pool;
   a.bounds = (uint16_t*)bounds;
-  a.q_out = (uint16_t*)q_out;
   a.table = table;
   a.starts = starts;
   a.counts = counts;
@@ -1899,9 +1765,10 @@ SV_API int snowverify_kv_append(const void* k, int64_t k_stride, const void* v, 
   a.blocks = blocks;
   a.batch = (int)batch;
   a.T = (int)tokens;
-  a.Hq = (int)num_heads;
   a.Hkv = (int)num_kv_heads;
   a.half = (int)half;
+  a.rows = {(const uint16_t*)q, q_stride, (const uint16_t*)q_gamma, cos_in, sin_in, cs_stride, eps,
+            (uint16_t*)q_out, starts, counts, (int)batch, (int)tokens, (int)num_heads, (int)half};
   a.pages = (int)((tokens + PAGE - 2) / PAGE + 1);
   a.page_wgs = batch * a.pages * num_kv_heads;
   const int64_t groups = (num_heads + Q_HEADS - 1) / Q_HEADS;

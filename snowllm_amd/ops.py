@@ -19,6 +19,8 @@ from .attention import (kv_pool_bytes, paged_attention_explicit,  # noqa: F401
                         prefill_q_plan)
 from .sparse import (kv_append, page_bounds, page_select, page_select_scratch_bytes,  # noqa: F401
                      sparse_attention, sparse_attention_scratch_bytes)
+from .kv8 import (Kv8Cache, kv8_append, kv8_attention, kv8_attention_scratch_bytes,  # noqa: F401
+                  kv8_bytes, kv8_cache, kv8_read, rope_axes)
 from .inference import (KQuantProjWeight, KQuantExpertWeight, inference_qkv,  # noqa: F401
                         qkv_proj_scratch_bytes, inference_mlp, mlp_workspace_bytes,
                         inference_moe, inference_moe_norm, inference_moe_workspace_bytes,
