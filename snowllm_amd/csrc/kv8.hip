@@ -303,7 +303,7 @@ struct Query {
   float s;                 // scores' factor, as an exponent of 2
 };
 
-__device__ __forceinline__ int clamp_pos(int64_t p) { return p < 0x7fffffff ? (int)p : 0x7fffffff; }
+__device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
 __device__ __forceinline__ Row find_row(const AttendArgs& a, int b, int h, int r, int64_t start, int count) {
   Row x{-1, 0, 0, 0};
@@ -311,10 +311,13 @@ __device__ __forceinline__ Row find_row(const AttendArgs& a, int b, int h, int r
   if (t >= count) return x;
   x.m = (int64_t)b * a.T + t;
   x.head = h * a.G + g;
-  x.end = clamp_pos(start + t + 1);
+  // nothing past the table
+  const int64_t width = a.table_stride * PAGE;
+  const int64_t end = a.tree ? start : start + t + 1;
+  x.end = (int)(end < width ? end : width);
   if (a.tree) {
-    x.end = clamp_pos(start);
-    x.mask = a.tree[x.m] & (count < 64 ? (1ull << count) - 1 : ~0ull);
+    const int64_t left = width - start, n = count < left ? count : left;
+    x.mask = a.tree[x.m] & (n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0ull);
   }
   return x;
 }
@@ -470,33 +473,104 @@ __device__ __forceinline__ void clear(RowState<D>& st) {
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }   // NaN stays
 
-// A (request, kv head, tile, split) each; its waves take the split's 64-key chunks in turn, operands
-// straight from memory, and join their states through LDS.
+// What a workgroup does: tiles of a (request, kv head) against the chunks c0 .. c1 - 1 of 64 keys.
+struct Share {
+  int64_t start;           // position of the request's first row
+  int64_t end;             // one past the last position that the tiles see
+  int count;               // the request's rows; 0: nothing to do
+  int b, h, split, c0, c1;
+};
+
+// The first tile and how many: chunks up to the last position that one of their rows sees.
+__device__ __forceinline__ Share find_share(const AttendArgs& a, int b, int h, int split, int tile, int tiles) {
+  Share w{a.starts[b], 0, a.counts[b], b, h, split, 0, 0};
+  w.count = w.count < a.T ? w.count : a.T;
+  if (w.start < 0 || w.count <= 0 || tile * 16 >= w.count * a.G) {
+    w.count = 0;
+    return w;
+  }
+  int t_last = ((tile + tiles) * 16 - 1) / a.G;
+  t_last = t_last < w.count ? t_last : w.count - 1;
+  w.end = a.tree ? w.start + w.count : w.start + t_last + 1;
+  w.end = w.end < a.table_stride * PAGE ? w.end : a.table_stride * PAGE;
+  w.c0 = split * a.chunks;
+  w.c1 = (int)((w.end + 63) / 64);
+  w.c1 = w.c1 < w.c0 + a.chunks ? w.c1 : w.c0 + a.chunks;
+  return w;
+}
+
+// Four elements of a row's result.
+template <int D>
+__device__ __forceinline__ void write_out(const AttendArgs& a, const Share& w, int r, int d, floatx4 o, float f) {
+  const int64_t row = (int64_t)w.b * a.T + r / a.G;
+  *(u32x2*)(a.out + (row * a.Hq + w.h * a.G + r % a.G) * D + d) =
+      u32x2{pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f)};
+}
+
+// A row's place among the splits' states.
+__device__ __forceinline__ int64_t part_row(const AttendArgs& a, const Share& w, int r) {
+  return ((((int64_t)w.b * a.Hkv + w.h) * a.tiles + r / 16) * a.splits + w.split) * 16 + r % 16;
+}
+
+__device__ __forceinline__ void write_sums(const AttendArgs& a, int64_t part, float m, float l) {
+  a.part_ml[part * 2] = m;
+  a.part_ml[part * 2 + 1] = l;
+}
+
+// The states of the N waves of each of a workgroup's tiles joined through LDS (os: a pitch of D + 4
+// floats a row): wave n * tiles + i holds part n of tile i.
+template <int D, int N, int THREADS>
+__device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, const RowState<D>& st, float* os,
+                                           float (*ml)[16][2], int wave, int tile, int tiles) {
+  constexpr int P = D + 4;
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const float l = column_sum(st.l);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (wave * 16 + col) * P + t * 16 + 4 * quad) = st.o[t];
+  if (quad == 0) {
+    ml[wave][col][0] = st.m;
+    ml[wave][col][1] = l;
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < tiles * 16 * (D / 4); u += THREADS) {
+    const int i = u / (4 * D), r = u / (D / 4) % 16, d = u % (D / 4) * 4;
+    if ((tile + i) * 16 + r >= w.count * a.G) break;   // rows only grow
+    float m = NEG_INF, sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) m = fmaxf(m, ml[n * tiles + i][r][0]);
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[n * tiles + i][r][0] - m);
+      sum += f * ml[n * tiles + i][r][1];
+      o += f * *(const floatx4*)(os + ((n * tiles + i) * 16 + r) * P + d);
+    }
+    const int row = (tile + i) * 16 + r;
+    if (a.splits == 1) {
+      write_out<D>(a, w, row, d, o, inverse_sum(sum));
+    } else {
+      const int64_t part = part_row(a, w, row);
+      *(floatx4*)(a.part_o + part * D + d) = o;
+      if (d == 0) write_sums(a, part, m, sum);
+    }
+  }
+}
+
+// One or two tiles: a (request, kv head, tile, split) each; the waves take the split's chunks in turn,
+// operands straight from memory, and join their states at the end.
 constexpr int WAVES = 4;
 
 template <int D>
 __global__ void __launch_bounds__(64 * WAVES) attend_kernel(AttendArgs a) {
-  constexpr int OP = D + 4;   // pitch of a row in LDS
-  __shared__ __attribute__((aligned(16))) float os[WAVES][16][OP];
+  __shared__ __attribute__((aligned(16))) float os[WAVES * 16 * (D + 4)];
   __shared__ float ml[WAVES][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int split = blockIdx.x, tile = (int)(blockIdx.y % (unsigned)a.tiles), h = (int)(blockIdx.y / (unsigned)a.tiles);
-  const int b = blockIdx.z;
-  const int64_t start = a.starts[b];
-  int count = a.counts[b];
-  count = count < a.T ? count : a.T;
-  if (start < 0 || count <= 0 || tile * 16 >= count * a.G) return;
-  const Row x = find_row(a, b, h, tile * 16 + col, start, count);
-  // chunks up to the last position that a row of the tile sees
-  int t_last = (tile * 16 + 15) / a.G;
-  t_last = t_last < count ? t_last : count - 1;
-  int64_t end = a.tree ? start + count : start + t_last + 1;
-  end = end < a.table_stride * PAGE ? end : a.table_stride * PAGE;
-  const int c0 = split * a.chunks;
-  int c1 = (int)((end + 63) / 64);
-  c1 = c1 < c0 + a.chunks ? c1 : c0 + a.chunks;
+  const int tile = (int)(blockIdx.y % (unsigned)a.tiles), h = (int)(blockIdx.y / (unsigned)a.tiles), b = blockIdx.z;
+  const Share w = find_share(a, b, h, blockIdx.x, tile, 1);
+  if (w.count == 0) return;
+  const Row x = find_row(a, b, h, tile * 16 + col, w.start, w.count);
   // every row of the tile sees the positions below
-  const int common = a.tree ? clamp_pos(start) : clamp_pos(start + tile * 16 / a.G + 1);
+  const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
   RowState<D> st;
   clear(st);
   Query<D> q;
@@ -505,7 +579,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(AttendArgs a) {
   const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
   const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
   const int32_t* trow = a.table + (int64_t)b * a.table_stride;
-  for (int c = c0 + wave; c < c1; c += WAVES) {
+  for (int c = w.c0 + wave; c < w.c1; c += WAVES) {
     const int64_t pk = 4ll * c + (col >> 2), pv = 4ll * c + quad;
     int bk = pk < a.table_stride ? trow[pk] : -1, bv = pv < a.table_stride ? trow[pv] : -1;
     const bool there = bv >= 0 && bv < a.blocks;
@@ -523,40 +597,148 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(AttendArgs a) {
         [&](int n) { return *(const floatx4*)(vsp + 4 * n); }, all,
         there ? seen_from(x, c * 64 + quad * 16) : 0u);
   }
-  float l = column_sum(st.l);
+  join_waves<D, WAVES, 64 * WAVES>(a, w, st, os, ml, wave, tile, 1);
+}
+
+// More tiles: eight waves share the chunks of a split through a ring in LDS. Wave n * TILES + i takes
+// part n of every step of PARTS chunks for tile i; all eight load (each one plane, K or V, of one of a
+// chunk's four pages, and its scales), STEPS - 1 steps ahead of the products, straight into LDS.
+constexpr int RING_WAVES = 8;
+
+template <int D>
+struct ChunkImage {
+  static constexpr int KS = 16 * D + 64;     // a page of K: four pages' rows on different banks
+  static constexpr int VS = 16 * D;
+  static constexpr int V = 4 * KS, SCALES = V + 4 * VS, BYTES = SCALES + 512;
+  static constexpr int SLOTS = D == 256 ? 4 : 8;
+};
+typedef __attribute__((address_space(3))) void lds_void;
+
+// N times 1 KiB (16 bytes a lane) from src, this lane's place, straight into LDS at dst. Written out
+// because the compiler would wait for every such load before any LDS read; the ring's own waits say
+// which have to be done. To the compiler they are clobbers of memory: its own waits stay good, since
+// loads that it does not know of only make them longer. (m0 is used by nothing else in the kernel.)
+template <int N>
+__device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
+  static_assert(N == 1 || N == 2 || N == 4, "one, two or four loads; their offsets go to both sides");
+  if constexpr (N == 1)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                 "global_load_lds_dwordx4 %1, off offset:1024" ::"s"(dst), "v"(src) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                 "global_load_lds_dwordx4 %1, off offset:1024\n\tglobal_load_lds_dwordx4 %1, off offset:2048\n\t"
+                 "global_load_lds_dwordx4 %1, off offset:3072" ::"s"(dst), "v"(src) : "memory");
+}
+
+template <int D, int PARTS>
+__global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs a) {
+  using G = ChunkImage<D>;
+  constexpr int TILES = RING_WAVES / PARTS, STEPS = G::SLOTS / PARTS, LOADS = PARTS * (D / 64 + 1);
+  static_assert(PARTS == 1 || RING_WAVES * 16 * (D + 4) * 4 <= G::SLOTS * G::BYTES, "states are joined in the ring");
+  __shared__ __attribute__((aligned(16))) uint8_t ring[G::SLOTS * G::BYTES];
+  __shared__ float ml[RING_WAVES][16][2];
+  const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
+  const int groups = (a.tiles + TILES - 1) / TILES;
+  const int tile0 = (int)(blockIdx.y % (unsigned)groups) * TILES, h = (int)(blockIdx.y / (unsigned)groups);
+  const int b = blockIdx.z, tile = tile0 + wave % TILES, part = wave / TILES;
+  const Share w = find_share(a, b, h, blockIdx.x, tile0, TILES);
+  if (w.count == 0) return;
+  const bool idle = tile * 16 >= w.count * a.G;
+  const Row x = idle ? Row{-1, 0, 0, 0} : find_row(a, b, h, tile * 16 + col, w.start, w.count);
+  // every row of the tile sees the positions below `common`, none those from `until` on
+  const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
+  int t_last = (tile * 16 + 15) / a.G;
+  t_last = t_last < w.count ? t_last : w.count - 1;
+  const int until = idle ? 0 : (int)min64(w.end, a.tree ? w.start + w.count : w.start + t_last + 1);
+  RowState<D> st;
+  clear(st);
+  Query<D> q;
+  const int32_t* trow = a.table + (int64_t)b * a.table_stride;
+  const int n_chunks = w.c1 - w.c0;
+  // pages without a block are rare: whether there is one is found once, and each looked up only then
+  bool hole = false;
+  const int pages = (int)min64(4ll * w.c1, (w.end + PAGE - 1) / PAGE);
+  for (int p = 4 * w.c0 + threadIdx.x; p < pages; p += 64 * RING_WAVES) hole |= trow[p] < 0 || trow[p] >= a.blocks;
+  // blocks of this wave's page in 64 chunks, one a lane
+  auto window = [&](int first) {
+    const int64_t p = 4ll * (w.c0 + first + lane) + (wave & 3);
+    const int e = p < a.table_stride ? trow[p] : 0;
+    return e >= 0 && e < a.blocks ? e : 0;
+  };
+  int ids = window(0), ids_from = 0;
+  if (!idle) load_query(q, a, x, quad);
+  const bool holes = __syncthreads_or(hole);
+  const int64_t page_bytes = PAGE * D;
+  const int8_t* plane = wave < 4 ? a.cache.k : a.cache.v;
+  const float* scales = wave < 4 ? a.cache.k_scale : a.cache.v_scale;
+  const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_void*)ring;
+  auto load_step = [&](int step) {
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) *(floatx4*)&os[wave][col][t * 16 + 4 * quad] = st.o[t];
-  if (quad == 0) {
-    ml[wave][col][0] = st.m;
-    ml[wave][col][1] = l;
-  }
-  __syncthreads();
-  const int64_t part = (((int64_t)b * a.Hkv + h) * a.tiles + tile) * a.splits + split;
-  for (int u = threadIdx.x; u < 16 * (D / 4); u += 64 * WAVES) {
-    const int r = u / (D / 4), d = u % (D / 4) * 4;
-    const int t = (tile * 16 + r) / a.G;
-    if (t >= count) break;   // rows only grow
-    float m = ml[0][r][0], w[WAVES], sum = 0.f;
-#pragma unroll
-    for (int i = 1; i < WAVES; ++i) m = fmaxf(m, ml[i][r][0]);
-    floatx4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-      w[i] = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[i][r][0] - m);
-      sum += w[i] * ml[i][r][1];
-      o += w[i] * *(const floatx4*)&os[i][r][d];
-    }
-    if (a.splits == 1) {
-      const float f = inverse_sum(sum);
-      const int64_t row = (int64_t)b * a.T + t;
-      *(u32x2*)(a.out + (row * a.Hq + h * a.G + (tile * 16 + r) % a.G) * D + d) =
-          u32x2{pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f)};
-    } else {
-      *(floatx4*)(a.part_o + (part * 16 + r) * D + d) = o;
-      if (d == 0) {
-        a.part_ml[(part * 16 + r) * 2] = m;
-        a.part_ml[(part * 16 + r) * 2 + 1] = sum;
+    for (int n = 0; n < PARTS; ++n) {
+      int i = step * PARTS + n;
+      i = i < n_chunks ? i : n_chunks - 1;
+      if (i - ids_from >= 64) {   // (uniform)
+        ids_from = i;
+        ids = window(i);
       }
+      const int64_t at = (int64_t)__builtin_amdgcn_readlane(ids, i - ids_from) * a.Hkv + h;
+      const int8_t* src = plane + at * page_bytes + lane * 16;
+      const uint32_t slot = ring_at + (step % STEPS * PARTS + n) * G::BYTES;
+      load_to_lds<D / 64>(src, slot + (wave < 4 ? wave * G::KS : G::V + (wave - 4) * G::VS));
+      if (lane < 4) load_to_lds<1>(scales + at * PAGE + lane * 4, slot + G::SCALES + wave * 64);
+    }
+  };
+  const int steps = (n_chunks + PARTS - 1) / PARTS;
+#pragma unroll
+  for (int s = 0; s < STEPS - 1; ++s)
+    if (s < steps) load_step(s);
+  for (int s = 0; s < steps; ++s) {
+    // this wave's loads of the step have landed ..
+    if (s + STEPS - 2 < steps) wait_vmcnt<(STEPS - 2) * LOADS>();
+    else wait_vmcnt<0>();
+    wait_lgkmcnt0();
+    block_barrier();   // .. and every wave's; the step before is done with its slots
+    if (s + STEPS - 1 < steps) load_step(s + STEPS - 1);
+    const int c = w.c0 + s * PARTS + part;
+    if (c >= w.c1 || c * 64 >= until) continue;   // (uniform over the wave)
+    const uint8_t* slot = ring + (s % STEPS * PARTS + part) * G::BYTES;
+    bool there = true;
+    if (holes) {
+      const int64_t p = 4ll * c + quad;
+      const int e = p < a.table_stride ? trow[p] : -1;
+      there = e >= 0 && e < a.blocks;
+    }
+    const bool all = c * 64 + 64 <= common && (!holes || __builtin_amdgcn_ballot_w64(!there) == 0);
+    const uint8_t* kp = slot + (col >> 2) * G::KS + quad * 64 + (col & 3) * 16;
+    const uint8_t* vp = slot + G::V + quad * G::VS + col * 16;
+    const uint8_t* sp = slot + G::SCALES + quad * 64;
+    attend_keys<D>(
+        st, q, [&](int n, int t) { return *(const i32x4*)(kp + n * 4 * D + t * 256); },
+        [&](int t) { return *(const i32x4*)(vp + t * 256); },
+        [&](int n) { return *(const floatx4*)(sp + 16 * n); },
+        [&](int n) { return *(const floatx4*)(sp + 256 + 16 * n); }, all,
+        there ? seen_from(x, c * 64 + quad * 16) : 0u);
+  }
+  wait_vmcnt<0>();   // no load may still go to LDS
+  if constexpr (PARTS > 1) {
+    __syncthreads();
+    join_waves<D, PARTS, 64 * RING_WAVES>(a, w, st, (float*)ring, ml, wave, tile0, TILES);
+  } else if (!idle) {
+    const float l = column_sum(st.l);
+    if (x.m < 0) return;
+    const int row = tile * 16 + col;
+    if (a.splits == 1) {
+      const float f = inverse_sum(l);
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) write_out<D>(a, w, row, t * 16 + 4 * quad, st.o[t], f);
+    } else {
+      const int64_t part = part_row(a, w, row);
+      float* po = a.part_o + part * D + 4 * quad;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) *(floatx4*)(po + t * 16) = st.o[t];
+      if (quad == 0) write_sums(a, part, st.m, l);
     }
   }
 }
@@ -602,15 +784,17 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
 constexpr int64_t MAX_PAGES = 1 << 26;   // of a request: positions stay below 2^30
 
 struct Plan {
-  int64_t tiles, splits, chunks;
+  int64_t tiles, parts, groups, splits, chunks;   // parts: 0 without the ring
 };
 
 Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t width) {
   Plan p;
   p.tiles = (tokens * (Hq / Hkv) + 15) / 16;
-  const int64_t chunks = (width + 3) / 4, items = batch * Hkv * p.tiles;
-  int64_t splits = items < 512 ? 512 / items : 1;
-  const int64_t most = (chunks + WAVES - 1) / WAVES;
+  p.parts = p.tiles <= 2 ? 0 : p.tiles <= 4 ? 2 : 1;
+  p.groups = p.parts ? (p.tiles + RING_WAVES / p.parts - 1) / (RING_WAVES / p.parts) : p.tiles;
+  const int64_t chunks = (width + 3) / 4, items = batch * Hkv * p.groups, target = p.parts ? 256 : 512;
+  int64_t splits = items < target ? target / items : 1;
+  const int64_t least = p.parts ? p.parts : WAVES, most = (chunks + least - 1) / least;
   splits = splits < most ? splits : most;
   if (splits < 1) splits = 1;
   p.chunks = (chunks + splits - 1) / splits;
@@ -736,7 +920,7 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
       (table_stride && !table) || !starts || !counts || scratch_bytes < need || (need && !scratch))
     return SV_EINVAL;
   const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
-  if (batch > 65535 || p.tiles * num_kv_heads > 65535) return SV_ENOTSUP;
+  if (batch > 65535 || p.groups * num_kv_heads > 65535) return SV_ENOTSUP;
   AttendArgs a{};
   a.q = (const uint16_t*)q;
   a.q_stride = q_stride;
@@ -758,9 +942,12 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   a.scale = scale;
   a.part_o = (float*)scratch;
   a.part_ml = (float*)scratch + batch * num_kv_heads * p.tiles * p.splits * 16 * head_size;
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.tiles * num_kv_heads), (unsigned)batch);
-  auto kern = head_size == 64 ? attend_kernel<64> : head_size == 128 ? attend_kernel<128> : attend_kernel<256>;
-  hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), 0, S(stream), a);
+  const dim3 grid((unsigned)p.splits, (unsigned)(p.groups * num_kv_heads), (unsigned)batch);
+#define KV8_ATTEND(D)                                                              \
+  (p.parts == 0 ? attend_kernel<D> : p.parts == 1 ? attend_ring_kernel<D, 1> : attend_ring_kernel<D, 2>)
+  auto kern = head_size == 64 ? KV8_ATTEND(64) : head_size == 128 ? KV8_ATTEND(128) : KV8_ATTEND(256);
+#undef KV8_ATTEND
+  hipLaunchKernelGGL(kern, grid, dim3(64 * (p.parts ? RING_WAVES : WAVES)), 0, S(stream), a);
   SV_CHECK_LAUNCH();
   if (p.splits > 1) {
     auto join = head_size == 64 ? join_kernel<64> : head_size == 128 ? join_kernel<128> : join_kernel<256>;
