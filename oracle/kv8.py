@@ -6,7 +6,13 @@ import torch
 from .sparse import PAGE, block_of
 
 LEAST = 2.0 ** -100
-GROUP = 64   # keys whose weights share a factor
+GROUP = 64   # keys whose weights share a factor, or twice as many, in whole groups
+
+
+def largest_near(wv, group, groups):
+    """[groups] the largest of wv in a group or the one before or behind it."""
+    most = torch.zeros(groups + 2, dtype=torch.float64).scatter_reduce(0, group + 1, wv, "amax")
+    return torch.maximum(torch.maximum(most[:-2], most[1:-1]), most[2:])
 
 
 def axis_of(i, sections, interleaved):
@@ -75,7 +81,8 @@ def attention(q, cache, table, starts, counts, scale, T, tree=None):
       scores: q as 16-bit integers is off by half of max|q| / 32512 an element; the integer products are
         exact, their conversion, the two factors, the maximum's subtraction and the exponential are 8 u
         of the largest score plus 8 u; twice, for the weights and for their sum              -> 2 e W
-      weights times v's scale as 16-bit integers of the largest of GROUP keys: half a unit each
+      weights times v's scale as 16-bit integers of the largest of one or two GROUPs of keys (which two
+        follows from where the keys are split): half a unit each
       sums of the keys' groups and of splits, in any order: (n / GROUP + 64) u W."""
     u = 2.0 ** -24
     M, Hq, d = q.shape
@@ -111,8 +118,7 @@ def attention(q, cache, table, starts, counts, scale, T, tree=None):
                     off = off + 8 * u * (s.abs().max() + 1)
                     big = w @ val.abs()
                     wv = w * vs[vis, h].double()
-                    most = torch.zeros(n // GROUP + 1, dtype=torch.float64).scatter_reduce(
-                        0, group, wv, "amax")
+                    most = largest_near(wv, group, n // GROUP + 1)
                     out[m, h * G + e] = o
                     error[m, h * G + e] = (2 * off * big + (most[group] / 65024) @ v[vis, h].double().abs()
                                            + (n / GROUP + 64) * u * big)

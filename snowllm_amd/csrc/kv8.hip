@@ -253,10 +253,10 @@ __global__ void __launch_bounds__(2 * D) read_kernel(ReadArgs a) {
 //   q_d = qs (256 h_d + l_d),   qs = max |q| / 32512: off by at most 2^-16 of the row's largest
 //   S_k = scale qs ks_k (256 K_k.h + K_k.l)
 //   p_k = 2^(S_k log2 e - m),   l = sum p_k,   m the row's maximum
-//   p_k vs_k = g (256 a_k + b_k),  g = max_k (p_k vs_k) / 32512 over 64 keys
+//   p_k vs_k = g (256 a_k + b_k),  g = max_k (p_k vs_k) / 32512 over 64 or 128 keys
 //   o_d += g (256 V_d.a + V_d.b),  sums of integers below 2^31, o and l in fp32
-// h and l are signed bytes; a is in 0 .. 127, b signed. Because g follows the 64 keys, a key with a
-// large weight costs only its neighbours' weights precision (2^-16 of it), not the whole context's.
+// h and l are signed bytes; a is in 0 .. 127, b signed. Because g follows the keys, one with a large
+// weight costs only its neighbours' weights precision (2^-16 of it), not the whole context's.
 //
 // Rows of a kv head are ordered r = t * G + g, in tiles of 16 (columns of the products). For four
 // pages, product n = 0 .. 3 takes row 4 q + i of its K operand from page q, token 4 n + i; then the
@@ -383,24 +383,24 @@ __device__ __forceinline__ void load_query(Query<D>& q, const AttendArgs& a, con
     }
 }
 
-// 64 keys, four pages: k(n, s) the K operand of product n, elements 64 s .., v(t) the V operand of
-// elements 16 t .., ks(n) and vs(n) the scales of this lane's page, tokens 4 n ... Where !all, this
-// lane's row sees the tokens of its page whose bits `seen` has.
-template <int D, typename K, typename V, typename KS, typename VS>
+// N times 64 keys (four pages): of the c-th, k(c, n, s) is the K operand of product n, elements 64 s ..,
+// v(c, t) the V operand of elements 16 t .., ks(c, n) and vs(c, n) the scales of this lane's page, tokens
+// 4 n ... Where !all, this lane's row sees the tokens of its pages whose bits `seen` has, sixteen a page.
+template <int D, int N, typename K, typename V, typename KS, typename VS>
 __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, K k, V v, KS ks, VS vs,
                                             bool all, uint32_t seen) {
   constexpr int NS = D / 64;
-  float x[16], p[16];   // scores; scales of V, then weights times them
+  float x[16 * N], p[16 * N];   // scores; scales of V, then weights times them
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
+  for (int n = 0; n < 4 * N; ++n) {
     i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const i32x4 w = k(n, s);
+      const i32x4 w = k(n / 4, n % 4, s);
       hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q.h[s], hi, 0, 0, 0);
       lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q.l[s], lo, 0, 0, 0);
     }
-    const floatx4 f = ks(n), g = vs(n);
+    const floatx4 f = ks(n / 4, n % 4), g = vs(n / 4, n % 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[4 * n + i] = (float)(int)(((uint32_t)hi[i] << 8) + (uint32_t)lo[i]) * f[i];
@@ -409,14 +409,14 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
   }
   if (!all)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {   // the scales of a key that is not there may be anything
+    for (int j = 0; j < 16 * N; ++j) {   // the scales of a key that is not there may be anything
       const bool s = seen >> j & 1;
       x[j] = s ? x[j] : NEG_INF;
       p[j] = s ? p[j] : 0.f;
     }
   float top = x[0];
 #pragma unroll
-  for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+  for (int j = 1; j < 16 * N; ++j) top = fmaxf(top, x[j]);
   top *= q.s;
   // The maximum (the same in the four lanes of a row) moves only when a score is above it by more than
   // 2^8 somewhere in the wave; weights are at most 2^8 then.
@@ -431,32 +431,36 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
   const float nm = st.m == NEG_INF ? 0.f : -st.m;
   float most = 0.f;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < 16 * N; ++j) {
     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], q.s, nm));
     st.l += e;
     p[j] *= e;
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) most = __builtin_elementwise_maximum(most, p[j]);   // NaN stays
+  for (int j = 0; j < 16 * N; ++j) most = __builtin_elementwise_maximum(most, p[j]);   // NaN stays
   most = column_maximum(most);
   const float g = most * (1.f / TERM);
   const float f = fminf(__builtin_amdgcn_rcpf(g), 0x1p120f);
-  i32x4 pa, pb;
+  i32x4 pa[N], pb[N];
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
+  for (int n = 0; n < 4 * N; ++n) {
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = __builtin_fmaf(p[4 * n + i], f, 8388736.f);
     int h, l;
     two_terms(z, h, l);
-    pa[n] = h;
-    pb[n] = l;
+    pa[n / 4][n % 4] = h;
+    pb[n / 4][n % 4] = l;
   }
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) {
-    const i32x4 w = v(t), zero = {0, 0, 0, 0};
-    const i32x4 hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pa, zero, 0, 0, 0);
-    const i32x4 lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pb, zero, 0, 0, 0);
+    i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const i32x4 w = v(c, t);
+      hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pa[c], hi, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pb[c], lo, 0, 0, 0);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       st.o[t][i] = __builtin_fmaf((float)(int)(((uint32_t)hi[i] << 8) + (uint32_t)lo[i]), g, st.o[t][i]);
@@ -517,19 +521,21 @@ __device__ __forceinline__ void write_sums(const AttendArgs& a, int64_t part, fl
   a.part_ml[part * 2 + 1] = l;
 }
 
-// The states of the N waves of each of a workgroup's tiles joined through LDS (os: a pitch of D + 4
-// floats a row): wave n * tiles + i holds part n of tile i.
+// The states of N waves for each of the tiles from `tile` on joined through LDS (os: a pitch of D + 4
+// floats a row): state i * N + n is part n of tile i, -1: this wave has none.
 template <int D, int N, int THREADS>
 __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, const RowState<D>& st, float* os,
-                                           float (*ml)[16][2], int wave, int tile, int tiles) {
+                                           float (*ml)[16][2], int state, int tile, int tiles) {
   constexpr int P = D + 4;
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-  const float l = column_sum(st.l);
+  if (state >= 0) {
+    const float l = column_sum(st.l);
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (wave * 16 + col) * P + t * 16 + 4 * quad) = st.o[t];
-  if (quad == 0) {
-    ml[wave][col][0] = st.m;
-    ml[wave][col][1] = l;
+    for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (state * 16 + col) * P + t * 16 + 4 * quad) = st.o[t];
+    if (quad == 0) {
+      ml[state][col][0] = st.m;
+      ml[state][col][1] = l;
+    }
   }
   __syncthreads();
   for (int u = threadIdx.x; u < tiles * 16 * (D / 4); u += THREADS) {
@@ -537,13 +543,13 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, 
     if ((tile + i) * 16 + r >= w.count * a.G) break;   // rows only grow
     float m = NEG_INF, sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < N; ++n) m = fmaxf(m, ml[n * tiles + i][r][0]);
+    for (int n = 0; n < N; ++n) m = fmaxf(m, ml[i * N + n][r][0]);
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[n * tiles + i][r][0] - m);
-      sum += f * ml[n * tiles + i][r][1];
-      o += f * *(const floatx4*)(os + ((n * tiles + i) * 16 + r) * P + d);
+      const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[i * N + n][r][0] - m);
+      sum += f * ml[i * N + n][r][1];
+      o += f * *(const floatx4*)(os + ((i * N + n) * 16 + r) * P + d);
     }
     const int row = (tile + i) * 16 + r;
     if (a.splits == 1) {
@@ -590,19 +596,21 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(AttendArgs a) {
     const float* ksp = a.cache.k_scale + ((int64_t)bv * a.Hkv + h) * PAGE;
     const float* vsp = a.cache.v_scale + ((int64_t)bv * a.Hkv + h) * PAGE;
     const bool all = __builtin_amdgcn_ballot_w64(!there) == 0 && c * 64 + 64 <= common;
-    attend_keys<D>(
-        st, q, [&](int n, int s) { return *(const i32x4*)(kp + n * 4 * D + s * 256); },
-        [&](int t) { return *(const i32x4*)(vp + t * 256); },
-        [&](int n) { return *(const floatx4*)(ksp + 4 * n); },
-        [&](int n) { return *(const floatx4*)(vsp + 4 * n); }, all,
+    attend_keys<D, 1>(
+        st, q, [&](int, int n, int s) { return *(const i32x4*)(kp + n * 4 * D + s * 256); },
+        [&](int, int t) { return *(const i32x4*)(vp + t * 256); },
+        [&](int, int n) { return *(const floatx4*)(ksp + 4 * n); },
+        [&](int, int n) { return *(const floatx4*)(vsp + 4 * n); }, all,
         there ? seen_from(x, c * 64 + quad * 16) : 0u);
   }
   join_waves<D, WAVES, 64 * WAVES>(a, w, st, os, ml, wave, tile, 1);
 }
 
-// More tiles: eight waves share the chunks of a split through a ring in LDS. Wave n * TILES + i takes
-// part n of every step of PARTS chunks for tile i; all eight load (each one plane, K or V, of one of a
-// chunk's four pages, and its scales), STEPS - 1 steps ahead of the products, straight into LDS.
+// More tiles: eight waves share the chunks of a split, two a step, through a ring in LDS. All eight load
+// (each one plane, K or V, of one of a chunk's four pages, and its scales) straight into LDS, ahead of
+// the products. Of n tiles the first 2 n - 8 have a wave each, which takes both chunks of a step at once
+// (one conversion of the sums for 128 keys); the others two, a chunk each, so that the four SIMDs have
+// about the same to do: six tiles 1.5 tiles a chunk and SIMD instead of 2.
 constexpr int RING_WAVES = 8;
 
 template <int D>
@@ -632,20 +640,24 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
                  "global_load_lds_dwordx4 %1, off offset:3072" ::"s"(dst), "v"(src) : "memory");
 }
 
-template <int D, int PARTS>
+template <int D>
 __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs a) {
   using G = ChunkImage<D>;
-  constexpr int TILES = RING_WAVES / PARTS, STEPS = G::SLOTS / PARTS, LOADS = PARTS * (D / 64 + 1);
-  static_assert(PARTS == 1 || RING_WAVES * 16 * (D + 4) * 4 <= G::SLOTS * G::BYTES, "states are joined in the ring");
+  constexpr int STEPS = G::SLOTS / 2, LOADS = 2 * (D / 64 + 1);
+  static_assert(RING_WAVES * 16 * (D + 4) * 4 <= G::SLOTS * G::BYTES, "states are joined in the ring");
   __shared__ __attribute__((aligned(16))) uint8_t ring[G::SLOTS * G::BYTES];
   __shared__ float ml[RING_WAVES][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int groups = (a.tiles + TILES - 1) / TILES;
-  const int tile0 = (int)(blockIdx.y % (unsigned)groups) * TILES, h = (int)(blockIdx.y / (unsigned)groups);
-  const int b = blockIdx.z, tile = tile0 + wave % TILES, part = wave / TILES;
-  const Share w = find_share(a, b, h, blockIdx.x, tile0, TILES);
+  const int groups = (a.tiles + RING_WAVES - 1) / RING_WAVES;
+  const int tile0 = (int)(blockIdx.y % (unsigned)groups) * RING_WAVES, h = (int)(blockIdx.y / (unsigned)groups);
+  const int b = blockIdx.z;
+  const int tiles = a.tiles - tile0 < RING_WAVES ? a.tiles - tile0 : RING_WAVES;
+  const int whole = 2 * tiles > RING_WAVES ? 2 * tiles - RING_WAVES : 0;   // tiles of one wave
+  const bool pair = wave >= whole;
+  const int tile = tile0 + (pair ? whole + (wave - whole) / 2 : wave), part = (wave - whole) & 1;
+  const Share w = find_share(a, b, h, blockIdx.x, tile0, tiles);
   if (w.count == 0) return;
-  const bool idle = tile * 16 >= w.count * a.G;
+  const bool idle = tile >= tile0 + tiles || tile * 16 >= w.count * a.G;
   const Row x = idle ? Row{-1, 0, 0, 0} : find_row(a, b, h, tile * 16 + col, w.start, w.count);
   // every row of the tile sees the positions below `common`, none those from `until` on
   const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
@@ -676,8 +688,8 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
   const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_void*)ring;
   auto load_step = [&](int step) {
 #pragma unroll
-    for (int n = 0; n < PARTS; ++n) {
-      int i = step * PARTS + n;
+    for (int n = 0; n < 2; ++n) {
+      int i = step * 2 + n;
       i = i < n_chunks ? i : n_chunks - 1;
       if (i - ids_from >= 64) {   // (uniform)
         ids_from = i;
@@ -685,12 +697,12 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
       }
       const int64_t at = (int64_t)__builtin_amdgcn_readlane(ids, i - ids_from) * a.Hkv + h;
       const int8_t* src = plane + at * page_bytes + lane * 16;
-      const uint32_t slot = ring_at + (step % STEPS * PARTS + n) * G::BYTES;
+      const uint32_t slot = ring_at + (step % STEPS * 2 + n) * G::BYTES;
       load_to_lds<D / 64>(src, slot + (wave < 4 ? wave * G::KS : G::V + (wave - 4) * G::VS));
       if (lane < 4) load_to_lds<1>(scales + at * PAGE + lane * 4, slot + G::SCALES + wave * 64);
     }
   };
-  const int steps = (n_chunks + PARTS - 1) / PARTS;
+  const int steps = (n_chunks + 1) / 2;
 #pragma unroll
   for (int s = 0; s < STEPS - 1; ++s)
     if (s < steps) load_step(s);
@@ -701,33 +713,37 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
     wait_lgkmcnt0();
     block_barrier();   // .. and every wave's; the step before is done with its slots
     if (s + STEPS - 1 < steps) load_step(s + STEPS - 1);
-    const int c = w.c0 + s * PARTS + part;
+    const int c = w.c0 + s * 2 + (pair ? part : 0);
     if (c >= w.c1 || c * 64 >= until) continue;   // (uniform over the wave)
-    const uint8_t* slot = ring + (s % STEPS * PARTS + part) * G::BYTES;
-    bool there = true;
+    const bool two = !pair && c + 1 < w.c1 && c * 64 + 64 < until;
+    bool there = true, there2 = true;
     if (holes) {
       const int64_t p = 4ll * c + quad;
-      const int e = p < a.table_stride ? trow[p] : -1;
+      const int e = p < a.table_stride ? trow[p] : -1, e2 = p + 4 < a.table_stride ? trow[p + 4] : -1;
       there = e >= 0 && e < a.blocks;
+      there2 = e2 >= 0 && e2 < a.blocks;
     }
-    const bool all = c * 64 + 64 <= common && (!holes || __builtin_amdgcn_ballot_w64(!there) == 0);
+    const bool all = c * 64 + (two ? 128 : 64) <= common &&
+                     (!holes || __builtin_amdgcn_ballot_w64(!there || (two && !there2)) == 0);
+    uint32_t seen = there ? seen_from(x, c * 64 + quad * 16) : 0u;
+    const uint8_t* slot = ring + (s % STEPS * 2 + (pair ? part : 0)) * G::BYTES;
     const uint8_t* kp = slot + (col >> 2) * G::KS + quad * 64 + (col & 3) * 16;
     const uint8_t* vp = slot + G::V + quad * G::VS + col * 16;
     const uint8_t* sp = slot + G::SCALES + quad * 64;
-    attend_keys<D>(
-        st, q, [&](int n, int t) { return *(const i32x4*)(kp + n * 4 * D + t * 256); },
-        [&](int t) { return *(const i32x4*)(vp + t * 256); },
-        [&](int n) { return *(const floatx4*)(sp + 16 * n); },
-        [&](int n) { return *(const floatx4*)(sp + 256 + 16 * n); }, all,
-        there ? seen_from(x, c * 64 + quad * 16) : 0u);
+    auto k = [&](int i, int n, int t) { return *(const i32x4*)(kp + i * G::BYTES + n * 4 * D + t * 256); };
+    auto v = [&](int i, int t) { return *(const i32x4*)(vp + i * G::BYTES + t * 256); };
+    auto ks = [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 16 * n); };
+    auto vs = [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); };
+    if (two) {
+      seen |= (there2 ? seen_from(x, c * 64 + 64 + quad * 16) : 0u) << 16;
+      attend_keys<D, 2>(st, q, k, v, ks, vs, all, seen);
+    } else {
+      attend_keys<D, 1>(st, q, k, v, ks, vs, all, seen);
+    }
   }
   wait_vmcnt<0>();   // no load may still go to LDS
-  if constexpr (PARTS > 1) {
-    __syncthreads();
-    join_waves<D, PARTS, 64 * RING_WAVES>(a, w, st, (float*)ring, ml, wave, tile0, TILES);
-  } else if (!idle) {
-    const float l = column_sum(st.l);
-    if (x.m < 0) return;
+  const float l = column_sum(st.l);
+  if (!pair && x.m >= 0) {
     const int row = tile * 16 + col;
     if (a.splits == 1) {
       const float f = inverse_sum(l);
@@ -741,14 +757,20 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
       if (quad == 0) write_sums(a, part, st.m, l);
     }
   }
+  if (whole < tiles) {
+    __syncthreads();   // the ring is free
+    join_waves<D, 2, 64 * RING_WAVES>(a, w, st, (float*)ring, ml, pair && tile < tile0 + tiles ? wave - whole : -1,
+                                      tile0 + whole, tiles - whole);
+  }
 }
 
-// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
-constexpr int JOIN = 256;
+// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. The threads of a row's
+// elements, D / 4, come in GROUPS, each with its splits, the loads of eight in flight.
+constexpr int JOIN = 512;
 
 template <int D>
 __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
-  constexpr int W = D / 4, GROUPS = JOIN / W;
+  constexpr int W = D / 4, GROUPS = JOIN / W, AHEAD = 8;
   __shared__ floatx4 red[GROUPS][W];
   const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = r / a.G;
   int count = a.counts[b];
@@ -757,16 +779,31 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
   const int lane = threadIdx.x & 63, g = threadIdx.x / W, c = threadIdx.x % W;
   const int64_t part = (((int64_t)b * a.Hkv + h) * a.tiles + r / 16) * a.splits;
   const float* ml = a.part_ml + (part * 16 + r % 16) * 2;
+  const float* po = a.part_o + (part * 16 + r % 16) * D + 4 * c;
+  floatx4 x[AHEAD];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int s = s0 + i * GROUPS;
+      if (s < a.splits) x[i] = *(const floatx4*)(po + (int64_t)s * 16 * D);
+    }
+  };
+  fetch(g);   // with the maxima and sums: one round trip
   float m = NEG_INF, l = 0.f;
   for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[s * 32]);
   m = wave_max(m);
   const float base = m == NEG_INF ? 0.f : m;
   for (int s = lane; s < a.splits; s += 64) l += __builtin_amdgcn_exp2f(ml[s * 32] - base) * ml[s * 32 + 1];
   l = wave_sum(l);
-  const float* po = a.part_o + (part * 16 + r % 16) * D + 4 * c;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = g; s < a.splits; s += GROUPS)
-    o += __builtin_amdgcn_exp2f(ml[s * 32] - base) * *(const floatx4*)(po + (int64_t)s * 16 * D);
+  for (int s0 = g; s0 < a.splits; s0 += AHEAD * GROUPS) {
+    if (s0 != g) fetch(s0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int s = s0 + i * GROUPS;
+      if (s < a.splits) o += __builtin_amdgcn_exp2f(ml[s * 32] - base) * x[i];
+    }
+  }
   red[g][c] = o;
   __syncthreads();
   if (g != 0) return;
@@ -784,17 +821,18 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
 constexpr int64_t MAX_PAGES = 1 << 26;   // of a request: positions stay below 2^30
 
 struct Plan {
-  int64_t tiles, parts, groups, splits, chunks;   // parts: 0 without the ring
+  int64_t tiles, groups, splits, chunks;
+  bool ring;
 };
 
 Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t width) {
   Plan p;
   p.tiles = (tokens * (Hq / Hkv) + 15) / 16;
-  p.parts = p.tiles <= 2 ? 0 : p.tiles <= 4 ? 2 : 1;
-  p.groups = p.parts ? (p.tiles + RING_WAVES / p.parts - 1) / (RING_WAVES / p.parts) : p.tiles;
-  const int64_t chunks = (width + 3) / 4, items = batch * Hkv * p.groups, target = p.parts ? 256 : 512;
+  p.ring = p.tiles > 2;
+  p.groups = p.ring ? (p.tiles + RING_WAVES - 1) / RING_WAVES : p.tiles;
+  const int64_t chunks = (width + 3) / 4, items = batch * Hkv * p.groups, target = p.ring ? 256 : 512;
   int64_t splits = items < target ? target / items : 1;
-  const int64_t least = p.parts ? p.parts : WAVES, most = (chunks + least - 1) / least;
+  const int64_t least = p.ring ? 2 : WAVES, most = (chunks + least - 1) / least;
   splits = splits < most ? splits : most;
   if (splits < 1) splits = 1;
   p.chunks = (chunks + splits - 1) / splits;
@@ -943,11 +981,10 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   a.part_o = (float*)scratch;
   a.part_ml = (float*)scratch + batch * num_kv_heads * p.tiles * p.splits * 16 * head_size;
   const dim3 grid((unsigned)p.splits, (unsigned)(p.groups * num_kv_heads), (unsigned)batch);
-#define KV8_ATTEND(D)                                                              \
-  (p.parts == 0 ? attend_kernel<D> : p.parts == 1 ? attend_ring_kernel<D, 1> : attend_ring_kernel<D, 2>)
-  auto kern = head_size == 64 ? KV8_ATTEND(64) : head_size == 128 ? KV8_ATTEND(128) : KV8_ATTEND(256);
-#undef KV8_ATTEND
-  hipLaunchKernelGGL(kern, grid, dim3(64 * (p.parts ? RING_WAVES : WAVES)), 0, S(stream), a);
+  auto few = head_size == 64 ? attend_kernel<64> : head_size == 128 ? attend_kernel<128> : attend_kernel<256>;
+  auto more = head_size == 64 ? attend_ring_kernel<64>
+              : head_size == 128 ? attend_ring_kernel<128> : attend_ring_kernel<256>;
+  hipLaunchKernelGGL(p.ring ? more : few, grid, dim3(64 * (p.ring ? RING_WAVES : WAVES)), 0, S(stream), a);
   SV_CHECK_LAUNCH();
   if (p.splits > 1) {
     auto join = head_size == 64 ? join_kernel<64> : head_size == 128 ? join_kernel<128> : join_kernel<256>;

@@ -382,7 +382,9 @@ def test_attention_of_a_sink_and_small_weights(gpu):
     got = run_attention(*on_gpu(q, cache, table, ints([n]), ints([1])), 1.0)
     want, error, live = R.attention(q, cache, table, ints([n]), ints([1]), 1.0, 1)
     check_attention(got, want, error, live)
-    assert (error[0] < 1e-3).all()
+    # 192 keys at most share the sink's factor: 192 * 33 * 0.47 * 0.02 / 65024 = 9e-4, and 2e-4 from the
+    # scores; with one factor for all 6000 it were 3e-2
+    assert (error[0] < 2e-3).all()
 
 
 @pytest.mark.parametrize("Hq,Hkv,d,T,start", [(16, 2, 256, 11, 20011), (8, 2, 64, 1, 33333), (32, 8, 128, 9, 9001)])
@@ -427,7 +429,7 @@ def whole_tree_row(q, cache, table, start, T, t, masks, scale):
             big = w @ val.abs()
             wv = w * vs[vis, h].double()
             group = torch.arange(n)[vis] // R.GROUP
-            most = torch.zeros(n // R.GROUP + 1, dtype=torch.float64).scatter_reduce(0, group, wv, "amax")
+            most = R.largest_near(wv, group, n // R.GROUP + 1)
             out[0, h * G + e] = w @ val
             error[0, h * G + e] = (2 * off * big + (most[group] / 65024) @ v[vis, h].double().abs()
                                    + (n / R.GROUP + 64) * U * big)
