@@ -18,6 +18,8 @@
 #include "common.h"
 #include "pages.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -293,7 +295,7 @@ struct Row {
 
 template <int D>
 struct RowState {
-  floatx4 o[D / 16];
+  float o[D / 4];          // elements 16 t + 4 quad + i at 4 t + i
   float m, l;
 };
 
@@ -391,29 +393,50 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
                                             bool all, uint32_t seen) {
   constexpr int NS = D / 64;
   float x[16 * N], p[16 * N];   // scores; scales of V, then weights times them
+  // stage n loads what product n + 1 takes, issues product n and converts product n - 2, whose sums are
+  // there by then
+  {
+    i32x4 w[2][NS], hi[3], lo[3];
+    floatx4 f[3];
 #pragma unroll
-  for (int n = 0; n < 4 * N; ++n) {
-    i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+    for (int n = -1; n < 4 * N + 2; ++n) {
+      if (n + 1 < 4 * N) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const i32x4 w = k(n / 4, n % 4, s);
-      hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q.h[s], hi, 0, 0, 0);
-      lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, q.l[s], lo, 0, 0, 0);
-    }
-    const floatx4 f = ks(n / 4, n % 4), g = vs(n / 4, n % 4);
+        for (int s = 0; s < NS; ++s) w[(n + 1) & 1][s] = k((n + 1) / 4, (n + 1) % 4, s);
+      }
+      if (n >= 0 && n < 4 * N) {
+        f[n % 3] = ks(n / 4, n % 4);
+        hi[n % 3] = lo[n % 3] = i32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[4 * n + i] = (float)(int)(((uint32_t)hi[i] << 8) + (uint32_t)lo[i]) * f[i];
-      p[4 * n + i] = g[i];
+        for (int s = 0; s < NS; ++s) {
+          hi[n % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[n & 1][s], q.h[s], hi[n % 3], 0, 0, 0);
+          lo[n % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[n & 1][s], q.l[s], lo[n % 3], 0, 0, 0);
+        }
+      }
+      if (n >= 2) {
+        const int m = n - 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[4 * m + i] = (float)(int)(((uint32_t)hi[m % 3][i] << 8) + (uint32_t)lo[m % 3][i]) * f[m % 3][i];
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if (!all)
+#pragma unroll
+  for (int n = 0; n < 4 * N; ++n) {
+    const floatx4 g = vs(n / 4, n % 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[4 * n + i] = g[i];
+  }
+  if (!all) {
+    asm volatile("" : "+v"(seen));   // stays a branch: most keys are seen by every row
 #pragma unroll
     for (int j = 0; j < 16 * N; ++j) {   // the scales of a key that is not there may be anything
       const bool s = seen >> j & 1;
       x[j] = s ? x[j] : NEG_INF;
       p[j] = s ? p[j] : 0.f;
     }
+  }
   float top = x[0];
 #pragma unroll
   for (int j = 1; j < 16 * N; ++j) top = fmaxf(top, x[j]);
@@ -424,7 +447,7 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
     const float m = fmaxf(st.m, column_max(top));
     const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) st.o[t] *= f;
+    for (int d = 0; d < D / 4; ++d) st.o[d] *= f;
     st.l *= f;
     st.m = m;
   }
@@ -441,7 +464,9 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
   most = column_maximum(most);
   const float g = most * (1.f / TERM);
   const float f = fminf(__builtin_amdgcn_rcpf(g), 0x1p120f);
-  i32x4 pa[N], pb[N];
+  i32x4 pa[N], pb[N], w[2][N];
+#pragma unroll
+  for (int c = 0; c < N; ++c) w[0][c] = v(c, 0);
 #pragma unroll
   for (int n = 0; n < 4 * N; ++n) {
     float z[4];
@@ -452,27 +477,45 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
     pa[n / 4][n % 4] = h;
     pb[n / 4][n % 4] = l;
   }
+  __builtin_amdgcn_sched_barrier(0);
+  constexpr int T = D / 16;
+  i32x4 hi[3], lo[3];
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) {
-    i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+  for (int t = 0; t < T + 2; ++t) {
+    if (t + 1 < T) {
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const i32x4 w = v(c, t);
-      hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pa[c], hi, 0, 0, 0);
-      lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, pb[c], lo, 0, 0, 0);
+      for (int c = 0; c < N; ++c) w[(t + 1) & 1][c] = v(c, t + 1);
     }
+    if (t < T) {
+      hi[t % 3] = lo[t % 3] = i32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      st.o[t][i] = __builtin_fmaf((float)(int)(((uint32_t)hi[i] << 8) + (uint32_t)lo[i]), g, st.o[t][i]);
+      for (int c = 0; c < N; ++c) {
+        hi[t % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t & 1][c], pa[c], hi[t % 3], 0, 0, 0);
+        lo[t % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t & 1][c], pb[c], lo[t % 3], 0, 0, 0);
+      }
+    }
+    if (t >= 2) {
+      const int m = t - 2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        st.o[4 * m + i] = __builtin_fmaf((float)(int)(((uint32_t)hi[m % 3][i] << 8) + (uint32_t)lo[m % 3][i]), g,
+                                         st.o[4 * m + i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 template <int D>
 __device__ __forceinline__ void clear(RowState<D>& st) {
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) st.o[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < D / 4; ++d) st.o[d] = 0.f;
   st.m = NEG_INF;
   st.l = 0.f;
+}
+
+template <int D>
+__device__ __forceinline__ floatx4 elements(const RowState<D>& st, int t) {
+  return floatx4{st.o[4 * t], st.o[4 * t + 1], st.o[4 * t + 2], st.o[4 * t + 3]};
 }
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }   // NaN stays
@@ -531,7 +574,7 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, 
   if (state >= 0) {
     const float l = column_sum(st.l);
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (state * 16 + col) * P + t * 16 + 4 * quad) = st.o[t];
+    for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (state * 16 + col) * P + t * 16 + 4 * quad) = elements(st, t);
     if (quad == 0) {
       ml[state][col][0] = st.m;
       ml[state][col][1] = l;
@@ -706,41 +749,45 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
 #pragma unroll
   for (int s = 0; s < STEPS - 1; ++s)
     if (s < steps) load_step(s);
-  for (int s = 0; s < steps; ++s) {
-    // this wave's loads of the step have landed ..
-    if (s + STEPS - 2 < steps) wait_vmcnt<(STEPS - 2) * LOADS>();
-    else wait_vmcnt<0>();
-    wait_lgkmcnt0();
-    block_barrier();   // .. and every wave's; the step before is done with its slots
-    if (s + STEPS - 1 < steps) load_step(s + STEPS - 1);
-    const int c = w.c0 + s * 2 + (pair ? part : 0);
-    if (c >= w.c1 || c * 64 >= until) continue;   // (uniform over the wave)
-    const bool two = !pair && c + 1 < w.c1 && c * 64 + 64 < until;
-    bool there = true, there2 = true;
-    if (holes) {
-      const int64_t p = 4ll * c + quad;
-      const int e = p < a.table_stride ? trow[p] : -1, e2 = p + 4 < a.table_stride ? trow[p + 4] : -1;
-      there = e >= 0 && e < a.blocks;
-      there2 = e2 >= 0 && e2 < a.blocks;
+  // a wave's steps: N = 2, both chunks of each, or 1, the part-th
+  auto walk = [&](auto chunks) {
+    constexpr int N = decltype(chunks)::value;
+    for (int s = 0; s < steps; ++s) {
+      // this wave's loads of the step have landed ..
+      if (s + STEPS - 2 < steps) wait_vmcnt<(STEPS - 2) * LOADS>();
+      else wait_vmcnt<0>();
+      wait_lgkmcnt0();
+      block_barrier();   // .. and every wave's; the step before is done with its slots
+      if (s + STEPS - 1 < steps) load_step(s + STEPS - 1);
+      const int o = N == 2 ? 0 : part, c = w.c0 + s * 2 + o;
+      if (c >= w.c1 || c * 64 >= until) continue;   // (uniform over the wave)
+      uint32_t seen = 0, there = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        bool page = c + i < w.c1;
+        if (holes && page) {
+          const int64_t p = 4ll * (c + i) + quad;
+          const int e = p < a.table_stride ? trow[p] : -1;
+          page = e >= 0 && e < a.blocks;
+        }
+        there |= (uint32_t)page << i;
+        if (page) seen |= seen_from(x, (c + i) * 64 + quad * 16) << (16 * i);
+      }
+      const bool all =
+          c + N <= w.c1 && c * 64 + 64 * N <= common && (!holes || __builtin_amdgcn_ballot_w64(there != (1u << N) - 1) == 0);
+      const uint8_t* slot = ring + (s % STEPS * 2 + o) * G::BYTES;
+      const uint8_t* kp = slot + (col >> 2) * G::KS + quad * 64 + (col & 3) * 16;
+      const uint8_t* vp = slot + G::V + quad * G::VS + col * 16;
+      const uint8_t* sp = slot + G::SCALES + quad * 64;
+      attend_keys<D, N>(
+          st, q, [&](int i, int n, int t) { return *(const i32x4*)(kp + i * G::BYTES + n * 4 * D + t * 256); },
+          [&](int i, int t) { return *(const i32x4*)(vp + i * G::BYTES + t * 256); },
+          [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 16 * n); },
+          [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); }, all, seen);
     }
-    const bool all = c * 64 + (two ? 128 : 64) <= common &&
-                     (!holes || __builtin_amdgcn_ballot_w64(!there || (two && !there2)) == 0);
-    uint32_t seen = there ? seen_from(x, c * 64 + quad * 16) : 0u;
-    const uint8_t* slot = ring + (s % STEPS * 2 + (pair ? part : 0)) * G::BYTES;
-    const uint8_t* kp = slot + (col >> 2) * G::KS + quad * 64 + (col & 3) * 16;
-    const uint8_t* vp = slot + G::V + quad * G::VS + col * 16;
-    const uint8_t* sp = slot + G::SCALES + quad * 64;
-    auto k = [&](int i, int n, int t) { return *(const i32x4*)(kp + i * G::BYTES + n * 4 * D + t * 256); };
-    auto v = [&](int i, int t) { return *(const i32x4*)(vp + i * G::BYTES + t * 256); };
-    auto ks = [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 16 * n); };
-    auto vs = [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); };
-    if (two) {
-      seen |= (there2 ? seen_from(x, c * 64 + 64 + quad * 16) : 0u) << 16;
-      attend_keys<D, 2>(st, q, k, v, ks, vs, all, seen);
-    } else {
-      attend_keys<D, 1>(st, q, k, v, ks, vs, all, seen);
-    }
-  }
+  };
+  if (pair) walk(std::integral_constant<int, 1>());
+  else walk(std::integral_constant<int, 2>());
   wait_vmcnt<0>();   // no load may still go to LDS
   const float l = column_sum(st.l);
   if (!pair && x.m >= 0) {
@@ -748,12 +795,12 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
     if (a.splits == 1) {
       const float f = inverse_sum(l);
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) write_out<D>(a, w, row, t * 16 + 4 * quad, st.o[t], f);
+      for (int t = 0; t < D / 16; ++t) write_out<D>(a, w, row, t * 16 + 4 * quad, elements(st, t), f);
     } else {
       const int64_t part = part_row(a, w, row);
       float* po = a.part_o + part * D + 4 * quad;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) *(floatx4*)(po + t * 16) = st.o[t];
+      for (int t = 0; t < D / 16; ++t) *(floatx4*)(po + t * 16) = elements(st, t);
       if (quad == 0) write_sums(a, part, st.m, l);
     }
   }
@@ -837,6 +884,7 @@ Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t
   if (splits < 1) splits = 1;
   p.chunks = (chunks + splits - 1) / splits;
   p.chunks = p.chunks > 0 ? p.chunks : 1;
+  if (p.ring) p.chunks += p.chunks & 1;   // whole steps
   p.splits = (chunks + p.chunks - 1) / p.chunks;
   p.splits = p.splits > 0 ? p.splits : 1;
   return p;
