@@ -277,7 +277,8 @@ struct AttendArgs {
   float* part_o;           // [batch, Hkv, tiles, splits, 16, D]
   float* part_ml;          // [batch, Hkv, tiles, splits, 16, 2]
   int64_t table_stride, blocks;
-  int T, Hq, Hkv, G, tiles, splits, chunks;   // chunks: of 64 keys per split
+  int T, Hq, Hkv, G, tiles, splits;
+  int units;               // of STEP chunks of 64 keys in a request's pages, which the splits share evenly
   float scale;
 };
 
@@ -342,22 +343,37 @@ __device__ __forceinline__ void two_terms(const float (&z)[4], int& h, int& l) {
   h = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
+// A row as it is (zeros past the last), fetched before its request's lengths are known.
 template <int D>
-__device__ __forceinline__ void load_query(Query<D>& q, const AttendArgs& a, const Row& x, int quad) {
-  float v[D / 64][16], top = 0.f;
-  const uint16_t* p = a.q + x.m * a.q_stride + (int64_t)x.head * D + 16 * quad;
+struct RawQuery {
+  u32x4 w[D / 64][2];
+};
+
+template <int D>
+__device__ __forceinline__ void fetch_query(RawQuery<D>& raw, const AttendArgs& a, int b, int h, int r, int quad) {
+  const int t = r / a.G, g = r % a.G;
+  const uint16_t* p = a.q + ((int64_t)b * a.T + t) * a.q_stride + (int64_t)(h * a.G + g) * D + 16 * quad;
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (x.m >= 0) w = *(const u32x4*)(p + 64 * s + 8 * i);
+      raw.w[s][i] = u32x4{0u, 0u, 0u, 0u};
+      if (t < a.T) raw.w[s][i] = *(const u32x4*)(p + 64 * s + 8 * i);
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a, const RawQuery<D>& raw) {
+  float v[D / 64][16], top = 0.f;
+#pragma unroll
+  for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[s][8 * i + 2 * e] = __uint_as_float(w[e] << 16);
-        v[s][8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        v[s][8 * i + 2 * e] = __uint_as_float(raw.w[s][i][e] << 16);
+        v[s][8 * i + 2 * e + 1] = __uint_as_float(raw.w[s][i][e] & 0xffff0000u);
       }
-    }
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
 #pragma unroll
@@ -388,9 +404,10 @@ __device__ __forceinline__ void load_query(Query<D>& q, const AttendArgs& a, con
 // N times 64 keys (four pages): of the c-th, k(c, n, s) is the K operand of product n, elements 64 s ..,
 // v(c, t) the V operand of elements 16 t .., ks(c, n) and vs(c, n) the scales of this lane's page, tokens
 // 4 n ... Where !all, this lane's row sees the tokens of its pages whose bits `seen` has, sixteen a page.
-template <int D, int N, typename K, typename V, typename KS, typename VS>
+// scored() is called when k, ks and vs are done with.
+template <int D, int N, typename K, typename V, typename KS, typename VS, typename Scored>
 __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, K k, V v, KS ks, VS vs,
-                                            bool all, uint32_t seen) {
+                                            Scored scored, bool all, uint32_t seen) {
   constexpr int NS = D / 64;
   float x[16 * N], p[16 * N];   // scores; scales of V, then weights times them
   // stage n loads what product n + 1 takes, issues product n and converts product n - 2, whose sums are
@@ -428,6 +445,7 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[4 * n + i] = g[i];
   }
+  scored();
   if (!all) {
     asm volatile("" : "+v"(seen));   // stays a branch: most keys are seen by every row
 #pragma unroll
@@ -528,9 +546,16 @@ struct Share {
   int b, h, split, c0, c1;
 };
 
+// The split's chunks, wherever the request ends.
+template <int STEP>
+__device__ __forceinline__ int split_chunk(const AttendArgs& a, int split) {
+  return STEP * (int)((int64_t)a.units * split / a.splits);
+}
+
 // The first tile and how many: chunks up to the last position that one of their rows sees.
+template <int STEP>
 __device__ __forceinline__ Share find_share(const AttendArgs& a, int b, int h, int split, int tile, int tiles) {
-  Share w{a.starts[b], 0, a.counts[b], b, h, split, 0, 0};
+  Share w{a.starts[b], 0, a.counts[b], b, h, split, split_chunk<STEP>(a, split), 0};
   w.count = w.count < a.T ? w.count : a.T;
   if (w.start < 0 || w.count <= 0 || tile * 16 >= w.count * a.G) {
     w.count = 0;
@@ -540,9 +565,7 @@ __device__ __forceinline__ Share find_share(const AttendArgs& a, int b, int h, i
   t_last = t_last < w.count ? t_last : w.count - 1;
   w.end = a.tree ? w.start + w.count : w.start + t_last + 1;
   w.end = w.end < a.table_stride * PAGE ? w.end : a.table_stride * PAGE;
-  w.c0 = split * a.chunks;
-  w.c1 = (int)((w.end + 63) / 64);
-  w.c1 = w.c1 < w.c0 + a.chunks ? w.c1 : w.c0 + a.chunks;
+  w.c1 = (int)min64((w.end + 63) / 64, split_chunk<STEP>(a, split + 1));
   return w;
 }
 
@@ -605,46 +628,98 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, 
   }
 }
 
-// One or two tiles: a (request, kv head, tile, split) each; the waves take the split's chunks in turn,
-// operands straight from memory, and join their states at the end.
+// One or two tiles: a (request, kv head, tile, split) each; the waves take the split's chunks in turn and
+// join their states at the end. Operands come straight from memory into registers, the next chunk's K as
+// soon as the scores are done and its V after the products, so that a wave has 16 D .. 32 D bytes in
+// flight all the time.
 constexpr int WAVES = 4;
 
+// The arguments that the first loads take come again in front, where they arrive in registers.
+#define KV8_FRONT                                                                                             \
+  const int32_t *__restrict__ h_table, const int32_t *__restrict__ h_starts, const int32_t *__restrict__ h_counts, \
+      const uint16_t *__restrict__ h_q, int64_t h_table_stride, int h_T, int h_G, int h_units, int h_splits,  \
+      int h_tiles, int h_Hkv, AttendArgs a
+#define KV8_TAKE_FRONT                                                                     \
+  a.table = h_table, a.starts = h_starts, a.counts = h_counts, a.q = h_q;                  \
+  a.table_stride = h_table_stride, a.T = h_T, a.G = h_G, a.units = h_units, a.splits = h_splits; \
+  a.tiles = h_tiles, a.Hkv = h_Hkv
+
 template <int D>
-__global__ void __launch_bounds__(64 * WAVES) attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
+  KV8_TAKE_FRONT;
+  constexpr int NS = D / 64, T = D / 16;
   __shared__ __attribute__((aligned(16))) float os[WAVES * 16 * (D + 4)];
   __shared__ float ml[WAVES][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
   const int tile = (int)(blockIdx.y % (unsigned)a.tiles), h = (int)(blockIdx.y / (unsigned)a.tiles), b = blockIdx.z;
-  const Share w = find_share(a, b, h, blockIdx.x, tile, 1);
+  const int64_t page_bytes = PAGE * D, block_bytes = page_bytes * a.Hkv;
+  const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
+  const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
+  const int32_t* trow = a.table + (int64_t)b * a.table_stride;
+  // the blocks of this lane's page of K and of V, -1: none
+  struct Pages {
+    int k, v;
+  };
+  auto look_up = [&](int c) {
+    const int64_t pk = 4ll * c + (col >> 2), pv = 4ll * c + quad;
+    Pages p{-1, -1};
+    if (pk < a.table_stride) p.k = trow[pk];
+    if (pv < a.table_stride) p.v = trow[pv];
+    return p;
+  };
+  auto valid = [&](int e) { return e >= 0 && e < a.blocks; };
+  int c = split_chunk<WAVES>(a, blockIdx.x) + wave;
+  Pages here = look_up(c), next = look_up(c + WAVES);
+  RawQuery<D> raw;
+  fetch_query(raw, a, b, h, tile * 16 + col, quad);
+  const Share w = find_share<WAVES>(a, b, h, blockIdx.x, tile, 1);
   if (w.count == 0) return;
+  i32x4 kw[4][NS], vw[T];
+  floatx4 kf[4], vf[4];
+  auto load_k = [&](Pages p) {
+    const int64_t bk = valid(p.k) ? p.k : 0, bv = valid(p.v) ? p.v : 0;
+    const int8_t* kp = kh + bk * block_bytes;
+    const int64_t at = (bv * a.Hkv + h) * PAGE;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kw[n][s] = *(const i32x4*)(kp + n * 4 * D + s * 256);
+      kf[n] = *(const floatx4*)(a.cache.k_scale + at + 4 * n);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) vf[n] = *(const floatx4*)(a.cache.v_scale + at + 4 * n);
+  };
+  auto load_v = [&](Pages p) {
+    const int8_t* vp = vh + (int64_t)(valid(p.v) ? p.v : 0) * block_bytes;
+#pragma unroll
+    for (int t = 0; t < T; ++t) vw[t] = *(const i32x4*)(vp + t * 256);
+  };
+  if (c < w.c1) {
+    load_k(here);
+    load_v(here);
+  }
   const Row x = find_row(a, b, h, tile * 16 + col, w.start, w.count);
   // every row of the tile sees the positions below
   const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
   RowState<D> st;
   clear(st);
   Query<D> q;
-  load_query(q, a, x, quad);
-  const int64_t page_bytes = PAGE * D, block_bytes = page_bytes * a.Hkv;
-  const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
-  const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
-  const int32_t* trow = a.table + (int64_t)b * a.table_stride;
-  for (int c = w.c0 + wave; c < w.c1; c += WAVES) {
-    const int64_t pk = 4ll * c + (col >> 2), pv = 4ll * c + quad;
-    int bk = pk < a.table_stride ? trow[pk] : -1, bv = pv < a.table_stride ? trow[pv] : -1;
-    const bool there = bv >= 0 && bv < a.blocks;
-    bk = bk >= 0 && bk < a.blocks ? bk : 0;
-    bv = there ? bv : 0;
-    const int8_t* kp = kh + bk * block_bytes;
-    const int8_t* vp = vh + bv * block_bytes;
-    const float* ksp = a.cache.k_scale + ((int64_t)bv * a.Hkv + h) * PAGE;
-    const float* vsp = a.cache.v_scale + ((int64_t)bv * a.Hkv + h) * PAGE;
+  quantise_query(q, a, raw);
+  for (; c < w.c1; c += WAVES) {
+    const bool there = valid(here.v), more = c + WAVES < w.c1;
     const bool all = __builtin_amdgcn_ballot_w64(!there) == 0 && c * 64 + 64 <= common;
     attend_keys<D, 1>(
-        st, q, [&](int, int n, int s) { return *(const i32x4*)(kp + n * 4 * D + s * 256); },
-        [&](int, int t) { return *(const i32x4*)(vp + t * 256); },
-        [&](int, int n) { return *(const floatx4*)(ksp + 4 * n); },
-        [&](int, int n) { return *(const floatx4*)(vsp + 4 * n); }, all,
-        there ? seen_from(x, c * 64 + quad * 16) : 0u);
+        st, q, [&](int, int n, int s) { return kw[n][s]; }, [&](int, int t) { return vw[t]; },
+        [&](int, int n) { return kf[n]; }, [&](int, int n) { return vf[n]; },
+        [&] {
+          if (more) load_k(next);
+        },
+        all, there ? seen_from(x, c * 64 + quad * 16) : 0u);
+    if (more) {
+      load_v(next);
+      here = next;
+      next = look_up(c + 2 * WAVES);
+    }
   }
   join_waves<D, WAVES, 64 * WAVES>(a, w, st, os, ml, wave, tile, 1);
 }
@@ -684,7 +759,8 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT) {
+  KV8_TAKE_FRONT;
   using G = ChunkImage<D>;
   constexpr int STEPS = G::SLOTS / 2, LOADS = 2 * (D / 64 + 1);
   static_assert(RING_WAVES * 16 * (D + 4) * 4 <= G::SLOTS * G::BYTES, "states are joined in the ring");
@@ -698,33 +774,28 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
   const int whole = 2 * tiles > RING_WAVES ? 2 * tiles - RING_WAVES : 0;   // tiles of one wave
   const bool pair = wave >= whole;
   const int tile = tile0 + (pair ? whole + (wave - whole) / 2 : wave), part = (wave - whole) & 1;
-  const Share w = find_share(a, b, h, blockIdx.x, tile0, tiles);
-  if (w.count == 0) return;
-  const bool idle = tile >= tile0 + tiles || tile * 16 >= w.count * a.G;
-  const Row x = idle ? Row{-1, 0, 0, 0} : find_row(a, b, h, tile * 16 + col, w.start, w.count);
-  // every row of the tile sees the positions below `common`, none those from `until` on
-  const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
-  int t_last = (tile * 16 + 15) / a.G;
-  t_last = t_last < w.count ? t_last : w.count - 1;
-  const int until = idle ? 0 : (int)min64(w.end, a.tree ? w.start + w.count : w.start + t_last + 1);
-  RowState<D> st;
-  clear(st);
-  Query<D> q;
   const int32_t* trow = a.table + (int64_t)b * a.table_stride;
+  const int c0 = split_chunk<2>(a, blockIdx.x);
+  // blocks of this wave's page in 64 chunks, one a lane
+  auto window = [&](int first) {
+    const int64_t p = 4ll * (c0 + first + lane) + (wave & 3);
+    const int e = p < a.table_stride ? trow[p] : 0;
+    return e >= 0 && e < a.blocks ? e : 0;
+  };
+  int ids = window(0), ids_from = 0;
+  RawQuery<D> raw;
+  fetch_query(raw, a, b, h, tile * 16 + col, quad);
+  const Share w = find_share<2>(a, b, h, blockIdx.x, tile0, tiles);
+  if (w.count == 0) return;
   const int n_chunks = w.c1 - w.c0;
   // pages without a block are rare: whether there is one is found once, and each looked up only then
   bool hole = false;
   const int pages = (int)min64(4ll * w.c1, (w.end + PAGE - 1) / PAGE);
   for (int p = 4 * w.c0 + threadIdx.x; p < pages; p += 64 * RING_WAVES) hole |= trow[p] < 0 || trow[p] >= a.blocks;
-  // blocks of this wave's page in 64 chunks, one a lane
-  auto window = [&](int first) {
-    const int64_t p = 4ll * (w.c0 + first + lane) + (wave & 3);
-    const int e = p < a.table_stride ? trow[p] : 0;
-    return e >= 0 && e < a.blocks ? e : 0;
-  };
-  int ids = window(0), ids_from = 0;
-  if (!idle) load_query(q, a, x, quad);
   const bool holes = __syncthreads_or(hole);
+  // the query is waited for here: later a wait for it would be one for the loads behind it too
+#pragma unroll
+  for (int s = 0; s < D / 64; ++s) asm volatile("" ::"v"(raw.w[s][0]), "v"(raw.w[s][1]));
   const int64_t page_bytes = PAGE * D;
   const int8_t* plane = wave < 4 ? a.cache.k : a.cache.v;
   const float* scales = wave < 4 ? a.cache.k_scale : a.cache.v_scale;
@@ -749,6 +820,17 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
 #pragma unroll
   for (int s = 0; s < STEPS - 1; ++s)
     if (s < steps) load_step(s);
+  const bool idle = tile >= tile0 + tiles || tile * 16 >= w.count * a.G;
+  const Row x = idle ? Row{-1, 0, 0, 0} : find_row(a, b, h, tile * 16 + col, w.start, w.count);
+  // every row of the tile sees the positions below `common`, none those from `until` on
+  const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
+  int t_last = (tile * 16 + 15) / a.G;
+  t_last = t_last < w.count ? t_last : w.count - 1;
+  const int until = idle ? 0 : (int)min64(w.end, a.tree ? w.start + w.count : w.start + t_last + 1);
+  RowState<D> st;
+  clear(st);
+  Query<D> q;
+  quantise_query(q, a, raw);
   // a wave's steps: N = 2, both chunks of each, or 1, the part-th
   auto walk = [&](auto chunks) {
     constexpr int N = decltype(chunks)::value;
@@ -783,7 +865,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
           st, q, [&](int i, int n, int t) { return *(const i32x4*)(kp + i * G::BYTES + n * 4 * D + t * 256); },
           [&](int i, int t) { return *(const i32x4*)(vp + i * G::BYTES + t * 256); },
           [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 16 * n); },
-          [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); }, all, seen);
+          [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); }, [] {}, all, seen);
     }
   };
   if (pair) walk(std::integral_constant<int, 1>());
@@ -811,51 +893,65 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(AttendArgs
   }
 }
 
-// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. The threads of a row's
-// elements, D / 4, come in GROUPS, each with its splits, the loads of eight in flight.
-constexpr int JOIN = 512;
+// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. The D / 4 threads of a
+// row's elements come GROUPS times, each with its splits, eight loads in flight: eight times for many
+// splits, once for a few (2304 rows of 8 splits: 9.0 us in eight groups).
+constexpr int JOIN = 512, AHEAD = 8;
 
-template <int D>
+template <int D, int GROUPS>
 __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
-  constexpr int W = D / 4, GROUPS = JOIN / W, AHEAD = 8;
-  __shared__ floatx4 red[GROUPS][W];
-  const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = r / a.G;
+  constexpr int W = D / 4, ROWS = JOIN / W / GROUPS;
+  __shared__ floatx4 red[GROUPS > 1 ? GROUPS : 1][ROWS][W];
+  const int c = threadIdx.x % W, g = threadIdx.x / W % GROUPS, i = threadIdx.x / W / GROUPS;
+  const int r = blockIdx.x * ROWS + i, h = blockIdx.y, b = blockIdx.z, t = r / a.G;
   int count = a.counts[b];
   count = count < a.T ? count : a.T;
-  if (a.starts[b] < 0 || t >= count) return;
-  const int lane = threadIdx.x & 63, g = threadIdx.x / W, c = threadIdx.x % W;
-  const int64_t part = (((int64_t)b * a.Hkv + h) * a.tiles + r / 16) * a.splits;
-  const float* ml = a.part_ml + (part * 16 + r % 16) * 2;
-  const float* po = a.part_o + (part * 16 + r % 16) * D + 4 * c;
-  floatx4 x[AHEAD];
-  auto fetch = [&](int s0) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int s = s0 + i * GROUPS;
-      if (s < a.splits) x[i] = *(const floatx4*)(po + (int64_t)s * 16 * D);
-    }
-  };
-  fetch(g);   // with the maxima and sums: one round trip
-  float m = NEG_INF, l = 0.f;
-  for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[s * 32]);
-  m = wave_max(m);
-  const float base = m == NEG_INF ? 0.f : m;
-  for (int s = lane; s < a.splits; s += 64) l += __builtin_amdgcn_exp2f(ml[s * 32] - base) * ml[s * 32 + 1];
-  l = wave_sum(l);
+  const bool live = a.starts[b] >= 0 && t < count;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = g; s0 < a.splits; s0 += AHEAD * GROUPS) {
-    if (s0 != g) fetch(s0);
+  float m = NEG_INF, l = 0.f;
+  if (live) {
+    const int64_t part = ((((int64_t)b * a.Hkv + h) * a.tiles + r / 16) * a.splits) * 16 + r % 16;
+    const float2* ml = (const float2*)a.part_ml + part;
+    const float* po = a.part_o + part * D + 4 * c;
+    floatx4 x[AHEAD];
+    auto fetch = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int s = s0 + i * GROUPS;
-      if (s < a.splits) o += __builtin_amdgcn_exp2f(ml[s * 32] - base) * x[i];
+      for (int k = 0; k < AHEAD; ++k) {
+        const int s = s0 + k * GROUPS;
+        if (s < a.splits) x[k] = *(const floatx4*)(po + (int64_t)s * 16 * D);
+      }
+    };
+    fetch(g);   // with the maxima and sums: one round trip
+    // a row's maximum and sum, by W threads or more
+    constexpr int L = W < 64 ? W : 64;
+    const int lane = threadIdx.x % L;
+    for (int s = lane; s < a.splits; s += L) m = fmaxf(m, ml[s * 16].x);
+#pragma unroll
+    for (int k = L / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, L));
+    const float base = m == NEG_INF ? 0.f : m;
+    for (int s = lane; s < a.splits; s += L) {
+      const float2 e = ml[s * 16];
+      l += __builtin_amdgcn_exp2f(e.x - base) * e.y;
+    }
+#pragma unroll
+    for (int k = L / 2; k > 0; k >>= 1) l += __shfl_xor(l, k, L);
+    for (int s0 = g; s0 < a.splits; s0 += AHEAD * GROUPS) {
+      if (s0 != g) fetch(s0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int s = s0 + k * GROUPS;
+        if (s < a.splits) o += __builtin_amdgcn_exp2f(ml[s * 16].x - base) * x[k];
+      }
     }
   }
-  red[g][c] = o;
-  __syncthreads();
-  if (g != 0) return;
+  if constexpr (GROUPS > 1) {
+    red[g][i][c] = o;
+    __syncthreads();
+    if (g != 0) return;
 #pragma unroll
-  for (int i = 1; i < GROUPS; ++i) o += red[i][c];
+    for (int k = 1; k < GROUPS; ++k) o += red[k][i][c];
+  }
+  if (!live) return;
   const float f = inverse_sum(l);
   const int64_t row = (int64_t)b * a.T + t;
   *(u32x2*)(a.out + (row * a.Hq + h * a.G + r % a.G) * D + 4 * c) =
@@ -868,7 +964,7 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
 constexpr int64_t MAX_PAGES = 1 << 26;   // of a request: positions stay below 2^30
 
 struct Plan {
-  int64_t tiles, groups, splits, chunks;
+  int64_t tiles, groups, splits, units;
   bool ring;
 };
 
@@ -877,17 +973,22 @@ Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t
   p.tiles = (tokens * (Hq / Hkv) + 15) / 16;
   p.ring = p.tiles > 2;
   p.groups = p.ring ? (p.tiles + RING_WAVES - 1) / RING_WAVES : p.tiles;
-  const int64_t chunks = (width + 3) / 4, items = batch * Hkv * p.groups, target = p.ring ? 256 : 512;
-  int64_t splits = items < target ? target / items : 1;
-  const int64_t least = p.ring ? 2 : WAVES, most = (chunks + least - 1) / least;
-  splits = splits < most ? splits : most;
-  if (splits < 1) splits = 1;
-  p.chunks = (chunks + splits - 1) / splits;
-  p.chunks = p.chunks > 0 ? p.chunks : 1;
-  if (p.ring) p.chunks += p.chunks & 1;   // whole steps
-  p.splits = (chunks + p.chunks - 1) / p.chunks;
-  p.splits = p.splits > 0 ? p.splits : 1;
+  const int64_t chunks = (width + 3) / 4, step = p.ring ? 2 : WAVES;
+  p.units = (chunks + step - 1) / step;
+  const int64_t items = batch * Hkv * p.groups, target = p.ring ? 256 : 512;
+  p.splits = items < target ? target / items : 1;
+  p.splits = p.splits < p.units ? p.splits : p.units;
+  if (p.splits < 1) p.splits = 1;
   return p;
+}
+
+template <int D>
+void launch_join(const AttendArgs& a, int64_t batch, hipStream_t s) {
+  const bool few = a.splits <= AHEAD;
+  const int rows = JOIN / (D / 4) / (few ? 1 : 8);
+  const dim3 grid((unsigned)((a.T * a.G + rows - 1) / rows), (unsigned)a.Hkv, (unsigned)batch);
+  if (few) hipLaunchKernelGGL((join_kernel<D, 1>), grid, dim3(JOIN), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<D, 8>), grid, dim3(JOIN), 0, s, a);
 }
 
 }  // namespace
@@ -1024,7 +1125,7 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   a.G = (int)(num_heads / num_kv_heads);
   a.tiles = (int)p.tiles;
   a.splits = (int)p.splits;
-  a.chunks = (int)p.chunks;
+  a.units = (int)p.units;
   a.scale = scale;
   a.part_o = (float*)scratch;
   a.part_ml = (float*)scratch + batch * num_kv_heads * p.tiles * p.splits * 16 * head_size;
@@ -1032,12 +1133,13 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   auto few = head_size == 64 ? attend_kernel<64> : head_size == 128 ? attend_kernel<128> : attend_kernel<256>;
   auto more = head_size == 64 ? attend_ring_kernel<64>
               : head_size == 128 ? attend_ring_kernel<128> : attend_ring_kernel<256>;
-  hipLaunchKernelGGL(p.ring ? more : few, grid, dim3(64 * (p.ring ? RING_WAVES : WAVES)), 0, S(stream), a);
+  hipLaunchKernelGGL(p.ring ? more : few, grid, dim3(64 * (p.ring ? RING_WAVES : WAVES)), 0, S(stream), a.table,
+                     a.starts, a.counts, a.q, a.table_stride, a.T, a.G, a.units, a.splits, a.tiles, a.Hkv, a);
   SV_CHECK_LAUNCH();
   if (p.splits > 1) {
-    auto join = head_size == 64 ? join_kernel<64> : head_size == 128 ? join_kernel<128> : join_kernel<256>;
-    hipLaunchKernelGGL(join, dim3((unsigned)(tokens * a.G), (unsigned)num_kv_heads, (unsigned)batch),
-                       dim3(JOIN), 0, S(stream), a);
+    if (head_size == 64) launch_join<64>(a, batch, S(stream));
+    else if (head_size == 128) launch_join<128>(a, batch, S(stream));
+    else launch_join<256>(a, batch, S(stream));
     SV_CHECK_LAUNCH();
   }
   return SV_OK;
