@@ -18,6 +18,7 @@
 #include "common.h"
 #include "pages.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -278,7 +279,8 @@ struct AttendArgs {
   float* part_ml;          // [batch, Hkv, tiles, splits, 16, 2]
   int64_t table_stride, blocks;
   int T, Hq, Hkv, G, tiles, splits;
-  int units;               // of STEP chunks of 64 keys in a request's pages, which the splits share evenly
+  int unit, longer;        // a split's share of a request's steps; the first `longer` have one more
+  uint32_t g_inv;          // floor(2^32 / G), at most 2^32 - 1
   float scale;
 };
 
@@ -306,14 +308,25 @@ struct Query {
   float s;                 // scores' factor, as an exponent of 2
 };
 
+// Row r of a kv head as (token, head of its group). r g_inv / 2^32 is below r / G by less than r / 2^32 + 1.
+struct RowPlace {
+  int t, g;
+};
+__device__ __forceinline__ RowPlace place(const AttendArgs& a, int r) {
+  int t = (int)__umulhi((uint32_t)r, a.g_inv), g = r - t * a.G;
+  if (g >= a.G) ++t, g -= a.G;
+  return {t, g};
+}
+
 __device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
 __device__ __forceinline__ Row find_row(const AttendArgs& a, int b, int h, int r, int64_t start, int count) {
   Row x{-1, 0, 0, 0};
-  const int t = r / a.G, g = r % a.G;
+  const RowPlace at = place(a, r);
+  const int t = at.t;
   if (t >= count) return x;
   x.m = (int64_t)b * a.T + t;
-  x.head = h * a.G + g;
+  x.head = h * a.G + at.g;
   // nothing past the table
   const int64_t width = a.table_stride * PAGE;
   const int64_t end = a.tree ? start : start + t + 1;
@@ -343,7 +356,7 @@ __device__ __forceinline__ void two_terms(const float (&z)[4], int& h, int& l) {
   h = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// A row as it is (zeros past the last), fetched before its request's lengths are known.
+// A row as it is, fetched before its request's lengths are known (one past the last: the first one's).
 template <int D>
 struct RawQuery {
   u32x4 w[D / 64][2];
@@ -351,15 +364,13 @@ struct RawQuery {
 
 template <int D>
 __device__ __forceinline__ void fetch_query(RawQuery<D>& raw, const AttendArgs& a, int b, int h, int r, int quad) {
-  const int t = r / a.G, g = r % a.G;
-  const uint16_t* p = a.q + ((int64_t)b * a.T + t) * a.q_stride + (int64_t)(h * a.G + g) * D + 16 * quad;
+  const RowPlace at = place(a, r);
+  const uint16_t* p =
+      a.q + ((int64_t)b * a.T + (at.t < a.T ? at.t : 0)) * a.q_stride + (int64_t)(h * a.G + at.g) * D + 16 * quad;
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      raw.w[s][i] = u32x4{0u, 0u, 0u, 0u};
-      if (t < a.T) raw.w[s][i] = *(const u32x4*)(p + 64 * s + 8 * i);
-    }
+    for (int i = 0; i < 2; ++i) raw.w[s][i] = *(const u32x4*)(p + 64 * s + 8 * i);
 }
 
 template <int D>
@@ -404,10 +415,11 @@ __device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a,
 // N times 64 keys (four pages): of the c-th, k(c, n, s) is the K operand of product n, elements 64 s ..,
 // v(c, t) the V operand of elements 16 t .., ks(c, n) and vs(c, n) the scales of this lane's page, tokens
 // 4 n ... Where !all, this lane's row sees the tokens of its pages whose bits `seen` has, sixteen a page.
-// scored() is called when k, ks and vs are done with.
-template <int D, int N, typename K, typename V, typename KS, typename VS, typename Scored>
+// scored() is called when k, ks and vs are done with, feed(i) with i = 0, 1, .. once a stage of the
+// products, 4 N + D / 16 times.
+template <int D, int N, typename K, typename V, typename KS, typename VS, typename Scored, typename Feed>
 __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, K k, V v, KS ks, VS vs,
-                                            Scored scored, bool all, uint32_t seen) {
+                                            Scored scored, Feed feed, bool all, uint32_t seen) {
   constexpr int NS = D / 64;
   float x[16 * N], p[16 * N];   // scores; scales of V, then weights times them
   // stage n loads what product n + 1 takes, issues product n and converts product n - 2, whose sums are
@@ -429,6 +441,7 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
           hi[n % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[n & 1][s], q.h[s], hi[n % 3], 0, 0, 0);
           lo[n % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[n & 1][s], q.l[s], lo[n % 3], 0, 0, 0);
         }
+        feed(n);
       }
       if (n >= 2) {
         const int m = n - 2;
@@ -511,6 +524,7 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
         hi[t % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t & 1][c], pa[c], hi[t % 3], 0, 0, 0);
         lo[t % 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t & 1][c], pb[c], lo[t % 3], 0, 0, 0);
       }
+      feed(4 * N + t);
     }
     if (t >= 2) {
       const int m = t - 2;
@@ -549,19 +563,20 @@ struct Share {
 // The split's chunks, wherever the request ends.
 template <int STEP>
 __device__ __forceinline__ int split_chunk(const AttendArgs& a, int split) {
-  return STEP * (int)((int64_t)a.units * split / a.splits);
+  return STEP * (split * a.unit + (split < a.longer ? split : a.longer));
 }
 
 // The first tile and how many: chunks up to the last position that one of their rows sees.
 template <int STEP>
-__device__ __forceinline__ Share find_share(const AttendArgs& a, int b, int h, int split, int tile, int tiles) {
-  Share w{a.starts[b], 0, a.counts[b], b, h, split, split_chunk<STEP>(a, split), 0};
+__device__ __forceinline__ Share find_share(const AttendArgs& a, int start, int count, int b, int h, int split, int tile,
+                                            int tiles) {
+  Share w{start, 0, count, b, h, split, split_chunk<STEP>(a, split), 0};
   w.count = w.count < a.T ? w.count : a.T;
-  if (w.start < 0 || w.count <= 0 || tile * 16 >= w.count * a.G) {
+  if (w.start < 0 || w.count <= 0 || (int64_t)tile * 16 >= (int64_t)w.count * a.G) {
     w.count = 0;
     return w;
   }
-  int t_last = ((tile + tiles) * 16 - 1) / a.G;
+  int t_last = place(a, (tile + tiles) * 16 - 1).t;
   t_last = t_last < w.count ? t_last : w.count - 1;
   w.end = a.tree ? w.start + w.count : w.start + t_last + 1;
   w.end = w.end < a.table_stride * PAGE ? w.end : a.table_stride * PAGE;
@@ -571,9 +586,8 @@ __device__ __forceinline__ Share find_share(const AttendArgs& a, int b, int h, i
 
 // Four elements of a row's result.
 template <int D>
-__device__ __forceinline__ void write_out(const AttendArgs& a, const Share& w, int r, int d, floatx4 o, float f) {
-  const int64_t row = (int64_t)w.b * a.T + r / a.G;
-  *(u32x2*)(a.out + (row * a.Hq + w.h * a.G + r % a.G) * D + d) =
+__device__ __forceinline__ void write_out(const AttendArgs& a, int64_t m, int head, int d, floatx4 o, float f) {
+  *(u32x2*)(a.out + (m * a.Hq + head) * D + d) =
       u32x2{pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f)};
 }
 
@@ -587,39 +601,36 @@ __device__ __forceinline__ void write_sums(const AttendArgs& a, int64_t part, fl
   a.part_ml[part * 2 + 1] = l;
 }
 
-// The states of N waves for each of the tiles from `tile` on joined through LDS (os: a pitch of D + 4
-// floats a row): state i * N + n is part n of tile i, -1: this wave has none.
-template <int D, int N, int THREADS>
+// The states of a tile's N waves joined through LDS (os: a pitch of D + 4 floats a row).
+template <int D, int N>
 __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, const RowState<D>& st, float* os,
-                                           float (*ml)[16][2], int state, int tile, int tiles) {
+                                           float (*ml)[16][2], int wave, int tile) {
   constexpr int P = D + 4;
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-  if (state >= 0) {
-    const float l = column_sum(st.l);
+  const float l = column_sum(st.l);
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (state * 16 + col) * P + t * 16 + 4 * quad) = elements(st, t);
-    if (quad == 0) {
-      ml[state][col][0] = st.m;
-      ml[state][col][1] = l;
-    }
+  for (int t = 0; t < D / 16; ++t) *(floatx4*)(os + (wave * 16 + col) * P + t * 16 + 4 * quad) = elements(st, t);
+  if (quad == 0) {
+    ml[wave][col][0] = st.m;
+    ml[wave][col][1] = l;
   }
   __syncthreads();
-  for (int u = threadIdx.x; u < tiles * 16 * (D / 4); u += THREADS) {
-    const int i = u / (4 * D), r = u / (D / 4) % 16, d = u % (D / 4) * 4;
-    if ((tile + i) * 16 + r >= w.count * a.G) break;   // rows only grow
+  for (int u = threadIdx.x; u < 16 * (D / 4); u += 64 * N) {
+    const int r = u / (D / 4), d = u % (D / 4) * 4, row = tile * 16 + r;
+    const RowPlace at = place(a, row);
+    if (at.t >= w.count) break;   // rows only grow
     float m = NEG_INF, sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < N; ++n) m = fmaxf(m, ml[i * N + n][r][0]);
+    for (int n = 0; n < N; ++n) m = fmaxf(m, ml[n][r][0]);
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[i * N + n][r][0] - m);
-      sum += f * ml[i * N + n][r][1];
-      o += f * *(const floatx4*)(os + ((i * N + n) * 16 + r) * P + d);
+      const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(ml[n][r][0] - m);
+      sum += f * ml[n][r][1];
+      o += f * *(const floatx4*)(os + (n * 16 + r) * P + d);
     }
-    const int row = (tile + i) * 16 + r;
     if (a.splits == 1) {
-      write_out<D>(a, w, row, d, o, inverse_sum(sum));
+      write_out<D>(a, (int64_t)w.b * a.T + at.t, w.h * a.G + at.g, d, o, inverse_sum(sum));
     } else {
       const int64_t part = part_row(a, w, row);
       *(floatx4*)(a.part_o + part * D + d) = o;
@@ -637,12 +648,12 @@ constexpr int WAVES = 4;
 // The arguments that the first loads take come again in front, where they arrive in registers.
 #define KV8_FRONT                                                                                             \
   const int32_t *__restrict__ h_table, const int32_t *__restrict__ h_starts, const int32_t *__restrict__ h_counts, \
-      const uint16_t *__restrict__ h_q, int64_t h_table_stride, int h_T, int h_G, int h_units, int h_splits,  \
-      int h_tiles, int h_Hkv, AttendArgs a
+      const uint16_t *__restrict__ h_q, int64_t h_table_stride, int h_T, int h_G, int h_unit, int h_longer,   \
+      int h_tiles, int h_Hkv, uint32_t h_g_inv, AttendArgs a
 #define KV8_TAKE_FRONT                                                                     \
   a.table = h_table, a.starts = h_starts, a.counts = h_counts, a.q = h_q;                  \
-  a.table_stride = h_table_stride, a.T = h_T, a.G = h_G, a.units = h_units, a.splits = h_splits; \
-  a.tiles = h_tiles, a.Hkv = h_Hkv
+  a.table_stride = h_table_stride, a.T = h_T, a.G = h_G, a.unit = h_unit, a.longer = h_longer; \
+  a.tiles = h_tiles, a.Hkv = h_Hkv, a.g_inv = h_g_inv
 
 template <int D>
 __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
@@ -651,7 +662,8 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   __shared__ __attribute__((aligned(16))) float os[WAVES * 16 * (D + 4)];
   __shared__ float ml[WAVES][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int tile = (int)(blockIdx.y % (unsigned)a.tiles), h = (int)(blockIdx.y / (unsigned)a.tiles), b = blockIdx.z;
+  const int start = a.starts[blockIdx.z], count = a.counts[blockIdx.z];
+  const int h = a.tiles == 1 ? blockIdx.y : blockIdx.y >> 1, tile = a.tiles == 1 ? 0 : blockIdx.y & 1, b = blockIdx.z;
   const int64_t page_bytes = PAGE * D, block_bytes = page_bytes * a.Hkv;
   const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
   const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
@@ -662,9 +674,10 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   };
   auto look_up = [&](int c) {
     const int64_t pk = 4ll * c + (col >> 2), pv = 4ll * c + quad;
-    Pages p{-1, -1};
-    if (pk < a.table_stride) p.k = trow[pk];
-    if (pv < a.table_stride) p.v = trow[pv];
+    const int64_t last = a.table_stride - 1;
+    if (last < 0) return Pages{-1, -1};   // (uniform)
+    Pages p{trow[pk < last ? pk : last], trow[pv < last ? pv : last]};
+    p.v = pv <= last ? p.v : -1;   // (a K of another page is a V that is not there: hidden)
     return p;
   };
   auto valid = [&](int e) { return e >= 0 && e < a.blocks; };
@@ -672,7 +685,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   Pages here = look_up(c), next = look_up(c + WAVES);
   RawQuery<D> raw;
   fetch_query(raw, a, b, h, tile * 16 + col, quad);
-  const Share w = find_share<WAVES>(a, b, h, blockIdx.x, tile, 1);
+  const Share w = find_share<WAVES>(a, start, count, b, h, blockIdx.x, tile, 1);
   if (w.count == 0) return;
   i32x4 kw[4][NS], vw[T];
   floatx4 kf[4], vf[4];
@@ -700,7 +713,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   }
   const Row x = find_row(a, b, h, tile * 16 + col, w.start, w.count);
   // every row of the tile sees the positions below
-  const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
+  const int common = (int)min64(w.end, a.tree ? w.start : w.start + place(a, tile * 16).t + 1);
   RowState<D> st;
   clear(st);
   Query<D> q;
@@ -714,14 +727,14 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
         [&] {
           if (more) load_k(next);
         },
-        all, there ? seen_from(x, c * 64 + quad * 16) : 0u);
+        [](int) {}, all, there ? seen_from(x, c * 64 + quad * 16) : 0u);
     if (more) {
       load_v(next);
       here = next;
       next = look_up(c + 2 * WAVES);
     }
   }
-  join_waves<D, WAVES, 64 * WAVES>(a, w, st, os, ml, wave, tile, 1);
+  join_waves<D, WAVES>(a, w, st, os, ml, wave, tile);
 }
 
 // More tiles: eight waves share the chunks of a split, two a step, through a ring in LDS. All eight load
@@ -733,29 +746,22 @@ constexpr int RING_WAVES = 8;
 
 template <int D>
 struct ChunkImage {
-  static constexpr int KS = 16 * D + 64;     // a page of K: four pages' rows on different banks
+  // a page of K, padded: a read of 16 bytes a lane goes in quarters of lanes 0 .. 3, 12 .. 15, 20 .. 23 and
+  // 24 .. 27 and the like, whose four pages are on different banks then
+  static constexpr int KS = 16 * D + 128;
   static constexpr int VS = 16 * D;
   static constexpr int V = 4 * KS, SCALES = V + 4 * VS, BYTES = SCALES + 512;
   static constexpr int SLOTS = D == 256 ? 4 : 8;
 };
 typedef __attribute__((address_space(3))) void lds_void;
 
-// N times 1 KiB (16 bytes a lane) from src, this lane's place, straight into LDS at dst. Written out
-// because the compiler would wait for every such load before any LDS read; the ring's own waits say
-// which have to be done. To the compiler they are clobbers of memory: its own waits stay good, since
-// loads that it does not know of only make them longer. (m0 is used by nothing else in the kernel.)
-template <int N>
-__device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
-  static_assert(N == 1 || N == 2 || N == 4, "one, two or four loads; their offsets go to both sides");
-  if constexpr (N == 1)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
-  else if constexpr (N == 2)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                 "global_load_lds_dwordx4 %1, off offset:1024" ::"s"(dst), "v"(src) : "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                 "global_load_lds_dwordx4 %1, off offset:1024\n\tglobal_load_lds_dwordx4 %1, off offset:2048\n\t"
-                 "global_load_lds_dwordx4 %1, off offset:3072" ::"s"(dst), "v"(src) : "memory");
+// 1 KiB (16 bytes a lane) from src, this lane's place, straight into LDS at dst, both `offset` bytes on.
+// Written out because the compiler would wait for every such load before any LDS read; the ring's own
+// waits say which have to be done. To the compiler they are clobbers of memory: its own waits stay good,
+// since loads that it does not know of only make them longer. (m0 is used by nothing else in the kernel.)
+__device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst, int offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(dst), "v"(src), "i"(offset)
+               : "memory");
 }
 
 template <int D>
@@ -763,13 +769,17 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   KV8_TAKE_FRONT;
   using G = ChunkImage<D>;
   constexpr int STEPS = G::SLOTS / 2, LOADS = 2 * (D / 64 + 1);
-  static_assert(RING_WAVES * 16 * (D + 4) * 4 <= G::SLOTS * G::BYTES, "states are joined in the ring");
+  static_assert(RING_WAVES / 2 * 16 * D * 4 <= G::SLOTS * G::BYTES, "states are joined in the ring");
   __shared__ __attribute__((aligned(16))) uint8_t ring[G::SLOTS * G::BYTES];
-  __shared__ float ml[RING_WAVES][16][2];
+  __shared__ float ml[RING_WAVES / 2][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int groups = (a.tiles + RING_WAVES - 1) / RING_WAVES;
-  const int tile0 = (int)(blockIdx.y % (unsigned)groups) * RING_WAVES, h = (int)(blockIdx.y / (unsigned)groups);
-  const int b = blockIdx.z;
+  const int start = a.starts[blockIdx.z], count = a.counts[blockIdx.z];
+  const int groups = (a.tiles + RING_WAVES - 1) / RING_WAVES, b = blockIdx.z;
+  int h = blockIdx.y, tile0 = 0;
+  if (groups > 1) {
+    tile0 = (int)(blockIdx.y % (unsigned)groups) * RING_WAVES;
+    h = (int)(blockIdx.y / (unsigned)groups);
+  }
   const int tiles = a.tiles - tile0 < RING_WAVES ? a.tiles - tile0 : RING_WAVES;
   const int whole = 2 * tiles > RING_WAVES ? 2 * tiles - RING_WAVES : 0;   // tiles of one wave
   const bool pair = wave >= whole;
@@ -777,22 +787,26 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   const int32_t* trow = a.table + (int64_t)b * a.table_stride;
   const int c0 = split_chunk<2>(a, blockIdx.x);
   // blocks of this wave's page in 64 chunks, one a lane
-  auto window = [&](int first) {
+  auto look_up = [&](int first) {   // (past the table: its last page)
     const int64_t p = 4ll * (c0 + first + lane) + (wave & 3);
-    const int e = p < a.table_stride ? trow[p] : 0;
-    return e >= 0 && e < a.blocks ? e : 0;
+    return a.table_stride > 0 ? trow[p < a.table_stride ? p : a.table_stride - 1] : 0;
   };
-  int ids = window(0), ids_from = 0;
+  auto valid = [&](int e) { return e >= 0 && e < a.blocks; };
+  int ids = look_up(0), ids_from = 0;
   RawQuery<D> raw;
   fetch_query(raw, a, b, h, tile * 16 + col, quad);
-  const Share w = find_share<2>(a, b, h, blockIdx.x, tile0, tiles);
+  const Share w = find_share<2>(a, start, count, b, h, blockIdx.x, tile0, tiles);
   if (w.count == 0) return;
   const int n_chunks = w.c1 - w.c0;
   // pages without a block are rare: whether there is one is found once, and each looked up only then
-  bool hole = false;
-  const int pages = (int)min64(4ll * w.c1, (w.end + PAGE - 1) / PAGE);
-  for (int p = 4 * w.c0 + threadIdx.x; p < pages; p += 64 * RING_WAVES) hole |= trow[p] < 0 || trow[p] >= a.blocks;
+  const int64_t pages = (w.end + PAGE - 1) / PAGE;
+  auto hole_in = [&](int first, int e) {
+    return first + lane < n_chunks && 4ll * (c0 + first + lane) + (wave & 3) < pages && !valid(e);
+  };
+  bool hole = hole_in(0, ids);
+  for (int i = 64; i < n_chunks; i += 64) hole |= hole_in(i, look_up(i));
   const bool holes = __syncthreads_or(hole);
+  ids = valid(ids) ? ids : 0;
   // the query is waited for here: later a wait for it would be one for the loads behind it too
 #pragma unroll
   for (int s = 0; s < D / 64; ++s) asm volatile("" ::"v"(raw.w[s][0]), "v"(raw.w[s][1]));
@@ -800,31 +814,47 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   const int8_t* plane = wave < 4 ? a.cache.k : a.cache.v;
   const float* scales = wave < 4 ? a.cache.k_scale : a.cache.v_scale;
   const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_void*)ring;
-  auto load_step = [&](int step) {
+  // the loads of a step: load i of LOADS, of chunk i / (LOADS / 2)
+  const int8_t* src[2];
+  const float* src_scale[2];
+  uint32_t dst[2];
+  auto aim = [&](int step) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       int i = step * 2 + n;
       i = i < n_chunks ? i : n_chunks - 1;
       if (i - ids_from >= 64) {   // (uniform)
         ids_from = i;
-        ids = window(i);
+        ids = look_up(i);
+        ids = valid(ids) ? ids : 0;
       }
       const int64_t at = (int64_t)__builtin_amdgcn_readlane(ids, i - ids_from) * a.Hkv + h;
-      const int8_t* src = plane + at * page_bytes + lane * 16;
-      const uint32_t slot = ring_at + (step % STEPS * 2 + n) * G::BYTES;
-      load_to_lds<D / 64>(src, slot + (wave < 4 ? wave * G::KS : G::V + (wave - 4) * G::VS));
-      if (lane < 4) load_to_lds<1>(scales + at * PAGE + lane * 4, slot + G::SCALES + wave * 64);
+      src[n] = plane + at * page_bytes + lane * 16;
+      src_scale[n] = scales + at * PAGE + lane * 4;
+      dst[n] = ring_at + (step % STEPS * 2 + n) * G::BYTES;
     }
+  };
+  auto load = [&](int i) {
+    const int n = i / (LOADS / 2), j = i % (LOADS / 2);
+    if (j < D / 64)
+      load_to_lds(src[n], dst[n] + (wave < 4 ? wave * G::KS : G::V + (wave - 4) * G::VS), j * 1024);
+    else if (lane < 4)
+      load_to_lds(src_scale[n], dst[n] + G::SCALES + wave * 64, 0);
+  };
+  auto load_step = [&](int step) {
+    aim(step);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(i);
   };
   const int steps = (n_chunks + 1) / 2;
 #pragma unroll
   for (int s = 0; s < STEPS - 1; ++s)
     if (s < steps) load_step(s);
-  const bool idle = tile >= tile0 + tiles || tile * 16 >= w.count * a.G;
+  const bool idle = tile >= tile0 + tiles || (int64_t)tile * 16 >= (int64_t)w.count * a.G;
   const Row x = idle ? Row{-1, 0, 0, 0} : find_row(a, b, h, tile * 16 + col, w.start, w.count);
   // every row of the tile sees the positions below `common`, none those from `until` on
-  const int common = (int)min64(w.end, a.tree ? w.start : w.start + tile * 16 / a.G + 1);
-  int t_last = (tile * 16 + 15) / a.G;
+  const int common = (int)min64(w.end, a.tree ? w.start : w.start + place(a, tile * 16).t + 1);
+  int t_last = place(a, tile * 16 + 15).t;
   t_last = t_last < w.count ? t_last : w.count - 1;
   const int until = idle ? 0 : (int)min64(w.end, a.tree ? w.start + w.count : w.start + t_last + 1);
   RowState<D> st;
@@ -840,9 +870,15 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
       else wait_vmcnt<0>();
       wait_lgkmcnt0();
       block_barrier();   // .. and every wave's; the step before is done with its slots
-      if (s + STEPS - 1 < steps) load_step(s + STEPS - 1);
+      const bool more = s + STEPS - 1 < steps;   // a step to load, between the products where there are any
+      if (more) aim(s + STEPS - 1);
       const int o = N == 2 ? 0 : part, c = w.c0 + s * 2 + o;
-      if (c >= w.c1 || c * 64 >= until) continue;   // (uniform over the wave)
+      if (c >= w.c1 || c * 64 >= until) {   // (uniform over the wave)
+        if (more)
+#pragma unroll
+          for (int i = 0; i < LOADS; ++i) load(i);
+        continue;
+      }
       uint32_t seen = 0, there = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -865,48 +901,74 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
           st, q, [&](int i, int n, int t) { return *(const i32x4*)(kp + i * G::BYTES + n * 4 * D + t * 256); },
           [&](int i, int t) { return *(const i32x4*)(vp + i * G::BYTES + t * 256); },
           [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 16 * n); },
-          [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); }, [] {}, all, seen);
+          [&](int i, int n) { return *(const floatx4*)(sp + i * G::BYTES + 256 + 16 * n); }, [] {},
+          [&](int i) {
+            if (i < LOADS && more) load(i);
+          },
+          all, seen);
     }
   };
   if (pair) walk(std::integral_constant<int, 1>());
   else walk(std::integral_constant<int, 2>());
   wait_vmcnt<0>();   // no load may still go to LDS
-  const float l = column_sum(st.l);
-  if (!pair && x.m >= 0) {
-    const int row = tile * 16 + col;
-    if (a.splits == 1) {
-      const float f = inverse_sum(l);
+  float l = column_sum(st.l);
+  if (whole < tiles) {   // the second waves of the pairs pass their states on, in lanes' places
+    floatx4(*os)[D / 16][64] = (floatx4(*)[D / 16][64])ring;
+    const int i = (wave - whole) / 2;
+    __syncthreads();   // the ring is free
+    if (pair && part == 1) {
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) write_out<D>(a, w, row, t * 16 + 4 * quad, elements(st, t), f);
-    } else {
-      const int64_t part = part_row(a, w, row);
-      float* po = a.part_o + part * D + 4 * quad;
+      for (int t = 0; t < D / 16; ++t) os[i][t][lane] = elements(st, t);
+      if (quad == 0) {
+        ml[i][col][0] = st.m;
+        ml[i][col][1] = l;
+      }
+    }
+    __syncthreads();
+    if (pair && part == 1) return;
+    if (pair) {
+      const float m1 = ml[i][col][0], m = fmaxf(st.m, m1);
+      const float f0 = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+      const float f1 = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(m1 - m);
+      st.m = m;
+      l = f0 * l + f1 * ml[i][col][1];
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) *(floatx4*)(po + t * 16) = elements(st, t);
-      if (quad == 0) write_sums(a, part, st.m, l);
+      for (int t = 0; t < D / 16; ++t) {
+        const floatx4 o = os[i][t][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[4 * t + e] = f0 * st.o[4 * t + e] + f1 * o[e];
+      }
     }
   }
-  if (whole < tiles) {
-    __syncthreads();   // the ring is free
-    join_waves<D, 2, 64 * RING_WAVES>(a, w, st, (float*)ring, ml, pair && tile < tile0 + tiles ? wave - whole : -1,
-                                      tile0 + whole, tiles - whole);
+  if (x.m < 0) return;
+  if (a.splits == 1) {
+    const float f = inverse_sum(l);
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) write_out<D>(a, x.m, x.head, t * 16 + 4 * quad, elements(st, t), f);
+  } else {
+    const int64_t part_at = part_row(a, w, tile * 16 + col);
+    float* po = a.part_o + part_at * D + 4 * quad;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) *(floatx4*)(po + t * 16) = elements(st, t);
+    if (quad == 0) write_sums(a, part_at, st.m, l);
   }
 }
 
-// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. The D / 4 threads of a
-// row's elements come GROUPS times, each with its splits, eight loads in flight: eight times for many
-// splits, once for a few (2304 rows of 8 splits: 9.0 us in eight groups).
+// The splits of a row joined: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. The threads of COLS
+// elements come GROUPS times, each with its splits, eight loads in flight: once for a few splits, else as
+// often as a workgroup holds.
 constexpr int JOIN = 512, AHEAD = 8;
 
-template <int D, int GROUPS>
+template <int D, int COLS, int GROUPS>
 __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
-  constexpr int W = D / 4, ROWS = JOIN / W / GROUPS;
+  constexpr int W = COLS / 4, ROWS = JOIN / W / GROUPS;
   __shared__ floatx4 red[GROUPS > 1 ? GROUPS : 1][ROWS][W];
-  const int c = threadIdx.x % W, g = threadIdx.x / W % GROUPS, i = threadIdx.x / W / GROUPS;
-  const int r = blockIdx.x * ROWS + i, h = blockIdx.y, b = blockIdx.z, t = r / a.G;
+  const int c = threadIdx.x % W + blockIdx.x % (D / COLS) * W, g = threadIdx.x / W % GROUPS;
+  const int i = threadIdx.x / W / GROUPS, r = blockIdx.x / (D / COLS) * ROWS + i, h = blockIdx.y, b = blockIdx.z;
+  const RowPlace at = place(a, r);
   int count = a.counts[b];
   count = count < a.T ? count : a.T;
-  const bool live = a.starts[b] >= 0 && t < count;
+  const bool live = a.starts[b] >= 0 && at.t < count;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   float m = NEG_INF, l = 0.f;
   if (live) {
@@ -945,17 +1007,14 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
     }
   }
   if constexpr (GROUPS > 1) {
-    red[g][i][c] = o;
+    red[g][i][c % W] = o;
     __syncthreads();
     if (g != 0) return;
 #pragma unroll
-    for (int k = 1; k < GROUPS; ++k) o += red[k][i][c];
+    for (int k = 1; k < GROUPS; ++k) o += red[k][i][c % W];
   }
   if (!live) return;
-  const float f = inverse_sum(l);
-  const int64_t row = (int64_t)b * a.T + t;
-  *(u32x2*)(a.out + (row * a.Hq + h * a.G + r % a.G) * D + 4 * c) =
-      u32x2{pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f)};
+  write_out<D>(a, (int64_t)b * a.T + at.t, h * a.G + at.g, 4 * c, o, inverse_sum(l));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -984,11 +1043,12 @@ Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t
 
 template <int D>
 void launch_join(const AttendArgs& a, int64_t batch, hipStream_t s) {
+  constexpr int COLS = D < 128 ? D : 128, GROUPS = JOIN / (COLS / 4);
   const bool few = a.splits <= AHEAD;
-  const int rows = JOIN / (D / 4) / (few ? 1 : 8);
-  const dim3 grid((unsigned)((a.T * a.G + rows - 1) / rows), (unsigned)a.Hkv, (unsigned)batch);
-  if (few) hipLaunchKernelGGL((join_kernel<D, 1>), grid, dim3(JOIN), 0, s, a);
-  else hipLaunchKernelGGL((join_kernel<D, 8>), grid, dim3(JOIN), 0, s, a);
+  const int rows = a.T * a.G, per = JOIN / (D / 4);
+  const dim3 grid((unsigned)(few ? (rows + per - 1) / per : rows * (D / COLS)), (unsigned)a.Hkv, (unsigned)batch);
+  if (few) hipLaunchKernelGGL((join_kernel<D, D, 1>), grid, dim3(JOIN), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<D, COLS, GROUPS>), grid, dim3(JOIN), 0, s, a);
 }
 
 }  // namespace
@@ -1125,7 +1185,9 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   a.G = (int)(num_heads / num_kv_heads);
   a.tiles = (int)p.tiles;
   a.splits = (int)p.splits;
-  a.units = (int)p.units;
+  a.unit = (int)(p.units / p.splits);
+  a.longer = (int)(p.units % p.splits);
+  a.g_inv = (uint32_t)std::min<uint64_t>((1ull << 32) / (uint64_t)a.G, 0xffffffffull);
   a.scale = scale;
   a.part_o = (float*)scratch;
   a.part_ml = (float*)scratch + batch * num_kv_heads * p.tiles * p.splits * 16 * head_size;
@@ -1134,7 +1196,7 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   auto more = head_size == 64 ? attend_ring_kernel<64>
               : head_size == 128 ? attend_ring_kernel<128> : attend_ring_kernel<256>;
   hipLaunchKernelGGL(p.ring ? more : few, grid, dim3(64 * (p.ring ? RING_WAVES : WAVES)), 0, S(stream), a.table,
-                     a.starts, a.counts, a.q, a.table_stride, a.T, a.G, a.units, a.splits, a.tiles, a.Hkv, a);
+                     a.starts, a.counts, a.q, a.table_stride, a.T, a.G, a.unit, a.longer, a.tiles, a.Hkv, a.g_inv, a);
   SV_CHECK_LAUNCH();
   if (p.splits > 1) {
     if (head_size == 64) launch_join<64>(a, batch, S(stream));
