@@ -51,27 +51,77 @@ struct AxesArgs {
   int count[MAX_AXES];     // pairs of each axis
 };
 
+// cos and sin of 2 pi t for |t| <= 1/2: a quarter turn and what is left, |z| <= pi / 4, whose Taylor series
+// to z^9 and z^8 leave less than 2^-24.
+__device__ __forceinline__ void cos_sin_turns(float t, float& c, float& s) {
+  const float quarter = rintf(4.f * t);
+  const float z = __builtin_fmaf(-0.25f, quarter, t) * 6.28318530717958648f, y = z * z;
+  float a = __builtin_fmaf(y, 1.f / 362880.f, -1.f / 5040.f);
+  a = __builtin_fmaf(y, a, 1.f / 120.f);
+  a = __builtin_fmaf(y, a, -1.f / 6.f);
+  a = __builtin_fmaf(y * z, a, z);
+  float b = __builtin_fmaf(y, 1.f / 40320.f, -1.f / 720.f);
+  b = __builtin_fmaf(y, b, 1.f / 24.f);
+  b = __builtin_fmaf(y, b, -0.5f);
+  b = __builtin_fmaf(y, b, 1.f);
+  const int q = (int)quarter;   // -2 .. 2
+  const float x = q & 1 ? a : b, w = q & 1 ? b : a;
+  c = __uint_as_float(__float_as_uint(x) ^ ((uint32_t)(q + 1) & 2u) << 30);
+  s = __uint_as_float(__float_as_uint(w) ^ ((uint32_t)q & 2u) << 30);
+}
+
 // The angle in turns, pos * inv_freq / 2 pi, is taken in 64 bits and without its whole turns: a
-// 32-bit product at position 220000 is off by up to 2^-7 of a radian.
+// 32-bit product at position 220000 is off by up to 2^-7 of a radian. A thread takes V pairs of AXES_ROWS
+// rows, whose frequencies it converts once; bound by its writes (262144 rows of 32 pairs).
+constexpr int AXES_ROWS = 4;
+
+template <int V>
 __global__ void __launch_bounds__(256) axes_kernel(AxesArgs a) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (idx >= a.rows * a.half) return;
-  const int64_t m = idx / a.half;
-  const int i = (int)(idx % a.half);
-  int axis = 0;
-  if (a.interleaved) {
-    axis = i % a.axes;
-    if (i / a.axes >= a.count[axis]) axis = 0;
-  } else {
-    int end = a.count[0];
-    while (i >= end && axis + 1 < a.axes) end += a.count[++axis];
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, cols = (uint32_t)(a.half / V);
+  const int64_t m0 = (int64_t)(idx / cols) * AXES_ROWS;
+  const int i0 = (int)(idx % cols) * V;
+  if (m0 >= a.rows) return;
+  int axis[V];
+  double freq[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = i0 + v;
+    axis[v] = 0;
+    if (a.interleaved) {
+      const int x = i % a.axes;
+#pragma unroll
+      for (int k = 0; k < MAX_AXES; ++k)
+        if (k == x && i / a.axes < a.count[k]) axis[v] = k;
+    } else {
+      int end = 0;
+#pragma unroll
+      for (int k = 0; k < MAX_AXES - 1; ++k) {
+        end += a.count[k];
+        if (k + 1 < a.axes && i >= end) axis[v] = k + 1;
+      }
+    }
+    freq[v] = (double)a.inv_freq[i] * 0.15915494309189533577;
   }
-  const double turns = (double)a.pos[axis * a.rows + m] * (double)a.inv_freq[i] * 0.15915494309189533577;
-  const float x = 2.f * (float)(turns - rint(turns));
-  float s, c;
-  sincospif(x, &s, &c);
-  a.cosv[idx] = c;
-  a.sinv[idx] = s;
+#pragma unroll
+  for (int r = 0; r < AXES_ROWS; ++r) {
+    const int64_t m = m0 + r;
+    if (m >= a.rows) return;
+    float c[V], s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const double turns = (double)a.pos[axis[v] * a.rows + m] * freq[v];
+      cos_sin_turns((float)(turns - rint(turns)), c[v], s[v]);
+    }
+    float* cp = a.cosv + m * a.half + i0;
+    float* sp = a.sinv + m * a.half + i0;
+    if constexpr (V == 4) {
+      *(floatx4*)cp = floatx4{c[0], c[1], c[2], c[3]};
+      *(floatx4*)sp = floatx4{s[0], s[1], s[2], s[3]};
+    } else {
+      *cp = c[0];
+      *sp = s[0];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1043,12 +1093,13 @@ Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t
 
 template <int D>
 void launch_join(const AttendArgs& a, int64_t batch, hipStream_t s) {
-  constexpr int COLS = D < 128 ? D : 128, GROUPS = JOIN / (COLS / 4);
-  const bool few = a.splits <= AHEAD;
-  const int rows = a.T * a.G, per = JOIN / (D / 4);
-  const dim3 grid((unsigned)(few ? (rows + per - 1) / per : rows * (D / COLS)), (unsigned)a.Hkv, (unsigned)batch);
-  if (few) hipLaunchKernelGGL((join_kernel<D, D, 1>), grid, dim3(JOIN), 0, s, a);
-  else hipLaunchKernelGGL((join_kernel<D, COLS, GROUPS>), grid, dim3(JOIN), 0, s, a);
+  constexpr int COLS = D < 128 ? D : 128, MOST = JOIN / (COLS / 4);
+  const int rows = a.T * a.G, groups = a.splits <= AHEAD ? 1 : a.splits <= 8 * AHEAD ? 8 : MOST;
+  const int per = groups == MOST ? 1 : JOIN / (D / 4) / groups;
+  const dim3 grid((unsigned)((rows + per - 1) / per * (groups == MOST ? D / COLS : 1)), (unsigned)a.Hkv, (unsigned)batch);
+  if (groups == 1) hipLaunchKernelGGL((join_kernel<D, D, 1>), grid, dim3(JOIN), 0, s, a);
+  else if (groups == 8) hipLaunchKernelGGL((join_kernel<D, D, 8>), grid, dim3(JOIN), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<D, COLS, MOST>), grid, dim3(JOIN), 0, s, a);
 }
 
 }  // namespace
@@ -1068,10 +1119,11 @@ SV_API int snowverify_rope_axes(const int64_t* pos, const float* inv_freq, float
   }
   if (sum != half) return SV_EINVAL;
   if (rows == 0) return SV_OK;
-  if (!pos || !inv_freq || !cosv || !sinv || rows > ((int64_t)1 << 40) / half) return SV_EINVAL;
-  const int64_t grid = (rows * half + 255) / 256;
-  if (!grid_ok(grid, 256)) return SV_EINVAL;
-  hipLaunchKernelGGL(axes_kernel, dim3((unsigned)grid), dim3(256), 0, S(stream), a);
+  if (!pos || !inv_freq || !cosv || !sinv || rows > ((int64_t)1 << 33) / half) return SV_EINVAL;
+  const bool four = half % 4 == 0 && (((uintptr_t)cosv | (uintptr_t)sinv) & 15) == 0;
+  const int64_t threads = (rows + AXES_ROWS - 1) / AXES_ROWS * (four ? half / 4 : half);
+  hipLaunchKernelGGL(four ? axes_kernel<4> : axes_kernel<1>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0,
+                     S(stream), a);
   SV_CHECK_LAUNCH();
   return SV_OK;
 }

@@ -160,13 +160,14 @@ __device__ __forceinline__ void rotate_queries(uint32_t u, int c, const QueryRow
 #pragma unroll
   for (int i = 0; i < Q_HEADS; ++i) {
     raw[i] = u32x4{0u, 0u, 0u, 0u};
-    if (i < heads) raw[i] = *(const u32x4*)(a.q + mr * a.stride + (int64_t)(head + i) * D + 8 * c);
+    if (i < heads)
+      raw[i] = __builtin_nontemporal_load((const u32x4*)(a.q + mr * a.stride + (int64_t)(head + i) * D + 8 * c));
   }
 #pragma unroll
   for (int i = 0; i < Q_HEADS; ++i) {
     const u32x4 o = rotate_norm<D>(raw[i], c, a.gamma, a.eps, a.cosv + mr * a.cs_stride,
                                    a.sinv + mr * a.cs_stride, a.half);
-    if (i < heads) *(u32x4*)(a.out + (mr * a.Hq + head + i) * D + 8 * c) = o;
+    if (i < heads) __builtin_nontemporal_store(o, (u32x4*)(a.out + (mr * a.Hq + head + i) * D + 8 * c));
   }
 }
 
