@@ -353,17 +353,17 @@ def save_gguf(path, cfg: VerifyConfig, tensors, *, parts: int = 1):
 
 
 def load_gguf(path, *, context: int, block: int, tree_parents=(), kv_std: float = 1.0,
-              seed: int = 0, name: str = None, sparse_pages: int = 0) -> VerifyModel:
+              seed: int = 0, name: str = None, sparse_pages: int = 0, kv8: bool = False) -> VerifyModel:
     """A VerifyModel whose weights come from the GGUF checkpoint at `path` (one file or the
     first part of a split one). The KV cache is random (kv_std, seed) and holds `context` prior
     tokens; `block` rows are verified per step, over selected pages of the context where
-    sparse_pages says how many. Installs the checkpoint's geometry (the repack
-    entry points read their shapes from it) and leaves it active."""
+    sparse_pages says how many, the cache in 8 bits where kv8 says so. Installs the checkpoint's
+    geometry (the repack entry points read their shapes from it) and leaves it active."""
     g = GGUF(path)
     try:
         cfg = config_from_gguf(g, context=context, block=block, tree_parents=tree_parents,
                                name=name)
-        cfg = replace(cfg, sparse_pages=sparse_pages)
+        cfg = replace(cfg, sparse_pages=sparse_pages, kv8=kv8)
         ops.define_geometry(**geometry_fields(cfg))
 
         def install(model: VerifyModel):

@@ -12,6 +12,9 @@ qwen3_5.py:32-78, layers.py:75-228) and its verify drivers (snowllm/engine/spec_
 263-309, 527-581). Every launch goes to torch's current stream and nothing allocates or
 synchronises inside step(), so the step can be captured in one HIP graph.
 
+With VerifyConfig.kv8 the KV cache is held in 8 bits (snowllm_amd.kv8): half the bytes per token, so that
+twice the context fits and its attention reads half as much; rope_sections gives positions several axes.
+
 With VerifyConfig.sparse_pages the attention is the one over selected pages (snowllm_amd.sparse):
 the cache write keeps the bounds of each page's keys, every row chooses the pages it reads, and
 only those are read, however long the context.
@@ -70,6 +73,11 @@ class VerifyConfig:
     sparse_pages: int = 0
     sparse_sink: int = 1
     sparse_recent: int = 2
+    # KV cache in 8 bits: KV8_GAIN
+    kv8: bool = False
+    # rotated pairs of every position axis (time, height, width), rot_half in all; empty: one axis
+    rope_sections: tuple = ()
+    rope_interleaved: bool = False   # the axes' pairs in turn instead of one section behind the other
 
     @property
     def moe(self):
@@ -252,6 +260,10 @@ class VerifyModel:
                     or cfg.sparse_sink + cfg.sparse_recent > cfg.sparse_pages):
                 raise SnowLLMError(f"sparse_pages {cfg.sparse_pages} does not hold the first "
                                    f"{cfg.sparse_sink} and the last {cfg.sparse_recent} (at least 1)")
+        if cfg.kv8 and cfg.sparse_pages:
+            raise SnowLLMError("attention over selected pages takes the bf16 cache")
+        if cfg.rope_sections and sum(cfg.rope_sections) != cfg.rot_half:
+            raise SnowLLMError(f"rope_sections {cfg.rope_sections} do not share {cfg.rot_half} pairs")
         self.batch = batch
         self.cfg = c = cfg
         self.keep_raw = keep_raw
@@ -286,18 +298,12 @@ class VerifyModel:
         self.pages = (c.context + T + c.page - 1) // c.page
         self.blocks = batch * self.pages + 8
         kvg = torch.Generator(device=dev).manual_seed(seed + 7)
-        shape_k = (self.blocks, c.kv_heads, c.head_dim // 16, c.page, 16)
-        shape_v = (self.blocks, c.kv_heads, c.page // 4, c.head_dim, 4)
-        self.k_pools, self.v_pools = [], []
-        for _ in range(c.layers):
-            k = torch.empty(shape_k, dtype=torch.bfloat16, device=dev)
-            v = torch.empty(shape_v, dtype=torch.bfloat16, device=dev)
-            k.normal_(0, kv_std, generator=kvg)
-            v.normal_(0, kv_std, generator=kvg)
-            self.k_pools.append(k)
-            self.v_pools.append(v)
+        if not c.kv8:
+            self._fill_pools(kvg, kv_std)
         perm = torch.randperm(self.blocks, device=dev, generator=kvg)[:batch * self.pages]
         self.table = perm.int().view(batch, -1).contiguous()
+        if c.kv8:
+            self._fill_caches(kvg, kv_std)
         self._alloc_step_buffers()
         if c.sparse_pages:
             # the prior tokens' pages come from elsewhere: their bounds, once
@@ -306,6 +312,32 @@ class VerifyModel:
             # per request, the pages whose bounds may leave out keys behind a block that ended in them
             self.cut_pages = [set() for _ in range(batch)]
             self._page_bounds([(0, self.pages)] * batch)
+
+    def _fill_pools(self, generator, std):
+        c = self.cfg
+        shape_k = (self.blocks, c.kv_heads, c.head_dim // 16, c.page, 16)
+        shape_v = (self.blocks, c.kv_heads, c.page // 4, c.head_dim, 4)
+        self.k_pools, self.v_pools = [], []
+        for _ in range(c.layers):
+            k = torch.empty(shape_k, dtype=torch.bfloat16, device="cuda")
+            v = torch.empty(shape_v, dtype=torch.bfloat16, device="cuda")
+            k.normal_(0, std, generator=generator)
+            v.normal_(0, std, generator=generator)
+            self.k_pools.append(k)
+            self.v_pools.append(v)
+
+    def _fill_caches(self, generator, std):
+        """The prior tokens' keys and values, quantised as the step writes them."""
+        c, B = self.cfg, self.batch
+        self.caches = [ops.kv8_cache(self.blocks, c.kv_heads, c.head_dim) for _ in range(c.layers)]
+        for cache in self.caches:
+            for first in range(0, c.context, 8192):
+                n = min(8192, c.context - first)
+                k, v = torch.empty(2, B * n, c.kv_heads, c.head_dim, dtype=torch.bfloat16,
+                                   device="cuda").normal_(0, std, generator=generator)
+                none = torch.empty(B * n, 0, device="cuda")
+                starts = torch.full((B,), first, dtype=torch.int32, device="cuda")
+                ops.kv8_append(k, v, none, none, cache, self.table, starts, torch.full_like(starts, n))
 
     def _page_bounds(self, spans):
         """Every layer's bounds of whole pages, from the K pools: request b's pages spans[b][0] ..
@@ -391,7 +423,8 @@ class VerifyModel:
         H = c.hidden
         bf = torch.bfloat16
         self.ids = torch.zeros(T, dtype=torch.int64, device=dev)
-        self.positions = torch.zeros(T, dtype=torch.int64, device=dev)
+        axes = (len(c.rope_sections),) if c.rope_sections else ()
+        self.positions = torch.zeros(*axes, T, dtype=torch.int64, device=dev)
         self.slots = torch.zeros(T, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(B, dtype=torch.int32, device=dev)
         self.lengths = [c.block] * B   # rows per request (ragged batches: set_batch)
@@ -407,7 +440,7 @@ class VerifyModel:
         self.res = [torch.empty(T, H, dtype=bf, device=dev) for _ in range(2)]
         self.proj = torch.empty(T, c.qkv_n, dtype=bf, device=dev)
         self.q = torch.empty(T, c.heads, c.head_dim, dtype=bf, device=dev)
-        self.attn = torch.empty(T, c.heads, c.head_dim, dtype=bf, device=dev)
+        self.attn = torch.zeros(T, c.heads, c.head_dim, dtype=bf, device=dev)
         self.o = torch.empty(T, H, dtype=bf, device=dev)
         self.h2 = torch.empty(T, H, dtype=bf, device=dev)
         wsH = ops.gemm_kquant_a_ws_bytes(T, H)
@@ -415,9 +448,13 @@ class VerifyModel:
         self.ws_h2 = torch.empty(wsH, dtype=torch.uint8, device=dev)
         self.ws_a = torch.empty(ops.gemm_kquant_a_ws_bytes(T, c.heads * c.head_dim),
                                 dtype=torch.uint8, device=dev)
-        if c.sparse_pages:
+        if c.sparse_pages or c.kv8:
             i32 = dict(dtype=torch.int32, device=dev)
             self.starts, self.counts = torch.zeros(B, **i32), torch.full((B,), c.block, **i32)
+        if c.kv8:
+            self.attn_scratch = ops.empty_bytes(max(16, ops.kv8_attention_scratch_bytes(
+                B, c.block, c.heads, c.kv_heads, c.head_dim, self.pages)))
+        elif c.sparse_pages:
             self.row_positions = torch.zeros(T, **i32)       # -1: a padding row
             self.row_pages = torch.empty(T, c.kv_heads, c.sparse_pages, **i32)
             shape = (B, c.block, c.heads, c.kv_heads, c.head_dim)
@@ -460,7 +497,7 @@ class VerifyModel:
         ctx = self.cfg.context if context is None else context
         self.set_batch(ids, [ctx] * B)
 
-    def set_batch(self, ids, contexts, lengths=None):
+    def set_batch(self, ids, contexts, lengths=None, positions=None):
         """Stage a batch: ids [batch, T] (each request's last token + drafts; a ragged request
         uses its first lengths[b] ids), request b's rows at positions contexts[b] + t (tree
         blocks: + depth) with its K/V written at those positions of its pages. Ragged batches
@@ -469,7 +506,8 @@ class VerifyModel:
         of the chain), and their logits are ignored. Host-side, outside the captured step; a
         graph captured with one ragged/uniform shape must be replayed with the same kind. With
         sparse_pages the contexts may move back and forth, and keys that something else writes into
-        the pools need ops.page_bounds."""
+        the pools need ops.page_bounds. positions: int [axes, batch, T] where the config has
+        rope_sections and a row's axes differ from its place in the cache (images)."""
         c, B, T = self.cfg, self.batch, self.cfg.block
         dev = "cuda"
         ids = torch.as_tensor(ids, dtype=torch.int64).view(B, T)
@@ -490,14 +528,22 @@ class VerifyModel:
                 slots.append(int(tbl[b, p // c.page]) * c.page + p % c.page if t < lengths[b]
                              else -1)
         self.ids.copy_(ids.reshape(-1).to(dev))
-        self.positions.copy_(torch.tensor(pos, dtype=torch.int64, device=dev))
+        if positions is None:
+            self.positions.copy_(torch.tensor(pos, dtype=torch.int64, device=dev))   # (of every axis)
+        elif not c.rope_sections:
+            raise SnowLLMError("set_batch: positions are for configurations with rope_sections")
+        else:
+            self.positions.copy_(torch.as_tensor(positions, dtype=torch.int64).reshape(-1, B * T))
         self.slots.copy_(torch.tensor(slots, dtype=torch.int32, device=dev))
         self.lens.copy_(torch.tensor([x + T for x in contexts], dtype=torch.int32, device=dev))
         self.lengths = lengths
-        if c.sparse_pages:
-            self._stage_bounds(contexts, lengths)
+        if c.sparse_pages or c.kv8:
             self.starts.copy_(torch.tensor(contexts, dtype=torch.int32, device=dev))
             self.counts.copy_(torch.tensor(lengths, dtype=torch.int32, device=dev))
+        if c.kv8:
+            return   # starts and counts say what a row sees, within a tree its masks too
+        if c.sparse_pages:
+            self._stage_bounds(contexts, lengths)
             self.row_positions.copy_(torch.tensor(
                 [x + t if t < n else -1 for x, n in zip(contexts, lengths) for t in range(T)],
                 dtype=torch.int32, device=dev))
@@ -524,7 +570,11 @@ class VerifyModel:
             gather_embedding_q4_k(self.ids, self.embed, self.x)
         else:
             Lops.gather_embedding(self.ids, self.embed, self.x)
-        Lops.rope_cos_sin(self.positions, self.inv_freq, self.cos, self.sin)
+        if c.rope_sections:
+            ops.rope_axes(self.positions, self.inv_freq, self.cos, self.sin, c.rope_sections,
+                          interleaved=c.rope_interleaved)
+        else:
+            Lops.rope_cos_sin(self.positions, self.inv_freq, self.cos, self.sin)
         res_in, res_out = None, self.res[0]
         n_layers = c.layers if upto_layer is None else upto_layer
         moe_out = False  # the previous layer's MoE output is still in (pairs, shared_out)
@@ -554,6 +604,8 @@ class VerifyModel:
                                            c.qkv_n - nqk, H, self.ws_h, col=nqk)
             if c.sparse_pages:
                 self._sparse_attention(i, lw)
+            elif c.kv8:
+                self._kv8_attention(i, lw)
             elif c.rot_half <= ops.FUSED_QK_MAX_HALF:
                 # QK-norm + RoPE + the block's K/V cache write inside the attention's launches
                 # with 256-wide heads the merge also writes the O projection's operands
@@ -571,7 +623,8 @@ class VerifyModel:
                 ops.paged_attention_explicit(self.q, self.k_pools[i], self.v_pools[i], self.attn,
                                              self.table, self.lens, c.head_dim ** -0.5,
                                              self.attn_scratch, tree=self.tree)
-            if not c.sparse_pages and c.rot_half <= ops.FUSED_QK_MAX_HALF and c.head_dim == 256:
+            if (not c.sparse_pages and not c.kv8 and c.rot_half <= ops.FUSED_QK_MAX_HALF
+                    and c.head_dim == 256):
                 ops.gemm_kquant_a_prepared(lw.o_fmt or c.attn_fmt, lw.o[0], lw.o[1], self.o, T,
                                            H, c.heads * c.head_dim, self.ws_a)
             else:
@@ -642,14 +695,28 @@ class VerifyModel:
         self.final_residual = res_out
         return self.logits
 
+    def _heads(self):
+        """q, k and v as views of self.proj."""
+        c = self.cfg
+        nq, nk = c.heads * c.head_dim, c.kv_heads * c.head_dim
+        return (self.proj[:, :nq].unflatten(1, (c.heads, c.head_dim)),
+                self.proj[:, nq:nq + nk].unflatten(1, (c.kv_heads, c.head_dim)),
+                self.proj[:, nq + nk:].unflatten(1, (c.kv_heads, c.head_dim)))
+
+    def _kv8_attention(self, i, lw):
+        """Layer i's quantising cache write and the attention over the cache: self.proj -> self.attn."""
+        c = self.cfg
+        q, k, v = self._heads()
+        ops.kv8_append(k, v, self.cos, self.sin, self.caches[i], self.table, self.starts, self.counts, q=q,
+                       q_out=self.q, q_gamma=lw.q_norm, k_gamma=lw.k_norm, eps=c.eps)
+        ops.kv8_attention(self.q, self.caches[i], self.attn, self.table, self.starts, self.counts,
+                          c.head_dim ** -0.5, self.attn_scratch, tree=self.tree)
+
     def _sparse_attention(self, i, lw):
         """Layer i's cache write with the bounds of its pages, the rows' choice of pages, and the
         attention over them: self.proj -> self.attn."""
         c = self.cfg
-        nq, nk = c.heads * c.head_dim, c.kv_heads * c.head_dim
-        q = self.proj[:, :nq].unflatten(1, (c.heads, c.head_dim))
-        k = self.proj[:, nq:nq + nk].unflatten(1, (c.kv_heads, c.head_dim))
-        v = self.proj[:, nq + nk:].unflatten(1, (c.kv_heads, c.head_dim))
+        q, k, v = self._heads()
         ops.kv_append(k, v, self.cos, self.sin, self.k_pools[i], self.v_pools[i], self.table,
                       self.starts, self.counts, bounds=self.bounds[i], q=q, q_out=self.q,
                       q_gamma=lw.q_norm, k_gamma=lw.k_norm, eps=c.eps)
