@@ -65,21 +65,34 @@ def _cache(cache):
         raise SnowLLMError(f"K pool: expected [blocks, Hkv, 4, d/16, 4, 16] with d in {HEAD_SIZES}, "
                            f"got {tuple(shape)}")
     dev = k.get_device()
-    if dev < 0:
-        _refuse(k, "K pool", I8, shape, dev)
     blocks, hkv, d = shape[0], shape[1], shape[3] * 16
-    kp = _need(k, "K pool", I8, shape, dev)
-    vp = _need(v, "V pool", I8, (blocks, hkv, d, PAGE), dev)
-    ksp = _need(ks, "K scales", F32, (blocks, hkv, PAGE), dev)
-    vsp = _need(vs, "V scales", F32, (blocks, hkv, PAGE), dev)
+    per_token = (blocks, hkv, PAGE)
+    # (as _need, in one condition)
+    if (dev < 0 or k.dtype is not I8 or v.dtype is not I8 or ks.dtype is not F32 or vs.dtype is not F32
+            or v.shape != (blocks, hkv, d, PAGE) or ks.shape != per_token or vs.shape != per_token
+            or v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev
+            or not k.is_contiguous() or not v.is_contiguous() or not ks.is_contiguous()
+            or not vs.is_contiguous()):
+        if dev < 0:
+            _refuse(k, "K pool", I8, shape, dev)
+        _need(k, "K pool", I8, shape, dev)
+        _need(v, "V pool", I8, (blocks, hkv, d, PAGE), dev)
+        _need(ks, "K scales", F32, per_token, dev)
+        _need(vs, "V scales", F32, per_token, dev)
+    kp, vp, ksp, vsp = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
     if (kp | vp | ksp | vsp) & 15:
         raise SnowLLMError("cache: every part must be 16-byte aligned")
     return kp, vp, ksp, vsp, blocks, hkv, d, dev
 
 
 @lru_cache(maxsize=64)
-def _sections(sections):
-    return (ctypes.c_int64 * len(sections))(*sections)
+def _sections(sections, axes, half, interleaved):
+    """The C array of an axes' sections, checked."""
+    if len(sections) != axes or min(sections) < 0 or sum(sections) != half or half < 1:
+        raise SnowLLMError(f"sections {sections} do not share {half} pairs between {axes} axes")
+    if interleaved and any(n and a + axes * (n - 1) >= half for a, n in enumerate(sections) if a):
+        raise SnowLLMError(f"sections {sections} of {half} pairs cannot take turns")
+    return (ctypes.c_int64 * axes)(*sections)
 
 
 def rope_axes(positions, inv_freq, cos, sin, sections, *, interleaved=False):
@@ -90,24 +103,20 @@ def rope_axes(positions, inv_freq, cos, sin, sections, *, interleaved=False):
     turn: pair i to axis i % axes while i // axes < sections[axis], to the first axis else. Angles
     are taken in 64 bits.
     """
-    if positions.dim() != 2 or not 1 <= positions.shape[0] <= 4:
-        raise SnowLLMError(f"positions: expected [axes, M] with one to four axes, got {tuple(positions.shape)}")
-    axes, M = positions.shape
+    shape = positions.shape
+    if len(shape) != 2 or not 1 <= shape[0] <= 4:
+        raise SnowLLMError(f"positions: expected [axes, M] with one to four axes, got {tuple(shape)}")
+    axes, M = shape
     half = inv_freq.shape[0] if inv_freq.dim() == 1 else 0
-    sections = tuple(sections)
-    if len(sections) != axes or min(sections) < 0 or sum(sections) != half or half < 1:
-        raise SnowLLMError(f"sections {sections} do not share {half} pairs between {axes} axes")
-    if interleaved and any(n and a + axes * (n - 1) >= half for a, n in enumerate(sections) if a):
-        raise SnowLLMError(f"sections {sections} of {half} pairs cannot take turns")
+    shares = _sections(tuple(sections), axes, half, bool(interleaved))
     dev = positions.get_device()
     if dev < 0:
-        _refuse(positions, "positions", I64, positions.shape, dev)
-    pp = _need(positions, "positions", I64, (axes, M), dev)
+        _refuse(positions, "positions", I64, shape, dev)
+    pp = _need(positions, "positions", I64, shape, dev)
     fp = _need(inv_freq, "inv_freq", F32, (half,), dev)
     cp = _need(cos, "cos", F32, (M, half), dev)
     sp = _need(sin, "sin", F32, (M, half), dev)
-    check(lib.snowverify_rope_axes(pp, fp, cp, sp, M, half, axes, _sections(sections), bool(interleaved),
-                                   _stream(dev)), "rope_axes")
+    check(lib.snowverify_rope_axes(pp, fp, cp, sp, M, half, axes, shares, interleaved, _stream(dev)), "rope_axes")
 
 
 def kv8_append(k, v, cos, sin, cache, table, starts, counts, *, q=None, q_out=None, q_gamma=None,
