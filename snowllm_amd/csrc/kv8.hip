@@ -325,10 +325,13 @@ struct AttendArgs {
   const int32_t* starts;
   const int32_t* counts;
   const uint64_t* tree;    // [rows] ancestor masks or null (causal)
-  float* part_o;           // [batch, Hkv, tiles, splits, 16, D]
-  float* part_ml;          // [batch, Hkv, tiles, splits, 16, 2]
+  float* part_o;           // [Hkv, slots, tiles, 16, D]
+  float* part_ml;          // [Hkv, slots, tiles, 16, 2]
   int64_t table_stride, blocks;
-  int T, Hq, Hkv, G, tiles, splits;
+  int T, Hq, Hkv, G, tiles;
+  int slots;               // workgroups of a kv head and tiles
+  int splits;              // of every request, 0: by the requests' lengths, batch <= 64 and <= slots
+  int batch;
   int unit, longer;        // a split's share of a request's steps; the first `longer` have one more
   uint32_t g_inv;          // floor(2^32 / G), at most 2^32 - 1
   float scale;
@@ -602,25 +605,65 @@ __device__ __forceinline__ floatx4 elements(const RowState<D>& st, int t) {
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }   // NaN stays
 
+// A slot's part of a request, as far as the keys go: the splits of the request are the slots from `first`.
+struct Slot {
+  int b, first, splits, c0, c1;
+};
+
+// Steps of STEP chunks of 64 keys that request b's rows see.
+template <int STEP>
+__device__ __forceinline__ int request_steps(const AttendArgs& a, int b) {
+  const int64_t start = a.starts[b];
+  int64_t count = a.counts[b], end;
+  count = count < a.T ? count : a.T;
+  end = start + count < a.table_stride * PAGE ? start + count : a.table_stride * PAGE;
+  return start < 0 || count <= 0 ? 0 : (int)((end + 64 * STEP - 1) / (64 * STEP));
+}
+
+// The slot `slot`, or the first one of request b (slot < 0). Where the lengths decide, every wave finds
+// the least steps a slot, from the mean on, with which all requests' splits have slots: lane b has request
+// b. (Sixteen blocks of 9 rows behind 4K to 8K tokens: 7 steps at most instead of 9.)
+template <int STEP>
+__device__ __forceinline__ Slot find_slot(const AttendArgs& a, int slot, int b) {
+  if (a.splits) {
+    if (slot >= 0) b = slot / a.splits;
+    const int split = slot - b * a.splits;
+    return {b, b * a.splits, a.splits, STEP * (split * a.unit + (split < a.longer ? split : a.longer)),
+            STEP * ((split + 1) * a.unit + (split + 1 < a.longer ? split + 1 : a.longer))};
+  }
+  const int lane = threadIdx.x & 63;
+  const int steps = lane < a.batch ? request_steps<STEP>(a, lane) : 0;
+  const int total = __builtin_amdgcn_readlane(wave_scan(steps), 63);
+  int share = (total + a.slots - 1) / a.slots, mine, upto;
+  share = share > 0 ? share : 1;
+  for (;;) {   // ends: with a share of the longest request, requests need no more slots than there are
+    mine = (int)((unsigned)(steps + share - 1) / (unsigned)share);
+    upto = wave_scan(mine);
+    if (__builtin_amdgcn_readlane(upto, 63) <= a.slots) break;
+    share += 1 + share / 16;
+  }
+  if (slot >= 0) {
+    const uint64_t found = __builtin_amdgcn_ballot_w64(slot < upto);
+    if (found == 0) return {-1, 0, 0, 0, 0};   // no part is left for it
+    b = __builtin_ctzll(found);
+  }
+  const int splits = __builtin_amdgcn_readlane(mine, b), first = __builtin_amdgcn_readlane(upto, b) - splits;
+  return {b, first, splits, STEP * share * (slot - first), STEP * share * (slot - first + 1)};
+}
+
 // What a workgroup does: tiles of a (request, kv head) against the chunks c0 .. c1 - 1 of 64 keys.
 struct Share {
   int64_t start;           // position of the request's first row
   int64_t end;             // one past the last position that the tiles see
   int count;               // the request's rows; 0: nothing to do
-  int b, h, split, c0, c1;
+  int b, h, slot, c0, c1;
+  bool single;             // no other split
 };
 
-// The split's chunks, wherever the request ends.
-template <int STEP>
-__device__ __forceinline__ int split_chunk(const AttendArgs& a, int split) {
-  return STEP * (split * a.unit + (split < a.longer ? split : a.longer));
-}
-
 // The first tile and how many: chunks up to the last position that one of their rows sees.
-template <int STEP>
-__device__ __forceinline__ Share find_share(const AttendArgs& a, int start, int count, int b, int h, int split, int tile,
-                                            int tiles) {
-  Share w{start, 0, count, b, h, split, split_chunk<STEP>(a, split), 0};
+__device__ __forceinline__ Share find_share(const AttendArgs& a, int start, int count, const Slot& at, int slot, int h,
+                                            int tile, int tiles) {
+  Share w{start, 0, count, at.b, h, slot, at.c0, 0, at.splits == 1};
   w.count = w.count < a.T ? w.count : a.T;
   if (w.start < 0 || w.count <= 0 || (int64_t)tile * 16 >= (int64_t)w.count * a.G) {
     w.count = 0;
@@ -630,7 +673,7 @@ __device__ __forceinline__ Share find_share(const AttendArgs& a, int start, int 
   t_last = t_last < w.count ? t_last : w.count - 1;
   w.end = a.tree ? w.start + w.count : w.start + t_last + 1;
   w.end = w.end < a.table_stride * PAGE ? w.end : a.table_stride * PAGE;
-  w.c1 = (int)min64((w.end + 63) / 64, split_chunk<STEP>(a, split + 1));
+  w.c1 = (int)min64((w.end + 63) / 64, at.c1);
   return w;
 }
 
@@ -643,7 +686,7 @@ __device__ __forceinline__ void write_out(const AttendArgs& a, int64_t m, int he
 
 // A row's place among the splits' states.
 __device__ __forceinline__ int64_t part_row(const AttendArgs& a, const Share& w, int r) {
-  return ((((int64_t)w.b * a.Hkv + w.h) * a.tiles + r / 16) * a.splits + w.split) * 16 + r % 16;
+  return (((int64_t)w.h * a.slots + w.slot) * a.tiles + r / 16) * 16 + r % 16;
 }
 
 __device__ __forceinline__ void write_sums(const AttendArgs& a, int64_t part, float m, float l) {
@@ -679,7 +722,7 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, 
       sum += f * ml[n][r][1];
       o += f * *(const floatx4*)(os + (n * 16 + r) * P + d);
     }
-    if (a.splits == 1) {
+    if (w.single) {
       write_out<D>(a, (int64_t)w.b * a.T + at.t, w.h * a.G + at.g, d, o, inverse_sum(sum));
     } else {
       const int64_t part = part_row(a, w, row);
@@ -698,11 +741,11 @@ constexpr int WAVES = 4;
 // The arguments that the first loads take come again in front, where they arrive in registers.
 #define KV8_FRONT                                                                                             \
   const int32_t *__restrict__ h_table, const int32_t *__restrict__ h_starts, const int32_t *__restrict__ h_counts, \
-      const uint16_t *__restrict__ h_q, int64_t h_table_stride, int h_T, int h_G, int h_unit, int h_longer,   \
+      const uint16_t *__restrict__ h_q, int64_t h_table_stride, int h_splits, int h_unit, int h_longer,       \
       int h_tiles, int h_Hkv, uint32_t h_g_inv, AttendArgs a
 #define KV8_TAKE_FRONT                                                                     \
   a.table = h_table, a.starts = h_starts, a.counts = h_counts, a.q = h_q;                  \
-  a.table_stride = h_table_stride, a.T = h_T, a.G = h_G, a.unit = h_unit, a.longer = h_longer; \
+  a.table_stride = h_table_stride, a.splits = h_splits, a.unit = h_unit, a.longer = h_longer; \
   a.tiles = h_tiles, a.Hkv = h_Hkv, a.g_inv = h_g_inv
 
 template <int D>
@@ -712,8 +755,11 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   __shared__ __attribute__((aligned(16))) float os[WAVES * 16 * (D + 4)];
   __shared__ float ml[WAVES][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int start = a.starts[blockIdx.z], count = a.counts[blockIdx.z];
-  const int h = a.tiles == 1 ? blockIdx.y : blockIdx.y >> 1, tile = a.tiles == 1 ? 0 : blockIdx.y & 1, b = blockIdx.z;
+  const Slot slot = find_slot<WAVES>(a, blockIdx.y, 0);
+  const int b = slot.b;
+  if (b < 0) return;
+  const int start = a.starts[b], count = a.counts[b];
+  const int h = a.tiles == 1 ? blockIdx.x : blockIdx.x >> 1, tile = a.tiles == 1 ? 0 : blockIdx.x & 1;
   const int64_t page_bytes = PAGE * D, block_bytes = page_bytes * a.Hkv;
   const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
   const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
@@ -731,11 +777,11 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
     return p;
   };
   auto valid = [&](int e) { return e >= 0 && e < a.blocks; };
-  int c = split_chunk<WAVES>(a, blockIdx.x) + wave;
+  int c = slot.c0 + wave;
   Pages here = look_up(c), next = look_up(c + WAVES);
   RawQuery<D> raw;
   fetch_query(raw, a, b, h, tile * 16 + col, quad);
-  const Share w = find_share<WAVES>(a, start, count, b, h, blockIdx.x, tile, 1);
+  const Share w = find_share(a, start, count, slot, blockIdx.y, h, tile, 1);
   if (w.count == 0) return;
   i32x4 kw[4][NS], vw[T];
   floatx4 kf[4], vf[4];
@@ -823,19 +869,22 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   __shared__ __attribute__((aligned(16))) uint8_t ring[G::SLOTS * G::BYTES];
   __shared__ float ml[RING_WAVES / 2][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int start = a.starts[blockIdx.z], count = a.counts[blockIdx.z];
-  const int groups = (a.tiles + RING_WAVES - 1) / RING_WAVES, b = blockIdx.z;
-  int h = blockIdx.y, tile0 = 0;
+  const Slot at_slot = find_slot<2>(a, blockIdx.y, 0);
+  const int b = at_slot.b;
+  if (b < 0) return;
+  const int start = a.starts[b], count = a.counts[b];
+  const int groups = (a.tiles + RING_WAVES - 1) / RING_WAVES;
+  int h = blockIdx.x, tile0 = 0;
   if (groups > 1) {
-    tile0 = (int)(blockIdx.y % (unsigned)groups) * RING_WAVES;
-    h = (int)(blockIdx.y / (unsigned)groups);
+    tile0 = (int)(blockIdx.x % (unsigned)groups) * RING_WAVES;
+    h = (int)(blockIdx.x / (unsigned)groups);
   }
   const int tiles = a.tiles - tile0 < RING_WAVES ? a.tiles - tile0 : RING_WAVES;
   const int whole = 2 * tiles > RING_WAVES ? 2 * tiles - RING_WAVES : 0;   // tiles of one wave
   const bool pair = wave >= whole;
   const int tile = tile0 + (pair ? whole + (wave - whole) / 2 : wave), part = (wave - whole) & 1;
   const int32_t* trow = a.table + (int64_t)b * a.table_stride;
-  const int c0 = split_chunk<2>(a, blockIdx.x);
+  const int c0 = at_slot.c0;
   // blocks of this wave's page in 64 chunks, one a lane
   auto look_up = [&](int first) {   // (past the table: its last page)
     const int64_t p = 4ll * (c0 + first + lane) + (wave & 3);
@@ -845,7 +894,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   int ids = look_up(0), ids_from = 0;
   RawQuery<D> raw;
   fetch_query(raw, a, b, h, tile * 16 + col, quad);
-  const Share w = find_share<2>(a, start, count, b, h, blockIdx.x, tile0, tiles);
+  const Share w = find_share(a, start, count, at_slot, blockIdx.y, h, tile0, tiles);
   if (w.count == 0) return;
   const int n_chunks = w.c1 - w.c0;
   // pages without a block are rare: whether there is one is found once, and each looked up only then
@@ -991,7 +1040,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
     }
   }
   if (x.m < 0) return;
-  if (a.splits == 1) {
+  if (w.single) {
     const float f = inverse_sum(l);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) write_out<D>(a, x.m, x.head, t * 16 + 4 * quad, elements(st, t), f);
@@ -1009,7 +1058,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
 // often as a workgroup holds.
 constexpr int JOIN = 512, AHEAD = 8;
 
-template <int D, int COLS, int GROUPS>
+template <int D, int STEP, int COLS, int GROUPS>
 __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
   constexpr int W = COLS / 4, ROWS = JOIN / W / GROUPS;
   __shared__ floatx4 red[GROUPS > 1 ? GROUPS : 1][ROWS][W];
@@ -1018,11 +1067,14 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
   const RowPlace at = place(a, r);
   int count = a.counts[b];
   count = count < a.T ? count : a.T;
+  const Slot slot = find_slot<STEP>(a, -1, b);
+  if (slot.splits <= 1) return;   // (uniform: written already)
   const bool live = a.starts[b] >= 0 && at.t < count;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   float m = NEG_INF, l = 0.f;
   if (live) {
-    const int64_t part = ((((int64_t)b * a.Hkv + h) * a.tiles + r / 16) * a.splits) * 16 + r % 16;
+    const int64_t part = (((int64_t)h * a.slots + slot.first) * a.tiles + r / 16) * 16 + r % 16;
+    const int64_t next = (int64_t)a.tiles * 16;   // the next split's
     const float2* ml = (const float2*)a.part_ml + part;
     const float* po = a.part_o + part * D + 4 * c;
     floatx4 x[AHEAD];
@@ -1030,29 +1082,29 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int s = s0 + k * GROUPS;
-        if (s < a.splits) x[k] = *(const floatx4*)(po + (int64_t)s * 16 * D);
+        if (s < slot.splits) x[k] = *(const floatx4*)(po + s * next * D);
       }
     };
     fetch(g);   // with the maxima and sums: one round trip
     // a row's maximum and sum, by W threads or more
     constexpr int L = W < 64 ? W : 64;
     const int lane = threadIdx.x % L;
-    for (int s = lane; s < a.splits; s += L) m = fmaxf(m, ml[s * 16].x);
+    for (int s = lane; s < slot.splits; s += L) m = fmaxf(m, ml[s * next].x);
 #pragma unroll
     for (int k = L / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, L));
     const float base = m == NEG_INF ? 0.f : m;
-    for (int s = lane; s < a.splits; s += L) {
-      const float2 e = ml[s * 16];
+    for (int s = lane; s < slot.splits; s += L) {
+      const float2 e = ml[s * next];
       l += __builtin_amdgcn_exp2f(e.x - base) * e.y;
     }
 #pragma unroll
     for (int k = L / 2; k > 0; k >>= 1) l += __shfl_xor(l, k, L);
-    for (int s0 = g; s0 < a.splits; s0 += AHEAD * GROUPS) {
+    for (int s0 = g; s0 < slot.splits; s0 += AHEAD * GROUPS) {
       if (s0 != g) fetch(s0);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int s = s0 + k * GROUPS;
-        if (s < a.splits) o += __builtin_amdgcn_exp2f(ml[s * 16].x - base) * x[k];
+        if (s < slot.splits) o += __builtin_amdgcn_exp2f(ml[s * next].x - base) * x[k];
       }
     }
   }
@@ -1073,10 +1125,12 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
 constexpr int64_t MAX_PAGES = 1 << 26;   // of a request: positions stay below 2^30
 
 struct Plan {
-  int64_t tiles, groups, splits, units;
+  int64_t tiles, groups, slots, splits, units;
   bool ring;
 };
 
+// The split of the keys: workgroups for every CU (twice, of those of one or two tiles). Several requests
+// share them by their lengths.
 Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t width) {
   Plan p;
   p.tiles = (tokens * (Hq / Hkv) + 15) / 16;
@@ -1084,22 +1138,45 @@ Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t
   p.groups = p.ring ? (p.tiles + RING_WAVES - 1) / RING_WAVES : p.tiles;
   const int64_t chunks = (width + 3) / 4, step = p.ring ? 2 : WAVES;
   p.units = (chunks + step - 1) / step;
-  const int64_t items = batch * Hkv * p.groups, target = p.ring ? 256 : 512;
-  p.splits = items < target ? target / items : 1;
-  p.splits = p.splits < p.units ? p.splits : p.units;
+  const int64_t per_head = (p.ring ? 256 : 512) / (Hkv * p.groups);
+  if (batch > 1 && batch <= 64 && batch < per_head && p.units > 1) {
+    p.splits = 0;
+    p.slots = per_head < batch * p.units ? per_head : batch * p.units;
+    return p;
+  }
+  p.splits = per_head / batch < p.units ? per_head / batch : p.units;
   if (p.splits < 1) p.splits = 1;
+  p.slots = batch * p.splits;
   return p;
 }
 
-template <int D>
-void launch_join(const AttendArgs& a, int64_t batch, hipStream_t s) {
+int64_t attend_bytes(const Plan& p, int64_t Hkv, int64_t D) {
+  return p.splits == 1 ? 0 : Hkv * p.slots * p.tiles * 16 * (D + 2) * 4;
+}
+
+template <int D, int STEP>
+void launch_join(const AttendArgs& a, hipStream_t s) {
   constexpr int COLS = D < 128 ? D : 128, MOST = JOIN / (COLS / 4);
-  const int rows = a.T * a.G, groups = a.splits <= AHEAD ? 1 : a.splits <= 8 * AHEAD ? 8 : MOST;
+  const int splits = a.splits ? a.splits : a.slots / a.batch;   // (about: any count is right in any form)
+  const int rows = a.T * a.G, groups = splits <= AHEAD ? 1 : splits <= 8 * AHEAD ? 8 : MOST;
   const int per = groups == MOST ? 1 : JOIN / (D / 4) / groups;
-  const dim3 grid((unsigned)((rows + per - 1) / per * (groups == MOST ? D / COLS : 1)), (unsigned)a.Hkv, (unsigned)batch);
-  if (groups == 1) hipLaunchKernelGGL((join_kernel<D, D, 1>), grid, dim3(JOIN), 0, s, a);
-  else if (groups == 8) hipLaunchKernelGGL((join_kernel<D, D, 8>), grid, dim3(JOIN), 0, s, a);
-  else hipLaunchKernelGGL((join_kernel<D, COLS, MOST>), grid, dim3(JOIN), 0, s, a);
+  const dim3 grid((unsigned)((rows + per - 1) / per * (groups == MOST ? D / COLS : 1)), (unsigned)a.Hkv,
+                  (unsigned)a.batch);
+  if (groups == 1) hipLaunchKernelGGL((join_kernel<D, STEP, D, 1>), grid, dim3(JOIN), 0, s, a);
+  else if (groups == 8) hipLaunchKernelGGL((join_kernel<D, STEP, D, 8>), grid, dim3(JOIN), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<D, STEP, COLS, MOST>), grid, dim3(JOIN), 0, s, a);
+}
+
+template <int D>
+void launch_attend(const AttendArgs& a, const Plan& p, hipStream_t s) {
+  // the heads of a page side by side: they lie behind one another in memory
+  const dim3 grid((unsigned)(p.groups * a.Hkv), (unsigned)p.slots);
+  hipLaunchKernelGGL(p.ring ? attend_ring_kernel<D> : attend_kernel<D>, grid, dim3(64 * (p.ring ? RING_WAVES : WAVES)),
+                     0, s, a.table, a.starts, a.counts, a.q, a.table_stride, a.splits, a.unit, a.longer, a.tiles, a.Hkv,
+                     a.g_inv, a);
+  if (p.splits == 1 || hipPeekAtLastError() != hipSuccess) return;
+  if (p.ring) launch_join<D, 2>(a, s);
+  else launch_join<D, WAVES>(a, s);
 }
 
 }  // namespace
@@ -1198,7 +1275,7 @@ SV_API int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tok
       table_stride > MAX_PAGES || batch * tokens == 0)
     return 0;
   const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
-  return p.splits == 1 ? 0 : batch * num_kv_heads * p.tiles * p.splits * 16 * (head_size + 2) * 4;
+  return attend_bytes(p, num_kv_heads, head_size);
 }
 
 SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void* k_pool,
@@ -1236,25 +1313,18 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   a.Hkv = (int)num_kv_heads;
   a.G = (int)(num_heads / num_kv_heads);
   a.tiles = (int)p.tiles;
+  a.slots = (int)p.slots;
   a.splits = (int)p.splits;
-  a.unit = (int)(p.units / p.splits);
-  a.longer = (int)(p.units % p.splits);
+  a.batch = (int)batch;
+  a.unit = p.splits ? (int)(p.units / p.splits) : 0;
+  a.longer = p.splits ? (int)(p.units % p.splits) : 0;
   a.g_inv = (uint32_t)std::min<uint64_t>((1ull << 32) / (uint64_t)a.G, 0xffffffffull);
   a.scale = scale;
   a.part_o = (float*)scratch;
-  a.part_ml = (float*)scratch + batch * num_kv_heads * p.tiles * p.splits * 16 * head_size;
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.groups * num_kv_heads), (unsigned)batch);
-  auto few = head_size == 64 ? attend_kernel<64> : head_size == 128 ? attend_kernel<128> : attend_kernel<256>;
-  auto more = head_size == 64 ? attend_ring_kernel<64>
-              : head_size == 128 ? attend_ring_kernel<128> : attend_ring_kernel<256>;
-  hipLaunchKernelGGL(p.ring ? more : few, grid, dim3(64 * (p.ring ? RING_WAVES : WAVES)), 0, S(stream), a.table,
-                     a.starts, a.counts, a.q, a.table_stride, a.T, a.G, a.unit, a.longer, a.tiles, a.Hkv, a.g_inv, a);
+  a.part_ml = (float*)scratch + num_kv_heads * p.slots * p.tiles * 16 * head_size;
+  if (head_size == 64) launch_attend<64>(a, p, S(stream));
+  else if (head_size == 128) launch_attend<128>(a, p, S(stream));
+  else launch_attend<256>(a, p, S(stream));
   SV_CHECK_LAUNCH();
-  if (p.splits > 1) {
-    if (head_size == 64) launch_join<64>(a, batch, S(stream));
-    else if (head_size == 128) launch_join<128>(a, batch, S(stream));
-    else launch_join<256>(a, batch, S(stream));
-    SV_CHECK_LAUNCH();
-  }
   return SV_OK;
 }

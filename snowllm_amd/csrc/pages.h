@@ -65,6 +65,17 @@ __device__ __forceinline__ float column_sum(float v) {
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+// Inclusive prefix sums over the wave's lanes, by row shifts and broadcasts.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // lanes 1, 2, 4, 8 back in a row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // lane 15 to the next row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
+  return v;
+}
+
 // Eight elements y of a head, d = 8 c .. 8 c + 7, normalised (gamma not null) and rotated in fp32; the
 // D / 8 threads of a head are neighbours in one wave. The rotation partner's raw words come from its
 // thread.

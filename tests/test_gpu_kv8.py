@@ -279,6 +279,11 @@ ATTEND = [
     (3, 3, 64, 130, [0, 50], [130, 129], False),
     (16, 1, 128, 2, [-1, 17], [2, 9], False),
     (34, 2, 64, 2, [77], [2], False),
+    # requests of very different lengths share the workgroups
+    (16, 2, 256, 9, [1700, 3, 800, 0, -1], [9, 9, 4, 1, 9], False),
+    (8, 2, 64, 1, [3000, 100, 0, 1999], [1, 1, 1, 0], False),
+    (8, 1, 128, 7, [900, 5, 640], [7, 7, 5], True),
+    (4, 1, 128, 1, [40 * i for i in range(40)], [1] * 40, False),
 ]
 
 
