@@ -378,7 +378,7 @@ int snowverify_rope_axes(const int64_t* pos, const float* inv_freq, float* cosv,
                          int64_t rows, int64_t half, int64_t axes, const int64_t* sections,
                          int interleaved, void* stream);
 /* snowverify_kv_append's cache write into a cache in 8 bits: K (normalised, rotated) and V quantised
- * from fp32, queries rotated alongside. */
+ * from fp32, queries rotated alongside. No page may be written twice in a call. */
 int snowverify_kv8_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                           const void* q, int64_t q_stride, const float* cos_in,
                           const float* sin_in, int64_t cs_stride, int64_t half,
@@ -403,7 +403,7 @@ int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, in
  * 64), those before starts[b] and the block's rows j < counts[b] whose bit j is set. Keys in pages
  * without a block or past the table are passed over; a row that sees none gets zeros; rows past a
  * request's count are left as they were. out must not overlap q; scale is finite. At most 65535
- * requests, and 65535 * 16 rows of (tokens * num_heads). */
+ * requests, and about 2^30 rows of (tokens * num_heads). */
 int snowverify_kv8_attention(const void* q, int64_t q_stride, const void* k_pool,
                              const void* v_pool, const float* k_scale, const float* v_scale,
                              void* out, const int32_t* table, const int32_t* starts,

@@ -340,7 +340,6 @@ struct AttendArgs {
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float TERM = 32512.f;      // the largest value of two terms, 127 * 256
 constexpr float RESCALE = 8.f;       // the maximum moves when a score exceeds it by 2^8
-typedef __attribute__((address_space(4))) const int32_t cint32;
 
 // One row of a lane's column: it sees the positions below `end`, and those from there on by its mask.
 struct Row {
@@ -610,14 +609,15 @@ struct Slot {
   int b, first, splits, c0, c1;
 };
 
-// Steps of STEP chunks of 64 keys that request b's rows see.
+// Steps of STEP chunks of 64 keys that request b's rows see (one where there are rows and no key).
 template <int STEP>
 __device__ __forceinline__ int request_steps(const AttendArgs& a, int b) {
   const int64_t start = a.starts[b];
   int64_t count = a.counts[b], end;
   count = count < a.T ? count : a.T;
   end = start + count < a.table_stride * PAGE ? start + count : a.table_stride * PAGE;
-  return start < 0 || count <= 0 ? 0 : (int)((end + 64 * STEP - 1) / (64 * STEP));
+  if (start < 0 || count <= 0) return 0;
+  return end > 0 ? (int)((end + 64 * STEP - 1) / (64 * STEP)) : 1;
 }
 
 // The slot `slot`, or the first one of request b (slot < 0). Where the lengths decide, every wave finds
@@ -1296,7 +1296,7 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
       (table_stride && !table) || !starts || !counts || scratch_bytes < need || (need && !scratch))
     return SV_EINVAL;
   const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
-  if (batch > 65535 || p.groups * num_kv_heads > 65535) return SV_ENOTSUP;
+  if (batch > 65535 || !grid_ok(p.groups * num_kv_heads, 64 * RING_WAVES)) return SV_ENOTSUP;
   AttendArgs a{};
   a.q = (const uint16_t*)q;
   a.q_stride = q_stride;

@@ -128,7 +128,8 @@ def kv8_append(k, v, cos, sin, cache, table, starts, counts, *, q=None, q_out=No
     K (and q, into q_out) is normalised per head where its gamma [d] is given and its first 2 half
     elements rotated in the pairs (i, i + half); K and V are quantised from fp32, q_out is rounded
     once to bf16 and may be q. Rows past a request's count are left as they were, in the pages and in
-    q_out. Requests must not share the pages they write.
+    q_out. No page may be written twice in a call: requests must not share those they write, and a
+    request's are different ones.
     """
     kp, vp, ksp, vsp, blocks, hkv, d, dev = _cache(cache)
     M = k.shape[0]

@@ -335,6 +335,26 @@ def test_attention_over_holes(gpu):
     assert (got.cpu()[8] == 0).all()
 
 
+@pytest.mark.parametrize("B", [1, 3, 70])
+@pytest.mark.parametrize("T", [1, 9])
+def test_attention_without_blocks_or_pages(gpu, B, T):
+    """A cache of no blocks, tables of no pages or of none that is there: zeros for every row of a request."""
+    Hq, Hkv, d = 16, 2, 128
+    g = torch.Generator().manual_seed(20)
+    q = torch.randn(B * T, Hq, d, generator=g).bfloat16().cuda()
+    counts = torch.tensor([T - b % 2 for b in range(B)], dtype=torch.int32)
+    live = torch.arange(T)[None] < counts[:, None]
+    empty = (torch.empty(0, Hkv, 4, 8, 4, 16, dtype=torch.int8), torch.empty(0, Hkv, d, 16, dtype=torch.int8),
+             torch.empty(0, Hkv, 16), torch.empty(0, Hkv, 16))
+    some = random_cache(g, 2, Hkv, d)
+    for cache, table in ((empty, torch.zeros(B, 100, dtype=torch.int32)), (some, torch.zeros(B, 0, dtype=torch.int32)),
+                         (some, torch.full((B, 100), -1, dtype=torch.int32)),
+                         (some, torch.full((B, 100), 2, dtype=torch.int32))):
+        starts = torch.tensor([(37 * b) % 1500 for b in range(B)], dtype=torch.int32)
+        got = run_attention(*on_gpu(q, cache, table, starts, counts), 0.1).cpu()
+        assert (got[live.view(-1)] == 0).all() and (got[~live.view(-1)] == 3).all()
+
+
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("T", [1, 9])
 def test_attention_nan_reaches_the_rows_that_see_it(gpu, which, T):
@@ -537,6 +557,64 @@ def test_graph(gpu):
         step()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, (*cache, qo, out, ko, vo, cos, sin)))
+
+
+def test_two_graphs_share_a_scratch_and_two_streams_do_not(gpu):
+    """Graphs of single tokens and of blocks over one scratch, replayed in turn; then both at once, each
+    with its own: the bits of the calls."""
+    from snowllm_amd import ops
+    g = torch.Generator().manual_seed(21)
+    Hq, Hkv, d, n = 16, 2, 128, 5000
+    W = n // PAGE + 2
+    cache, table = on_gpu(random_cache(g, W, Hkv, d), tables(g, 1, W, W))
+    sizes = (1, 9)
+    qs = [torch.randn(T, Hq, d, generator=g).bfloat16().cuda() for T in sizes]
+    outs = [torch.empty_like(q) for q in qs]
+    spans = [on_gpu(ints([n - 77 * T]), ints([T])) for T in sizes]
+    needs = [ops.kv8_attention_scratch_bytes(1, T, Hq, Hkv, d, W) for T in sizes]
+    assert min(needs) > 0
+    shared = ops.empty_bytes(max(needs))
+    own = [ops.empty_bytes(x) for x in needs]
+    want = [run_attention(q, cache, table, *span, 0.1) for q, span in zip(qs, spans)]
+    graphs = []
+    for q, out, span in zip(qs, outs, spans):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ops.kv8_attention(q, cache, out, table, *span, 0.1, shared)
+    for _ in range(3):
+        for i in (0, 1, 1, 0):
+            outs[i].fill_(5.0)
+            graphs[i].replay()
+            assert torch.equal(outs[i], want[i])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for out in outs:
+        out.fill_(5.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                ops.kv8_attention(qs[i], cache, outs[i], table, *spans[i], 0.1, own[i])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_attention_of_many_heads(gpu):
+    """More workgroups of heads and rows than 65535: the first and the last heads as by themselves."""
+    heads, d, T = 4096, 64, 2049
+    W = T // PAGE + 1
+    g = torch.Generator(device="cuda").manual_seed(22)
+    codes = dict(dtype=torch.int8, device="cuda", generator=g)
+    cache = (torch.randint(-127, 128, (W, heads, 4, 4, 4, 16), **codes),
+             torch.randint(-127, 128, (W, heads, d, 16), **codes),
+             torch.rand(W, heads, 16, device="cuda", generator=g) * 0.02,
+             torch.rand(W, heads, 16, device="cuda", generator=g) * 0.02)
+    q = torch.empty(T, heads, d, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    table = torch.randperm(W, device="cuda", generator=g).int()[None]
+    span = on_gpu(ints([0]), ints([T]))
+    got = run_attention(q, cache, table, *span, 0.1)
+    for at in (slice(0, 64), slice(heads - 64, heads)):
+        want = run_attention(q[:, at].contiguous(), tuple(x[:, at].contiguous() for x in cache), table, *span, 0.1)
+        assert torch.equal(got[:, at], want) and want.isfinite().all()
 
 
 def test_a_prompt_and_its_continuation(gpu):

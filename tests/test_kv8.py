@@ -89,7 +89,8 @@ def test_attention_takes_no_rows_and_no_grid():
     assert need > 0 and need % 16 == 0
     assert lib.snowverify_kv8_attention_scratch_bytes(1, 2, 8, 2, 64, 0) == 0
     assert lib.snowverify_kv8_attention_scratch_bytes(1, 2, 8, 3, 64, 9) == 0
-    # more requests than a launch holds
+    # more heads' rows than a launch holds, more requests
+    assert lib.snowverify_kv8_attention(*attention_args(tokens=1 << 24, heads=4096, hkv=64), None) == 801
     assert lib.snowverify_kv8_attention(*attention_args(batch=70000, scratch=16, n=1 << 60), None) == 801
 
 
