@@ -112,6 +112,10 @@ def test_refusals(gpu):
         VerifyModel(replace(cfg, kv8=True, sparse_pages=8))
     with pytest.raises(SnowLLMError, match="do not share"):
         VerifyModel(replace(cfg, rope_sections=(20, 20, 20)))
+    with pytest.raises(SnowLLMError, match="four axes"):
+        VerifyModel(replace(cfg, rope_sections=(8, 8, 8, 8, 0)))
+    with pytest.raises(SnowLLMError, match="take turns"):
+        VerifyModel(replace(cfg, rope_sections=(0, cfg.rot_half), rope_interleaved=True))
     m = VerifyModel(replace(cfg, kv8=True), seed=1)
     with pytest.raises(SnowLLMError, match="rope_sections"):
         m.set_batch(torch.zeros(1, 9), [10], positions=torch.zeros(3, 1, 9))
