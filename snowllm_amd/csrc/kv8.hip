@@ -150,11 +150,7 @@ __device__ __forceinline__ u32x2 quantise(const float (&y)[8], float& scale) {
     const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
     top = b > top ? b : top;
   }
-#pragma unroll
-  for (int s = D / 16; s > 0; s >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)top, s, D / 8);
-    top = o > top ? o : top;
-  }
+  top = over_head<D / 8>(top, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
   const bool fine = top < 0x7f800000u;
   const float most = fmaxf(__uint_as_float(top), LEAST);
   scale = fine ? __fdiv_rn(most, 127.f) : __uint_as_float(0x7fc00000u);
@@ -204,8 +200,8 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
       vraw = *(const u32x4*)(a.v + m * a.v_stride + (int64_t)h * D + 8 * c);
     }
     float y[8], z[8], k_scale, v_scale;
-    rotate_norm_f32<D>(y, kraw, c, a.k_gamma, a.rows.eps, a.rows.cosv + m * a.rows.cs_stride,
-                       a.rows.sinv + m * a.rows.cs_stride, a.rows.half);
+    rotate_norm_f32<D>(y, kraw, load_rotation(c, a.k_gamma, a.rows.eps, a.rows.cosv + m * a.rows.cs_stride,
+                                              a.rows.sinv + m * a.rows.cs_stride, a.rows.half));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       z[2 * i] = __uint_as_float(vraw[i] << 16);

@@ -76,31 +76,81 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Eight elements y of a head, d = 8 c .. 8 c + 7, normalised (gamma not null) and rotated in fp32; the
-// D / 8 threads of a head are neighbours in one wave. The rotation partner's raw words come from its
-// thread.
+// op over the W neighbouring lanes of a head, in every lane: lanes 16 apart, then 8, 4, 2 and 1.
+template <int W, typename Op>
+__device__ __forceinline__ uint32_t over_head(uint32_t v, Op op) {
+  static_assert(W == 8 || W == 16 || W == 32, "lanes of a head");
+  if constexpr (W == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  if constexpr (W >= 16) {
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));   // 8 round a row of 16
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));   // 4: eighths are alike
+  } else {
+    const int up = __builtin_amdgcn_update_dpp((int)v, (int)v, 0x104, 0xf, 0x5, false);    // 4 on, lanes 0 .. 3 of 8
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(up, (int)v, 0x114, 0xf, 0xa, false));  // 4 back, lanes 4 .. 7
+  }
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));
+  return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));
+}
+
+// What the norm and rotation of elements 8 c .. 8 c + 7 take besides the row: gammas of these and of
+// their partners, and angles, the sine with the sign of its term. Loaded once for a thread's heads.
+struct Rotation {
+  u32x4 gamma, other_gamma;
+  float cosv[8], sinv[8];
+  float eps;
+  int partner;             // the thread of the rotation's other half
+  bool norm, turn;
+};
+
+__device__ __forceinline__ Rotation load_rotation(int c, const uint16_t* gamma, float eps, const float* cr,
+                                                  const float* sr, int half) {
+  Rotation a;
+  const int h8 = half / 8;
+  a.eps = eps;
+  a.partner = c < h8 ? c + h8 : c < 2 * h8 ? c - h8 : c;
+  a.norm = gamma != nullptr;
+  a.turn = c < 2 * h8;
+  if (a.norm) {
+    a.gamma = *(const u32x4*)(gamma + 8 * c);
+    a.other_gamma = *(const u32x4*)(gamma + 8 * a.partner);
+  }
+  if (a.turn) {
+    const int i0 = c < h8 ? 8 * c : 8 * (c - h8);
+    const float sign = c < h8 ? -1.f : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      a.cosv[e] = cr[i0 + e];
+      a.sinv[e] = sign * sr[i0 + e];
+    }
+  }
+  return a;
+}
+
+// Eight elements y of a head, d = 8 c .. 8 c + 7, normalised and rotated in fp32; the D / 8 threads of a
+// head are neighbours in one wave. The rotation partner's raw words come from its thread.
 template <int D>
-__device__ __forceinline__ void rotate_norm_f32(float (&y)[8], u32x4 raw, int c, const uint16_t* gamma,
-                                                float eps, const float* cr, const float* sr, int half) {
+__device__ __forceinline__ void rotate_norm_f32(float (&y)[8], u32x4 raw, const Rotation& a) {
   constexpr int W = D / 8;
   float inv = 1.f;
-  if (gamma) {
+  if (a.norm) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float a = __uint_as_float(raw[i] << 16), b = __uint_as_float(raw[i] & 0xffff0000u);
-      ss = __builtin_fmaf(a, a, ss);
-      ss = __builtin_fmaf(b, b, ss);
+      const float lo = __uint_as_float(raw[i] << 16), hi = __uint_as_float(raw[i] & 0xffff0000u);
+      ss = __builtin_fmaf(lo, lo, ss);
+      ss = __builtin_fmaf(hi, hi, ss);
     }
-#pragma unroll
-    for (int s = W / 2; s > 0; s >>= 1) ss += __shfl_xor(ss, s, W);
-    inv = __frsqrt_rn(ss / (float)D + eps);
+    ss = __uint_as_float(over_head<W>(__float_as_uint(ss), [](uint32_t x, uint32_t y) {
+      return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+    }));
+    inv = __frsqrt_rn(ss / (float)D + a.eps);
   }
-  const int h8 = half / 8;
-  const int pc = c < h8 ? c + h8 : c < 2 * h8 ? c - h8 : c;
   u32x4 other;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)raw[i], pc, W);
+  for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)raw[i], a.partner, W);
   float z[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -109,30 +159,26 @@ __device__ __forceinline__ void rotate_norm_f32(float (&y)[8], u32x4 raw, int c,
     z[2 * i] = __uint_as_float(other[i] << 16) * inv;
     z[2 * i + 1] = __uint_as_float(other[i] & 0xffff0000u) * inv;
   }
-  if (gamma) {
-    const u32x4 g = *(const u32x4*)(gamma + 8 * c), go = *(const u32x4*)(gamma + 8 * pc);
+  if (a.norm) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      y[2 * i] *= __uint_as_float(g[i] << 16);
-      y[2 * i + 1] *= __uint_as_float(g[i] & 0xffff0000u);
-      z[2 * i] *= __uint_as_float(go[i] << 16);
-      z[2 * i + 1] *= __uint_as_float(go[i] & 0xffff0000u);
+      y[2 * i] *= __uint_as_float(a.gamma[i] << 16);
+      y[2 * i + 1] *= __uint_as_float(a.gamma[i] & 0xffff0000u);
+      z[2 * i] *= __uint_as_float(a.other_gamma[i] << 16);
+      z[2 * i + 1] *= __uint_as_float(a.other_gamma[i] & 0xffff0000u);
     }
   }
-  if (c < 2 * h8) {
-    const int i0 = c < h8 ? 8 * c : 8 * (c - h8);
-    const float sign = c < h8 ? -1.f : 1.f;
+  if (a.turn) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(y[e], cr[i0 + e], sign * (z[e] * sr[i0 + e]));
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(y[e], a.cosv[e], z[e] * a.sinv[e]);
   }
 }
 
 // The same, rounded once to bf16.
 template <int D>
-__device__ __forceinline__ u32x4 rotate_norm(u32x4 raw, int c, const uint16_t* gamma, float eps,
-                                             const float* cr, const float* sr, int half) {
+__device__ __forceinline__ u32x4 rotate_norm(u32x4 raw, const Rotation& a) {
   float y[8];
-  rotate_norm_f32<D>(y, raw, c, gamma, eps, cr, sr, half);
+  rotate_norm_f32<D>(y, raw, a);
   u32x4 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
@@ -174,10 +220,11 @@ __device__ __forceinline__ void rotate_queries(uint32_t u, int c, const QueryRow
     if (i < heads)
       raw[i] = __builtin_nontemporal_load((const u32x4*)(a.q + mr * a.stride + (int64_t)(head + i) * D + 8 * c));
   }
+  const Rotation turn =
+      load_rotation(c, a.gamma, a.eps, a.cosv + mr * a.cs_stride, a.sinv + mr * a.cs_stride, a.half);
 #pragma unroll
   for (int i = 0; i < Q_HEADS; ++i) {
-    const u32x4 o = rotate_norm<D>(raw[i], c, a.gamma, a.eps, a.cosv + mr * a.cs_stride,
-                                   a.sinv + mr * a.cs_stride, a.half);
+    const u32x4 o = rotate_norm<D>(raw[i], turn);
     if (i < heads) __builtin_nontemporal_store(o, (u32x4*)(a.out + (mr * a.Hq + head + i) * D + 8 * c));
   }
 }

@@ -114,8 +114,8 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
       kraw = *(const u32x4*)(a.k + m * a.k_stride + (int64_t)h * D + 8 * c);
       vraw = *(const u32x4*)(a.v + m * a.v_stride + (int64_t)h * D + 8 * c);
     }
-    const u32x4 o = rotate_norm<D>(kraw, c, a.k_gamma, a.eps, a.cosv + m * a.cs_stride,
-                                   a.sinv + m * a.cs_stride, a.half);
+    const u32x4 o = rotate_norm<D>(kraw, load_rotation(c, a.k_gamma, a.eps, a.cosv + m * a.cs_stride,
+                                                       a.sinv + m * a.cs_stride, a.half));
     if (live) {
       *(u32x4*)(ks + r * LD + 8 * c) = o;
       *(u32x4*)(vs + r * LD + 8 * c) = vraw;
