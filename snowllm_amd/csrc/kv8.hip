@@ -150,7 +150,7 @@ __device__ __forceinline__ u32x2 quantise(const float (&y)[8], float& scale) {
     const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
     top = b > top ? b : top;
   }
-  top = over_head<D / 8>(top, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+  top = over_lanes<D / 8>(top, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
   const bool fine = top < 0x7f800000u;
   const float most = fmaxf(__uint_as_float(top), LEAST);
   scale = fine ? __fdiv_rn(most, 127.f) : __uint_as_float(0x7fc00000u);
@@ -1061,47 +1061,46 @@ __global__ void __launch_bounds__(JOIN) join_kernel(AttendArgs a) {
   const int c = threadIdx.x % W + blockIdx.x % (D / COLS) * W, g = threadIdx.x / W % GROUPS;
   const int i = threadIdx.x / W / GROUPS, r = blockIdx.x / (D / COLS) * ROWS + i, h = blockIdx.y, b = blockIdx.z;
   const RowPlace at = place(a, r);
-  int count = a.counts[b];
-  count = count < a.T ? count : a.T;
   const Slot slot = find_slot<STEP>(a, -1, b);
   if (slot.splits <= 1) return;   // (uniform: written already)
+  const int most = a.tiles * 16 - 1, rc = r < most ? r : most;
+  const int64_t part = (((int64_t)h * a.slots + slot.first) * a.tiles + rc / 16) * 16 + rc % 16;
+  const int64_t next = (int64_t)a.tiles * 16;   // the next split's
+  const float2* ml = (const float2*)a.part_ml + part;
+  const float* po = a.part_o + part * D + 4 * c;
+  floatx4 x[AHEAD];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int s = s0 + k * GROUPS;
+      if (s < slot.splits) x[k] = *(const floatx4*)(po + s * next * D);
+    }
+  };
+  fetch(g);   // with the maxima, the sums and the request's lengths: one round trip
+  int count = a.counts[b];
+  count = count < a.T ? count : a.T;
   const bool live = a.starts[b] >= 0 && at.t < count;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   float m = NEG_INF, l = 0.f;
-  if (live) {
-    const int64_t part = (((int64_t)h * a.slots + slot.first) * a.tiles + r / 16) * 16 + r % 16;
-    const int64_t next = (int64_t)a.tiles * 16;   // the next split's
-    const float2* ml = (const float2*)a.part_ml + part;
-    const float* po = a.part_o + part * D + 4 * c;
-    floatx4 x[AHEAD];
-    auto fetch = [&](int s0) {
+  // a row's maximum and sum, by W threads or more
+  constexpr int L = W < 64 ? W : 64;
+  const int lane = threadIdx.x % L;
+  for (int s = lane; s < slot.splits; s += L) m = fmaxf(m, ml[s * next].x);
+  m = __uint_as_float(over_lanes<L>(__float_as_uint(m), [](uint32_t x, uint32_t y) {
+    return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+  }));
+  const float base = m == NEG_INF ? 0.f : m;
+  for (int s = lane; s < slot.splits; s += L) {
+    const float2 e = ml[s * next];
+    l += __builtin_amdgcn_exp2f(e.x - base) * e.y;
+  }
+  l = sum_over_lanes<L>(l);
+  for (int s0 = g; s0 < slot.splits; s0 += AHEAD * GROUPS) {
+    if (s0 != g) fetch(s0);
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int s = s0 + k * GROUPS;
-        if (s < slot.splits) x[k] = *(const floatx4*)(po + s * next * D);
-      }
-    };
-    fetch(g);   // with the maxima and sums: one round trip
-    // a row's maximum and sum, by W threads or more
-    constexpr int L = W < 64 ? W : 64;
-    const int lane = threadIdx.x % L;
-    for (int s = lane; s < slot.splits; s += L) m = fmaxf(m, ml[s * next].x);
-#pragma unroll
-    for (int k = L / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, L));
-    const float base = m == NEG_INF ? 0.f : m;
-    for (int s = lane; s < slot.splits; s += L) {
-      const float2 e = ml[s * next];
-      l += __builtin_amdgcn_exp2f(e.x - base) * e.y;
-    }
-#pragma unroll
-    for (int k = L / 2; k > 0; k >>= 1) l += __shfl_xor(l, k, L);
-    for (int s0 = g; s0 < slot.splits; s0 += AHEAD * GROUPS) {
-      if (s0 != g) fetch(s0);
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int s = s0 + k * GROUPS;
-        if (s < slot.splits) o += __builtin_amdgcn_exp2f(ml[s * next].x - base) * x[k];
-      }
+    for (int k = 0; k < AHEAD; ++k) {
+      const int s = s0 + k * GROUPS;
+      if (s < slot.splits) o += __builtin_amdgcn_exp2f(ml[s * next].x - base) * x[k];
     }
   }
   if constexpr (GROUPS > 1) {

@@ -76,11 +76,15 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// op over the W neighbouring lanes of a head, in every lane: lanes 16 apart, then 8, 4, 2 and 1.
+// op over W neighbouring lanes, in every one of them: lanes 32 apart, then 16, 8, 4, 2 and 1.
 template <int W, typename Op>
-__device__ __forceinline__ uint32_t over_head(uint32_t v, Op op) {
-  static_assert(W == 8 || W == 16 || W == 32, "lanes of a head");
-  if constexpr (W == 32) {
+__device__ __forceinline__ uint32_t over_lanes(uint32_t v, Op op) {
+  static_assert(W == 8 || W == 16 || W == 32 || W == 64, "neighbours that have a head's row or part of it");
+  if constexpr (W == 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  if constexpr (W >= 32) {
     const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = op(r[0], r[1]);
   }
@@ -93,6 +97,13 @@ __device__ __forceinline__ uint32_t over_head(uint32_t v, Op op) {
   }
   v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));
   return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));
+}
+
+template <int W>
+__device__ __forceinline__ float sum_over_lanes(float v) {
+  return __uint_as_float(over_lanes<W>(__float_as_uint(v), [](uint32_t x, uint32_t y) {
+    return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+  }));
 }
 
 // What the norm and rotation of elements 8 c .. 8 c + 7 take besides the row: gammas of these and of
@@ -143,9 +154,7 @@ __device__ __forceinline__ void rotate_norm_f32(float (&y)[8], u32x4 raw, const 
       ss = __builtin_fmaf(lo, lo, ss);
       ss = __builtin_fmaf(hi, hi, ss);
     }
-    ss = __uint_as_float(over_head<W>(__float_as_uint(ss), [](uint32_t x, uint32_t y) {
-      return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
-    }));
+    ss = sum_over_lanes<W>(ss);
     inv = __frsqrt_rn(ss / (float)D + a.eps);
   }
   u32x4 other;
