@@ -647,6 +647,26 @@ __device__ __forceinline__ Slot find_slot(const AttendArgs& a, int slot, int b) 
   return {b, first, splits, STEP * share * (slot - first), STEP * share * (slot - first + 1)};
 }
 
+// The workgroup's kv head, group of tiles and slot. Workgroups go to the eight XCDs in turn: those that
+// read the same keys, the groups of a (head, slot), are eight apart, so that their XCD's cache has the keys
+// (9 rows of 16 heads behind 24000 tokens 20 us; 28 with the groups side by side).
+struct Spot {
+  int h, group, slot;
+};
+
+__device__ __forceinline__ Spot find_spot(int Hkv, int groups) {
+  if (groups == 1) return {(int)blockIdx.x, 0, (int)blockIdx.y};   // heads side by side, as in memory
+  const uint32_t n = (uint32_t)groups, pairs = (uint32_t)Hkv * gridDim.y, whole = pairs / 8 * 8;
+  uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, first = 0, wide = 8;
+  if (at >= whole * n) {
+    at -= whole * n;
+    first = whole;
+    wide = pairs - whole;
+  }
+  const uint32_t row = at / wide, pair = first + row / n * wide + (at - row * wide);
+  return {(int)(pair % (uint32_t)Hkv), (int)(row % n), (int)(pair / (uint32_t)Hkv)};
+}
+
 // What a workgroup does: tiles of a (request, kv head) against the chunks c0 .. c1 - 1 of 64 keys.
 struct Share {
   int64_t start;           // position of the request's first row
@@ -728,7 +748,7 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, 
   }
 }
 
-// One or two tiles: a (request, kv head, tile, split) each; the waves take the split's chunks in turn and
+// A workgroup for each (request, kv head, tile, split); the waves take the split's chunks in turn and
 // join their states at the end. Operands come straight from memory into registers, the next chunk's K as
 // soon as the scores are done and its V after the products, so that a wave has 16 D .. 32 D bytes in
 // flight all the time.
@@ -751,11 +771,12 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   __shared__ __attribute__((aligned(16))) float os[WAVES * 16 * (D + 4)];
   __shared__ float ml[WAVES][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const Slot slot = find_slot<WAVES>(a, blockIdx.y, 0);
+  const Spot spot = find_spot(a.Hkv, a.tiles);
+  const int h = spot.h, tile = spot.group;
+  const Slot slot = find_slot<WAVES>(a, spot.slot, 0);
   const int b = slot.b;
   if (b < 0) return;
   const int start = a.starts[b], count = a.counts[b];
-  const int h = a.tiles == 1 ? blockIdx.x : blockIdx.x >> 1, tile = a.tiles == 1 ? 0 : blockIdx.x & 1;
   const int64_t page_bytes = PAGE * D, block_bytes = page_bytes * a.Hkv;
   const int8_t* kh = a.cache.k + h * page_bytes + quad * 64 + (col & 3) * 16;
   const int8_t* vh = a.cache.v + h * page_bytes + col * 16;
@@ -777,7 +798,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   Pages here = look_up(c), next = look_up(c + WAVES);
   RawQuery<D> raw;
   fetch_query(raw, a, b, h, tile * 16 + col, quad);
-  const Share w = find_share(a, start, count, slot, blockIdx.y, h, tile, 1);
+  const Share w = find_share(a, start, count, slot, spot.slot, h, tile, 1);
   if (w.count == 0) return;
   i32x4 kw[4][NS], vw[T];
   floatx4 kf[4], vf[4];
@@ -829,7 +850,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   join_waves<D, WAVES>(a, w, st, os, ml, wave, tile);
 }
 
-// More tiles: eight waves share the chunks of a split, two a step, through a ring in LDS. All eight load
+// Up to eight tiles: eight waves share the chunks of a split, two a step, through a ring in LDS. All eight load
 // (each one plane, K or V, of one of a chunk's four pages, and its scales) straight into LDS, ahead of
 // the products. Of n tiles the first 2 n - 8 have a wave each, which takes both chunks of a step at once
 // (one conversion of the sums for 128 keys); the others two, a chunk each, so that the four SIMDs have
@@ -865,16 +886,12 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   __shared__ __attribute__((aligned(16))) uint8_t ring[G::SLOTS * G::BYTES];
   __shared__ float ml[RING_WAVES / 2][16][2];
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const Slot at_slot = find_slot<2>(a, blockIdx.y, 0);
+  const Spot spot = find_spot(a.Hkv, (a.tiles + RING_WAVES - 1) / RING_WAVES);
+  const int h = spot.h, tile0 = spot.group * RING_WAVES;
+  const Slot at_slot = find_slot<2>(a, spot.slot, 0);
   const int b = at_slot.b;
   if (b < 0) return;
   const int start = a.starts[b], count = a.counts[b];
-  const int groups = (a.tiles + RING_WAVES - 1) / RING_WAVES;
-  int h = blockIdx.x, tile0 = 0;
-  if (groups > 1) {
-    tile0 = (int)(blockIdx.x % (unsigned)groups) * RING_WAVES;
-    h = (int)(blockIdx.x / (unsigned)groups);
-  }
   const int tiles = a.tiles - tile0 < RING_WAVES ? a.tiles - tile0 : RING_WAVES;
   const int whole = 2 * tiles > RING_WAVES ? 2 * tiles - RING_WAVES : 0;   // tiles of one wave
   const bool pair = wave >= whole;
@@ -890,7 +907,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   int ids = look_up(0), ids_from = 0;
   RawQuery<D> raw;
   fetch_query(raw, a, b, h, tile * 16 + col, quad);
-  const Share w = find_share(a, start, count, at_slot, blockIdx.y, h, tile0, tiles);
+  const Share w = find_share(a, start, count, at_slot, spot.slot, h, tile0, tiles);
   if (w.count == 0) return;
   const int n_chunks = w.c1 - w.c0;
   // pages without a block are rare: whether there is one is found once, and each looked up only then
@@ -1124,22 +1141,35 @@ struct Plan {
   bool ring;
 };
 
-// The split of the keys: workgroups for every CU (twice, of those of one or two tiles). Several requests
-// share them by their lengths.
-Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t width) {
+// The form, and the split of the keys.
+Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D, int64_t width) {
   Plan p;
   p.tiles = (tokens * (Hq / Hkv) + 15) / 16;
-  p.ring = p.tiles > 2;
+  const int64_t chunks = (width + 3) / 4, heads = batch * Hkv;
+  // In the ring's form a head's tiles share what is loaded, but a workgroup takes longer to start and its
+  // 128 rows make more to join. It is taken from a megabyte of keys a CU on that the tiles would each load
+  // (9 rows of 16 heads of 256 behind 220K tokens 78 us instead of 109; behind 24000 tokens 29 instead of
+  // 20; of 32 heads of 128 behind 64000 tokens 44 instead of 48, behind 8192 17 instead of 14.4), and for
+  // the tiles of many short prompts (8 of 128 rows, heads of 128: 11 us instead of 23).
+  p.ring = p.tiles > 1 && (p.tiles * heads * chunks >= (1 << 21) / D ||
+                           (p.tiles >= RING_WAVES && p.tiles * heads >= (1 << 18) / D));
   p.groups = p.ring ? (p.tiles + RING_WAVES - 1) / RING_WAVES : p.tiles;
-  const int64_t chunks = (width + 3) / 4, step = p.ring ? 2 : WAVES;
+  const int64_t step = p.ring ? 2 : WAVES;
   p.units = (chunks + step - 1) / step;
-  const int64_t per_head = (p.ring ? 256 : 512) / (Hkv * p.groups);
+  // A workgroup for every CU, in the ring and with heads of 256, of which one has 128 KiB in flight (two
+  // for every CU: 100K tokens 37 us instead of 29); two with the others (16 requests of 4K to 8K tokens,
+  // heads of 128: 50 us instead of 55).
+  const int64_t per_head = (p.ring || D == 256 ? 256 : 512) / (Hkv * p.groups);
   if (batch > 1 && batch <= 64 && batch < per_head && p.units > 1) {
+    // several requests share them by their lengths (16 blocks of 9 rows behind 4K to 8K tokens: 44 us
+    // instead of 47)
     p.splits = 0;
     p.slots = per_head < batch * p.units ? per_head : batch * p.units;
     return p;
   }
-  p.splits = per_head / batch < p.units ? per_head / batch : p.units;
+  p.splits = per_head / batch;
+  if (p.splits > 128) p.splits = 256 / (Hkv * p.groups * batch);   // (100K tokens, heads of 64: 17 us instead of 21)
+  if (p.splits > p.units) p.splits = p.units;
   if (p.splits < 1) p.splits = 1;
   p.slots = batch * p.splits;
   return p;
@@ -1269,7 +1299,7 @@ SV_API int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tok
   if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
       table_stride > MAX_PAGES || batch * tokens == 0)
     return 0;
-  const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
+  const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, head_size, table_stride);
   return attend_bytes(p, num_kv_heads, head_size);
 }
 
@@ -1290,7 +1320,7 @@ SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void*
   if (!q || !out || out == q || (blocks && (!k_pool || !v_pool || !k_scale || !v_scale)) ||
       (table_stride && !table) || !starts || !counts || scratch_bytes < need || (need && !scratch))
     return SV_EINVAL;
-  const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, table_stride);
+  const Plan p = attend_plan(batch, tokens, num_heads, num_kv_heads, head_size, table_stride);
   if (batch > 65535 || !grid_ok(p.groups * num_kv_heads, 64 * RING_WAVES)) return SV_ENOTSUP;
   AttendArgs a{};
   a.q = (const uint16_t*)q;

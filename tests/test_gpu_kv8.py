@@ -243,6 +243,21 @@ def test_append_q_in_place_and_without_rows(gpu):
 # ------------------------------------------------------------------------------------------
 # attention
 # ------------------------------------------------------------------------------------------
+def form_tables(table, form, Hq, Hkv, d, T):
+    """The same requests for one of the attention's two forms: tables of many pages that are not there
+    take the one whose tiles of 16 rows of a head share their keys (from 2^21 / d tiles times chunks of
+    four pages times heads on)."""
+    if form == "tiles":
+        return table
+    B, width = table.shape
+    tiles = -(-T * (Hq // Hkv) // 16)
+    most = 4 * -(-(1 << 21) // (d * tiles * B * Hkv))
+    return torch.nn.functional.pad(table, (0, max(0, most - width)), value=-1)
+
+
+FORMS = ["tiles", "ring"]
+
+
 def run_attention(q, cache, table, starts, counts, scale, tree=None, fill=3.0, out=None):
     from snowllm_amd import ops
     M, Hq, d = q.shape
@@ -284,17 +299,21 @@ ATTEND = [
     (8, 2, 64, 1, [3000, 100, 0, 1999], [1, 1, 1, 0], False),
     (8, 1, 128, 7, [900, 5, 640], [7, 7, 5], True),
     (4, 1, 128, 1, [40 * i for i in range(40)], [1] * 40, False),
+    (8, 2, 64, 9, [(53 * i) % 300 for i in range(66)], [9 - i % 10 for i in range(66)], False),
+    # tiles of many short prompts
+    (32, 16, 128, 64, [11 * i for i in range(16)], [64 - i for i in range(16)], False),
 ]
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("Hq,Hkv,d,T,starts,counts,tree", ATTEND)
-def test_attention(gpu, Hq, Hkv, d, T, starts, counts, tree):
-    say("attention", Hq, Hkv, d, T, starts, counts, tree)
+def test_attention(gpu, Hq, Hkv, d, T, starts, counts, tree, form):
+    say("attention", Hq, Hkv, d, T, starts, counts, tree, form)
     g = torch.Generator().manual_seed(Hq * 1000 + T)
     B = len(starts)
     width = max(max(s, 0) + T for s in starts) // PAGE + 1
     blocks = B * width + 3
-    table = tables(g, B, width, blocks)
+    table = form_tables(tables(g, B, width, blocks), form, Hq, Hkv, d, T)
     cache = random_cache(g, blocks, Hkv, d)
     q = (torch.randn(B * T, Hq, d, generator=g) * 2).bfloat16()
     masks = torch.cat([tree_masks(g, T) for _ in range(B)]) if tree else None
@@ -304,12 +323,14 @@ def test_attention(gpu, Hq, Hkv, d, T, starts, counts, tree):
     check_attention(got, *R.attention(q, cache, table, st, ct, scale, T, masks))
 
 
-def test_attention_over_holes(gpu):
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_over_holes(gpu, form):
     """Pages without a block and positions past the table; a row that sees nothing; masks of nothing;
     NaN in the places that no row sees."""
     g = torch.Generator().manual_seed(11)
-    Hq, Hkv, d, T = 8, 2, 128, 4
+    Hq, Hkv, d, T = 16, 2, 128, 4
     table = ints([[3, -1, 2, 9, 1], [-1, -1, -1, -1, -1], [0, 4, 5, 6, 7]])
+    table = form_tables(table, form, Hq, Hkv, d, T)
     st, ct = ints([78, 20, 0]), ints([4, 4, 4])
     cache = random_cache(g, 9, Hkv, d)
     for x in cache[2:]:
@@ -336,8 +357,8 @@ def test_attention_over_holes(gpu):
 
 
 @pytest.mark.parametrize("B", [1, 3, 70])
-@pytest.mark.parametrize("T", [1, 9])
-def test_attention_without_blocks_or_pages(gpu, B, T):
+@pytest.mark.parametrize("T,W", [(1, 100), (9, 100), (9, 9000)])
+def test_attention_without_blocks_or_pages(gpu, B, T, W):
     """A cache of no blocks, tables of no pages or of none that is there: zeros for every row of a request."""
     Hq, Hkv, d = 16, 2, 128
     g = torch.Generator().manual_seed(20)
@@ -347,21 +368,21 @@ def test_attention_without_blocks_or_pages(gpu, B, T):
     empty = (torch.empty(0, Hkv, 4, 8, 4, 16, dtype=torch.int8), torch.empty(0, Hkv, d, 16, dtype=torch.int8),
              torch.empty(0, Hkv, 16), torch.empty(0, Hkv, 16))
     some = random_cache(g, 2, Hkv, d)
-    for cache, table in ((empty, torch.zeros(B, 100, dtype=torch.int32)), (some, torch.zeros(B, 0, dtype=torch.int32)),
-                         (some, torch.full((B, 100), -1, dtype=torch.int32)),
-                         (some, torch.full((B, 100), 2, dtype=torch.int32))):
+    for cache, table in ((empty, torch.zeros(B, W, dtype=torch.int32)), (some, torch.zeros(B, 0, dtype=torch.int32)),
+                         (some, torch.full((B, W), -1, dtype=torch.int32)),
+                         (some, torch.full((B, W), 2, dtype=torch.int32))):
         starts = torch.tensor([(37 * b) % 1500 for b in range(B)], dtype=torch.int32)
         got = run_attention(*on_gpu(q, cache, table, starts, counts), 0.1).cpu()
         assert (got[live.view(-1)] == 0).all() and (got[~live.view(-1)] == 3).all()
 
 
 @pytest.mark.parametrize("which", ["k", "v"])
-@pytest.mark.parametrize("T", [1, 9])
-def test_attention_nan_reaches_the_rows_that_see_it(gpu, which, T):
+@pytest.mark.parametrize("T,form", [(1, "tiles"), (9, "tiles"), (9, "ring")])
+def test_attention_nan_reaches_the_rows_that_see_it(gpu, which, T, form):
     g = torch.Generator().manual_seed(12)
     Hq, Hkv, d = 8, 2, 64
     cache = random_cache(g, 30, Hkv, d)
-    table = ints([list(range(29, -1, -1))])
+    table = form_tables(ints([list(range(29, -1, -1))]), form, Hq, Hkv, d, T)
     cache[2 if which == "k" else 3][29 - 2, 1, 5] = NAN          # position 37 of kv head 1
     for start in (0, 37 - T // 2, 400):
         q = torch.randn(T, Hq, d, generator=g).bfloat16()
@@ -412,7 +433,8 @@ def test_attention_of_a_sink_and_small_weights(gpu):
     assert (error[0] < 2e-3).all()
 
 
-@pytest.mark.parametrize("Hq,Hkv,d,T,start", [(16, 2, 256, 11, 20011), (8, 2, 64, 1, 33333), (32, 8, 128, 9, 9001)])
+@pytest.mark.parametrize("Hq,Hkv,d,T,start", [(16, 2, 256, 11, 20011), (16, 2, 256, 11, 50011), (8, 2, 64, 1, 33333), (32, 8, 128, 9, 9001),
+                                                   (32, 8, 128, 9, 45001), (16, 2, 64, 33, 62001)])
 def test_attention_long(gpu, Hq, Hkv, d, T, start):
     """Many splits, joined."""
     say("long", Hq, Hkv, d, T, start)
