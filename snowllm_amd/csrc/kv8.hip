@@ -1160,14 +1160,15 @@ Plan attend_plan(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t
   // for every CU: 100K tokens 37 us instead of 29); two with the others (16 requests of 4K to 8K tokens,
   // heads of 128: 50 us instead of 55).
   const int64_t per_head = (p.ring || D == 256 ? 256 : 512) / (Hkv * p.groups);
-  if (batch > 1 && batch <= 64 && batch < per_head && p.units > 1) {
+  if (batch > 1 && batch <= 64 && batch < per_head && p.units > 2) {
     // several requests share them by their lengths (16 blocks of 9 rows behind 4K to 8K tokens: 44 us
     // instead of 47)
     p.splits = 0;
     p.slots = per_head < batch * p.units ? per_head : batch * p.units;
     return p;
   }
-  p.splits = per_head / batch;
+  // two steps stay together: joining them takes longer (400 tokens 12.2 us instead of 7.9)
+  p.splits = p.units > 2 ? per_head / batch : 1;
   if (p.splits > 128) p.splits = 256 / (Hkv * p.groups * batch);   // (100K tokens, heads of 64: 17 us instead of 21)
   if (p.splits > p.units) p.splits = p.units;
   if (p.splits < 1) p.splits = 1;
