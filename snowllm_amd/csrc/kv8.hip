@@ -72,7 +72,7 @@ __device__ __forceinline__ void cos_sin_turns(float t, float& c, float& s) {
 
 // The angle in turns, pos * inv_freq / 2 pi, is taken in 64 bits and without its whole turns: a
 // 32-bit product at position 220000 is off by up to 2^-7 of a radian. A thread takes V pairs of AXES_ROWS
-// rows, whose frequencies it converts once; bound by its writes (262144 rows of 32 pairs).
+// rows, whose frequencies it converts once; bound by its writes (262144 rows of 32 pairs: 73 MB in 15 us).
 constexpr int AXES_ROWS = 4;
 
 template <int V>
@@ -164,7 +164,9 @@ __device__ __forceinline__ u32x2 quantise(const float (&y)[8], float& scale) {
 }
 
 // 2 D threads: sixteen rows of D / 8 threads each. A page workgroup owns one (request, page, kv head):
-// its threads take a token's row each, and the codes go through LDS into the page's layout.
+// its threads take a token's row each, and the codes go through LDS into the page's layout, so that every
+// write is of 16 bytes but in pages that begin or end a request. Bound by bytes, most of them the
+// queries' (8192 rows of 16 + 2 heads of 256: 145 MB in 31 us).
 template <int D>
 __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   constexpr int W = D / 8, VP = D + 8;   // VP: pitch of V's codes in LDS, by token
@@ -259,7 +261,8 @@ __device__ __forceinline__ u32x4 values(u32x2 w, float scale) {
   return o;
 }
 
-// 2 D threads take a (request, page, kv head): sixteen rows of D / 8 threads each.
+// 2 D threads take a (request, page, kv head): sixteen rows of D / 8 threads each; V goes through LDS. Bound
+// by bytes (131071 rows of 2 heads of 256: 405 MB in 79 us).
 template <int D>
 __global__ void __launch_bounds__(2 * D) read_kernel(ReadArgs a) {
   constexpr int W = D / 8, VP = D + 8;
@@ -750,8 +753,9 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Share& w, 
 
 // A workgroup for each (request, kv head, tile, split); the waves take the split's chunks in turn and
 // join their states at the end. Operands come straight from memory into registers, the next chunk's K as
-// soon as the scores are done and its V after the products, so that a wave has 16 D .. 32 D bytes in
-// flight all the time.
+// soon as the scores are done and its V after the products, so that a wave has 64 D .. 128 D bytes in
+// flight all the time. Bound by bytes for single tokens (64 requests of 8192 tokens, 8 kv heads of 128: 836 MB
+// in 154 us), by the chain of table, keys, join where there are few (one: 8 us and 3 for the join).
 constexpr int WAVES = 4;
 
 // The arguments that the first loads take come again in front, where they arrive in registers.
@@ -854,7 +858,10 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
 // (each one plane, K or V, of one of a chunk's four pages, and its scales) straight into LDS, ahead of
 // the products. Of n tiles the first 2 n - 8 have a wave each, which takes both chunks of a step at once
 // (one conversion of the sums for 128 keys); the others two, a chunk each, so that the four SIMDs have
-// about the same to do: six tiles 1.5 tiles a chunk and SIMD instead of 2.
+// about the same to do: six tiles 1.5 tiles a chunk and SIMD instead of 2. Bound by the products and the
+// softmax beside them (1024 rows of 16 heads of 256 behind 16001 tokens: 277 GFLOP, twice that in 8 bits, in
+// 288 us with the join); with few rows about as long for the loads (11 rows behind 220K tokens: 229 MB in
+// 65 us, either alone 53).
 constexpr int RING_WAVES = 8;
 
 template <int D>
