@@ -85,6 +85,23 @@ def _cache(cache):
     return kp, vp, ksp, vsp, blocks, hkv, d, dev
 
 
+def _spans(table, starts, counts, M, dev):
+    """(addresses of the three, batch, tokens, pages per request) of M padded rows."""
+    shape = table.shape
+    # (as _requests and _need, in one condition)
+    if (len(shape) == 2 and table.dtype is I32 and starts.dtype is I32 and counts.dtype is I32
+            and starts.shape == shape[:1] and counts.shape == shape[:1] and table.get_device() == dev
+            and starts.get_device() == dev and counts.get_device() == dev and table.is_contiguous()
+            and starts.is_contiguous() and counts.is_contiguous()):
+        batch, width = shape
+        if batch and M % batch == 0:
+            return table.data_ptr(), starts.data_ptr(), counts.data_ptr(), batch, M // batch, width
+    tp, batch, tokens, width = _requests(table, M, dev)
+    st = _need(starts, "starts", I32, (batch,), dev)
+    ct = _need(counts, "counts", I32, (batch,), dev)
+    return tp, st, ct, batch, tokens, width
+
+
 @lru_cache(maxsize=64)
 def _sections(sections, axes, half, interleaved):
     """The C array of an axes' sections, checked."""
@@ -133,7 +150,7 @@ def kv8_append(k, v, cos, sin, cache, table, starts, counts, *, q=None, q_out=No
     """
     kp, vp, ksp, vsp, blocks, hkv, d, dev = _cache(cache)
     M = k.shape[0]
-    tp, batch, tokens, width = _requests(table, M, dev)
+    tp, st, ct, batch, tokens, width = _spans(table, starts, counts, M, dev)
     rows = (M, hkv, d)
     k_at, ks = _rows(k, "k", rows, dev)
     v_at, vs = _rows(v, "v", rows, dev)
@@ -143,8 +160,6 @@ def kv8_append(k, v, cos, sin, cache, table, starts, counts, *, q=None, q_out=No
                            f"got {tuple(cos.shape)}")
     cp = _need(cos, "cos", F32, (M, half), dev)
     sp = _need(sin, "sin", F32, (M, half), dev)
-    st = _need(starts, "starts", I32, (batch,), dev)
-    ct = _need(counts, "counts", I32, (batch,), dev)
     qg = 0 if q_gamma is None else _need(q_gamma, "q gamma", BF16, (d,), dev)
     kg = 0 if k_gamma is None else _need(k_gamma, "k gamma", BF16, (d,), dev)
     heads, qp, qs, qo = hkv, 0, 0, 0
@@ -166,13 +181,11 @@ def kv8_read(cache, table, starts, counts, k, v):
     pages without a block, are left as they were."""
     kp, vp, ksp, vsp, blocks, hkv, d, dev = _cache(cache)
     M = k.shape[0]
-    tp, batch, tokens, width = _requests(table, M, dev)
+    tp, st, ct, batch, tokens, width = _spans(table, starts, counts, M, dev)
     ko = _need(k, "k", BF16, (M, hkv, d), dev)
     vo = _need(v, "v", BF16, (M, hkv, d), dev)
     if ko == vo and M:
         raise SnowLLMError("v must not be k")
-    st = _need(starts, "starts", I32, (batch,), dev)
-    ct = _need(counts, "counts", I32, (batch,), dev)
     check(lib.snowverify_kv8_read(kp, vp, ksp, vsp, tp, st, ct, ko, vo, batch, tokens, hkv, d, width,
                                   blocks, _stream(dev)), "kv8_read")
 
@@ -199,14 +212,13 @@ def kv8_attention(q, cache, out, table, starts, counts, scale, scratch=None, *, 
     if q.dim() != 3:
         raise SnowLLMError(f"q: expected [rows, Hq, d], got {tuple(q.shape)}")
     M, heads = q.shape[0], q.shape[1]
-    tp, batch, tokens, width = _requests(table, M, dev)
+    tp, st, ct, batch, tokens, width = _spans(table, starts, counts, M, dev)
     _groups(heads, hkv)
-    qp, qs = _rows(q, "q", (M, heads, d), dev)
-    op = _need(out, "out", BF16, (M, heads, d), dev)
+    shape = (M, heads, d)
+    qp, qs = _rows(q, "q", shape, dev)
+    op = _need(out, "out", BF16, shape, dev)
     if op == qp and M:
         raise SnowLLMError("out must not be q")
-    st = _need(starts, "starts", I32, (batch,), dev)
-    ct = _need(counts, "counts", I32, (batch,), dev)
     if tree is None:
         mp = 0
     else:
