@@ -265,6 +265,8 @@ class VerifyModel:
                                    f"{cfg.sparse_sink} and the last {cfg.sparse_recent} (at least 1)")
         if cfg.kv8 and cfg.sparse_pages:
             raise SnowLLMError("attention over selected pages takes the bf16 cache")
+        if cfg.kv8 and cfg.page != 16:
+            raise SnowLLMError(f"the cache in 8 bits has pages of 16 tokens, not {cfg.page}")
         if cfg.rope_sections:
             if len(cfg.rope_sections) > 4:
                 raise SnowLLMError(f"rope_sections {cfg.rope_sections}: at most four axes")
@@ -523,6 +525,12 @@ class VerifyModel:
             raise SnowLLMError("set_batch: ragged lengths apply to chain blocks of <= 64 rows")
         if any(x < 0 or x + T > self.pages * c.page for x in contexts):
             raise SnowLLMError("set_batch: a request's block runs past its pages")
+        if positions is not None:
+            positions = torch.as_tensor(positions, dtype=torch.int64)
+            if positions.shape != (len(c.rope_sections), B, T):
+                raise SnowLLMError(f"set_batch: positions are [axes of rope_sections, {B}, {T}], got "
+                                   f"{tuple(positions.shape)}")
+            positions = positions.reshape(-1, B * T)
         depth = tree_depths(c.tree_parents) if c.tree_parents else list(range(T))
         tbl = self.table.cpu().long()
         pos, slots = [], []
@@ -533,13 +541,7 @@ class VerifyModel:
                 slots.append(int(tbl[b, p // c.page]) * c.page + p % c.page if t < lengths[b]
                              else -1)
         self.ids.copy_(ids.reshape(-1).to(dev))
-        if positions is None:
-            self.positions.copy_(torch.tensor(pos, dtype=torch.int64, device=dev))   # (of every axis)
-        elif not c.rope_sections:
-            raise SnowLLMError("set_batch: positions are for configurations with rope_sections")
-        else:
-            self.positions.copy_(torch.as_tensor(positions, dtype=torch.int64).reshape(
-                len(c.rope_sections), B * T))
+        self.positions.copy_(torch.tensor(pos, dtype=torch.int64, device=dev) if positions is None else positions)
         self.slots.copy_(torch.tensor(slots, dtype=torch.int32, device=dev))
         self.lens.copy_(torch.tensor([x + T for x in contexts], dtype=torch.int32, device=dev))
         self.lengths = lengths

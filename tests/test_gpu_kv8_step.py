@@ -117,5 +117,14 @@ def test_refusals(gpu):
     with pytest.raises(SnowLLMError, match="take turns"):
         VerifyModel(replace(cfg, rope_sections=(0, cfg.rot_half), rope_interleaved=True))
     m = VerifyModel(replace(cfg, kv8=True), seed=1)
+    with pytest.raises(SnowLLMError, match="pages of 16"):
+        VerifyModel(replace(cfg, kv8=True, page=32))
     with pytest.raises(SnowLLMError, match="rope_sections"):
         m.set_batch(torch.zeros(1, 9), [10], positions=torch.zeros(3, 1, 9))
+    n = VerifyModel(replace(cfg, kv8=True, rope_sections=(cfg.rot_half - 8, 4, 4)), seed=1)
+    n.set_block(torch.arange(9))
+    kept = n.ids.clone(), n.positions.clone()
+    for wrong in ((1, 1, 9), (3, 9), (3, 1, 8)):
+        with pytest.raises(SnowLLMError, match="axes of rope_sections"):
+            n.set_batch(torch.ones(1, 9), [10], positions=torch.zeros(wrong))
+    assert torch.equal(kept[0], n.ids) and torch.equal(kept[1], n.positions)   # nothing was staged
