@@ -51,11 +51,11 @@ struct AxesArgs {
   int count[MAX_AXES];     // pairs of each axis
 };
 
-// cos and sin of 2 pi t for |t| <= 1/2: a quarter turn and what is left, |z| <= pi / 4, whose Taylor series
-// to z^9 and z^8 leave less than 2^-24.
-__device__ __forceinline__ void cos_sin_turns(float t, float& c, float& s) {
-  const float quarter = rintf(4.f * t);
-  const float z = __builtin_fmaf(-0.25f, quarter, t) * 6.28318530717958648f, y = z * z;
+// cos and sin of 2 pi t for |t| <= 1/2: a quarter turn and what is left, |z| <= pi / 4, rounded to 32 bits
+// once; its Taylor series to z^9 and z^8 leave less than 2^-24.
+__device__ __forceinline__ void cos_sin_turns(double t, float& c, float& s) {
+  const double quarter = rint(4. * t);
+  const float z = (float)((t - 0.25 * quarter) * 6.28318530717958647693), y = z * z;
   float a = __builtin_fmaf(y, 1.f / 362880.f, -1.f / 5040.f);
   a = __builtin_fmaf(y, a, 1.f / 120.f);
   a = __builtin_fmaf(y, a, -1.f / 6.f);
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) axes_kernel(AxesArgs a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const double turns = (double)a.pos[axis[v] * a.rows + m] * freq[v];
-      cos_sin_turns((float)(turns - rint(turns)), c[v], s[v]);
+      cos_sin_turns(turns - rint(turns), c[v], s[v]);
     }
     float* cp = a.cosv + m * a.half + i0;
     float* sp = a.sinv + m * a.half + i0;
