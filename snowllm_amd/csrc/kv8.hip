@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(2 * D) read_kernel(ReadArgs a) {
 //   q_d = qs (256 h_d + l_d),   qs = max |q| / 32512: off by at most 2^-16 of the row's largest
 //   S_k = scale qs ks_k (256 K_k.h + K_k.l)
 //   p_k = 2^(S_k log2 e - m),   l = sum p_k,   m the row's maximum
-//   p_k vs_k = g (256 a_k + b_k),  g = max_k (p_k vs_k) / 32512 over 64 or 128 keys
+//   p_k vs_k = g (256 a_k + b_k),  g = max(max_k (p_k vs_k) / 32512, 2^-126) over 64 or 128 keys
 //   o_d += g (256 V_d.a + V_d.b),  sums of integers below 2^31, o and l in fp32
 // h and l are signed bytes; a is in 0 .. 127, b signed. Because g follows the keys, one with a large
 // weight costs only its neighbours' weights precision (2^-16 of it), not the whole context's.
@@ -544,8 +544,10 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
 #pragma unroll
   for (int j = 0; j < 16 * N; ++j) most = __builtin_elementwise_maximum(most, p[j]);   // NaN stays
   most = column_maximum(most);
-  const float g = most * (1.f / TERM);
-  const float f = fminf(__builtin_amdgcn_rcpf(g), 0x1p120f);
+  // g and its inverse are of one number that both can hold: products below 2^-111 get a unit of 2^-126, which
+  // is 2^-19 of V's least scale
+  const float g = __builtin_elementwise_maximum(most * (1.f / TERM), 0x1p-126f);   // NaN stays
+  const float f = __builtin_amdgcn_rcpf(g);
   i32x4 pa[N], pb[N], w[2][N];
 #pragma unroll
   for (int c = 0; c < N; ++c) w[0][c] = v(c, 0);
