@@ -403,7 +403,8 @@ int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, in
  * 64), those before starts[b] and the block's rows j < counts[b] whose bit j is set. Keys in pages
  * without a block or past the table are passed over; a row that sees none gets zeros; rows past a
  * request's count are left as they were. out must not overlap q; scale is finite. At most 65535
- * requests, and about 2^30 rows of (tokens * num_heads). */
+ * requests, and about 2^30 rows of (tokens * num_heads). Range: keys up to 2^104 in magnitude, scores and
+ * the sum of a row's values times their weights relative to its largest within fp32. */
 int snowverify_kv8_attention(const void* q, int64_t q_stride, const void* k_pool,
                              const void* v_pool, const float* k_scale, const float* v_scale,
                              void* out, const int32_t* table, const int32_t* starts,

@@ -83,7 +83,7 @@ def attention(q, cache, table, starts, counts, scale, T, tree=None):
         of the largest score plus 8 u; twice, for the weights and for their sum              -> 2 e W
       weights times v's scale as 16-bit integers of the largest of one or two GROUPs of keys (which two
         follows from where the keys are split): half a unit each, which is at least 2^-127 (2^-126 is the
-        least unit) beside a sum of weights of at least 1
+        least unit) beside a sum of weights of at least 2^-4
       sums of the keys' groups and of splits, in any order: (n / GROUP + 64) u W."""
     u = 2.0 ** -24
     M, Hq, d = q.shape
@@ -121,7 +121,7 @@ def attention(q, cache, table, starts, counts, scale, T, tree=None):
                     wv = w * vs[vis, h].double()
                     most = largest_near(wv, group, n // GROUP + 1)
                     out[m, h * G + e] = o
-                    unit = most[group] / 65024 + 2.0 ** -127
+                    unit = most[group] / 65024 + 2.0 ** -123
                     error[m, h * G + e] = (2 * off * big + unit @ v[vis, h].double().abs()
                                            + (n / GROUP + 64) * u * big)
     return out, error, live

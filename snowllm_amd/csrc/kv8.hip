@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(2 * D) read_kernel(ReadArgs a) {
 // The products run on the 8-bit matrix cores, exactly, with q and the weights as two 8-bit terms:
 //   q_d = qs (256 h_d + l_d),   qs = max |q| / 32512: off by at most 2^-16 of the row's largest
 //   S_k = scale qs ks_k (256 K_k.h + K_k.l)
-//   p_k = 2^(S_k log2 e - m),   l = sum p_k,   m the row's maximum
+//   p_k = 2^(S_k log2 e - m),   l = sum p_k,   m from the row's maximum to 2^4 above it
 //   p_k vs_k = g (256 a_k + b_k),  g = max(max_k (p_k vs_k) / 32512, 2^-126) over 64 or 128 keys
 //   o_d += g (256 V_d.a + V_d.b),  sums of integers below 2^31, o and l in fp32
 // h and l are signed bytes; a is in 0 .. 127, b signed. Because g follows the keys, one with a large
@@ -338,7 +338,7 @@ struct AttendArgs {
 
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float TERM = 32512.f;      // the largest value of two terms, 127 * 256
-constexpr float RESCALE = 8.f;       // the maximum moves when a score exceeds it by 2^8
+constexpr float MARGIN = 4.f;        // how far m is set above a row's maximum, as an exponent of 2
 
 // One row of a lane's column: it sees the positions below `end`, and those from there on by its mask.
 struct Row {
@@ -523,10 +523,11 @@ __device__ __forceinline__ void attend_keys(RowState<D>& st, const Query<D>& q, 
 #pragma unroll
   for (int j = 1; j < 16 * N; ++j) top = fmaxf(top, x[j]);
   top *= q.s;
-  // The maximum (the same in the four lanes of a row) moves only when a score is above it by more than
-  // 2^8 somewhere in the wave; weights are at most 2^8 then.
-  if (__builtin_amdgcn_ballot_w64(top > st.m + RESCALE) != 0) {
-    const float m = fmaxf(st.m, column_max(top));
+  // m (the same in the four lanes of a row) moves only when a score is above it somewhere in the wave, and
+  // then past it: weights are at most 1, so that with any V in bf16 their products are finite, and the
+  // largest at least 2^-4, so that 2^15 units of them are with V's least scale too.
+  if (__builtin_amdgcn_ballot_w64(top > st.m) != 0) {
+    const float m = fmaxf(st.m, column_max(top) + MARGIN);
     const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
 #pragma unroll
     for (int d = 0; d < D / 4; ++d) st.o[d] *= f;

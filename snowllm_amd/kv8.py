@@ -207,6 +207,10 @@ def kv8_attention(q, cache, out, table, starts, counts, scale, scratch=None, *, 
     bit j is set. The rows' own K and V must be in the cache. Keys in pages without a block, or past
     the table, are passed over; a row that sees no key gets zeros; rows past a request's count are
     left as they were. out must not overlap q. scratch: kv8_attention_scratch_bytes (may be 0: None).
+
+    Range: cached keys up to 2^104 in magnitude, scores and, summed over the keys, a row's values times
+    their weights relative to its largest within fp32; beyond that a row may not be finite. Queries
+    count from 2^-101 / 32512 on.
     """
     kp, vp, ksp, vsp, blocks, hkv, d, dev = _cache(cache)
     if q.dim() != 3:

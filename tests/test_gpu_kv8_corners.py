@@ -28,3 +28,52 @@ def test_values_near_the_least_scale(gpu, Hq, Hkv, d, T, start, form):
     want, error, live = R.attention(q, cache, table, st, ct, d ** -0.5, T)
     assert (error < 0.1 * want.abs().amax()).all()
     check_attention(got, want, error, live)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("Hq,Hkv,d,T,start", [(8, 2, 64, 9, 700), (16, 2, 128, 5, 300), (16, 2, 256, 9, 1500)])
+def test_values_near_the_largest_number(gpu, Hq, Hkv, d, T, start, form):
+    """A key whose score is 2^6 above those before it and whose value is the largest that bf16 holds, so that
+    the weights, relative to the row's first keys, times its value are past fp32.
+    Relative to the largest score the weights times the values are within it."""
+    say("largest", Hq, Hkv, d, T, start, form)
+    g = torch.Generator().manual_seed(d + T)
+    W = (start + T) // 16 + 1
+    cache = list(random_cache(g, W, Hkv, d))
+    q = 1 + 0.1 * torch.randn(T, Hq, d, generator=g)
+    q = q.bfloat16()
+    # scores 0.02 nats about 0, but for position 270: about 4.5
+    cache[0] = torch.randint(-127, 128, cache[0].shape, generator=g).to(torch.int8)
+    cache[2][:] = 0.02 / 127 / d ** 0.5
+    page, at = 270 // 16, 270 % 16
+    cache[0][page, :, at // 4, :, at % 4], cache[2][page, :, at] = 127, 4.5 / 127 / d
+    cache[3][page, :, at] = 2.0 ** 128 * (1 - 2.0 ** -8) / 127
+    cache = tuple(cache)
+    table = form_tables(torch.arange(W).int().view(1, W), form, Hq, Hkv, d, T)
+    st, ct = ints([start]), ints([T])
+    got = run_attention(*on_gpu(q, cache, table, st, ct), 1.0)
+    want, error, live = R.attention(q, cache, table, st, ct, 1.0, T)
+    assert want.isfinite().all() and (error < 0.1 * want.abs().amax()).all()
+    check_attention(got, want, error, live)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("Hq,Hkv,d,T,start", [(8, 2, 64, 9, 700), (16, 2, 128, 5, 300), (16, 2, 256, 9, 1500)])
+def test_keys_and_queries_far_from_one(gpu, Hq, Hkv, d, T, start, form):
+    """The largest keys that scores are held for (2^104) against queries of 2^-98, and the other way round:
+    keys of 2^-98 against the largest queries."""
+    say("far", Hq, Hkv, d, T, start, form)
+    g = torch.Generator().manual_seed(d + T)
+    W = (start + T) // 16 + 1
+    first = random_cache(g, W, Hkv, d)
+    table = form_tables(tables(g, 1, W, W), form, Hq, Hkv, d, T)
+    x = torch.randn(T, Hq, d, generator=g).clamp(-3, 3)
+    st, ct = ints([start]), ints([T])
+    # codes of 42, scores of about 42 / 127 * sqrt(d) * 2^6 scale
+    for key, query, scale in ((2.0 ** 104, 2.0 ** -98, 2.0 ** -6), (2.0 ** -98, 2.0 ** 126, 2.0 ** -28)):
+        cache = (*first[:2], torch.full_like(first[2], key / 127), first[3])
+        q = (x * query).bfloat16()
+        got = run_attention(*on_gpu(q, cache, table, st, ct), scale)
+        want, error, live = R.attention(q, cache, table, st, ct, scale, T)
+        assert (error < 0.1 * want.abs().amax()).all()
+        check_attention(got, want, error, live)
