@@ -424,8 +424,10 @@ __device__ __forceinline__ void fetch_query(RawQuery<D>& raw, const AttendArgs& 
     for (int i = 0; i < 2; ++i) raw.w[s][i] = *(const u32x4*)(p + 64 * s + 8 * i);
 }
 
+// A row that is not `there` (past the request's count) as zeros: whatever its memory holds would have a say in
+// when the maxima of the tile's other rows move, and so in their bits.
 template <int D>
-__device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a, const RawQuery<D>& raw) {
+__device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a, const RawQuery<D>& raw, bool there) {
   float v[D / 64][16], top = 0.f;
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
@@ -433,8 +435,9 @@ __device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a,
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[s][8 * i + 2 * e] = __uint_as_float(raw.w[s][i][e] << 16);
-        v[s][8 * i + 2 * e + 1] = __uint_as_float(raw.w[s][i][e] & 0xffff0000u);
+        const uint32_t w = there ? raw.w[s][i][e] : 0u;
+        v[s][8 * i + 2 * e] = __uint_as_float(w << 16);
+        v[s][8 * i + 2 * e + 1] = __uint_as_float(w & 0xffff0000u);
       }
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
@@ -837,7 +840,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   RowState<D> st;
   clear(st);
   Query<D> q;
-  quantise_query(q, a, raw);
+  quantise_query(q, a, raw, x.m >= 0);
   for (; c < w.c1; c += WAVES) {
     const bool there = valid(here.v), more = c + WAVES < w.c1;
     const bool all = __builtin_amdgcn_ballot_w64(!there) == 0 && c * 64 + 64 <= common;
@@ -982,7 +985,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   RowState<D> st;
   clear(st);
   Query<D> q;
-  quantise_query(q, a, raw);
+  quantise_query(q, a, raw, x.m >= 0);
   // a wave's steps: N = 2, both chunks of each, or 1, the part-th
   auto walk = [&](auto chunks) {
     constexpr int N = decltype(chunks)::value;

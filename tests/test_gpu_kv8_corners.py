@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from oracle import kv8 as R
-from tests.test_gpu_kv8 import FORMS, check_attention, form_tables, ints, on_gpu, random_cache, run_attention, say, tables
+from tests.test_gpu_kv8 import (FORMS, check_attention, form_tables, ints, on_gpu, random_cache, run_attention,
+                                say, tables, tree_masks)
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,30 @@ def test_keys_and_queries_far_from_one(gpu, Hq, Hkv, d, T, start, form):
         want, error, live = R.attention(q, cache, table, st, ct, scale, T)
         assert (error < 0.1 * want.abs().amax()).all()
         check_attention(got, want, error, live)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("Hq,Hkv,d,T,starts,counts,tree", [
+    (8, 1, 64, 9, [3000], [5], False), (16, 2, 256, 9, [2000], [3], True), (32, 8, 128, 4, [700, 90], [1, 3], False),
+    (8, 2, 128, 70, [400], [33], False), (64, 8, 64, 9, [6000], [5], False)])
+def test_padding_rows_do_not_reach_the_others(gpu, Hq, Hkv, d, T, starts, counts, tree, form):
+    """The bits of a request's rows are the same whatever the rows past its count hold."""
+    say("padding", Hq, Hkv, d, T, starts, counts, tree, form)
+    g = torch.Generator().manual_seed(d + T)
+    B = len(starts)
+    W = (max(starts) + T) // 16 + 1
+    cache = random_cache(g, B * W, Hkv, d)
+    table = form_tables(tables(g, B, W, B * W), form, Hq, Hkv, d, T)
+    q = torch.randn(B * T, Hq, d, generator=g).bfloat16()
+    noise = torch.randn(B * T, Hq, d, generator=g)
+    masks = torch.cat([tree_masks(g, T) for _ in range(B)]) if tree else None
+    live = (torch.arange(T)[None] < torch.tensor(counts)[:, None]).view(-1)
+    gc, gt, gs, gn, gm = on_gpu(cache, table, ints(starts), ints(counts), masks)
+    seen = []
+    for padding in (torch.zeros_like(noise), noise * 40, noise * 1e30, torch.full_like(noise, float("nan")),
+                    torch.full_like(noise, float("inf"))):
+        x = torch.where(live[:, None, None], q, padding.bfloat16())
+        seen.append(run_attention(x.cuda(), gc, gt, gs, gn, d ** -0.5, gm).cpu())
+    check_attention(seen[0], *R.attention(q, cache, table, ints(starts), ints(counts), d ** -0.5, T, masks))
+    for other in seen[1:]:
+        assert torch.equal(other, seen[0])
