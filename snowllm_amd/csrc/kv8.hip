@@ -425,9 +425,10 @@ __device__ __forceinline__ void fetch_query(RawQuery<D>& raw, const AttendArgs& 
 }
 
 // A row that is not `there` (past the request's count) as zeros: whatever its memory holds would have a say in
-// when the maxima of the tile's other rows move, and so in their bits.
+// when the maxima of the tile's other rows move, and so in their bits. False where an element is not finite: such a
+// row's scores are finite and mean nothing, so that its sum says whether it sees a key (see sum_of).
 template <int D>
-__device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a, const RawQuery<D>& raw, bool there) {
+__device__ __forceinline__ bool quantise_query(Query<D>& q, const AttendArgs& a, const RawQuery<D>& raw, bool there) {
   float v[D / 64][16], top = 0.f;
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
@@ -445,13 +446,12 @@ __device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a,
     for (int e = 0; e < 16; ++e)
       top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[s][e]));   // NaN stays
   top = column_maximum(top);
-  // rows below 2^-100 as zeros, as in the cache; an element that is not finite makes the scores NaN
+  // rows below 2^-100 as zeros, as in the cache
   const float most = fmaxf(top, LEAST);
   const float f = a.scale < 0.f ? -TERM / most : TERM / most;
   // (never zero: a hidden key's -inf times it stays -inf)
-  q.s = top < __builtin_huge_valf()
-            ? fmaxf(most * (1.f / TERM) * __builtin_fabsf(a.scale) * kLog2e, 0x1p-126f)
-            : __uint_as_float(0x7fc00000u);
+  const bool fine = top < __builtin_huge_valf();
+  q.s = fine ? fmaxf(most * (1.f / TERM) * __builtin_fabsf(a.scale) * kLog2e, 0x1p-126f) : 0x1p-126f;
 #pragma unroll
   for (int s = 0; s < D / 64; ++s)
 #pragma unroll
@@ -464,6 +464,12 @@ __device__ __forceinline__ void quantise_query(Query<D>& q, const AttendArgs& a,
       q.h[s][e] = h;
       q.l[s][e] = l;
     }
+  return fine;
+}
+
+// The sum l of a row's weights, NaN where its query is not finite and it sees a key.
+__device__ __forceinline__ float sum_of(float l, bool fine) {
+  return fine || l == 0.f ? l : __uint_as_float(0x7fc00000u);
 }
 
 // N times 64 keys (four pages): of the c-th, k(c, n, s) is the K operand of product n, elements 64 s ..,
@@ -840,7 +846,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
   RowState<D> st;
   clear(st);
   Query<D> q;
-  quantise_query(q, a, raw, x.m >= 0);
+  const bool fine = quantise_query(q, a, raw, x.m >= 0);
   for (; c < w.c1; c += WAVES) {
     const bool there = valid(here.v), more = c + WAVES < w.c1;
     const bool all = __builtin_amdgcn_ballot_w64(!there) == 0 && c * 64 + 64 <= common;
@@ -857,6 +863,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_kernel(KV8_FRONT) {
       next = look_up(c + 2 * WAVES);
     }
   }
+  st.l = sum_of(st.l, fine);
   join_waves<D, WAVES>(a, w, st, os, ml, wave, tile);
 }
 
@@ -985,7 +992,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
   RowState<D> st;
   clear(st);
   Query<D> q;
-  quantise_query(q, a, raw, x.m >= 0);
+  const bool fine = quantise_query(q, a, raw, x.m >= 0);
   // a wave's steps: N = 2, both chunks of each, or 1, the part-th
   auto walk = [&](auto chunks) {
     constexpr int N = decltype(chunks)::value;
@@ -1066,6 +1073,7 @@ __global__ void __launch_bounds__(64 * RING_WAVES) attend_ring_kernel(KV8_FRONT)
     }
   }
   if (x.m < 0) return;
+  l = sum_of(l, fine);
   if (w.single) {
     const float f = inverse_sum(l);
 #pragma unroll

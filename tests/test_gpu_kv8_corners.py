@@ -105,3 +105,35 @@ def test_padding_rows_do_not_reach_the_others(gpu, Hq, Hkv, d, T, starts, counts
     check_attention(seen[0], *R.attention(q, cache, table, ints(starts), ints(counts), d ** -0.5, T, masks))
     for other in seen[1:]:
         assert torch.equal(other, seen[0])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("Hq,Hkv,d,start", [(16, 2, 256, 0), (8, 2, 64, 0), (16, 2, 128, 3000), (8, 1, 128, 300)])
+def test_queries_that_are_not_finite_and_see_nothing(gpu, Hq, Hkv, d, start, form):
+    """Zeros for a row that sees no key, NaN for one that does: by ancestor masks, over pages without a block."""
+    say("nothing", Hq, Hkv, d, start, form)
+    g = torch.Generator().manual_seed(d + start)
+    T = 8
+    W = (start + T) // 16 + 1
+    cache = random_cache(g, W, Hkv, d)
+    table = tables(g, 1, W, W)
+    if start:
+        table[0, :start // 16] = -1     # the context has no block but for its last page
+        start = start // 16 * 16
+    table = form_tables(table, form, Hq, Hkv, d, T)
+    q = torch.randn(T, Hq, d, generator=g).bfloat16()
+    q[0, :, 3], q[1, 0, 5], q[2, :, 7], q[3, 1, 9] = float("nan"), float("inf"), float("-inf"), float("nan")
+    masks = torch.tensor([0, 0, 4, 1, 16, 0, 64, 255])
+    args = on_gpu(q, cache, table, ints([start]), ints([T]))
+    got = run_attention(*args, d ** -0.5, masks.cuda()).cpu()
+    fine = q.isfinite().all(-1)
+    nothing = masks == 0
+    assert (got[nothing] == 0).all()
+    assert got[~nothing][~fine[~nothing]].isnan().all()
+    want, error, live = R.attention(torch.where(fine[..., None], q, 0), cache, table, ints([start]), ints([T]),
+                                    d ** -0.5, T, masks)
+    rest = fine & ~nothing[:, None]
+    assert rest.any() and ((got.double() - want).abs() <= 2.0 ** -8 * (want.abs() + error) + error)[rest].all()
+    # nothing at all
+    args[2] = torch.full_like(args[2], -1)
+    assert (run_attention(*args, d ** -0.5).cpu() == 0).all()
