@@ -167,7 +167,7 @@ __device__ __forceinline__ u32x2 quantise(const float (&y)[8], float& scale) {
 // its threads take a token's row each, and the codes go through LDS into the page's layout, so that every
 // write is of 16 bytes but in pages that begin or end a request. Bound by bytes, most of them the
 // queries' (8192 rows of 16 + 2 heads of 256: 145 MB in 31 us).
-template <int D>
+template <int D, bool PASS_BY>
 __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   constexpr int W = D / 8, VP = D + 8;   // VP: pitch of V's codes in LDS, by token
   __shared__ __attribute__((aligned(16))) uint8_t ks[PAGE * D];
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   const int tid = threadIdx.x, r = tid / W, c = tid % W;
   int64_t wg = blockIdx.x;
   if (wg >= a.page_wgs) {
-    rotate_queries<D>((uint32_t)(wg - a.page_wgs) * 16 + r, c, a.rows);
+    rotate_queries<D, PASS_BY>((uint32_t)(wg - a.page_wgs) * 16 + r, c, a.rows);
     return;
   }
   const int h = (int)(wg % a.Hkv);
@@ -1287,7 +1287,10 @@ SV_API int snowverify_kv8_append(const void* k, int64_t k_stride, const void* v,
   const int64_t groups = (num_heads + Q_HEADS - 1) / Q_HEADS;
   const int64_t grid = a.page_wgs + (q ? (batch * tokens * groups + 15) / 16 : 0);
   if (!grid_ok(grid, 2 * head_size)) return SV_EINVAL;
-  auto kern = head_size == 64 ? append_kernel<64> : head_size == 128 ? append_kernel<128> : append_kernel<256>;
+  const bool by = q && queries_pass_by(batch * tokens, num_heads, head_size);
+  auto kern = head_size == 64    ? by ? append_kernel<64, true> : append_kernel<64, false>
+              : head_size == 128 ? by ? append_kernel<128, true> : append_kernel<128, false>
+              : by               ? append_kernel<256, true> : append_kernel<256, false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3((unsigned)(2 * head_size)), 0, S(stream), a);
   SV_CHECK_LAUNCH();
   return SV_OK;

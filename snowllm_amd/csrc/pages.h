@@ -212,8 +212,8 @@ struct QueryRows {
 constexpr int Q_HEADS = 4;   // heads of a row that a thread rotates: their loads are in flight at once
 
 // The queries of a cache write: D / 8 neighbouring threads take unit u, Q_HEADS heads of one row
-// (ceil(heads / Q_HEADS) units a row), c of them this thread.
-template <int D>
+// (ceil(heads / Q_HEADS) units a row), c of them this thread. PASS_BY: past the caches (queries_pass_by).
+template <int D, bool PASS_BY>
 __device__ __forceinline__ void rotate_queries(uint32_t u, int c, const QueryRows& a) {
   const uint32_t groups = (uint32_t)(a.Hq + Q_HEADS - 1) / Q_HEADS;
   const uint32_t m = u / groups;
@@ -226,15 +226,18 @@ __device__ __forceinline__ void rotate_queries(uint32_t u, int c, const QueryRow
 #pragma unroll
   for (int i = 0; i < Q_HEADS; ++i) {
     raw[i] = u32x4{0u, 0u, 0u, 0u};
-    if (i < heads)
-      raw[i] = __builtin_nontemporal_load((const u32x4*)(a.q + mr * a.stride + (int64_t)(head + i) * D + 8 * c));
+    const u32x4* p = (const u32x4*)(a.q + mr * a.stride + (int64_t)(head + i) * D + 8 * c);
+    if (i < heads) raw[i] = PASS_BY ? __builtin_nontemporal_load(p) : *p;
   }
   const Rotation turn =
       load_rotation(c, a.gamma, a.eps, a.cosv + mr * a.cs_stride, a.sinv + mr * a.cs_stride, a.half);
 #pragma unroll
   for (int i = 0; i < Q_HEADS; ++i) {
     const u32x4 o = rotate_norm<D>(raw[i], turn);
-    if (i < heads) __builtin_nontemporal_store(o, (u32x4*)(a.out + (mr * a.Hq + head + i) * D + 8 * c));
+    u32x4* p = (u32x4*)(a.out + (mr * a.Hq + head + i) * D + 8 * c);
+    if (i >= heads) continue;
+    if (PASS_BY) __builtin_nontemporal_store(o, p);
+    else *p = o;
   }
 }
 
@@ -245,6 +248,11 @@ constexpr int64_t MAX_BATCH_ROWS = 1 << 24;   // batch * tokens
 
 // A launch holds fewer than 2^32 threads.
 inline bool grid_ok(int64_t wgs, int64_t threads) { return wgs <= 0xffffffffll / threads; }
+
+// Whether a cache write's queries go past the caches: from 40 MiB of them on, which go in and out beside the
+// keys and values. Over three sets of buffers in turn, 34 MB of queries take 18.3 us and past the caches 20.3
+// (17 MB 11.7 and 13.3, 1.2 MB 4.4 and 4.9), 50 MB 28.4 and 27.0, 134 MB 68 and 62.
+inline bool queries_pass_by(int64_t rows, int64_t Hq, int64_t D) { return rows * Hq * D * 2 >= (40ll << 20); }
 
 inline bool head_shape_ok(int64_t batch, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D) {
   return batch >= 0 && tokens >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq <= 4096 &&

@@ -67,15 +67,16 @@ struct AppendArgs {
   int64_t page_wgs;        // workgroups over (request, page, kv head); the rest rotate queries
 };
 
-// Bound by its bytes: four prompts of about 2048 rows (q and k normalised, 150 MB) take 41 us (3.7 TB/s),
-// 34 of them in the kernel; one row of a 128-wide model 4 us, a dependent load of start, table entry and
-// rows each. A thread's four heads of queries: 41 us against 47 with one.
+// Bound by its bytes: four prompts of about 2048 rows (q and k normalised, 150 MB) take 31 us (4.8 TB/s); one
+// row of a 128-wide model 4 us, a dependent load of start, table entry and rows each. A thread has four heads
+// of queries (41 us against 47 with one, when gammas and angles were loaded for each head and the queries went
+// through the caches).
 // 2 D threads: sixteen heads of D / 8 threads each. A page workgroup owns one (request, page, kv
 // head): its threads take a token's row each, normalise and rotate it, and pass it through LDS into
 // the page's layout, so that global reads and writes are both contiguous. The page's bounds are
 // taken from the same LDS image, to which the page's older keys are loaded first: they come out the
 // same whatever was in the page behind the last row (rejected drafts) and need no atomics.
-template <int D>
+template <int D, bool PASS_BY>
 __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   constexpr int W = D / 8, LD = D + 8;   // row pitch of the LDS tiles: 16 bytes more than a row
   __shared__ __attribute__((aligned(16))) uint16_t ks[PAGE * LD];
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
   const int tid = threadIdx.x, r = tid / W, c = tid % W;
   int64_t wg = blockIdx.x;
   if (wg >= a.page_wgs) {   // queries: sixteen units of a row and Q_HEADS heads
-    rotate_queries<D>((uint32_t)(wg - a.page_wgs) * 16 + r, c, a.rows);
+    rotate_queries<D, PASS_BY>((uint32_t)(wg - a.page_wgs) * 16 + r, c, a.rows);
     return;
   }
   const int h = (int)(wg % a.Hkv);
@@ -1774,7 +1775,10 @@ SV_API int snowverify_kv_append(const void* k, int64_t k_stride, const void* v, 
   const int64_t groups = (num_heads + Q_HEADS - 1) / Q_HEADS;
   const int64_t grid = a.page_wgs + (q ? (batch * tokens * groups + 15) / 16 : 0);
   if (!grid_ok(grid, 2 * head_size)) return SV_EINVAL;
-  auto kern = head_size == 64 ? append_kernel<64> : head_size == 128 ? append_kernel<128> : append_kernel<256>;
+  const bool by = q && queries_pass_by(batch * tokens, num_heads, head_size);
+  auto kern = head_size == 64    ? by ? append_kernel<64, true> : append_kernel<64, false>
+              : head_size == 128 ? by ? append_kernel<128, true> : append_kernel<128, false>
+              : by               ? append_kernel<256, true> : append_kernel<256, false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3((unsigned)(2 * head_size)), 0, S(stream), a);
   SV_CHECK_LAUNCH();
   return SV_OK;

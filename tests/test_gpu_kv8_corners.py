@@ -137,3 +137,35 @@ def test_queries_that_are_not_finite_and_see_nothing(gpu, Hq, Hkv, d, start, for
     # nothing at all
     args[2] = torch.full_like(args[2], -1)
     assert (run_attention(*args, d ** -0.5).cpu() == 0).all()
+
+
+@pytest.mark.parametrize("writer", ["kv_append", "kv8_append"])
+def test_many_queries_as_in_parts(gpu, writer):
+    """A cache write whose queries go past the caches (40 MiB of them) and the same rows in two calls whose do
+    not: the same bits."""
+    from snowllm_amd import ops
+    say("many queries", writer)
+    Hq, Hkv, d, half, T = 32, 2, 128, 64, 5121
+    W = T // 16 + 1
+    g = torch.Generator(device="cuda").manual_seed(9)
+    bf = dict(dtype=torch.bfloat16, device="cuda")
+    q = torch.empty(T, Hq, d, **bf).normal_(generator=g)
+    k, v = torch.empty(2, T, Hkv, d, **bf).normal_(generator=g)
+    gamma = torch.empty(d, **bf).normal_(generator=g)
+    cos, sin = torch.rand(2, T, half, device="cuda", generator=g)
+    table = torch.randperm(W, device="cuda", generator=g).int()[None]
+    got = []
+    for cuts in ((0, T), (0, 2000, T)):
+        if writer == "kv8_append":
+            cache = list(ops.kv8_cache(W, Hkv, d))
+        else:
+            cache = [torch.zeros(W, Hkv, d // 16, 16, 16, **bf), torch.zeros(W, Hkv, 4, d, 4, **bf)]
+        out = torch.zeros_like(q)
+        for a, b in zip(cuts, cuts[1:]):
+            rows = slice(a, b)
+            span = on_gpu(ints([a]), ints([b - a - (b == T)]))      # the last row is none of the request's
+            args = (k[rows], v[rows], cos[rows], sin[rows], *((cache,) if writer == "kv8_append" else cache), table, *span)
+            getattr(ops, writer)(*args, q=q[rows], q_out=out[rows], q_gamma=gamma, k_gamma=gamma)
+        got.append(cache + [out])
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    assert (got[0][-1][-1] == 0).all() and (got[0][-1][:-1] != 0).any()
