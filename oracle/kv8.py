@@ -78,7 +78,7 @@ def attention(q, cache, table, starts, counts, scale, T, tree=None):
     may be from it before its last rounding (see below), live [M] the rows that are written.
 
     error counts, with u = 2^-24 and W = sum_k w_k |v_k| of the normalised weights w:
-      scores: q as 16-bit integers is off by half of max|q| / 32512 an element; the integer products are
+      scores: q as 16-bit integers is off by half of max(max|q|, LEAST) / 32512 an element; the integer products are
         exact, their conversion, the two factors, the maximum's subtraction and the exponential are 8 u
         of the largest score plus 8 u; twice, for the weights and for their sum              -> 2 e W
       weights times v's scale as 16-bit integers of the largest of one or two GROUPs of keys (which two
@@ -115,7 +115,7 @@ def attention(q, cache, table, starts, counts, scale, T, tree=None):
                     s = key @ x * scale
                     w = s.softmax(0)
                     o = w @ val
-                    off = abs(scale) * x.abs().max() / 65024 * key.abs().sum(1).max()
+                    off = abs(scale) * x.abs().max().clamp(min=LEAST) / 65024 * key.abs().sum(1).max()
                     off = off + 8 * u * (s.abs().max() + 1)
                     big = w @ val.abs()
                     wv = w * vs[vis, h].double()

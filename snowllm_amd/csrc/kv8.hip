@@ -9,8 +9,8 @@
 //   scale = max(max_d |x_d|, 2^-100) / 127,  code_d = rint(x_d / scale),  x_d ~ code_d * scale,
 // in pages of 16 tokens: K [blocks, Hkv, 4, d/16, 4, 16] (token t is group t / 4, place t % 4), V
 // [blocks, Hkv, d, 16], scales [blocks, Hkv, 16]. A row with an element that is not finite has a NaN
-// scale and zero codes. The least scale keeps 127 / max finite and every scale a normal number; rows
-// below 2^-100 read back as zeros.
+// scale and zero codes. The least scale keeps 127 / max finite and every scale a normal number; elements
+// below half of it (2^-101 / 127) read back as zeros.
 //
 // The layouts are the operands of the attention's 64-key products (v_mfma_i32_16x16x64_i8): 16 bytes
 // of K are 16 elements of a token, 16 bytes of V the 16 tokens of a page at one element, and a lane's
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(2 * D) read_kernel(ReadArgs a) {
 // attend
 // ---------------------------------------------------------------------------------------
 // The products run on the 8-bit matrix cores, exactly, with q and the weights as two 8-bit terms:
-//   q_d = qs (256 h_d + l_d),   qs = max |q| / 32512: off by at most 2^-16 of the row's largest
+//   q_d = qs (256 h_d + l_d),   qs = max(max |q|, 2^-100) / 32512: off by at most 2^-16 of the row's largest
 //   S_k = scale qs ks_k (256 K_k.h + K_k.l)
 //   p_k = 2^(S_k log2 e - m),   l = sum p_k,   m from the row's maximum to 2^4 above it
 //   p_k vs_k = g (256 a_k + b_k),  g = max(max_k (p_k vs_k) / 32512, 2^-126) over 64 or 128 keys
@@ -446,7 +446,7 @@ __device__ __forceinline__ bool quantise_query(Query<D>& q, const AttendArgs& a,
     for (int e = 0; e < 16; ++e)
       top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[s][e]));   // NaN stays
   top = column_maximum(top);
-  // rows below 2^-100 as zeros, as in the cache
+  // in units of 2^-100 / 32512 at least: elements below half of that count as zeros
   const float most = fmaxf(top, LEAST);
   const float f = a.scale < 0.f ? -TERM / most : TERM / most;
   // (never zero: a hidden key's -inf times it stays -inf)

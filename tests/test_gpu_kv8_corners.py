@@ -4,8 +4,8 @@ import pytest
 import torch
 
 from oracle import kv8 as R
-from tests.test_gpu_kv8 import (FORMS, check_attention, form_tables, ints, on_gpu, random_cache, run_attention,
-                                say, tables, tree_masks)
+from tests.test_gpu_kv8 import (FORMS, check_attention, check_code, form_tables, ints, on_gpu, random_cache,
+                                run_attention, say, tables, tree_masks)
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +169,46 @@ def test_many_queries_as_in_parts(gpu, writer):
         got.append(cache + [out])
     assert all(torch.equal(x, y) for x, y in zip(*got))
     assert (got[0][-1][-1] == 0).all() and (got[0][-1][:-1] != 0).any()
+
+
+def test_rows_about_the_least_scale_read_back(gpu):
+    """Rows whose largest magnitude is below 2^-100 keep what half of the least scale resolves."""
+    from snowllm_amd import ops
+    g = torch.Generator().manual_seed(8)
+    T, Hkv, d = 16, 2, 64
+    x = torch.randn(T, Hkv, d, generator=g)
+    x = x / x.abs().amax(-1, keepdim=True)
+    size = 2.0 ** -torch.tensor([100, 100.2, 101, 102, 103, 104, 105, 106, 107, 108, 108.5, 110, 120, 126, 130, 133])
+    x = (x * size[:, None, None]).bfloat16()
+    cache = ops.kv8_cache(1, Hkv, d)
+    none = torch.zeros(T, 0).cuda()
+    args = on_gpu(ints([[0]]), ints([0]), ints([T]))
+    ops.kv8_append(x.cuda(), x.cuda(), none, none, cache, *args)
+    k, v = torch.ones(2, T, Hkv, d, dtype=torch.bfloat16, device="cuda")
+    ops.kv8_read(cache, *args, k, v)
+    host = tuple(y.cpu() for y in cache)
+    for t in range(T):
+        ck, cv, ks, vs = R.code_of(host, 0, t)
+        check_code(ck, ks, x[t].double(), torch.zeros(1), "K")
+        check_code(cv, vs, x[t].double(), torch.zeros(1), "V")
+    # half of the least scale is 2^-107.99: rows of 2^-107 are there, those of 2^-108.5 are not
+    there = (size >= 2.0 ** -107)
+    for y in (k.cpu(), v.cpu()):
+        assert (y[there].abs().amax(-1) > 0).all() and (y[size < 2.0 ** -108.2] == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_queries_below_the_least_unit(gpu, form):
+    """Queries of 2^-104 to 2^-102 against keys of 2^104: their scores count."""
+    g = torch.Generator().manual_seed(10)
+    Hq, Hkv, d, T, start = 16, 2, 128, 5, 300
+    W = (start + T) // 16 + 1
+    first = random_cache(g, W, Hkv, d)
+    cache = (*first[:2], torch.full_like(first[2], 2.0 ** 104 / 127), first[3])
+    table = form_tables(tables(g, 1, W, W), form, Hq, Hkv, d, T)
+    q = (torch.randn(T, Hq, d, generator=g).clamp(-4, 4) * 2.0 ** -104).bfloat16()
+    got = run_attention(*on_gpu(q, cache, table, ints([start]), ints([T])), 0.5)
+    want, error, live = R.attention(q, cache, table, ints([start]), ints([T]), 0.5, T)
+    mean, _, _ = R.attention(q * 0, cache, table, ints([start]), ints([T]), 0.5, T)
+    assert (error < 0.1 * want.abs().amax()).all() and ((want - mean).abs() > error).any(-1).all()
+    check_attention(got, want, error, live)
