@@ -398,6 +398,10 @@ int snowverify_kv8_read(const void* k_pool, const void* v_pool, const float* k_s
 int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t num_heads,
                                                int64_t num_kv_heads, int64_t head_size,
                                                int64_t table_stride);
+/* Which form of the kernel a call of this shape takes: 0 a workgroup for each tile of 16 rows of a kv head,
+ * 1 up to eight tiles that share their keys, -1 no such shape. Both give a result within the same bounds. */
+int snowverify_kv8_attention_form(int64_t batch, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                                  int64_t head_size, int64_t table_stride);
 /* out[m, h] = softmax(scale q k^T) v: row t of request b (q row m = b * tokens + t at q + m * q_stride)
  * sees the positions up to starts[b] + t, or, with tree (ancestor masks u64 [batch*tokens], tokens <=
  * 64), those before starts[b] and the block's rows j < counts[b] whose bit j is set. Keys in pages

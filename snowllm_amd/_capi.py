@@ -123,6 +123,7 @@ _SIGS = [
      [P] * 8 + [c_int64] * 7 + [S]),
     ("snowverify_kv8_read", c_int, [P] * 9 + [c_int64] * 6 + [S]),
     ("snowverify_kv8_attention_scratch_bytes", c_int64, [c_int64] * 6),
+    ("snowverify_kv8_attention_form", c_int, [c_int64] * 6),
     ("snowverify_kv8_attention", c_int, [P, c_int64] + [P] * 9 + [c_int64] * 7 +
      [c_float, P, c_int64, S]),
     # geometry-driven operator entry points (reference signatures)

@@ -1328,6 +1328,14 @@ SV_API int64_t snowverify_kv8_attention_scratch_bytes(int64_t batch, int64_t tok
   return attend_bytes(p, num_kv_heads, head_size);
 }
 
+SV_API int snowverify_kv8_attention_form(int64_t batch, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                                         int64_t head_size, int64_t table_stride) {
+  if (!head_shape_ok(batch, tokens, num_heads, num_kv_heads, head_size) || table_stride < 0 ||
+      table_stride > MAX_PAGES || batch * tokens == 0)
+    return -1;
+  return attend_plan(batch, tokens, num_heads, num_kv_heads, head_size, table_stride).ring;
+}
+
 SV_API int snowverify_kv8_attention(const void* q, int64_t q_stride, const void* k_pool,
                                     const void* v_pool, const float* k_scale, const float* v_scale,
                                     void* out, const int32_t* table, const int32_t* starts,
