@@ -211,6 +211,11 @@ def kv8_attention(q, cache, out, table, starts, counts, scale, scratch=None, *, 
     Range: cached keys up to 2^104 in magnitude, scores and, summed over the keys, a row's values times
     their weights relative to its largest within fp32; beyond that a row may not be finite. Queries
     count from 2^-101 / 32512 on.
+
+    Time: two to 64 requests share the workgroups by their lengths, where there are enough for a split of
+    each; one request, or more than 64, are split by the table's width, so that a table much wider
+    than its contexts costs time (9 rows of 32 heads of 128 behind 8K tokens 14 us, with a table
+    for 131K 66).
     """
     kp, vp, ksp, vsp, blocks, hkv, d, dev = _cache(cache)
     if q.dim() != 3:

@@ -75,7 +75,7 @@ class VerifyConfig:
     sparse_sink: int = 1
     sparse_recent: int = 2
     # KV cache in 8 bits: half the memory always. A layer of 9 rows with 8 kv heads of 128 takes 2 us more
-    # behind 8K tokens, 5 less behind 32K; with 2 of 256 5 more behind 8K, 1 more behind 64K, 19 less
+    # behind 8K tokens, 5 less behind 32K; with 2 of 256 5 more behind 8K, 1 more behind 64K, 20 less
     # behind 220K (a launch more than the bf16 step, whose attention writes the cache itself)
     kv8: bool = False
     # rotated pairs of every position axis (time, height, width), rot_half in all; empty: one axis
