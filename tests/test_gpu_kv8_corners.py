@@ -212,3 +212,31 @@ def test_queries_below_the_least_unit(gpu, form):
     mean, _, _ = R.attention(q * 0, cache, table, ints([start]), ints([T]), 0.5, T)
     assert (error < 0.1 * want.abs().amax()).all() and ((want - mean).abs() > error).any(-1).all()
     check_attention(got, want, error, live)
+
+
+@pytest.mark.parametrize("kind,change", [("dense", {}), ("moe", {}), ("dense", dict(sparse_pages=8)), ("moe", dict(kv8=True))])
+def test_step_with_several_axes_over_every_cache(gpu, monkeypatch, kind, change):
+    """rope_sections beside each kind of cache: the step's angles are those of the axes, and with the same
+    angles the step is the one of a single axis, bit for bit."""
+    from dataclasses import replace
+
+    from snowllm_amd import layers, ops
+    from snowllm_amd.verify import VerifyModel
+    from tests.test_gpu_batch import tiny
+    say("step", kind, change)
+    cfg = replace(tiny(kind), **change)
+    half = cfg.rot_half
+    several = replace(cfg, rope_sections=(half - 16, 8, 8), rope_interleaved=False)
+    one, m = VerifyModel(cfg, seed=3), VerifyModel(several, seed=3)
+    ids = torch.arange(cfg.block).view(1, -1) * 7 % cfg.vocab
+    for x in (one, m):
+        x.set_batch(ids, [200])
+    want = one.forward().clone()
+    m.forward()
+    angles = R.angles(m.positions.cpu(), m.inv_freq.cpu(), several.rope_sections, False)
+    assert ((m.cos.cpu() - angles.cos()).abs() <= 8 * 2.0 ** -24).all()
+    assert ((m.sin.cpu() - angles.sin()).abs() <= 8 * 2.0 ** -24).all()
+    again = VerifyModel(several, seed=3)
+    again.set_batch(ids, [200])
+    monkeypatch.setattr(ops, "rope_axes", lambda p, f, c, s, *_, **__: layers.rope_cos_sin(p[0].contiguous(), f, c, s))
+    assert torch.equal(again.forward(), want)
