@@ -1,4 +1,5 @@
-"""The attention over the cache in 8 bits at the ends of its range of values. Tolerances are those of
+"""The cache in 8 bits where it can go wrong: the ends of the attention's range of values, rows that are not
+there or see nothing, writes of many queries, several position axes in the step. Tolerances are those of
 test_gpu_kv8.py and of the oracle (oracle/kv8.py)."""
 import pytest
 import torch
